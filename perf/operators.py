@@ -170,7 +170,8 @@ def _values(codes, scales):
 def _exponent(amax, least=-40):
     """The smallest integer e >= least with amax <= 127 * 2^e."""
     m, x = torch.frexp(amax)
-    return torch.where(m <= 127.0 / 128.0, x - 7, x - 6).clamp(min=least).to(torch.int32)
+    e = torch.where(m <= 127.0 / 128.0, x - 7, x - 6).clamp(min=least)
+    return torch.where(amax > 0, e, torch.full_like(e, least)).to(torch.int32)
 
 
 def _bounds(codes, scales, valid):

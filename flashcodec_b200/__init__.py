@@ -16,6 +16,7 @@ from .attention import attention_status, block_basis, codec_decode_attention
 from .cache import CodecKVCache, _CodecStream, make_codec
 from .codecs import (JPEGCodec, PNGCodec, dct_basis, dct_compress, dct_decompress,
                      dequantize_coeffs, png_filter, png_reconstruct, quantize_coeffs)
+from .paged import PagedInt4Cache, rotary_table
 from .patch import (apply_flash_codec, find_attention_modules, remove_flash_codec,
                     undo_flash_codec)
 from .patch_attention import (apply_codec_attention, codec_attention_stats,
@@ -45,5 +46,6 @@ __all__ = [
     "dct_basis", "dct_compress", "dct_decompress",
     "quantize_coeffs", "dequantize_coeffs",
     "png_filter", "png_reconstruct",
+    "PagedInt4Cache", "rotary_table",
     "__version__",
 ]

@@ -25,7 +25,9 @@ SYMBOLS = ("fc_version", "fc_last_error_string", "fc_jpeg_encode", "fc_jpeg_deco
            "fc_decode_attn_noalloc_status", "fc_append_tokens", "fc_gather_batch", "fc_rope_kv_append", "fc_decode_attn_masked",
            "fc_set_attn_kernel",
            "fc_selftest_bounded_wait", "fc_selftest_noalloc_wait", "fc_decode_attn_peers",
-           "fc_peers_wait", "fc_ipc_get_handle", "fc_ipc_open_handle", "fc_ipc_close_handle")
+           "fc_peers_wait", "fc_ipc_get_handle", "fc_ipc_open_handle", "fc_ipc_close_handle",
+           "fc_kv4_page_bytes", "fc_kv4_append", "fc_kv4_read", "fc_kv4_attn_workspace_size",
+           "fc_kv4_attn", "fc_kv4_select_workspace_size", "fc_kv4_select")
 FC_MAX_PEERS, FC_IPC_HANDLE_BYTES = 8, 64
 FC_ATTN_AUTO, FC_ATTN_CUDA_CORE, FC_ATTN_TENSOR_CORE = 0, 1, 2
 
@@ -152,6 +154,22 @@ _SIGS = {
     "fc_ipc_get_handle": ([_P, _P, _P], _I32),
     "fc_ipc_open_handle": ([_P, _P], _I32),
     "fc_ipc_close_handle": ([_P], _I32),
+    "fc_kv4_page_bytes": ([_I64, _I64, _I64], _I64),
+    "fc_kv4_append": ([_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64,
+                       _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I32,
+                       _I64, _I64, _I64, _P, _P, _P,
+                       _P, _P, _I32, _F32, _P, _I64, _I32, _I32,
+                       _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P], _I32),
+    "fc_kv4_read": ([_P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P,
+                     _P, _P, _I32, _I64, _I64, _I64, _P, _P], _I32),
+    "fc_kv4_attn_workspace_size": ([_I64, _I64, _I64, _I64, _I64], ctypes.c_size_t),
+    "fc_kv4_attn": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _I64,
+                     _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _F32,
+                     _P, _I64, _I64, _I64, _P, _P, ctypes.c_size_t, _P, _P], _I32),
+    "fc_kv4_select_workspace_size": ([_I64, _I64, _I64], ctypes.c_size_t),
+    "fc_kv4_select": ([_P, _I32, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64,
+                       _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, ctypes.c_size_t, _P, _P],
+                      _I32),
 }
 
 _lock = threading.Lock()

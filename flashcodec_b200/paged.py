@@ -1,0 +1,326 @@
+"""A paged 4-bit KV cache for batches of sequences that come and go.
+
+The codec streams (``cache.py``) hold one batch that grows in step.  A serving
+engine instead keeps one pool of pages per layer and a table that says which
+pages a sequence owns; sequences join, grow by different amounts and leave.
+``PagedInt4Cache`` is that pool for one layer: K and V as 4-bit codes with one
+fp16 scale for each token and 32 channels (4.5 bits a value), and the four
+operations on it:
+
+* ``append``  -- new tokens in: RMS norm of the query and key heads, rotary
+  positions, quantisation and the page write, one launch;
+* ``attend``  -- attention of the newest token(s) of every sequence, one launch;
+* ``select``  -- the pages of a long context worth attending to, by a bound on
+  their scores; ``attend(..., selected=pages)`` reads only those;
+* ``read``    -- the values held, gathered back (the prefix of a prompt's next
+  chunk).
+
+    cache = PagedInt4Cache(num_pages, num_kv_heads, head_dim)
+    table = rotary_table(131072, head_dim, base=1e6)
+    q = cache.append(q, k, v, page_table, lengths, q_weight=wq, k_weight=wk, rotary=table)
+    lengths += 1
+    out = cache.attend(q, page_table, lengths)
+
+``page_table`` (B, n) and ``lengths`` (B,) are int32 CUDA tensors which the
+kernels read when they run: a captured CUDA graph follows their contents.  The
+caller owns page allocation; entries past a sequence's pages are never read.
+Kernels check pages, lengths and positions against the buffers: what does not
+fit is skipped or clamped and noted in ``status`` (see ``check``).  The
+reference has no paged cache; its notes on 4-bit K/V quantisation
+(docs/llama-cpp-kv-quantization.md) are the nearest it has.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _kernels as K
+from . import _lib
+
+_STATUS = ((1, "a page outside the pool"),
+           (2, "a length or position past what the page table holds"),
+           (4, "a position outside the rotary table"))
+
+
+def rotary_table(max_positions, rotary_dim, base=10000.0, *, scaling=None, factor=1.0,
+                 original_max_positions=None, low_freq_factor=1.0, high_freq_factor=4.0,
+                 beta_fast=32.0, beta_slow=1.0, attention_factor=None, device="cuda"):
+    """(max_positions, rotary_dim) fp32: the cosines, then the sines, of every
+    position's angles ``position * base ** (-2 i / rotary_dim)``, evaluated in
+    fp64 and rounded once.
+
+    scaling: how the frequencies are stretched for contexts ``factor`` times
+    ``original_max_positions``:
+        None      not at all;
+        "linear"  positions divided by ``factor``;
+        "ntk"     ``base`` times ``factor ** (R / (R - 2))``;
+        "llama3"  wavelengths over ``original / low_freq_factor`` divided by
+                  ``factor``, those under ``original / high_freq_factor`` kept,
+                  a linear ramp between;
+        "yarn"    frequencies of fewer than ``beta_slow`` turns over the original
+                  context divided by ``factor``, those of more than ``beta_fast``
+                  kept, a linear ramp over the channels between; cosines and
+                  sines times ``attention_factor`` (0.1 ln factor + 1).
+    """
+    R = int(rotary_dim)
+    if R <= 0 or R % 2 or max_positions <= 0:
+        raise ValueError(f"rotary_dim must be even and positive (got {rotary_dim}), "
+                         f"max_positions positive (got {max_positions})")
+    if factor < 1.0:
+        raise ValueError(f"factor must be at least 1 (got {factor})")
+    if scaling in ("llama3", "yarn") and not original_max_positions:
+        raise ValueError(f"scaling {scaling!r} needs original_max_positions")
+    if scaling == "ntk":
+        base = base * factor ** (R / max(R - 2, 1))
+    freq = base ** (-torch.arange(0, R, 2, dtype=torch.float64) / R)
+    gain = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "llama3":
+        turns = original_max_positions * freq / (2 * math.pi)
+        keep = ((turns - low_freq_factor) / (high_freq_factor - low_freq_factor)).clamp(0, 1)
+        freq = freq * keep + freq / factor * (1 - keep)
+    elif scaling == "yarn":
+        def channel(turns):  # where a frequency makes so many turns over the original context
+            return R * math.log(original_max_positions / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low, high = max(math.floor(channel(beta_fast)), 0), min(math.ceil(channel(beta_slow)), R - 1)
+        ramp = ((torch.arange(R // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
+        freq = freq * (1 - ramp) + freq / factor * ramp
+        gain = attention_factor if attention_factor is not None else \
+            (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"unknown rotary scaling {scaling!r}")
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq.to(device)
+    return (torch.cat([angle.cos(), angle.sin()], 1) * gain).float()
+
+
+class PagedInt4Cache:
+    """One layer's pool of 4-bit K/V pages.
+
+    Args:
+        num_pages: pages of the pool.
+        num_kv_heads, head_dim: of the model (head_dim 64, 96, 128, 192 or 256).
+        page_size: tokens of a page, a power of two from 16 to 1024.
+        bounds: keep every page's least and largest key values per channel,
+            which ``select`` needs (2 * head_dim + 4 bytes per page and KV head).
+        device: a CUDA device.
+
+    Attributes: ``pool`` (num_pages, bytes) uint8; ``bounds`` (num_pages, Hk, 2,
+    D) int8 and ``exponents`` (num_pages, Hk) int32, or None; ``status`` int32.
+    """
+
+    def __init__(self, num_pages, num_kv_heads, head_dim, page_size=64, bounds=False,
+                 device="cuda"):
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise RuntimeError("flashcodec_b200 runs on CUDA devices only (got "
+                               f"{dev}); there is no CPU implementation")
+        if num_pages <= 0 or num_pages > 0x7fffffff:
+            raise ValueError(f"num_pages must be positive (got {num_pages})")
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.device = dev
+        self.num_pages, self.num_kv_heads = int(num_pages), int(num_kv_heads)
+        self.head_dim, self.page_size = int(head_dim), int(page_size)
+        self.page_bytes = K.kv4_page_bytes(self.num_kv_heads, self.head_dim, self.page_size)
+        self.pool = torch.empty(self.num_pages, self.page_bytes, dtype=torch.uint8, device=dev)
+        self.bounds = self.exponents = None
+        if bounds:
+            self.bounds = torch.zeros(self.num_pages, self.num_kv_heads, 2, self.head_dim,
+                                      dtype=torch.int8, device=dev)
+            self.exponents = torch.zeros(self.num_pages, self.num_kv_heads, dtype=torch.int32,
+                                         device=dev)
+        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._pool_ptr, self._status_ptr = self.pool.data_ptr(), self.status.data_ptr()
+        self._bounds_ptr = self.bounds.data_ptr() if bounds else None
+        self._exponents_ptr = self.exponents.data_ptr() if bounds else None
+
+    # ------------------------------------------------------------ argument checks
+    def _check(self, *tensors):
+        grad = torch.is_grad_enabled()
+        for t in tensors:
+            if t is None:
+                continue
+            if t.device != self.device:
+                K.require_cuda(t)
+                raise ValueError(f"a tensor is on {t.device}, the cache on {self.device}")
+            if grad and t.requires_grad:
+                raise RuntimeError("the 4-bit cache holds rounded values and has no gradient: "
+                                   "call it under torch.no_grad()")
+
+    def _index(self, name, t, shape):
+        if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} "
+                             f"(got {t.dtype}, {tuple(t.shape)})")
+
+    def _table(self, page_table):
+        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[1] == 0 \
+                or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError("page_table must be an int32 (B, n) tensor with unit stride along n")
+        return page_table.shape[0]
+
+    def _rows(self, name, t, dims, heads=None):
+        s = t.shape
+        if len(s) not in dims or s[-1] != self.head_dim or (heads is not None and s[-2] != heads):
+            raise ValueError(f"{name}: expected (..., {heads or 'heads'}, {self.head_dim}), got "
+                             f"{tuple(s)}")
+        if t.stride(-1) != 1:
+            raise ValueError(f"{name}: the head dim must have unit stride")
+
+    # ----------------------------------------------------------------- operations
+    def append(self, q, k, v, page_table, lengths, *, cu_seqlens=None, q_weight=None,
+               k_weight=None, eps=1e-6, rotary=None, interleaved=False, positions=None,
+               q_out=None):
+        """Put new tokens at the ends of their sequences; returns the queries.
+
+        q, k, v: (B, S, H, D), (B, H, D) for one token each, or packed (T, H, D)
+            with ``cu_seqlens`` (B + 1,) int32; fp32, bf16 or fp16, any strides
+            with unit stride along D.  q may be None.
+        lengths: (B,) int32, tokens held before the call (unchanged by it); a
+            negative one skips the sequence.
+        q_weight, k_weight: (D,) weights of a per-head RMS norm (``eps``), or None.
+        rotary: ``rotary_table``'s (positions, R) fp32, R a multiple of 16, or
+            None; its first R channels turn, in pairs (i, i + R/2), or (2i, 2i+1)
+            with ``interleaved``.
+        positions: (B, S) or (T,) int32 rows of the table (default: the cache
+            positions, lengths + i).
+        q_out: where the queries go (default: a new tensor; may be q).
+
+        Arithmetic is fp32 and rounded in a fixed order, so what is stored does
+        not depend on how tokens are split into calls.
+        """
+        self._check(q, k, v, page_table, lengths, cu_seqlens, q_weight, k_weight, rotary,
+                    positions, q_out)
+        B = self._table(page_table)
+        packed = cu_seqlens is not None
+        dims = (3,) if packed else (3, 4)
+        self._rows("k", k, dims, self.num_kv_heads)
+        self._rows("v", v, dims, self.num_kv_heads)
+        lead = k.shape[:-2]
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError("k and v must have one shape and dtype")
+        if packed:
+            self._index("cu_seqlens", cu_seqlens, (B + 1,))
+            S, T = 0, lead[0]
+        else:
+            S = lead[1] if len(lead) == 2 else 1
+            T = B * S
+            if lead[0] != B:
+                raise ValueError(f"k has {lead[0]} sequences, the page table {B}")
+        self._index("lengths", lengths, (B,))
+        if q is not None:
+            self._rows("q", q, dims)
+            if q.shape[:-2] != lead or q.dtype != k.dtype:
+                raise ValueError("q must have the tokens and the dtype of k")
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            else:
+                self._rows("q_out", q_out, dims)
+                if q_out.shape != q.shape or q_out.dtype != q.dtype:
+                    raise ValueError("q_out must have the shape and dtype of q")
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None and (w.shape != (self.head_dim,) or w.stride(0) != 1):
+                raise ValueError(f"{name} must be a contiguous ({self.head_dim},) tensor")
+        if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+            raise ValueError("q_weight and k_weight must have one dtype")
+        if rotary is not None and (rotary.dtype != torch.float32 or rotary.dim() != 2
+                                   or not rotary.is_contiguous()):
+            raise ValueError("rotary must be a contiguous fp32 (positions, R) tensor")
+        if positions is not None:
+            self._index("positions", positions, lead if len(lead) == positions.dim() else (T,))
+        K.kv4_append(self, q, k, v, q_out, B, S, T, cu_seqlens, page_table, lengths, positions,
+                     q_weight, k_weight, eps, rotary, bool(interleaved))
+        return q_out
+
+    def attend(self, q, page_table, lengths, *, scale=None, selected=None, out=None,
+               return_lse=False):
+        """Attention of every sequence's newest tokens over what the cache holds.
+
+        q: (B, Hq, D), or (B, Sq, Hq, D) for the last Sq tokens of each sequence
+            (query i sees lengths - Sq + 1 + i tokens); Hq a multiple of the KV heads.
+        lengths: (B,) int32, tokens held, the queries' own among them.
+        scale: of the scores (default D ** -0.5).
+        selected: (B, Hk, n) int32 from ``select`` (one query per sequence): only
+            the tokens of these pages, each named once, count.
+        Returns the outputs in q's shape and dtype, and with ``return_lse`` the
+        natural log of the softmax sums, q.shape[:-1] fp32.  A query that sees no
+        token gives zeros (and -inf).
+        """
+        self._check(q, page_table, lengths, selected, out)
+        B = self._table(page_table)
+        self._rows("q", q, (3, 4))
+        if q.shape[0] != B:
+            raise ValueError(f"q has {q.shape[0]} sequences, the page table {B}")
+        self._index("lengths", lengths, (B,))
+        if selected is not None:
+            if q.dim() == 4 and q.shape[1] != 1:
+                raise ValueError("selected pages go with one query per sequence")
+            self._index("selected", selected, (B, self.num_kv_heads, selected.shape[-1]))
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            self._rows("out", out, (3, 4))
+            if out.shape != q.shape or out.dtype != q.dtype:
+                raise ValueError("out must have the shape and dtype of q")
+        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+        K.kv4_attn(self, q, page_table, lengths, selected,
+                   self.head_dim ** -0.5 if scale is None else scale, out, lse)
+        return (out, lse) if return_lse else out
+
+    def select(self, q, page_table, lengths, count, *, sink=1, recent=1):
+        """(B, Hk, count) int32: for every KV head the pages to attend to, ascending,
+        then -1.
+
+        A page's score bounds the sum over the group's query heads of q . k for
+        every key in it; the first ``sink`` and last ``recent`` pages of a sequence
+        are always taken, the rest by score (ties: the lower index).  q (B, Hq, D).
+        The cache needs ``bounds=True``.
+        """
+        if self.bounds is None:
+            raise ValueError("this cache keeps no page bounds (bounds=True)")
+        self._check(q, page_table, lengths)
+        B = self._table(page_table)
+        self._rows("q", q, (3,))
+        if q.shape[0] != B:
+            raise ValueError(f"q has {q.shape[0]} sequences, the page table {B}")
+        self._index("lengths", lengths, (B,))
+        if count <= 0:
+            raise ValueError(f"count must be positive (got {count})")
+        pages = torch.empty(B, self.num_kv_heads, count, dtype=torch.int32, device=q.device)
+        K.kv4_select(self, q, page_table, lengths, count, sink, recent, pages)
+        return pages
+
+    def read(self, page_table, starts=None, *, count=None, cu_seqlens=None, dtype=torch.bfloat16):
+        """The values held, as (k, v): ``count`` tokens of every sequence from
+        position ``starts`` ((B,) int32; None: 0) as (B, count, Hk, D), or, with
+        ``cu_seqlens``, cu_seqlens[b + 1] - cu_seqlens[b] of sequence b, ``count``
+        in all, packed as (count, Hk, D)."""
+        self._check(page_table, starts, cu_seqlens)
+        B = self._table(page_table)
+        if count is None or count < 0:
+            raise ValueError("read needs the number of tokens (count)")
+        if starts is not None:
+            self._index("starts", starts, (B,))
+        if cu_seqlens is not None:
+            self._index("cu_seqlens", cu_seqlens, (B + 1,))
+            shape, S, T = (count,), 0, count
+        else:
+            shape, S, T = (B, count), count, B * count
+        k, v = torch.empty(2, *shape, self.num_kv_heads, self.head_dim, dtype=dtype,
+                           device=self.device)
+        K.kv4_read(self, page_table, starts, B, S, T, cu_seqlens, k, v)
+        return k, v
+
+    def check(self):
+        """Raise if a kernel met a bad page, length or position since the last
+        check, and clear the word (synchronises)."""
+        word = int(self.status.item())
+        if word:
+            self.status.zero_()
+            raise _lib.FlashCodecError(_lib.FC_ERANGE, "paged cache: " + "; ".join(
+                text for bit, text in _STATUS if word & bit))
+
+
+__all__ = ["PagedInt4Cache", "rotary_table"]

@@ -537,6 +537,127 @@ FC_API int fc_ipc_get_handle(const void *ptr, void *handle, int64_t *offset);
 FC_API int fc_ipc_open_handle(const void *handle, void **base);
 FC_API int fc_ipc_close_handle(void *base);
 
+/* ---- paged 4-bit KV cache ------------------------------------------------
+ *
+ * No counterpart in the reference beyond the 4-bit K/V quantisers its notes
+ * compare with (docs/llama-cpp-kv-quantization.md): a cache for batches of
+ * sequences that come and go.  One layer's pool is `num_pages` pages of
+ * fc_kv4_page_bytes bytes; a page holds `page_size` tokens (a power of two,
+ * 16 .. 1024) of every KV head, K and V, as 4-bit codes with one fp16 scale
+ * for each token and group of 32 channels:
+ *     scale = fp16(min(amax * fl32(1/7), 65504)),
+ *     code  = clamp(rint(x / scale), -7, 7)    (0 where the scale is 0)
+ * and a group with an infinity or a NaN gets a NaN scale.  Head dims 64, 96,
+ * 128, 192 and 256.  The byte layout of a page is in csrc/fc_kv4.cuh.
+ *
+ * page_table (B, max_pages) int32, row stride table_stride: page i of sequence
+ * b holds its positions i * page_size .. ; entries past a sequence's tokens are
+ * not read.  lengths (B) int32: tokens a sequence holds.  Both are device
+ * memory and read when the kernel runs, so a captured graph follows them.  A
+ * page that two sequences share (a common prefix) may be read by both, but no
+ * append may write it.
+ *
+ * status   device int, required: bits are OR-ed in when a kernel meets a page
+ *          outside the pool (FC_KV4_BAD_PAGE), a length or position past what
+ *          the table can hold (FC_KV4_BAD_LENGTH) or a position outside the
+ *          rotary table (FC_KV4_BAD_POSITION).  No kernel accesses memory
+ *          outside the buffers then; the output rows concerned are not valid
+ *          and appends skip the tokens.
+ * All entry points are asynchronous on `stream` and can be captured. */
+#define FC_KV4_BAD_PAGE 1
+#define FC_KV4_BAD_LENGTH 2
+#define FC_KV4_BAD_POSITION 4
+
+/* Bytes of one page of one layer (all its KV heads), or -1 for a head dim or
+ * page size that is not supported. */
+FC_API int64_t fc_kv4_page_bytes(int64_t Hk, int64_t D, int64_t page_size);
+
+/* Norm and rotate the heads of new tokens, quantise keys and values into the
+ * pages, and write the queries back.
+ * Tokens come as (B, S, H, D) with strides *_sb, *_ss, *_sh (cu_seqlens NULL,
+ * T = B * S), or packed as (T, H, D) with cu_seqlens (B + 1) int32 (S and the
+ * *_sb strides are not used).  Sequence b's tokens go to positions
+ * lengths[b], lengths[b] + 1, ...; a negative length skips the sequence
+ * (its queries are still turned).  lengths is not changed.
+ * q, q_out  (.., Hq, D) or NULL with Hq = 0.  q_out may be q.
+ * q_weight, k_weight  (D) weights of w_dtype of an RMS norm of every head, each
+ *          NULL for none:  x * r * w, r = 1 / sqrt(mean(x^2) + eps).
+ * rotary   (rotary_rows, rotary_dim) fp32, cosines then sines of the angles of
+ *          a position, or NULL for none; rotary_dim is a multiple of 16 up to
+ *          D.  The first rotary_dim channels turn in pairs (i, i +
+ *          rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`.
+ * positions (T) int32 rows of the table, or NULL for the cache positions.
+ * bounds, exponents  (num_pages, Hk, 2, D) int8 and (num_pages, Hk) int32: the
+ *          least and the largest value held of every key channel of a page, as
+ *          multiples of 2^exponent, rounded outward; or NULL, NULL.
+ * Arithmetic is fp32, every product and sum rounded by itself; the stored bits
+ * do not depend on how tokens are split into calls. */
+FC_API int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t q_sh, void *q_out,
+                         int64_t qo_sb, int64_t qo_ss, int64_t qo_sh, int64_t Hq,
+                         const void *k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                         const void *v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int dtype,
+                         int64_t B, int64_t S, int64_t T, const int *cu_seqlens,
+                         const int *lengths, const int *positions,
+                         const void *q_weight, const void *k_weight, int w_dtype, float eps,
+                         const float *rotary, int64_t rotary_rows, int rotary_dim,
+                         int interleaved, void *pool, int64_t num_pages, int64_t Hk, int64_t D,
+                         int64_t page_size, const int *page_table, int64_t table_stride,
+                         int64_t max_pages, signed char *bounds, int *exponents, int *status,
+                         void *stream);
+
+/* The values held, code * scale rounded to dtype: positions starts[b] + i
+ * (starts NULL: from 0) of every sequence, i < S, into k_out and v_out
+ * (B, S, Hk, D), or packed (T, Hk, D) with cu_seqlens; both of strides o_sb,
+ * o_ss, o_sh. */
+FC_API int fc_kv4_read(const void *pool, int64_t num_pages, int64_t Hk, int64_t D,
+                       int64_t page_size, const int *page_table, int64_t table_stride,
+                       int64_t max_pages, const int *starts, int64_t B, int64_t S, int64_t T,
+                       const int *cu_seqlens, void *k_out, void *v_out, int dtype, int64_t o_sb,
+                       int64_t o_ss, int64_t o_sh, int *status, void *stream);
+
+/* Bytes of workspace that fc_kv4_attn needs for these sizes (any lengths),
+ * zero-filled before its first use and left with zeroed counters by every call.
+ * Calls sharing one must not overlap on the GPU. */
+FC_API size_t fc_kv4_attn_workspace_size(int64_t B, int64_t Sq, int64_t Hq, int64_t Hk, int64_t D);
+
+/* Attention of the last Sq tokens of every sequence over the cache:
+ *     out = softmax(softmax_scale * q . K^T) . V
+ * q (B, Sq, Hq, D), out likewise (its dtype is q's).  Query i of sequence b sees
+ * positions 0 .. lengths[b] - Sq + i (lengths counts the Sq tokens); one that
+ * sees none, and every query of a sequence with lengths[b] <= 0, gets zeros.
+ * selected (B, Hk, n_selected) int32, or NULL: only the tokens of these pages
+ * (indices into the sequence's row of the page table, each at most once;
+ * negative or past the sequence's pages: none); Sq = 1 with it.
+ * lse (B, Sq, Hq) fp32 or NULL: the natural logarithm of the softmax sums, -inf
+ * where a query sees nothing.  Scores, sums and accumulation are fp32. */
+FC_API int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int64_t Hq, int64_t q_sb,
+                       int64_t q_ss, int64_t q_sh, const void *pool, int64_t num_pages, int64_t Hk,
+                       int64_t D, int64_t page_size, const int *page_table, int64_t table_stride,
+                       int64_t max_pages, const int *lengths, const int *selected,
+                       int64_t n_selected, float softmax_scale, void *out, int64_t o_sb,
+                       int64_t o_ss, int64_t o_sh, float *lse, void *workspace,
+                       size_t workspace_bytes, int *status, void *stream);
+
+/* Bytes of workspace of fc_kv4_select, as above. */
+FC_API size_t fc_kv4_select_workspace_size(int64_t B, int64_t Hk, int64_t max_pages);
+
+/* The pages of each sequence and KV head worth attending to.  With z the group's
+ * queries (Hq / Hk heads) rounded to multiples of a power of two 2^s (s the
+ * smallest integer >= -100 with |q| <= 127 * 2^s, plus ceil(log2(Hq/Hk * D /
+ * 1024)) where that is positive), a page scores
+ *     sum over heads and channels of max(z * least, z * largest) * 2^exponent,
+ * an upper bound of the sum of the heads' scores of any of its keys.  The first
+ * `sink` and the last `recent` pages of a sequence stay; the others follow by
+ * score, equal ones by index, to `count` pages.  pages (B, Hk, count) int32 gets
+ * their indices in ascending order, then -1.  Scores are whole numbers below
+ * 2^24 times powers of two, so the choice is exact. */
+FC_API int fc_kv4_select(const void *q, int dtype, int64_t B, int64_t Hq, int64_t q_sb, int64_t q_sh,
+                         const signed char *bounds, const int *exponents, int64_t num_pages,
+                         int64_t Hk, int64_t D, int64_t page_size, const int *page_table,
+                         int64_t table_stride, int64_t max_pages, const int *lengths, int64_t count,
+                         int64_t sink, int64_t recent, int *pages, void *workspace,
+                         size_t workspace_bytes, int *status, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

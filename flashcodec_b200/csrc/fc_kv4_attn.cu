@@ -6,20 +6,22 @@
 // below at 144 bytes a token and head at D = 128), and each value takes part in
 // Hq / Hk products on each side.  What competes with HBM is the issue rate: at
 // 6.4 TB/s an SM receives 46 values a cycle to unpack.  So the pages are stored in
-// the operand order of mma.m16n8k16 (fc_kv4.cuh): a lane's words become operands by
-// an AND and an OR per two values (fp16 1024 + code), tokens (K) or channels (V) in
-// the 16 rows, the group's query rows in the 8 columns, and nothing is exchanged
-// between lanes but a transposition of the weights (movmatrix).  Matrix instructions
-// that read shared memory (tcgen05) would need the unpacked values written back to
-// shared memory, 4 bytes moved for every half byte that arrives.
+// the operand order of mma.m16n8k16 (fc_kv4.cuh): tokens (K) or channels (V) in the 16
+// rows, the group's query rows in the 8 columns, and nothing is exchanged between lanes
+// but a transposition of the weights (movmatrix).  Matrix instructions that read shared
+// memory (tcgen05) would need the unpacked values written back there, 4 bytes moved for
+// every half byte that arrives.
 //
-// Scores.  A group of 32 channels is two matrix instructions; its fp16 scales come
-// in after it, in fp32.  With bf16 queries the +1032 that unpacking leaves on a code
-// is taken off by starting the group's sum from -1032 * (sum of q): exact products,
-// fp32 sums, an error of about 2^-24 * 1032 of the largest |q| of the group.  With
-// fp16 and fp32 queries the codes are made exact first, and a query is two fp16
-// parts in neighbouring columns (22 bits).  Queries are scaled by a power of two per
-// row so that fp16 holds them.
+// Codes.  A nibble in the low bits of an fp16 is a subnormal, its multiple of 2^-24, so
+// with bf16 queries a word becomes operands by five ANDs and shifts, and the products are
+// exact.  What is left is the 8 that is on every stored code: for the scores a product of
+// the tokens' scales with -8 * (sum of q of each group), one more matrix instruction for
+// 16 tokens; for the output the groups' sums of weight * scale, one with an operand of
+// eights for each group.  The tensor cores add subnormal products with about 2^-17 of the
+// largest, enough beside 2^-9 of a bf16 query; fp16 and fp32 queries get codes made exact
+// (fp16 1024 + u, minus 1032) and two fp16 parts in neighbouring columns (22 bits).
+// Queries are scaled by a power of two per row so that fp16 holds them.  A group of 32
+// channels is two matrix instructions; its scale comes in after it, in fp32.
 //
 // Weights.  Base-2 softmax with a running reference per row, moved only when a score
 // passes it by 2^4, and a running power of two above the values' scales, so that
@@ -32,6 +34,11 @@
 // with its own ring of asynchronous copies and its own running state.  Pieces of one
 // (sequence, head) are joined by the last block to finish, in order: the result does
 // not depend on timing.  No block waits for another.
+//
+// 16 sequences of 32768 tokens, 32/8 heads, D = 128, bf16 (604 MB): 112 us, 5.4 TB/s, 84 %
+// of the copy rate; the copies alone take 103 us.  3 blocks of 168 registers an SM; 4 of
+// 128 spill (123 us), 5 warps a block too (132).  Copies as bulk copies: 127 us.
+#include "fc_attn_common.cuh"
 #include "fc_kv4.cuh"
 
 namespace fc {
@@ -56,7 +63,12 @@ struct AttnArgs {
 };
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 3;
-constexpr int kMinChunks = 8;    // of a block's piece
+// What a segment costs beyond its chunks (queries, the pipeline's start, the joins), in
+// chunks of its block's 4 warps; a block's least piece is a chunk for every warp more.
+// Times in us with 0 / 8 / 16 / 32 (one column block): 16 sequences of 32768 tokens 115 /
+// 113 / 112 / 111, 61 of 1..12000 58 / 23 / 20 / 21; with two column blocks, whose joins
+// are twice as long: 24 sequences of 1..9000 with 16 rows 194 / 52 / 41 / 36.
+constexpr int overhead(int NT) { return NT == 1 ? 16 : 32; }
 constexpr float kSlack = 4.f;    // log2 of how far a score may pass the reference
 
 __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
@@ -64,6 +76,14 @@ __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32
         "{%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ... with nothing to add to
+__device__ __forceinline__ void mma16816_first(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -83,31 +103,30 @@ __device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__h
 
 // (x & mask) | 0x64006400: fp16 pairs 1024 + nibble (or + 16 nibble)
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask) {
-    return (x & mask) | 0x64006400u;
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "r"(mask), "r"(0x64006400u));
+    return y;
 }
 
-// The four pairs of a word as 1024 + u, 1024 + 16 u, 1024 + u, 1024 + 16 u.
-__device__ __forceinline__ void unpack_raw(uint32_t w, uint32_t p[4]) {
-    const uint32_t s = w >> 8;
-    p[0] = and_or(w, 0x000f000fu);
-    p[1] = and_or(w, 0x00f000f0u);
-    p[2] = and_or(s, 0x000f000fu);
-    p[3] = and_or(s, 0x00f000f0u);
-}
-
-// ... as codes (u - 8), exact
+// The four pairs of a word.  RAW: as fp16 subnormals u 2^-24, 16 u 2^-24, u 2^-24,
+// 16 u 2^-24 (u = code + 8: a nibble in the low bits of a half is that multiple of
+// 2^-24); else as codes.
+template <bool RAW>
 __device__ __forceinline__ void unpack(uint32_t w, uint32_t p[4]) {
-    unpack_raw(w, p);
-    const __half2 one = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f),
-                  off = __float2half2_rn(-72.f);
-    p[0] = u32(__hadd2(h2(p[0]), one));
-    p[1] = u32(__hfma2(h2(p[1]), sixteenth, off));
-    p[2] = u32(__hadd2(h2(p[2]), one));
-    p[3] = u32(__hfma2(h2(p[3]), sixteenth, off));
-}
-
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    const uint32_t s = w >> 8;
+    if constexpr (RAW) {
+        p[0] = w & 0x000f000fu;
+        p[1] = w & 0x00f000f0u;
+        p[2] = s & 0x000f000fu;
+        p[3] = s & 0x00f000f0u;
+    } else {
+        const __half2 one = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f),
+                      off = __float2half2_rn(-72.f);
+        p[0] = u32(__hadd2(h2(and_or(w, 0x000f000fu)), one));
+        p[1] = u32(__hfma2(h2(and_or(w, 0x00f000f0u)), sixteenth, off));
+        p[2] = u32(__hadd2(h2(and_or(s, 0x000f000fu)), one));
+        p[3] = u32(__hfma2(h2(and_or(s, 0x00f000f0u)), sixteenth, off));
+    }
 }
 
 // N 32-bit words from shared memory by the widest loads that their alignment
@@ -132,10 +151,12 @@ __device__ __forceinline__ void load_words(const void *p, uint32_t w[N]) {
     }
 }
 
-template <int W, int NT, int LIMBS>
+template <int W, int NT, int LIMBS, bool RUNS>
 struct Attn {
     static constexpr int D = 32 * W, TILE = tile_bytes(W), STAGE = 2 * TILE;
     static constexpr int RPC = 8 * NT / LIMBS;  // query rows of a block
+    static constexpr int H = (W + 1) / 2;       // pairs of groups
+    static constexpr bool RAW = LIMBS == 1;     // how codes become operands
     static constexpr int RING = kStages * STAGE;
     static constexpr int SMEM = kWarps * RING;
 
@@ -146,13 +167,14 @@ struct Attn {
     // this segment
     int b, h, rb, len, chunk0, chunk1;
     int log_tpp, pages;
-    // queries: operand words, offsets of a group's sum, factors and lengths seen
-    uint32_t qb[NT][2 * W][2];
-    float off[LIMBS == 1 ? NT : 1][LIMBS == 1 ? W : 1][2];
+    const unsigned char *base_ptr;
+    uint32_t page_stride;  // bytes
+    // queries: operand words, those of the groups' offsets, factors and lengths seen
+    uint32_t qb[NT][2 * W][2], qo[RAW ? NT : 1][2];
     float f[NT][2];
     int seen[NT][2], min_seen;
-    // running state
-    float M[NT][2], l[NT][2], acc[NT][2 * W][4];
+    // running state: references, sums, outputs, sums of weight * scale of each group
+    float M[NT][2], l[NT][2], acc[NT][2 * W][4], ws[RAW ? NT : 1][W][2];
     float lim, slim;
 
     __device__ __forceinline__ Attn(const AttnArgs &args, unsigned char *smem, int *pos)
@@ -210,35 +232,48 @@ struct Attn {
                 sum[j] = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
+                    const bool sixteen = RAW && (i >> 1) & 1;  // codes that come as 16 u
                     float u = x[8 * j + i] * up, v = x[8 * j + i + 1] * up;
+                    if (sixteen) { u *= 0.0625f; v *= 0.0625f; }
                     __half2 p = __floats2half2_rn(u, v);
                     if constexpr (LIMBS == 2) {
                         if (r & 1) {
                             const float2 hi = __half22float2(p);
                             p = __floats2half2_rn(u - hi.x, v - hi.y);
                         }
-                    } else {
-                        const bool sixteen = (i >> 1) & 1;  // its codes come as 1024 + 16 u
-                        if (sixteen) p = __floats2half2_rn(u * 0.0625f, v * 0.0625f);
-                        const float2 z = __half22float2(p);
-                        sum[j] -= (sixteen ? 1152.f : 1032.f) * (z.x + z.y);
                     }
+                    const float2 z = __half22float2(p);
+                    sum[j] -= (sixteen ? 128.f : 8.f) * 0x1p-24f * (z.x + z.y);
                     qb[nt][2 * j + (i >> 2)][(i >> 1) & 1] = u32(p);
                 }
-                if constexpr (LIMBS == 1) {
+                if constexpr (RAW) {
                     sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
                     sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
                 }
+            }
+            // -8 sum(q) of every group, as two fp16 parts: slot c (and c + 4) of the offsets'
+            // operand holds part slot / H of the groups 2 (slot % H) and the next
+#pragma unroll
+            for (int y = 0; y < (RAW ? 2 : 0); y++) {
+                float lo[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int slot = c + 4 * y, g = 2 * (slot % H) + e;
+                    float v = 0.f;
+#pragma unroll
+                    for (int j = 0; j < W; j++)
+                        if (g == j) v = sum[j];
+                    if (slot >= H) v -= __half2float(__float2half_rn(v));
+                    if (slot >= 2 * H) v = 0.f;
+                    lo[e] = v;
+                }
+                qo[nt][y] = u32(__floats2half2_rn(lo[0], lo[1]));
             }
             // what belongs to a column, from the lanes that hold it to those that score it
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 const int from = (2 * c + y) * 4;
-                f[nt][y] = __shfl_sync(0xffffffffu, down, from) * a.scale;
-                if constexpr (LIMBS == 1) {
-#pragma unroll
-                    for (int j = 0; j < W; j++) off[nt][j][y] = __shfl_sync(0xffffffffu, sum[j], from);
-                }
+                f[nt][y] = __shfl_sync(0xffffffffu, down, from) * a.scale * (RAW ? 0x1p24f : 1.f);
                 const int sq = min(row_of(nt, 2 * c + y), a.rows - 1) / a.G;
                 seen[nt][y] = len - (a.Sq - 1 - sq);
             }
@@ -253,44 +288,66 @@ struct Attn {
             for (int m = 0; m < 2 * W; m++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) acc[nt][m][i] = 0.f;
+            if constexpr (RAW) {
+#pragma unroll
+                for (int j = 0; j < W; j++) ws[nt][j][0] = ws[nt][j][1] = 0.f;
+            }
         }
         lim = 15.f;
         slim = 1.f;
     }
 
     // ------------------------------------------------------------------ copies
-    // Lanes 0 and 1 look the tiles of a chunk up (the others follow lane 1): the
-    // page of the sequence, and where it lies.
-    __device__ __forceinline__ int logical(int chunk) const {
-        const int tile = 2 * chunk + (lane & 1);
+    // The page of the sequence that holds tile `tile` (of its tokens, or of the
+    // selected pages), or -1; where that lies in the pool.
+    __device__ __forceinline__ int logical(int tile) const {
         int page = tile >> log_tpp;
         if (a.selected) {
             if (page >= a.n_selected) return -1;
             page = a.selected[((int64_t)b * a.Hk + h) * a.n_selected + page];
         }
-        return page < pages ? page : -1;
+        return (unsigned)page < (unsigned)pages ? page : -1;
     }
     __device__ __forceinline__ int physical(int page) const {
         return page < 0 ? -1 : a.table.page(b, page);
     }
-    __device__ __forceinline__ void issue(int chunk, int page, int id, int stage) {
-        const int tile = (2 * chunk + (lane & 1)) & ((1 << log_tpp) - 1);
-        int pos = page < 0 ? 0x7fffffff - 64 : (page << a.table.log_page) + tile * 16;
-        if (pos >= len) id = -1;  // nothing there
-        if (id < 0) pos = 0x7fffffff - 64;
-        const int64_t at = ((((int64_t)max(id, 0) * a.Hk + h) << log_tpp) + tile) * TILE;
-        if (lane < 2) pos_s[stage * 2 + lane] = pos;
-        const int id0 = __shfl_sync(0xffffffffu, id, 0), id1 = __shfl_sync(0xffffffffu, id, 1);
-        const unsigned char *s0 = a.pool + __shfl_sync(0xffffffffu, at, 0);
-        const unsigned char *s1 = a.pool + __shfl_sync(0xffffffffu, at, 1) - TILE;
-        const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(ring + stage * STAGE));
+    static constexpr int kNowhere = 0x7fffffff - 64;  // a position past every length
+
+    // The common case: all tokens of the sequence, pages of 32 tokens and more, so that a
+    // chunk is one run of bytes.  `tile`: of the page; n: tokens of the chunk that are held.
+    __device__ __forceinline__ void issue_run(int tile, int id, int n, int stage) const {
         constexpr int N = TILE / 16;  // 36 W pieces of a tile
+        unsigned char *dst = ring + stage * STAGE + lane * 16;
+        const unsigned char *s =
+            base_ptr + lane * 16 + (uint64_t)(uint32_t)id * page_stride + (uint32_t)(tile * TILE);
+        if (n > 16) {
 #pragma unroll
-        for (int i = 0; i < (2 * N + 31) / 32; i++) {
-            const int p = 32 * i + lane;
-            const bool second = 32 * i >= N || (32 * i + 31 >= N && p >= N);
-            if ((32 * i + 31 < 2 * N || p < 2 * N) && (second ? id1 : id0) >= 0)
-                copy16(dst + p * 16, (second ? s1 : s0) + p * 16);
+            for (int i = 0; i < (2 * N + 31) / 32; i++)
+                if (32 * i + 31 < 2 * N || lane < 2 * N - 32 * i) cp_async16(dst + 512 * i, s + 512 * i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < (N + 31) / 32; i++)
+                if (32 * i + 31 < N || lane < N - 32 * i) cp_async16(dst + 512 * i, s + 512 * i);
+        }
+    }
+
+    // Any other: lanes 0 and 1 have looked the two tiles up (`page` of the sequence, `id`).
+    __device__ __forceinline__ void issue_tiles(int chunk, int page, int id, int stage) const {
+        constexpr int N = TILE / 16;
+        const int tile = (2 * chunk + (lane & 1)) & ((1 << log_tpp) - 1);
+        const int p = (page << a.table.log_page) + tile * 16;
+        if (page < 0 || p >= len) id = -1;
+        if (lane < 2) pos_s[stage * 2 + lane] = id < 0 ? kNowhere : p;
+        const unsigned char *s = base_ptr + (uint64_t)(uint32_t)id * page_stride + (uint32_t)(tile * TILE);
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            const unsigned char *z = reinterpret_cast<const unsigned char *>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(s), y));
+            if (__shfl_sync(0xffffffffu, id, y) < 0) continue;
+#pragma unroll
+            for (int i = 0; i < (N + 31) / 32; i++)
+                if (32 * i + 31 < N || lane < N - 32 * i)
+                    cp_async16(ring + stage * STAGE + y * TILE + lane * 16 + 512 * i, z + lane * 16 + 512 * i);
         }
     }
 
@@ -307,36 +364,38 @@ struct Attn {
             s[2 * i] = z.x;
             s[2 * i + 1] = z.y;
         }
+        if constexpr (RAW) {
+            // the offsets of all groups: a product of the tokens' scales with -8 sum(q)
+            uint32_t o[4];
+            if constexpr (W % 2 == 0) {
+                const uint32_t *p = reinterpret_cast<const uint32_t *>(tile + ks_off(W)) + r * W;
+                o[0] = p[c % H];
+                o[1] = p[H + c % H];
+                o[2] = H > 2 ? p[(c + 4) % H] : o[0];
+                o[3] = H > 2 ? p[H + (c + 4) % H] : o[1];
+            } else {
+                const uint16_t *p = reinterpret_cast<const uint16_t *>(tile + ks_off(W)) + r * 2 * W;
+                const int g = 2 * (c % H), g1 = min(g + 1, W - 1);
+                o[0] = o[2] = p[g] | (uint32_t)p[g1] << 16;
+                o[1] = o[3] = p[W + g] | (uint32_t)p[W + g1] << 16;
+            }
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) S[nt][i] = 0.f;
+            for (int nt = 0; nt < NT; nt++) mma16816_first(S[nt], o, qo[nt][0], qo[nt][1]);
+        }
 #pragma unroll
         for (int j = 0; j < W; j++) {
             uint32_t x[4], y[4];
-            if constexpr (LIMBS == 1) {
-                unpack_raw(k0[j], x);
-                unpack_raw(k1[j], y);
-            } else {
-                unpack(k0[j], x);
-                unpack(k1[j], y);
-            }
+            unpack<RAW>(k0[j], x);
+            unpack<RAW>(k1[j], y);
             const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 float t[4];
-                if constexpr (LIMBS == 1) {
-                    t[0] = t[2] = off[nt][j][0];
-                    t[1] = t[3] = off[nt][j][1];
-                } else {
-                    t[0] = t[1] = t[2] = t[3] = 0.f;
-                }
-                mma16816(t, a0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
+                mma16816_first(t, a0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
                 mma16816(t, a1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
-                S[nt][0] = fmaf(s[j], t[0], S[nt][0]);
-                S[nt][1] = fmaf(s[j], t[1], S[nt][1]);
-                S[nt][2] = fmaf(s[W + j], t[2], S[nt][2]);
-                S[nt][3] = fmaf(s[W + j], t[3], S[nt][3]);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    S[nt][i] = RAW || j ? fmaf(s[(i >> 1) * W + j], t[i], S[nt][i]) : s[(i >> 1) * W + j] * t[i];
             }
         }
         if constexpr (LIMBS == 2) {  // the two parts of a query are neighbouring columns
@@ -366,9 +425,13 @@ struct Attn {
         }
     }
 
-    // acc += V . weights of one tile; p: the weights, in place of the scores
+    // out += V . weights of one tile; p: the weights.  RAW: in units of 2^-24 (channels
+    // r + 8: 2^-20) and without the 8 off every code; ws gets 8 times the groups' sums of
+    // weight * scale, in 2^-24 too.  MASKED: some weights are of tokens not seen, whose
+    // scales may be NaN.
+    template <bool MASKED>
     __device__ __forceinline__ void gather(const unsigned char *tile, const float p[NT][4],
-                                           float out[NT][2 * W][4]) const {
+                                           float out[NT][2 * W][4]) {
         uint32_t v[2 * W];
         constexpr int VW = v_vec(W);
 #pragma unroll
@@ -385,6 +448,10 @@ struct Attn {
                 for (int j = 0; j < W; j++) {
                     w[nt][j][0] = u32(__hmul2(h2(lo), h2(sc[2 * j])));
                     w[nt][j][1] = u32(__hmul2(h2(hi), h2(sc[2 * j + 1])));
+                    if constexpr (MASKED) {
+                        w[nt][j][0] &= __hne2_mask(h2(lo), h2(0u));
+                        w[nt][j][1] &= __hne2_mask(h2(hi), h2(0u));
+                    }
                 }
             }
         } else {
@@ -394,30 +461,70 @@ struct Attn {
                 const float s0 = __half2float(vs[4 * j]), s1 = __half2float(vs[4 * j + 2]);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    const float u = p[nt][0] * s0, v2 = p[nt][2] * s1;
-                    const __half uh = __float2half_rn(u), vh = __float2half_rn(v2);
+                    const float u = MASKED && p[nt][0] == 0.f ? 0.f : p[nt][0] * s0;
+                    const float z = MASKED && p[nt][2] == 0.f ? 0.f : p[nt][2] * s1;
+                    const __half uh = __float2half_rn(u), zh = __float2half_rn(z);
                     w[nt][j][0] = transpose8(u32(__halves2half2(uh, __float2half_rn(u - __half2float(uh)))));
-                    w[nt][j][1] = transpose8(u32(__halves2half2(vh, __float2half_rn(v2 - __half2float(vh)))));
+                    w[nt][j][1] = transpose8(u32(__halves2half2(zh, __float2half_rn(z - __half2float(zh)))));
                 }
             }
+        }
+        if constexpr (RAW) {
+            const uint32_t eight[4] = {0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u};
+#pragma unroll
+            for (int j = 0; j < W; j++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float sum[4];  // of every row
+                    mma16816_first(sum, eight, w[nt][j][0], w[nt][j][1]);
+                    const float2 s = __fadd2_rn(make_float2(ws[nt][j][0], ws[nt][j][1]), make_float2(sum[0], sum[1]));
+                    ws[nt][j][0] = s.x;
+                    ws[nt][j][1] = s.y;
+                }
         }
 #pragma unroll
         for (int m = 0; m < 2 * W; m++) {
             uint32_t x[4];
-            unpack(v[m], x);
+            unpack<RAW>(v[m], x);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) mma16816(out[nt][m], x, w[nt][m / 2][0], w[nt][m / 2][1]);
         }
     }
 
-    __device__ __forceinline__ void chunk(int stage) {
+    // Both tiles of a chunk.
+    template <bool MASKED>
+    __device__ __forceinline__ void gather_chunk(const unsigned char *tile, const float S[2][NT][4]) {
+        if constexpr (RAW) {
+            gather<MASKED>(tile, S[0], acc);
+            gather<MASKED>(tile + TILE, S[1], acc);
+        } else {
+            // a chunk's sum by itself: the long sum is then in rounded fp32 additions
+            float part[NT][2 * W][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int m = 0; m < 2 * W; m++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) part[nt][m][i] = 0.f;
+            gather<MASKED>(tile, S[0], part);
+            gather<MASKED>(tile + TILE, S[1], part);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int m = 0; m < 2 * W; m++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[nt][m][i] += part[nt][m][i];
+        }
+    }
+
+    // The staged chunk, whose tiles hold the positions from p0 and from p1.
+    __device__ __forceinline__ void chunk(int stage, int p0, int p1) {
         unsigned char *tile = ring + stage * STAGE;
-        const int p0 = pos_s[stage * 2], p1 = pos_s[stage * 2 + 1];
-        if (p0 >= len && p1 >= len) return;
         float S[2][NT][4];
         score(tile, S[0]);
         score(tile + TILE, S[1]);
-        if (max(p0, p1) + 16 > min_seen) {
+        const bool masked = max(p0, p1) + 16 > min_seen;
+        if (masked) {
             mask(tile, p0, S[0]);
             mask(tile + TILE, p1, S[1]);
             __syncwarp();
@@ -472,6 +579,10 @@ struct Attn {
                     const float g = exp2_fast(M[nt][y] - m);
                     M[nt][y] = m;
                     l[nt][y] *= g;
+                    if constexpr (RAW) {
+#pragma unroll
+                        for (int j = 0; j < W; j++) ws[nt][j][y] *= g;
+                    }
 #pragma unroll
                     for (int i = 0; i < 2 * W; i++) {
                         acc[nt][i][y] *= g;
@@ -484,60 +595,99 @@ struct Attn {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float p = exp2_fast(fmaf(S[t][nt][i], f[nt][i & 1], -M[nt][i & 1]));
-                    S[t][nt][i] = p;
-                    l[nt][i & 1] += p;
+                for (int i = 0; i < 4; i += 2) {
+                    const float2 x = __ffma2_rn(make_float2(S[t][nt][i], S[t][nt][i + 1]),
+                                                make_float2(f[nt][0], f[nt][1]),
+                                                make_float2(-M[nt][0], -M[nt][1]));
+                    S[t][nt][i] = exp2_fast(x.x);
+                    S[t][nt][i + 1] = exp2_fast(x.y);
+                    const float2 s = __fadd2_rn(make_float2(l[nt][0], l[nt][1]),
+                                                make_float2(S[t][nt][i], S[t][nt][i + 1]));
+                    l[nt][0] = s.x;
+                    l[nt][1] = s.y;
                 }
-        if constexpr (LIMBS == 1) {
-            gather(tile, S[0], acc);
-            gather(tile + TILE, S[1], acc);
-        } else {
-            // a chunk's sum by itself: the long sum is then in rounded fp32 additions
-            float part[NT][2 * W][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int m = 0; m < 2 * W; m++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) part[nt][m][i] = 0.f;
-            gather(tile, S[0], part);
-            gather(tile + TILE, S[1], part);
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int m = 0; m < 2 * W; m++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[nt][m][i] += part[nt][m][i];
-        }
+        if (masked)
+            gather_chunk<true>(tile, S);
+        else
+            gather_chunk<false>(tile, S);
     }
 
-    // This warp's chunks of the segment: chunk0 + warp, + 4, ...
+    // This warp's chunks of the segment: chunk0 + warp, + 4, ..., each copied two rounds
+    // before it is used.
     __device__ __forceinline__ void run() {
-        int next = chunk0 + warp;  // the next chunk to copy
-        int page = next < chunk1 ? logical(next) : -1;
-        int id = physical(page);
-        int page2 = next + kWarps < chunk1 ? logical(next + kWarps) : -1;
-        auto fetch = [&](int stage) {
-            if (next < chunk1) issue(next, page, id, stage);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            next += kWarps;
-            page = page2;
-            id = physical(page);
-            page2 = next + kWarps < chunk1 ? logical(next + kWarps) : -1;
-        };
+        pages = (len + (1 << a.table.log_page) - 1) >> a.table.log_page;
+        base_ptr = a.pool + ((int64_t)h << log_tpp) * TILE;
+        page_stride = (uint32_t)((a.Hk << log_tpp) * TILE);
+        if constexpr (RUNS)
+            run_pages();
+        else
+            run_tiles();
+    }
+
+    // fetch(stage) copies the next chunk, use(i, stage) works on chunk i.
+    template <typename Fetch, typename Use>
+    __device__ __forceinline__ void rounds(Fetch fetch, Use use) {
 #pragma unroll
-        for (int i = 0; i < kStages - 1; i++) fetch(i);
+        for (int i = 0; i < kStages - 1; i++) {
+            if (chunk0 + warp + i * kWarps < chunk1) fetch(i);
+            cp_async_commit();
+        }
+        load_queries();  // while the first chunks are on their way
         int stage = 0;
         for (int i = chunk0 + warp; i < chunk1; i += kWarps) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            cp_async_wait<kStages - 2>();
             __syncwarp();
-            fetch(stage == 0 ? kStages - 1 : stage - 1);
-            chunk(stage);
+            if (i + (kStages - 1) * kWarps < chunk1) fetch(stage == 0 ? kStages - 1 : stage - 1);
+            cp_async_commit();
+            use(i, stage);
             __syncwarp();
             stage = stage == kStages - 1 ? 0 : stage + 1;
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        cp_async_wait<0>();
+    }
+
+    __device__ __forceinline__ void run_pages() {
+        // lane i holds the page of the chunk i rounds into a window of 32 rounds; the
+        // window after it is on its way
+        const int shift = log_tpp - 1;
+        int next = chunk0 + warp, round = 0;
+        auto window = [&](int first) {
+            const int chunk = first + kWarps * lane;
+            return chunk < chunk1 ? a.table.page(b, chunk >> shift) : 0;
+        };
+        int ids = window(next), ids2 = window(next + 32 * kWarps);
+        rounds(
+            [&](int stage) {
+                const int id = __shfl_sync(0xffffffffu, ids, round);
+                issue_run(2 * (next & ((1 << shift) - 1)), id, len - 32 * next, stage);
+                next += kWarps;
+                if (++round == 32) {
+                    round = 0;
+                    ids = ids2;
+                    ids2 = window(next + 32 * kWarps);
+                }
+            },
+            [&](int i, int stage) { chunk(stage, 32 * i, 32 * i + 16); });
+    }
+
+    __device__ __forceinline__ void run_tiles() {
+        const int odd = lane & 1;
+        int next = chunk0 + warp;  // the next chunk to copy
+        int page = next < chunk1 ? logical(2 * next + odd) : -1;
+        int id = physical(page);
+        int page2 = next + kWarps < chunk1 ? logical(2 * (next + kWarps) + odd) : -1;
+        rounds(
+            [&](int stage) {
+                issue_tiles(next, page, id, stage);
+                next += kWarps;
+                page = page2;
+                id = physical(page);
+                page2 = next + kWarps < chunk1 ? logical(2 * (next + kWarps) + odd) : -1;
+            },
+            [&](int, int stage) {
+                const int p0 = pos_s[stage * 2], p1 = pos_s[stage * 2 + 1];
+                if (p0 < len || p1 < len) chunk(stage, p0, p1);
+            });
     }
 
     // -------------------------------------------------------------------- joins
@@ -583,11 +733,17 @@ struct Attn {
                 float m = ml[row * 2];
 #pragma unroll
                 for (int w = 1; w < kWarps; w++) m = fmaxf(m, ml[(w * RPC + row) * 2]);
-                const float g = exp2_fast(M[nt][y] - m);
+                const float g = exp2_fast(M[nt][y] - m) * (RAW ? 0x1p24f : 1.f);
 #pragma unroll
                 for (int i = 0; i < 2 * W; i++) {
                     float u = acc[nt][i][y], v = acc[nt][i][y + 2];
-                    if constexpr (LIMBS == 2) { u += acc[nt][i][1]; v += acc[nt][i][3]; }
+                    if constexpr (RAW) {
+                        u -= ws[nt][i / 2][y];
+                        v = fmaf(v, 0.0625f, -ws[nt][i / 2][y]);
+                    } else {
+                        u += acc[nt][i][1];
+                        v += acc[nt][i][3];
+                    }
                     o[(warp * RPC + row) * D + 16 * i + r] = u * g;
                     o[(warp * RPC + row) * D + 16 * i + r + 8] = v * g;
                 }
@@ -616,6 +772,39 @@ struct Attn {
             }
         }
     }
+
+    // Joins `count` parts of this unit: block `first`'s second one, then the first
+    // ones of the blocks after it.
+    __device__ __forceinline__ void merge(int first, int count) const {
+        const float *p0 = a.parts + ((int64_t)first * 2 + 1) * PART;
+        const float *p1 = a.parts + (int64_t)first * 2 * PART;  // block first + k: + 2 k PART
+        const int rows = min(RPC, a.rows - rb * RPC);
+        for (int i = threadIdx.x * 4; i < rows * D; i += kThreads * 4) {
+            const int row = i / D, at = RPC * D + 2 * row;
+            float m = __ldcg(p0 + at);
+#pragma unroll 4
+            for (int k = 1; k < count; k++) m = fmaxf(m, __ldcg(p1 + (int64_t)2 * k * PART + at));
+            float s = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int k = 0; k < count; k++) {
+                const float *p = k ? p1 + (int64_t)2 * k * PART : p0;
+                const float2 z = __ldcg(reinterpret_cast<const float2 *>(p + at));
+                const float4 o = __ldcg(reinterpret_cast<const float4 *>(p + i));
+                const float g = exp2_fast(z.x - m);
+                s = fmaf(g, z.y, s);
+                v.x = fmaf(g, o.x, v.x);
+                v.y = fmaf(g, o.y, v.y);
+                v.z = fmaf(g, o.z, v.z);
+                v.w = fmaf(g, o.w, v.w);
+            }
+            const float inv = s == 0.f ? 0.f : 1.f / s;
+            const float x[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+#pragma unroll
+            for (int j = 0; j < 4; j++) write_row(rb * RPC + row, i % D + j, x[j]);
+            if (a.lse && i % D == 0) write_lse(rb * RPC + row, m, s);
+        }
+    }
 };
 
 // Chunks of sequence b, 0 where it holds nothing.
@@ -626,28 +815,34 @@ __device__ __forceinline__ int chunks_of(const AttnArgs &a, int64_t b) {
     return (len + 31) / 32;
 }
 
-template <int W, int NT, int LIMBS>
-__global__ void __launch_bounds__(kThreads) attn_kernel(const __grid_constant__ AttnArgs a) {
-    using A = Attn<W, NT, LIMBS>;
+// The line: unit (sequence, KV head, row block) u of n > 0 chunks is n + OVERHEAD
+// long, the first OVERHEAD standing for what a segment costs beyond its chunks.
+// Block i of `blocks` has the piece [U i / blocks, U (i + 1) / blocks).
+template <int W, int NT, int LIMBS, bool RUNS>
+__global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kernel(const __grid_constant__ AttnArgs a) {
+    using A = Attn<W, NT, LIMBS, RUNS>;
+    constexpr int OVERHEAD = overhead(NT), MIN_PIECE = OVERHEAD + kWarps;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int64_t sums[kThreads], pre_s;
-    __shared__ int b_s, last_s;
+    __shared__ int64_t sums[kWarps], pre_s;
+    __shared__ int b_s, first_s, last_s;
     __shared__ int pos[kWarps * kStages * 2];
     __shared__ float ml[kWarps * A::RPC * 2];
 
-    // the line of chunks: before each thread's sequences, and in all
     const int HR = a.Hk * a.row_blocks;
     const int per = (a.B + kThreads - 1) / kThreads;
     const int b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
     int64_t mine = 0;
-    for (int b = b0; b < b1; b++) mine += chunks_of(a, b);
-    sums[threadIdx.x] = mine;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-    for (int i = 0; i < kThreads; i++) {
-        if (i < (int)threadIdx.x) before += sums[i];
-        all += sums[i];
+    for (int b = b0; b < b1; b++) {
+        const int n = chunks_of(a, b);
+        mine += n ? n + OVERHEAD : 0;
     }
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if ((threadIdx.x & 31) >= o) upto += v;
+    }
+    if ((threadIdx.x & 31) == 31) sums[threadIdx.x >> 5] = upto;
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {  // nothing held: zeros
         if (chunks_of(a, b)) continue;
         for (int i = threadIdx.x; i < a.Sq * a.Hq * A::D; i += kThreads) {
@@ -656,101 +851,92 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const __grid_constant__ 
             if (a.lse && i % A::D == 0) a.lse[(int64_t)b * a.Sq * a.Hq + row] = -INFINITY;
         }
     }
+    __syncthreads();
+    int64_t before = upto - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+        if (w < (int)(threadIdx.x >> 5)) before += sums[w];
+        all += sums[w];
+    }
     const int64_t U = all * HR;
-    const int64_t blocks = min((int64_t)gridDim.x, (U + kMinChunks - 1) / kMinChunks);
+    const int64_t blocks = min((int64_t)gridDim.x, (U + MIN_PIECE - 1) / MIN_PIECE);
     if ((int64_t)blockIdx.x >= blocks) return;
     int64_t x = U * blockIdx.x / blocks;
     const int64_t end = U * (blockIdx.x + 1) / blocks;
-    const int64_t start = x;
     // the sequence that x falls in
-    {
+    if (x >= before * HR && x < (before + mine) * HR) {
         int64_t at = before * HR;
-        if (x >= at && x < at + mine * HR) {
-            int b = b0;
-            for (;; b++) {
-                const int64_t n = (int64_t)chunks_of(a, b) * HR;
-                if (x < at + n) break;
-                at += n;
-            }
-            b_s = b;
-            pre_s = at;
+        int b = b0;
+        for (;; b++) {
+            const int n = chunks_of(a, b);
+            const int64_t w = n ? (int64_t)(n + OVERHEAD) * HR : 0;
+            if (x < at + w) break;
+            at += w;
         }
+        b_s = b;
+        pre_s = at;
     }
     __syncthreads();
     int b = b_s;
     int64_t base = pre_s;  // where the line of sequence b begins
+    int n = chunks_of(a, b);
+    int64_t unit = (x - base) / (n + OVERHEAD);
 
     A t(a, smem, pos);
     while (x < end) {
-        int n = chunks_of(a, b);
-        while (x >= base + (int64_t)n * HR) {
-            base += (int64_t)n * HR;
-            n = chunks_of(a, ++b);
-        }
-        const int unit = (int)((x - base) / n);
-        const int64_t u0 = base + (int64_t)unit * n;
-        t.b = b;
-        t.h = unit / a.row_blocks;
-        t.rb = unit % a.row_blocks;
-        t.len = a.table.length(a.lengths[b]);
-        t.pages = (t.len + (1 << a.table.log_page) - 1) >> a.table.log_page;
-        t.chunk0 = (int)(x - u0);
-        t.chunk1 = (int)min((int64_t)n, end - u0);
-        const bool whole = t.chunk0 == 0 && t.chunk1 == n;
-        t.load_queries();
-        t.run();
-        float *part = a.parts + ((int64_t)blockIdx.x * 2 + (x == start ? 0 : 1)) * A::PART;
-        t.join(smem, ml, whole, part);
-        if (!whole) {
-            // blocks that share this unit: from the one its first chunk falls to
-            const int64_t i0 = ((u0 + 1) * blocks - 1) / U, i1 = ((u0 + n) * blocks - 1) / U;
-            int *counter = a.counters + ((int64_t)b * HR + unit);
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) last_s = atomicAdd(counter, 1) == (int)(i1 - i0);
-            __syncthreads();
-            if (last_s) {
-                __threadfence();
-                const int rows = min(A::RPC, a.rows - t.rb * A::RPC);
-                for (int i = threadIdx.x; i < rows * A::D; i += kThreads) {
-                    const int row = i / A::D;
-                    auto of = [&](int64_t k) {
-                        const bool first = U * k / blocks >= u0;
-                        return a.parts + (k * 2 + (first ? 0 : 1)) * A::PART;
-                    };
-                    float m = -INFINITY, s = 0.f, v = 0.f;
-                    for (int64_t k = i0; k <= i1; k++) m = fmaxf(m, __ldcg(of(k) + A::RPC * A::D + 2 * row));
-                    for (int64_t k = i0; k <= i1; k++) {
-                        const float *p = of(k);
-                        const float g = exp2_fast(__ldcg(p + A::RPC * A::D + 2 * row) - m);
-                        s += g * __ldcg(p + A::RPC * A::D + 2 * row + 1);
-                        v += g * __ldcg(p + i);
-                    }
-                    t.write_row(t.rb * A::RPC + row, i % A::D, s == 0.f ? 0.f : v / s);
-                    if (a.lse && i % A::D == 0) t.write_lse(t.rb * A::RPC + row, m, s);
+        const int64_t u0 = base + unit * (n + OVERHEAD) + OVERHEAD, u1 = u0 + n;  // its chunks
+        t.chunk0 = (int)(max(x, u0) - u0);
+        t.chunk1 = (int)(min(end, u1) - u0);
+        if (t.chunk0 < t.chunk1) {
+            t.b = b;
+            t.h = (int)unit / a.row_blocks;
+            t.rb = (int)unit - t.h * a.row_blocks;
+            t.len = a.table.length(a.lengths[b]);
+            const bool whole = t.chunk0 == 0 && t.chunk1 == n;
+            t.run();
+            // parts of a block: 0 of a unit that began in an earlier one, 1 of one that ends in a later one
+            t.join(smem, ml, whole, a.parts + ((int64_t)blockIdx.x * 2 + (t.chunk0 == 0)) * A::PART);
+            if (!whole) {
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    // the blocks with chunks of this unit: i0 (its first chunk) to i1
+                    const int64_t i0 = ((u0 + 1) * blocks - 1) / U, i1 = (u1 * blocks - 1) / U;
+                    __threadfence();
+                    int *counter = a.counters + ((int64_t)b * HR + unit);
+                    const bool last = atomicAdd(counter, 1) == (int)(i1 - i0);
+                    if (last) *counter = 0;
+                    __threadfence();
+                    last_s = last ? (int)(i1 - i0) + 1 : 0;
+                    first_s = (int)i0;
                 }
-                if (threadIdx.x == 0) *counter = 0;
+                __syncthreads();
+                if (last_s) t.merge(first_s, last_s);
             }
+            __syncthreads();
         }
-        __syncthreads();
-        x = u0 + t.chunk1;
+        x = max(x, u1);
+        if (++unit == HR) {
+            unit = 0;
+            base = u1;
+            if (x < end) do { n = chunks_of(a, ++b); } while (n == 0);
+        }
     }
 }
 
 constexpr int kMaxBlocksPerSm = 8;
 
 // Blocks of a wave: what of the kernel fits on the device.
-template <int W, int NT, int LIMBS>
+template <int W, int NT, int LIMBS, bool RUNS>
 int wave() {
     static int cache[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
     if (cache[dev] == 0) {
-        constexpr int smem = Attn<W, NT, LIMBS>::SMEM;
+        constexpr int smem = Attn<W, NT, LIMBS, RUNS>::SMEM;
         int n = 0;
-        if (cudaFuncSetAttribute(attn_kernel<W, NT, LIMBS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+        if (cudaFuncSetAttribute(attn_kernel<W, NT, LIMBS, RUNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
                 cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_kernel<W, NT, LIMBS>, kThreads, smem) !=
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_kernel<W, NT, LIMBS, RUNS>, kThreads, smem) !=
                 cudaSuccess || n < 1)
             return 0;
         cache[dev] = num_sms() * (n < kMaxBlocksPerSm ? n : kMaxBlocksPerSm);
@@ -797,6 +983,10 @@ extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int6
     }
     if (B == 0 || Sq == 0) return FC_OK;
     if (!q || !out || !lengths) { set_error("kv4_attn: null pointer"); return FC_EINVAL; }
+    if (Hk * page_size * (tile_bytes((int)(D / 32)) / 16) > 0x7fffffff) {
+        set_error("kv4_attn: pages over 2 GiB");
+        return FC_ENOTSUP;
+    }
     if (selected && (Sq != 1 || n_selected < 0 || n_selected * page_size > 0x7fffffff)) {
         set_error("kv4_attn: selected pages go with one query per sequence");
         return FC_EINVAL;
@@ -832,16 +1022,20 @@ extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int6
     a.parts = reinterpret_cast<float *>(ws + counter_bytes(B * Hk * ((rows + 3) / 4)));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return by_head_dim(D, [&](auto w) {
-        auto launch = [&](auto n, auto lm) {
+        auto launch = [&](auto n, auto lm, auto runs) {
             constexpr int W = decltype(w)::value, NT = decltype(n)::value, L = decltype(lm)::value;
-            const int blocks = wave<W, NT, L>();
+            constexpr bool R = decltype(runs)::value;
+            const int blocks = wave<W, NT, L, R>();
             if (!blocks) { set_error("kv4_attn: the kernel does not fit this device"); return FC_ECUDA; }
-            attn_kernel<W, NT, L><<<blocks, kThreads, Attn<W, NT, L>::SMEM, st>>>(a);
+            attn_kernel<W, NT, L, R><<<blocks, kThreads, Attn<W, NT, L, R>::SMEM, st>>>(a);
             return check_launch("kv4_attn");
         };
         using I1 = std::integral_constant<int, 1>;
         using I2 = std::integral_constant<int, 2>;
-        if (limbs == 1) return nt == 1 ? launch(I1(), I1()) : launch(I2(), I1());
-        return nt == 1 ? launch(I1(), I2()) : launch(I2(), I2());
+        auto of_kind = [&](auto runs) {
+            if (limbs == 1) return nt == 1 ? launch(I1(), I1(), runs) : launch(I2(), I1(), runs);
+            return nt == 1 ? launch(I1(), I2(), runs) : launch(I2(), I2(), runs);
+        };
+        return page_size >= 32 && !selected ? of_kind(std::true_type()) : of_kind(std::false_type());
     });
 }

@@ -24,44 +24,93 @@ namespace fc {
 namespace kv4 {
 namespace {
 
+// 8 neighbouring channels of a head in one lane, as pairs for the paired fp32
+// instructions: even channels (0, 2), (4, 6) and odd ones (1, 3), (5, 7).
+struct Row {
+    float2 e[2], o[2];
+};
+
+__device__ __forceinline__ float2 pair(float x, float y) { return make_float2(x, y); }
+
+// A row as it is in memory: 8 elements of T.
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, bool vec, float x[8]) {
+struct Raw {
+    uint32_t w[2 * sizeof(T)];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T *p, bool vec) {
+    Raw<T> r;
     if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            load_vec_f32<T, 4>(p, x);
-            load_vec_f32<T, 4>(p + 4, x + 4);
-        } else {
-            load_vec_f32<T, 8>(p, x);
-        }
-    } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = Elem<T>::to_f32(p[i]);
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+            r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
+        }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+    } else {
+        const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.w[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
     }
+    return r;
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T *p, bool vec, const float x[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            store_vec_from_f32<T, 4>(p, x);
-            store_vec_from_f32<T, 4>(p + 4, x + 4);
-        } else {
-            uint32_t w[4];
+__device__ __forceinline__ Raw<T> zero_raw() {
+    Raw<T> r;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if constexpr (std::is_same<T, __half>::value) {
-                    const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t *>(&h);
-                } else {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t *>(&h);
-                }
-            }
-            *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < 2 * (int)sizeof(T); i++) r.w[i] = 0u;
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ Row widen(const Raw<T> &r) {
+    float x[8];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __uint_as_float(r.w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[2 * i] = __uint_as_float(r.w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) store_from_f32(p, i, Elem<T>::code, x[i]);
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r.w[i]));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+    return Row{{pair(x[0], x[2]), pair(x[4], x[6])}, {pair(x[1], x[3]), pair(x[5], x[7])}};
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row(T *p, bool vec, const Row &x) {
+    const float y[8] = {x.e[0].x, x.o[0].x, x.e[0].y, x.o[0].y, x.e[1].x, x.o[1].x, x.e[1].y, x.o[1].y};
+    if (!vec) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) store_from_f32(p, i, Elem<T>::code, y[i]);
+    } else if constexpr (sizeof(T) == 4) {
+        store_vec_from_f32<T, 4>(p, y);
+        store_vec_from_f32<T, 4>(p + 4, y + 4);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const __half2 h = __floats2half2_rn(y[2 * i], y[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -84,127 +133,209 @@ struct AppendArgs {
     int *exps;
     int vec;                         // 1 q, 2 q_out, 4 k, 8 v: rows on 16-byte boundaries
     int slots;                       // page slots; blocks < slots * Hk write the cache
-    int q_units;                     // head chunks of one token
+    int q_units, q_heads;            // warps of a token, heads of each
 };
 
-// What a lane needs to norm and rotate its 8 channels of a head.
-struct Turn {
-    float w[8], c[8], s[8];
-    int part;   // rotary halves: 0 outside, 1 first half, 2 second half, 3 pairs
-    int shift;  // lanes to the partner half
+// Cosines and sines of a lane's channels.  Halves: c.e, c.o and s.e, s.o as the
+// channels, the sines negative in the first half; pairs: c.e and s.e for the four pairs.
+struct Angles {
+    Row c, s;
+};
+
+// What a lane's place in the head makes of the rotation: 0 outside of it, 1 and 2 the
+// halves, 3 pairs; `from`: the lane of the other half.
+struct Place {
+    int part, from, index;
 };
 
 template <int LPT>
-__device__ __forceinline__ void turn_weights(Turn &t, const AppendArgs &a, const void *w, int li) {
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        t.w[i] = w && li * 8 < a.D ? load_as_f32(w, li * 8 + i, a.w_dtype) : 0.f;
-    const int d = li * 8;
-    t.shift = a.R / 16;
-    t.part = d >= a.R ? 0 : a.interleaved ? 3 : li < t.shift ? 1 : 2;
+__device__ __forceinline__ Place place_of(const AppendArgs &a, int lane) {
+    const int li = lane % LPT, shift = a.R / 16;
+    Place p;
+    p.part = li * 8 >= a.R ? 0 : a.interleaved ? 3 : li < shift ? 1 : 2;
+    p.from = p.part == 1 ? lane + shift : p.part == 2 ? lane - shift : lane;
+    p.index = p.part == 3 ? li * 4 : (p.part == 2 ? li - shift : li) * 8;
+    return p;
 }
 
-__device__ __forceinline__ void turn_angles(Turn &t, const AppendArgs &a, int li, int64_t pos) {
-    if (t.part == 0) return;
+__device__ __forceinline__ Row load_weights(const AppendArgs &a, const void *w, int li) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = w && li * 8 < a.D ? load_as_f32(w, li * 8 + i, a.w_dtype) : 0.f;
+    return Row{{pair(x[0], x[2]), pair(x[4], x[6])}, {pair(x[1], x[3]), pair(x[5], x[7])}};
+}
+
+__device__ __forceinline__ void load_angles(Angles &t, const AppendArgs &a, const Place &p, int64_t pos) {
+    if (p.part == 0) return;
     if (pos < 0 || pos >= a.rotary_rows) {
         atomicOr(a.table.status, kBadPosition);
         pos = pos < 0 ? 0 : a.rotary_rows - 1;
     }
-    const float *row = a.rotary + pos * a.R;
-    if (t.part == 3) {
-        const float4 c = *reinterpret_cast<const float4 *>(row + li * 4);
-        const float4 s = *reinterpret_cast<const float4 *>(row + a.R / 2 + li * 4);
-        t.c[0] = c.x; t.c[1] = c.y; t.c[2] = c.z; t.c[3] = c.w;
-        t.s[0] = s.x; t.s[1] = s.y; t.s[2] = s.z; t.s[3] = s.w;
+    const float *row = a.rotary + pos * a.R + p.index;
+    const float4 c = *reinterpret_cast<const float4 *>(row);
+    const float4 s = *reinterpret_cast<const float4 *>(row + a.R / 2);
+    if (p.part == 3) {
+        t.c.e[0] = pair(c.x, c.y);
+        t.c.e[1] = pair(c.z, c.w);
+        t.s.e[0] = pair(s.x, s.y);
+        t.s.e[1] = pair(s.z, s.w);
     } else {
-        const int i = (t.part == 1 ? li : li - t.shift) * 8;
-        load_vec_f32<float, 4>(row + i, t.c);
-        load_vec_f32<float, 4>(row + i + 4, t.c + 4);
-        load_vec_f32<float, 4>(row + a.R / 2 + i, t.s);
-        load_vec_f32<float, 4>(row + a.R / 2 + i + 4, t.s + 4);
+        const float4 d = *reinterpret_cast<const float4 *>(row + 4);
+        const float4 u = *reinterpret_cast<const float4 *>(row + a.R / 2 + 4);
+        const float2 g = p.part == 1 ? pair(-1.f, -1.f) : pair(1.f, 1.f);
+        t.c = Row{{pair(c.x, c.z), pair(d.x, d.z)}, {pair(c.y, c.w), pair(d.y, d.w)}};
+        t.s = Row{{__fmul2_rn(pair(s.x, s.z), g), __fmul2_rn(pair(u.x, u.z), g)},
+                  {__fmul2_rn(pair(s.y, s.w), g), __fmul2_rn(pair(u.y, u.w), g)}};
     }
 }
 
-// Norm and rotation of one head held by LPT lanes (8 channels each).  All lanes
-// of the warp call it.
-template <int LPT>
-__device__ __forceinline__ void turn_row(float x[8], const Turn &t, bool norm, float inv_d, float eps) {
-    if (norm) {
-        float s[8];
+// x c + y s, every operation rounded.  (The sums are scalar: the compiler joins paired
+// products and paired sums into fused ones, whatever rounding they are written with.)
+__device__ __forceinline__ float2 turn2(float2 x, float2 c, float2 y, float2 s) {
+    const float2 u = __fmul2_rn(x, c), v = __fmul2_rn(y, s);
+    return pair(__fadd_rn(u.x, v.x), __fadd_rn(u.y, v.y));
+}
+
+__device__ __forceinline__ float2 shfl2(float2 x, int from) {
+    return pair(__shfl_sync(0xffffffffu, x.x, from), __shfl_sync(0xffffffffu, x.y, from));
+}
+
+// Sum of a lane's 8 squares: neighbours first, then pairs of them, then fours.
+__device__ __forceinline__ float squares(const Row &x) {
+    const float2 u = turn2(x.e[0], x.e[0], x.o[0], x.o[0]);
+    const float2 v = turn2(x.e[1], x.e[1], x.o[1], x.o[1]);
+    return __fadd_rn(__fadd_rn(u.x, u.y), __fadd_rn(v.x, v.y));
+}
+
+__device__ __forceinline__ float norm_factor(float ss, const AppendArgs &a) {
+    return __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(ss, a.inv_d), a.eps)));
+}
+
+__device__ __forceinline__ void norm_row(Row &x, float r, const Row &w) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) s[i] = __fmul_rn(x[i], x[i]);
-        float ss = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3])),
-                             __fadd_rn(__fadd_rn(s[4], s[5]), __fadd_rn(s[6], s[7])));
-#pragma unroll
-        for (int m = 1; m < LPT; m *= 2) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, m));
-        const float r = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(ss, inv_d), eps)));
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), t.w[i]);
+    for (int i = 0; i < 2; i++) {
+        x.e[i] = __fmul2_rn(__fmul2_rn(x.e[i], pair(r, r)), w.e[i]);
+        x.o[i] = __fmul2_rn(__fmul2_rn(x.o[i], pair(r, r)), w.o[i]);
     }
-    if (t.shift == 0) return;  // no rotation (uniform over the launch)
+}
+
+// Norms of N heads, each held by LPT >= 8 lanes.  All lanes of the warp call it.  The
+// lanes share the heads out while they sum (the two halves of an exchange keep one half
+// of the heads each), so that a lane sums, and takes the root of, one head.
+template <int LPT, int N>
+__device__ __forceinline__ void norm_rows(Row x[N], const Row &w, const AppendArgs &a) {
     const int lane = threadIdx.x & 31;
-    const int from = t.part == 1 ? lane + t.shift : t.part == 2 ? lane - t.shift : lane;
-    float y[8];
+    float s[N];
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], from);
-    if (t.part == 3) {
+    for (int p = 0; p < N; p++) s[p] = squares(x[p]);
+    int n = N;  // heads this lane still sums
+#pragma unroll
+    for (int m = 1; m < LPT; m *= 2) {
+        if (n > 1) {
+            const bool up = lane & m;
+            n /= 2;
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) {
+                if (i >= n) break;
+                const float give = up ? s[i] : s[i + n], mine = up ? s[i + n] : s[i];
+                s[i] = __fadd_rn(mine, __shfl_xor_sync(0xffffffffu, give, m));
+            }
+        } else {
+            s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], m));
+        }
+    }
+    const float r = norm_factor(s[0], a);
+    // head p is with the lane whose low bits, the last halving first, spell p
+#pragma unroll
+    for (int p = 0; p < N; p++) {
+        int from = 0;
+#pragma unroll
+        for (int m = 1, h = N / 2; h; m *= 2, h /= 2) from += p & h ? m : 0;
+        norm_row(x[p], __shfl_sync(0xffffffffu, r, from, LPT), w);
+    }
+}
+
+// Rotation of one head held by LPT lanes.  All lanes of the warp call it.
+__device__ __forceinline__ void rotate_row(Row &x, const Angles &t, const Place &p, const AppendArgs &a) {
+    if (a.interleaved) {
+        if (p.part == 3) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float2 e = x.e[i], o = x.o[i], s = t.s.e[i];
+                x.e[i] = turn2(e, t.c.e[i], o, pair(-s.x, -s.y));
+                x.o[i] = turn2(o, t.c.e[i], e, s);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float2 e = shfl2(x.e[i], p.from), o = shfl2(x.o[i], p.from);
+            if (p.part) {
+                x.e[i] = turn2(x.e[i], t.c.e[i], e, t.s.e[i]);
+                x.o[i] = turn2(x.o[i], t.c.o[i], o, t.s.o[i]);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float max_nan(float x, float y) {  // a NaN stays
+    float z;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+}
+
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Codes of a lane's 8 channels, left in x as whole numbers, and the scale of their group,
+// which 4 lanes share; returns the word of the K layout: channel i in nibble
+// (i >> 1) + 4 (i & 1).  x / scale is taken as a product with 1 / scale, rounded by adding
+// 1.5 * 2^23; where that lies within 1e-5 of a half (its error is under 2e-6), or past 7
+// (scales at either end of fp16's range), divisions decide, so that the codes are those of
+// clamp(rint(x / scale), -7, 7).
+__device__ __forceinline__ uint32_t quantise(Row &x, __half &scale) {
+    float top = max_nan(max_nan(fabsf(x.e[0].x), fabsf(x.e[0].y)), max_nan(fabsf(x.e[1].x), fabsf(x.e[1].y)));
+    top = max_nan(top, max_nan(max_nan(fabsf(x.o[0].x), fabsf(x.o[0].y)), max_nan(fabsf(x.o[1].x), fabsf(x.o[1].y))));
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const bool bad = !(top < INFINITY);
+    scale = bad ? __ushort_as_half(0x7fff) : __float2half_rn(fminf(__fmul_rn(top, 1.f / 7.f), 65504.f));
+    const float s = __half2float(scale);
+    const float inv = s > 0.f ? rcp_fast(s) : 0.f;
+    float2 y[4];
+    const float2 inv2 = pair(inv, inv), up = pair(12582912.f, 12582912.f), down = pair(-12582912.f, -12582912.f);
+    float2 *const z[4] = {&x.e[0], &x.e[1], &x.o[0], &x.o[1]};
+    float off = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 t = __fmul2_rn(*z[i], inv2);
+        const float2 n = __fadd2_rn(__fadd2_rn(t, up), down);
+        const float2 d = __fadd2_rn(t, pair(-n.x, -n.y));
+        off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+        y[i] = n;
+    }
+    if (off > 0.5f - 1e-5f || !(top * inv <= 7.4f)) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float u = x[2 * i], v = x[2 * i + 1];
-            x[2 * i] = __fsub_rn(__fmul_rn(u, t.c[i]), __fmul_rn(v, t.s[i]));
-            x[2 * i + 1] = __fadd_rn(__fmul_rn(v, t.c[i]), __fmul_rn(u, t.s[i]));
+            y[i].x = bad ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(z[i]->x, s)), -7.f), 7.f);
+            y[i].y = bad ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(z[i]->y, s)), -7.f), 7.f);
         }
-    } else if (t.part == 1) {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            x[i] = __fsub_rn(__fmul_rn(x[i], t.c[i]), __fmul_rn(y[i], t.s[i]));
-    } else if (t.part == 2) {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            x[i] = __fadd_rn(__fmul_rn(x[i], t.c[i]), __fmul_rn(y[i], t.s[i]));
     }
-}
-
-// Codes (+8, one per byte) of a lane's 8 channels and the scale of their group,
-// which the 4 lanes of the group share.  x / scale is taken as a product with
-// 1 / scale; only where that is within 1e-5 of a half (its error is under 2e-6)
-// does the division itself decide, so the codes are those of rint(x / scale).
-__device__ __forceinline__ void quantise8(const float x[8], uint32_t code[2], __half &scale) {
-    uint32_t top = 0;  // of the bit patterns: a NaN is above an infinity is above a number
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const bool bad = top >= 0x7f800000u;
-    scale = __float2half_rn(fminf(__fmul_rn(__uint_as_float(top), 1.f / 7.f), 65504.f));
-    const float s = __half2float(scale);
-    if (bad) scale = __ushort_as_half(0x7fff);
-    const float inv = bad || !(s > 0.f) ? 0.f : 1.f / s;
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float t = x[i] * inv;
-        float n = rintf(t);
-        if (fabsf(fabsf(t - n) - 0.5f) < 1e-5f) n = rintf(__fdiv_rn(x[i], s));
-        n = fminf(fmaxf(n, -7.f), 7.f);
-        c[i] = bad ? 8u : (uint32_t)((int)n + 8);
-    }
-    code[0] = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-    code[1] = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
-}
-
-// 8 codes in bytes -> the K word: channel i in nibble (i >> 1) + 4 (i & 1)
-__device__ __forceinline__ uint32_t pack_k(const uint32_t code[2]) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        w |= ((code[i >> 2] >> (8 * (i & 3))) & 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
-    return w;
+    for (int i = 0; i < 4; i++) *z[i] = y[i];
+    // four codes (+8) as one number below 2^16, twice
+    const float2 u = __ffma2_rn(x.e[1], pair(256.f, 256.f), x.e[0]);
+    const float2 v = __ffma2_rn(x.o[1], pair(256.f, 256.f), x.o[0]);
+    const float lo = fmaf(u.y, 16.f, u.x) + (8388608.f + 34952.f), hi = fmaf(v.y, 16.f, v.x) + (8388608.f + 34952.f);
+    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
 }
 
 template <typename T, int W, int LPT>
 __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *smem) {
-    constexpr int D = 32 * W, ROW = D + 8, TPP = 32 / LPT;  // tokens of a pass
+    constexpr int D = 32 * W, ROW = 4 * W + 4, TPP = 32 / LPT;  // tokens of a pass
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int g = lane / LPT, li = lane % LPT;
     const bool live = li * 8 < D;
@@ -224,9 +355,10 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
         const int *cu = a.cu;
         const int lp = a.table.log_page;
         b = warp_find([=](int i) { return (int64_t)(cu[i] >> lp) + 2 * i; }, a.B, slot);
-        first = (int64_t)(cu[b] >> lp) + 2 * b;
-        n = max(0, (int)min((int64_t)cu[b + 1], a.T) - max(0, cu[b]));
-        t0 = max(0, cu[b]);
+        const int c0 = cu[b], c1 = cu[b + 1];
+        first = (int64_t)(c0 >> lp) + 2 * b;
+        n = max(0, (int)min((int64_t)c1, a.T) - max(0, c0));
+        t0 = max(0, c0);
     }
     const int len = a.lengths[b];
     if (len < 0 || n <= 0 || slot < first) return;
@@ -238,90 +370,110 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
         return;
     }
     const int id = a.table.pages[b * a.table.stride + page];
+    const int base = (int)page << a.table.log_page;  // position of the page's first token
+    const int lo = max(len, base), hi = (int)min(end, (int64_t)base + P);
+
+    const T *k0 = static_cast<const T *>(a.k) + b * (a.S ? a.k_sb : 0) + h * a.k_sh + li * 8;
+    const T *v0 = static_cast<const T *>(a.v) + b * (a.S ? a.v_sb : 0) + h * a.v_sh + li * 8;
+    const Place place = place_of<LPT>(a, lane);
+    Raw<T> kr, vr;   // of the next pass
+    Angles angles;
+    // pass p of a tile at position tb: token p + g of it
+    auto load = [&](int tb, int p) {
+        const int t = tb + p + g;
+        kr = zero_raw<T>();
+        vr = zero_raw<T>();
+        if (live && t >= lo && t < hi) {
+            const int64_t row = t0 + (t - len);
+            kr = load_raw(k0 + row * a.k_ss, a.vec & 4);
+            vr = load_raw(v0 + row * a.v_ss, a.vec & 8);
+            if (a.R) load_angles(angles, a, place, a.positions ? (int64_t)a.positions[a.S ? b * a.S + row : row] : t);
+        }
+    };
+    // the first tile of this warp that gets tokens
+    int tile = max(warp, (lo - base) / 16);
+    tile += ((warp - tile) % warps + warps) % warps;
+    if (tile < P / 16 && base + tile * 16 < hi) load(base + tile * 16, max(lo - base - tile * 16, 0) / TPP * TPP);
+    const Row kw = load_weights(a, a.norm_k ? a.kw : nullptr, li);
+
     if ((unsigned)id >= (unsigned)a.table.num_pages) {
         if (threadIdx.x == 0) atomicOr(a.table.status, kBadPage);
         return;
     }
     const int64_t record = (int64_t)id * a.Hk + h;
     unsigned char *tiles = a.pool + record * (P / 16) * tile_bytes(W);
-    const int base = (int)page << a.table.log_page;  // position of the page's first token
-    const int lo = max(len, base), hi = (int)min(end, (int64_t)base + P);
-
-    Turn turn;
-    turn_weights<LPT>(turn, a, a.norm_k ? a.kw : nullptr, li);
-    float mn[8], mx[8];
+    const bool older = lo > base;
+    float2 mn[4], mx[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) { mn[i] = INFINITY; mx[i] = -INFINITY; }
+    for (int i = 0; i < 4; i++) { mn[i] = pair(INFINITY, INFINITY); mx[i] = pair(-INFINITY, -INFINITY); }
 
-    unsigned char *stage = smem + warp * 16 * ROW;
-    const T *k0 = static_cast<const T *>(a.k) + b * (a.S ? a.k_sb : 0) + h * a.k_sh;
-    const T *v0 = static_cast<const T *>(a.v) + b * (a.S ? a.v_sb : 0) + h * a.v_sh;
-    for (int tile = warp; tile < P / 16; tile += warps) {
+    uint32_t *stage = reinterpret_cast<uint32_t *>(smem) + warp * 16 * ROW;
+    const int r = lane >> 2, c = lane & 3;
+    for (; tile < P / 16 && base + tile * 16 < hi; tile += warps) {
         const int tb = base + tile * 16;  // position of the tile's first token
         const int tlo = max(lo, tb) - tb, thi = min(hi, tb + 16) - tb;
-        if (tlo >= thi) continue;
         unsigned char *out = tiles + (int64_t)tile * tile_bytes(W);
+        uint32_t *vw = reinterpret_cast<uint32_t *>(out + v_off(W));
         for (int p = tlo / TPP * TPP; p < thi; p += TPP) {
-            const int t = p + g;
-            const bool on = t >= tlo && t < thi;
-            const int64_t row = t0 + (tb + t - len);
-            float x[8], y[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = y[i] = 0.f;
-            if (on && live) {
-                load8(k0 + row * a.k_ss + li * 8, a.vec & 4, x);
-                load8(v0 + row * a.v_ss + li * 8, a.vec & 8, y);
-                if (a.R)
-                    turn_angles(turn, a, li, a.positions ? a.positions[a.S ? b * a.S + row : row]
-                                                         : (int64_t)(tb + t));
-            }
-            turn_row<LPT>(x, turn, a.norm_k, a.inv_d, a.eps);
-            uint32_t kc[2], vc[2];
+            Row x = widen(kr), y = widen(vr);
+            const Angles now = angles;
+            if (p + TPP < thi)
+                load(tb, p + TPP);
+            else if (tile + warps < P / 16 && tb + 16 * warps < hi)
+                load(tb + 16 * warps, 0);
+            if (a.norm_k) norm_rows<LPT, 1>(&x, kw, a);
+            if (a.R) rotate_row(x, now, place, a);
             __half ks, vs;
-            quantise8(x, kc, ks);
-            quantise8(y, vc, vs);
-            if (on && live) {
-                const int j = li / 4, c = li % 4;
-                reinterpret_cast<uint32_t *>(out)[t * 4 * W + c * W + j] = pack_k(kc);
-                *reinterpret_cast<uint2 *>(stage + t * ROW + li * 8) = make_uint2(vc[0], vc[1]);
-                if (c == 0) {
+            const uint32_t kc = quantise(x, ks), vc = quantise(y, vs);
+            const int t = p + g;
+            if (live && t >= tlo && t < thi) {
+                const int j = li / 4, q = li % 4;
+                reinterpret_cast<uint32_t *>(out)[t * 4 * W + q * W + j] = kc;
+                stage[t * ROW + li] = vc;
+                if (q == 0) {
                     reinterpret_cast<__half *>(out + ks_off(W))[(2 * (t & 7) + (t >> 3)) * W + j] = ks;
                     reinterpret_cast<__half *>(out + vs_off(W))[4 * (((t & 7) >> 1) * W + j) +
                                                                 2 * (t >> 3) + (t & 1)] = vs;
                 }
                 if (a.bounds) {
                     const float s = __half2float(ks);
+                    const float2 z[4] = {__fmul2_rn(x.e[0], pair(s, s)), __fmul2_rn(x.e[1], pair(s, s)),
+                                         __fmul2_rn(x.o[0], pair(s, s)), __fmul2_rn(x.o[1], pair(s, s))};
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float z = (float)((int)((kc[i >> 2] >> (8 * (i & 3))) & 15u) - 8) * s;
-                        mn[i] = fminf(mn[i], z);
-                        mx[i] = fmaxf(mx[i], z);
+                    for (int i = 0; i < 4; i++) {
+                        mn[i] = pair(fminf(mn[i].x, z[i].x), fminf(mn[i].y, z[i].y));
+                        mx[i] = pair(fmaxf(mx[i].x, z[i].x), fmaxf(mx[i].y, z[i].y));
                     }
                 }
             }
         }
         __syncwarp();
-        // the V words: this lane's channels and tokens, older tokens kept
-        {
-            const int r = lane >> 2, c = lane & 3;
-            const int tok[4] = {2 * c, 2 * c + 1, 2 * c + 8, 2 * c + 9};
-            uint32_t mask = 0;  // nibbles 2 y + 4 e and the next one: both channel halves
+        // The V words of this lane: channels 16 m + r and + 8 of tokens 2c, 2c + 1, 2c + 8,
+        // 2c + 9, turned from their place in the staged words to nibble x + 2 y + 4 e.
+        uint32_t word[2 * W], mask = 0;
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (tok[u] >= tlo && tok[u] < thi) mask |= 0xffu << (4 * (2 * (u >> 1) + 4 * (u & 1)));
-            uint32_t *vw = reinterpret_cast<uint32_t *>(out + v_off(W));
-            const bool merge = tlo > 0;
+        for (int m = 0; m < 2 * W; m++) word[m] = 0u;
+        const int from = (r >> 1) + 4 * (r & 1);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int tok = 2 * c + 8 * (u >> 1) + (u & 1), to = 2 * (u >> 1) + 4 * (u & 1);
+            if (tok >= tlo && tok < thi) mask |= 0xffu << (4 * to);
+            const uint4 *z = reinterpret_cast<const uint4 *>(stage + tok * ROW);
+            const int s0 = 4 * (from - to), s1 = 4 * (from - to - 1);  // the funnel shifts take them mod 32
+#pragma unroll
+            for (int i = 0; i < W; i++) {
+                const uint4 y = z[i];
+                word[2 * i] |= (__funnelshift_r(y.x, y.x, s0) & (0x0fu << (4 * to))) |
+                               (__funnelshift_r(y.y, y.y, s1) & (0xf0u << (4 * to)));
+                word[2 * i + 1] |= (__funnelshift_r(y.z, y.z, s0) & (0x0fu << (4 * to))) |
+                                   (__funnelshift_r(y.w, y.w, s1) & (0xf0u << (4 * to)));
+            }
+        }
+        if (mask) {
 #pragma unroll
             for (int m = 0; m < 2 * W; m++) {
-                uint32_t w = 0;
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const unsigned char *s = stage + tok[u] * ROW + 16 * m + r;
-                    const int sh = 4 * (2 * (u >> 1) + 4 * (u & 1));
-                    w |= (uint32_t)(s[0] & 15) << sh | (uint32_t)(s[8] & 15) << (sh + 4);
-                }
                 const int at = v_word<W>(m, lane);
-                if (mask) vw[at] = (w & mask) | (merge ? vw[at] & ~mask : 0u);
+                vw[at] = (word[m] & mask) | (tlo > 0 ? vw[at] & ~mask : 0u);  // older tokens share words
             }
         }
         __syncwarp();
@@ -330,75 +482,85 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
     if (a.bounds) {
         // the block's tokens: over the lanes that share channels, then over the warps
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < 4; i++) {
 #pragma unroll
             for (int m = LPT; m < 32; m *= 2) {
-                mn[i] = fminf(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], m));
-                mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], m));
+                const float2 u = shfl2(mn[i], lane ^ m), v = shfl2(mx[i], lane ^ m);
+                mn[i] = pair(fminf(mn[i].x, u.x), fminf(mn[i].y, u.y));
+                mx[i] = pair(fmaxf(mx[i].x, v.x), fmaxf(mx[i].y, v.y));
             }
         }
         __syncthreads();
         float *lo_s = reinterpret_cast<float *>(smem), *hi_s = lo_s + warps * D;
         if (g == 0 && live) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                lo_s[warp * D + li * 8 + i] = mn[i];
-                hi_s[warp * D + li * 8 + i] = mx[i];
+            for (int i = 0; i < 4; i++) {  // channels 0 2, 4 6, 1 3, 5 7
+                const int d = warp * D + li * 8 + (i & 1) * 4 + (i >> 1);
+                lo_s[d] = mn[i].x;
+                lo_s[d + 2] = mn[i].y;
+                hi_s[d] = mx[i].x;
+                hi_s[d + 2] = mx[i].y;
             }
         }
         __syncthreads();
         if (warp == 0) {
-            float top = 0.f;
-            for (int d = lane; d < D; d += 32) {
-                float u = lo_s[d], v = hi_s[d];
+            const int e0 = older ? a.exps[record] : -40;
+            signed char *out = a.bounds + record * 2 * D;
+            float u[W], v[W], top = 0.f;
+            int o0[W], o1[W];
+#pragma unroll
+            for (int i = 0; i < W; i++) {
+                const int d = lane + 32 * i;
+                o0[i] = older ? out[d] : 0;
+                o1[i] = older ? out[D + d] : 0;
+                u[i] = lo_s[d];
+                v[i] = hi_s[d];
                 for (int w = 1; w < warps; w++) {
-                    u = fminf(u, lo_s[w * D + d]);
-                    v = fmaxf(v, hi_s[w * D + d]);
+                    u[i] = fminf(u[i], lo_s[w * D + d]);
+                    v[i] = fmaxf(v[i], hi_s[w * D + d]);
                 }
-                if (u > v) u = v = 0.f;  // no number among them
-                lo_s[d] = u;
-                hi_s[d] = v;
-                top = fmaxf(top, fmaxf(fabsf(u), fabsf(v)));
+                if (u[i] > v[i]) u[i] = v[i] = 0.f;  // no number among them
+                top = fmaxf(top, fmaxf(fabsf(u[i]), fabsf(v[i])));
             }
 #pragma unroll
             for (int m = 16; m; m /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-            int e = bound_exponent(top, -40);
-            const bool older = lo > base;
-            const int e0 = older ? a.exps[record] : e;
-            e = max(e, e0);
+            const int e = max(bound_exponent(top, -40), e0);
             const float f = pow2f(-e);
-            signed char *out = a.bounds + record * 2 * D;
-            for (int d = lane; d < D; d += 32) {
-                int u = (int)floorf(lo_s[d] * f), v = (int)ceilf(hi_s[d] * f);
+#pragma unroll
+            for (int i = 0; i < W; i++) {
+                int x = (int)floorf(u[i] * f), y = (int)ceilf(v[i] * f);
                 if (older) {
-                    u = min(u, (int)out[d] >> min(e - e0, 31));
-                    v = max(v, -(-(int)out[D + d] >> min(e - e0, 31)));
+                    x = min(x, o0[i] >> min(e - e0, 31));
+                    y = max(y, -(-o1[i] >> min(e - e0, 31)));
                 }
-                out[d] = (signed char)u;
-                out[D + d] = (signed char)v;
+                out[lane + 32 * i] = (signed char)x;
+                out[D + lane + 32 * i] = (signed char)y;
             }
-            __syncwarp();
             if (lane == 0) a.exps[record] = e;
         }
     }
 }
 
-constexpr int kQPasses = 4;  // passes of a warp over a token's query heads
+// Query heads: one warp for some heads of a token, kQPasses rows of lanes at a time, the
+// next ones on their way while these are turned.
+template <typename T>
+constexpr int kQPasses = sizeof(T) == 4 ? 2 : 4;
 
 template <typename T, int W, int LPT>
 __device__ __forceinline__ void turn_queries(const AppendArgs &a) {
-    constexpr int D = 32 * W, TPP = 32 / LPT;
+    constexpr int D = 32 * W, TPP = 32 / LPT, N = kQPasses<T>;
     const int lane = threadIdx.x & 31, g = lane / LPT, li = lane % LPT;
     const bool live = li * 8 < D;
     const int64_t unit = ((int64_t)blockIdx.x - (int64_t)a.slots * a.Hk) * (blockDim.x >> 5) +
                          (threadIdx.x >> 5);
-    const int64_t t = unit / a.q_units;
+    const int64_t t = (uint32_t)unit / (uint32_t)a.q_units;
     if (t >= a.T) return;
-    const int h0 = (int)(unit % a.q_units) * (kQPasses * TPP);
+    int h = (int)((uint32_t)unit - (uint32_t)t * a.q_units) * a.q_heads + g;
+    const int end = min(h - g + a.q_heads, a.Hq);
     int64_t b, row;
     if (a.S) {
-        b = t / a.S;
-        row = t % a.S;
+        b = (uint32_t)t / (uint32_t)a.S;
+        row = t - b * a.S;
     } else {
         const int *cu = a.cu;
         b = warp_find([=](int i) { return (int64_t)cu[i]; }, a.B, t);
@@ -406,31 +568,36 @@ __device__ __forceinline__ void turn_queries(const AppendArgs &a) {
     }
     const T *q = static_cast<const T *>(a.q) + (a.S ? b * a.q_sb : 0) + row * a.q_ss + li * 8;
     T *qo = static_cast<T *>(a.qo) + (a.S ? b * a.qo_sb : 0) + row * a.qo_ss + li * 8;
-    float x[kQPasses][8];
+    Raw<T> raw[N];
+    auto load = [&](int h0) {
 #pragma unroll
-    for (int p = 0; p < kQPasses; p++) {
-        const int h = h0 + p * TPP + g;
+        for (int p = 0; p < N; p++)
+            raw[p] = live && h0 + p * TPP < end ? load_raw(q + (h0 + p * TPP) * a.q_sh, a.vec & 1) : zero_raw<T>();
+    };
+    load(h);
+    const Place place = place_of<LPT>(a, lane);
+    const Row w = load_weights(a, a.norm_q ? a.qw : nullptr, li);
+    Angles angles;
+    if (a.R)
+        load_angles(angles, a, place,
+                    a.positions ? (int64_t)a.positions[t]
+                                : (int64_t)max(0, a.lengths[b]) + (a.S ? row : t - a.cu[b]));
+    for (; h - g < end; h += N * TPP) {
+        Row x[N];
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[p][i] = 0.f;
-        if (live && h < a.Hq) load8(q + h * a.q_sh, a.vec & 1, x[p]);
-    }
-    Turn turn;
-    turn_weights<LPT>(turn, a, a.norm_q ? a.qw : nullptr, li);
-    if (a.R) {
-        int64_t pos = a.positions ? (int64_t)a.positions[t]
-                                  : (int64_t)max(0, a.lengths[b]) + (a.S ? row : t - a.cu[b]);
-        turn_angles(turn, a, li, pos);
-    }
+        for (int p = 0; p < N; p++) x[p] = widen(raw[p]);
+        if (h - g + N * TPP < end) load(h + N * TPP);
+        if (a.norm_q) norm_rows<LPT, N>(x, w, a);
 #pragma unroll
-    for (int p = 0; p < kQPasses; p++) {
-        const int h = h0 + p * TPP + g;
-        turn_row<LPT>(x[p], turn, a.norm_q, a.inv_d, a.eps);
-        if (live && h < a.Hq) store8(qo + h * a.qo_sh, a.vec & 2, x[p]);
+        for (int p = 0; p < N; p++) {
+            if (a.R) rotate_row(x[p], angles, place, a);
+            if (live && h + p * TPP < end) store_row(qo + (h + p * TPP) * a.qo_sh, a.vec & 2, x[p]);
+        }
     }
 }
 
 template <typename T, int W, int LPT>
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(256, 2) append_kernel(const __grid_constant__ AppendArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     if ((int64_t)blockIdx.x < (int64_t)a.slots * a.Hk)
         write_page<T, W, LPT>(a, smem);
@@ -439,6 +606,10 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 }
 
 // ------------------------------------------------------------------------ read
+__device__ __forceinline__ Row row_of(const float x[8]) {
+    return Row{{pair(x[0], x[2]), pair(x[4], x[6])}, {pair(x[1], x[3]), pair(x[5], x[7])}};
+}
+
 struct ReadArgs {
     const unsigned char *pool;
     Table table;
@@ -505,7 +676,7 @@ __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ ReadA
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 x[i] = (float)((int)((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) - 8) * s;
-            store8(ko + row * a.o_ss + li * 8, a.vec & 1, x);
+            store_row(ko + row * a.o_ss + li * 8, a.vec & 1, row_of(x));
         }
         {
             const int vc = (t & 7) >> 1;
@@ -514,7 +685,7 @@ __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ ReadA
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 x[i] = (float)((int)((vw[v_word<W>(li >> 1, i * 4 + vc)] >> sh) & 15u) - 8) * s;
-            store8(vo + row * a.o_ss + li * 8, a.vec & 2, x);
+            store_row(vo + row * a.o_ss + li * 8, a.vec & 2, row_of(x));
         }
     }
 }
@@ -605,13 +776,18 @@ extern "C" int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t 
             using E = decltype(t);
             constexpr int W = decltype(w)::value, LPT = lanes_per_head(W);
             a.slots = (int)slots;
-            a.q_units = (int)((Hq + kQPasses * (32 / LPT) - 1) / (kQPasses * (32 / LPT)));
+            // heads of a query warp: all of a token's where there are tokens enough for
+            // 32 warps an SM, else fewer, down to one load's worth
+            constexpr int per = kQPasses<E> * (32 / LPT);
+            const int64_t loads = (Hq + per - 1) / per, want = (32 * (int64_t)num_sms() + T - 1) / T;
+            a.q_heads = (int)(per * ((loads + want - 1) / want));
+            a.q_units = a.q_heads ? (int)((Hq + a.q_heads - 1) / a.q_heads) : 0;
             const int64_t blocks = slots * Hk + (T * a.q_units + warps - 1) / warps;
-            if (slots > 0x7fffffff || blocks > 0x7fffffff) {
+            if (slots * Hk > 0x7fffffff || blocks * warps > 0x7fffffff) {
                 set_error("kv4_append: too many tokens for one call");
                 return FC_ENOTSUP;
             }
-            const size_t stage = (size_t)warps * 16 * (32 * W + 8), red = (size_t)warps * 32 * W * 8;
+            const size_t stage = (size_t)warps * 16 * (4 * W + 4) * 4, red = (size_t)warps * 32 * W * 8;
             append_kernel<E, W, LPT><<<(unsigned)blocks, warps * 32, stage > red ? stage : red, st>>>(a);
             return check_launch("kv4_append");
         });

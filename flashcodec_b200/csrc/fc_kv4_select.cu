@@ -9,6 +9,13 @@
 // z is the query in whole numbers (|z| <= 127, common power of two of the group),
 // so the sums are exact (below 2^24, also as fp32) and the choice of pages does not
 // depend on the order of any sum.
+//
+// The bounds, 2 D bytes a page, are read once; HBM bounds the scoring, a chain of short
+// steps the choice.  A lane takes 16 bytes of a page, 8 two-way integer dot products; a
+// warp 32 pages.  The block that finishes a (sequence, head) last chooses: the keys (scores
+// in unsigned order) are counted in 1024 equal bins between the least and the largest, the
+// bin that holds the last key wanted is counted in the same way, until what is wanted of it
+// is all or one value; one prefix sum over the pages then writes the indices in order.
 #include "fc_kv4.cuh"
 
 namespace fc {
@@ -26,12 +33,15 @@ struct SelectArgs {
     const int *lengths;
     int count, sink, recent;
     int *out;
+    int *counters;   // (B, Hk), zero between calls
     uint32_t *keys;  // (B, Hk, max_pages)
     int shift;       // ceil(log2(G * D / 1024)) where positive
 };
 
-constexpr int kScoreThreads = 256;
-constexpr int kScorePages = 128;  // pages of a scoring block
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kBlockPages = 32 * kWarps;  // pages of a block
+constexpr int kBins = 1024;
+constexpr int kHold = 16;                 // keys of a thread at a time
 
 // Order-preserving map of finite fp32 to unsigned.
 __device__ __forceinline__ uint32_t order_key(float f) {
@@ -39,113 +49,228 @@ __device__ __forceinline__ uint32_t order_key(float f) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+struct PickShared {
+    uint32_t hist[kBins];
+    uint32_t part[kWarps], part2[kWarps];
+    uint32_t bin, above, inside;
+};
+
+// Sum over the threads before this one, and over all of them.
+__device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t *part, uint32_t &all) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t upto = x;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    __syncthreads();  // earlier readers of part are done
+    if (lane == 31) part[warp] = upto;
+    __syncthreads();
+    uint32_t before = upto - x;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+        if (w < warp) before += part[w];
+        all += part[w];
+    }
+    return before;
+}
+
+// The choice for one (sequence, KV head): n > count keys.
+__device__ void pick(const SelectArgs &a, const uint32_t *keys, int n, int *out, PickShared &s) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int first = a.sink, last = n - a.recent;  // the pages between stand for choice
+    uint32_t rest = (uint32_t)(a.count - a.sink - a.recent);
+    // f(key, page) of every page that stands for choice, this thread's of each window
+    auto each = [&](auto f) {
+        for (int i0 = 0; i0 < n; i0 += kThreads * kHold) {
+            uint32_t k[kHold];
+#pragma unroll
+            for (int j = 0; j < kHold; j++) {
+                const int i = i0 + j * kThreads + (int)threadIdx.x;
+                k[j] = i >= first && i < last ? __ldcg(keys + i) : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < kHold; j++) {
+                const int i = i0 + j * kThreads + (int)threadIdx.x;
+                if (i >= first && i < last) f(k[j]);
+            }
+        }
+    };
+    // from `from` on a key is taken, but of those equal to `from` only `rest` if `some`
+    uint32_t from = 0xffffffffu;
+    bool some = false;
+    if (rest) {
+        uint32_t lo = 0xffffffffu, hi = 0;
+        each([&](uint32_t k) { lo = min(lo, k); hi = max(hi, k); });
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        if (lane == 0) { s.part[warp] = lo; s.part2[warp] = hi; }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) { lo = min(lo, s.part[w]); hi = max(hi, s.part2[w]); }
+        uint32_t range = hi - lo;
+        for (;;) {
+            const int shift = max(0, 22 - __clz(range));  // range >> shift < 1024
+            for (int i = threadIdx.x; i < kBins; i += kThreads) s.hist[i] = 0;
+            __syncthreads();
+            each([&](uint32_t k) {
+                if (k - lo <= range) atomicAdd(&s.hist[(k - lo) >> shift], 1u);
+            });
+            __syncthreads();
+            // bins from the top: this thread's four are 1023 - 4 t and the ones below
+            const int top = kBins - 1 - 4 * (int)threadIdx.x;
+            const uint32_t h[4] = {s.hist[top], s.hist[top - 1], s.hist[top - 2], s.hist[top - 3]};
+            uint32_t all, above = scan_before(h[0] + h[1] + h[2] + h[3], s.part, all);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (above < rest && rest <= above + h[i]) {
+                    s.bin = top - i;
+                    s.above = above;
+                    s.inside = h[i];
+                }
+                above += h[i];
+            }
+            __syncthreads();
+            rest -= s.above;
+            from = lo + (s.bin << shift);
+            if (rest == s.inside) break;  // all of the bin
+            if (shift == 0) { some = true; break; }
+            lo = from;
+            range = (1u << shift) - 1;
+            __syncthreads();  // s.bin is read
+        }
+    }
+    // indices in ascending order: a thread takes neighbouring pages
+    uint32_t done = 0, equal = 0;  // of the windows before
+    for (int i0 = 0; i0 < n; i0 += kThreads * kHold) {
+        const int per = min(kHold, (n - i0 + kThreads - 1) / kThreads);
+        const int b = i0 + (int)threadIdx.x * per, e = min(b + per, n);
+        uint32_t over = 0, same = 0;  // bit j: page b + j is taken; equals the last key
+#pragma unroll
+        for (int j = 0; j < kHold; j++) {
+            const int i = b + j;
+            if (i >= e || j >= per) continue;
+            if (i < first || i >= last) {
+                over |= 1u << j;
+            } else if (a.count > a.sink + a.recent) {
+                const uint32_t k = __ldcg(keys + i);
+                if (k > from || (k == from && !some)) over |= 1u << j;
+                if (k == from && some) same |= 1u << j;
+            }
+        }
+        uint32_t all;
+        const uint32_t eq = equal + scan_before(__popc(same), s.part, all);
+        equal += all;
+        // of the equal ones the first `rest`
+        uint32_t take = over, left = eq < rest ? rest - eq : 0u;
+        for (uint32_t m = same; m && left; m &= m - 1, left--) take |= m & -m;
+        uint32_t at = done + scan_before(__popc(take), s.part2, all);
+        done += all;
+        for (uint32_t m = take; m; m &= m - 1) out[at++] = b + __ffs(m) - 1;
+    }
+}
+
+// Lanes that share a page, 16 bytes each: a power of two of at least 4 W.
+constexpr int lanes_per_page(int W) { return W <= 2 ? 8 : W <= 4 ? 16 : 32; }
+
 template <int W>
-__global__ void __launch_bounds__(kScoreThreads) score_kernel(const __grid_constant__ SelectArgs a) {
-    constexpr int D = 32 * W;
-    __shared__ short z[2 * D];  // N then P, as the bounds: least then largest
-    __shared__ float wmax[kScoreThreads / 32];
+__global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ SelectArgs a) {
+    constexpr int D = 32 * W, GRP = lanes_per_page(W), PPW = 32 / GRP;
+    __shared__ __align__(16) short z[16 * GRP];  // N then P, as the bounds: least then largest
+    __shared__ float wmax[kWarps];
+    __shared__ PickShared pick_s;
+    __shared__ int last_s;
     const int h = blockIdx.y;
     const int64_t b = blockIdx.z;
-    const int len = a.table.length(a.lengths[b]);
-    const int n = (len + (1 << a.table.log_page) - 1) >> a.table.log_page;
-    const int p0 = blockIdx.x * kScorePages;
-    if (p0 >= n || n <= a.count) return;  // everything is taken: no scores needed
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.Hq / a.Hk;
     const int64_t q0 = b * a.q_sb + (int64_t)h * G * a.q_sh;
+    const int len = a.table.length(a.lengths[b]);
+    const int n = (len + (1 << a.table.log_page) - 1) >> a.table.log_page;
+    int *out = a.out + (b * a.Hk + h) * a.count;
+    if (n <= a.count) {  // everything is taken: no scores needed
+        if (blockIdx.x == 0)
+            for (int i = threadIdx.x; i < a.count; i += kThreads) out[i] = i < n ? i : -1;
+        return;
+    }
+    const int p0 = blockIdx.x * kBlockPages;
+    if (p0 >= n) return;
+    // this lane's page, its record and exponent
+    const int page = p0 + warp * 32 + lane;
+    int rec = 0, e_page = 0;
+    if (page < n) {
+        rec = a.table.page(b, page);
+        e_page = a.exps[(int64_t)rec * a.Hk + h];
+    }
+
     float top = 0.f;
-    for (int i = threadIdx.x; i < G * D; i += kScoreThreads)
+    for (int i = threadIdx.x; i < G * D; i += kThreads)
         top = fmaxf(top, fabsf(load_as_f32(a.q, q0 + (i / D) * a.q_sh + i % D, a.dtype)));
     for (int o = 16; o; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) wmax[warp] = top;
     __syncthreads();
-    for (int w = 0; w < kScoreThreads / 32; w++) top = fmaxf(top, wmax[w]);
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) top = fmaxf(top, wmax[w]);
     const int e = bound_exponent(fminf(top, 3e38f), -100) + a.shift;
-    for (int d = threadIdx.x; d < D; d += kScoreThreads) {
+    for (int d = threadIdx.x; d < 8 * GRP; d += kThreads) {
         int neg = 0, pos = 0;
-        for (int g = 0; g < G; g++) {
-            const float x = load_as_f32(a.q, q0 + g * a.q_sh + d, a.dtype);
-            const int v = (int)fminf(fmaxf(rintf(ldexpf(x, -e)), -127.f), 127.f);
-            neg += min(v, 0);
-            pos += max(v, 0);
+        if (d < D)
+            for (int g = 0; g < G; g++) {
+                const float x = load_as_f32(a.q, q0 + g * a.q_sh + d, a.dtype);
+                const int v = (int)fminf(fmaxf(rintf(ldexpf(x, -e)), -127.f), 127.f);
+                neg += min(v, 0);
+                pos += max(v, 0);
+            }
+        if (d < D) {
+            z[d] = (short)neg;
+            z[D + d] = (short)pos;
         }
-        z[d] = (short)neg;
-        z[D + d] = (short)pos;
     }
     __syncthreads();
-    const int p1 = min(p0 + kScorePages, n);
-    for (int p = p0 + warp; p < p1; p += kScoreThreads / 32) {
-        const int64_t rec = (int64_t)a.table.page(b, p) * a.Hk + h;
-        int sum = 0;
-        for (int d = lane; d < 2 * D; d += 32) sum += (int)a.bounds[rec * 2 * D + d] * z[d];
-        sum = __reduce_add_sync(0xffffffffu, sum);
-        if (lane == 0) {
-            uint32_t k = order_key((float)sum * pow2f(a.exps[rec]));
-            if (p < a.sink || p >= n - a.recent) k = 0xffffffffu;
-            a.keys[(b * a.Hk + h) * a.table.max_pages + p] = k;
+    const int li = lane % GRP, grp = lane / GRP;
+    const bool live = li < 4 * W;
+    int zr[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) zr[i] = live ? reinterpret_cast<const int *>(z)[li * 8 + i] : 0;
+    int mine = 0;
+    if (p0 + warp * 32 < n) {
+#pragma unroll 4
+        for (int it = 0; it < GRP; it++) {  // PPW pages at a time, one a group
+            const int id = __shfl_sync(0xffffffffu, rec, it * PPW + grp);
+            int4 v = make_int4(0, 0, 0, 0);
+            if (live)
+                v = __ldg(reinterpret_cast<const int4 *>(a.bounds + ((int64_t)id * a.Hk + h) * 2 * D) + li);
+            int sum = 0;
+            const int w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                sum = __dp2a_lo(zr[2 * i], w[i], sum);
+                sum = __dp2a_hi(zr[2 * i + 1], w[i], sum);
+            }
+#pragma unroll
+            for (int o = GRP / 2; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const int s = __shfl_sync(0xffffffffu, sum, (lane % PPW) * GRP);
+            if (lane / PPW == it) mine = s;
         }
     }
-}
-
-constexpr int kPickThreads = 1024;
-
-// The `count` largest keys, equal ones by index, in ascending order of index.
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const __grid_constant__ SelectArgs a) {
-    __shared__ uint32_t hist[256], want_s, rest_s, base[2], sums[2][kPickThreads / 32];
-    const int h = blockIdx.x;
-    const int64_t b = blockIdx.y;
-    const int len = a.table.length(a.lengths[b]);
-    const int n = (len + (1 << a.table.log_page) - 1) >> a.table.log_page;
-    int *out = a.out + (b * a.Hk + h) * a.count;
-    if (n <= a.count) {
-        for (int i = threadIdx.x; i < a.count; i += kPickThreads) out[i] = i < n ? i : -1;
-        return;
-    }
-    const uint32_t *keys = a.keys + (b * a.Hk + h) * a.table.max_pages;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint32_t prefix = 0, rest = (uint32_t)a.count;  // of keys with this prefix, `rest` are wanted
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += kPickThreads) hist[i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kPickThreads) {
-            const uint32_t k = keys[i];
-            if (shift == 24 || k >> (shift + 8) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int i = 255;
-            uint32_t left = rest;
-            while (hist[i] < left) left -= hist[i--];
-            want_s = (uint32_t)i;
-            rest_s = left;
-        }
-        __syncthreads();
-        prefix = prefix << 8 | want_s;
-        rest = rest_s;
-        __syncthreads();
-    }
-    // prefix is the smallest key taken, `rest` of its equals are
-    if (threadIdx.x < 2) base[threadIdx.x] = 0;
+    uint32_t *keys = a.keys + (b * a.Hk + h) * a.table.max_pages;
+    if (page < n) keys[page] = order_key((float)mine * pow2f(e_page));
     __syncthreads();
-    for (int i0 = 0; i0 < n; i0 += kPickThreads) {
-        const int i = i0 + threadIdx.x;
-        const uint32_t k = i < n ? keys[i] : 0u;
-        const bool over = i < n && k > prefix, same = i < n && k == prefix;
-        const uint32_t below = (1u << lane) - 1;
-        const uint32_t mo = __ballot_sync(0xffffffffu, over), ms = __ballot_sync(0xffffffffu, same);
-        if (lane == 0) { sums[0][warp] = __popc(mo); sums[1][warp] = __popc(ms); }
-        __syncthreads();
-        uint32_t no = base[0], ns = base[1];
-        for (int w = 0; w < warp; w++) { no += sums[0][w]; ns += sums[1][w]; }
-        no += __popc(mo & below);
-        ns += __popc(ms & below);
-        if (over || (same && ns < rest)) out[no + min(ns, rest)] = i;
-        __syncthreads();
-        if (threadIdx.x == 0)
-            for (int w = 0; w < kPickThreads / 32; w++) { base[0] += sums[0][w]; base[1] += sums[1][w]; }
-        __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        int *counter = a.counters + b * a.Hk + h;
+        const int blocks = (n + kBlockPages - 1) / kBlockPages;
+        last_s = atomicAdd(counter, 1) == blocks - 1;
+        if (last_s) *counter = 0;
+        __threadfence();
     }
+    __syncthreads();
+    if (last_s) pick(a, keys, n, out, pick_s);
 }
+
+int64_t counter_bytes(int64_t units) { return 256 + (units * 4 + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace kv4
@@ -155,7 +280,7 @@ using namespace fc;
 using namespace fc::kv4;
 
 extern "C" size_t fc_kv4_select_workspace_size(int64_t B, int64_t Hk, int64_t max_pages) {
-    return 256 + (size_t)B * Hk * max_pages * sizeof(uint32_t);
+    return (size_t)(counter_bytes(B * Hk) + B * Hk * max_pages * 4);
 }
 
 extern "C" int fc_kv4_select(const void *q, int dtype, int64_t B, int64_t Hq, int64_t q_sb, int64_t q_sh,
@@ -190,15 +315,13 @@ extern "C" int fc_kv4_select(const void *q, int dtype, int64_t B, int64_t Hq, in
     SelectArgs a{q, dtype, q_sb, q_sh, (int)Hq, (int)Hk, bounds, exponents,
                  Table{page_table, table_stride, (int)max_pages, (int)num_pages, ilog2(page_size), status},
                  lengths, (int)count, (int)sink, (int)recent, pages,
-                 reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + 256),
+                 reinterpret_cast<int *>(static_cast<char *>(workspace) + 256),
+                 reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + counter_bytes(B * Hk)),
                  Hq / Hk * D > 1024 ? ilog2((Hq / Hk * D + 1023) / 1024) : 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return by_head_dim(D, [&](auto w) {
-        score_kernel<decltype(w)::value><<<dim3((unsigned)((max_pages + kScorePages - 1) / kScorePages),
-                                                (unsigned)Hk, (unsigned)B), kScoreThreads, 0, st>>>(a);
-        int e = check_launch("kv4_select");
-        if (e) return e;
-        pick_kernel<<<dim3((unsigned)Hk, (unsigned)B), kPickThreads, 0, st>>>(a);
+        select_kernel<decltype(w)::value><<<dim3((unsigned)((max_pages + kBlockPages - 1) / kBlockPages),
+                                                 (unsigned)Hk, (unsigned)B), kThreads, 0, st>>>(a);
         return check_launch("kv4_select");
     });
 }

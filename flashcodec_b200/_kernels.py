@@ -551,6 +551,17 @@ def decode_attn_grouped(q, krows, vrows, kscales, vscales, group, kraw, vraw, A,
 
 
 # --------------------------------------------------------- paged 4-bit KV cache
+# These calls run once per layer and decode step, next to kernels of a few microseconds:
+# what is the same from call to call (addresses of the cache, workspaces, the library's
+# functions) is looked up once.
+try:  # the current stream's handle and device without building objects around them
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream, _cuda_getDevice as _current_device
+except ImportError:
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
+    _current_device = torch.cuda.current_device
+
 _kv4_workspaces: dict = {}
 
 
@@ -561,40 +572,36 @@ def kv4_page_bytes(Hk: int, D: int, page_size: int) -> int:
     return n
 
 
-def _kv4_workspace(what: str, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    """Zero-initialised workspace of one entry point, cached per (device, stream)."""
-    key = (what, device.index, stream)
-    ws = _kv4_workspaces.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-        _kv4_workspaces[key] = ws
-    return ws
+def _kv4_workspace(what, sizes, index, stream):
+    """(address, bytes) of the zero-initialised workspace of one entry point, shared by the
+    calls of a (device, stream); `sizes` are the arguments of its size function."""
+    key = (what, index, stream)
+    held = _kv4_workspaces.get(key)
+    if held is None:
+        held = _kv4_workspaces[key] = [None, 0, 0, set()]
+    if sizes not in held[3]:
+        nbytes = getattr(_lib.load(), f"fc_kv4_{what}_workspace_size")(*sizes)
+        if nbytes > held[2]:
+            held[0] = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+            held[1], held[2] = held[0].data_ptr(), nbytes
+        held[3].add(sizes)
+    return held
 
 
-class _On:
-    """The device made current for a launch, where it is not already."""
-    __slots__ = ("ctx",)
-
-    def __init__(self, device):
-        self.ctx = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
+def _kv4_call(fn, what, index, args, ws=None):
+    if _current_device() == index:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    if rc:
+        if ws is not None:
+            ws[0].zero_()
+        _lib.check(rc, what)
 
 
 def _token_strides(t, packed):
     """(sequence, token, head) strides of (B, S, H, D), (B, H, D) or packed (T, H, D)."""
-    if t is None:
-        return 0, 0, 0
     s = t.stride()
     if len(s) == 4:
         return s[0], s[1], s[2]
@@ -604,77 +611,59 @@ def _token_strides(t, packed):
 def kv4_append(cache, q, k, v, q_out, B, S, T, cu, table, lengths, positions, q_weight, k_weight,
                eps, rotary, interleaved) -> None:
     """fc_kv4_append on a PagedInt4Cache; shapes are the caller's to check."""
-    dev = cache.device
     packed = cu is not None
     w = q_weight if q_weight is not None else k_weight
-    with _On(dev):
-        rc = _lib.load().fc_kv4_append(
-            _addr(q), *_token_strides(q, packed), _addr(q_out), *_token_strides(q_out, packed),
-            0 if q is None else q.shape[-2],
-            k.data_ptr(), *_token_strides(k, packed), v.data_ptr(), *_token_strides(v, packed),
-            dtype_code(k), B, S, T, _addr(cu), lengths.data_ptr(), _addr(positions),
-            _addr(q_weight), _addr(k_weight), 0 if w is None else dtype_code(w), eps,
-            _addr(rotary), *((0, 0) if rotary is None else rotary.shape), interleaved,
-            cache._pool_ptr, cache.num_pages, cache.num_kv_heads, cache.head_dim, cache.page_size,
-            table.data_ptr(), table.stride(0), table.shape[1],
-            cache._bounds_ptr, cache._exponents_ptr, cache._status_ptr,
-            torch.cuda.current_stream(dev).cuda_stream)
-    if rc:
-        _lib.check(rc, "kv4_append")
+    index = cache._index
+    qs = (None, 0, 0, 0, None, 0, 0, 0, 0) if q is None else (
+        q.data_ptr(), *_token_strides(q, packed), q_out.data_ptr(), *_token_strides(q_out, packed),
+        q.shape[-2])
+    _kv4_call(_lib.load().fc_kv4_append, "kv4_append", index, (
+        *qs, k.data_ptr(), *_token_strides(k, packed), v.data_ptr(), *_token_strides(v, packed),
+        dtype_code(k), B, S, T, None if cu is None else cu.data_ptr(), lengths.data_ptr(),
+        None if positions is None else positions.data_ptr(),
+        None if q_weight is None else q_weight.data_ptr(),
+        None if k_weight is None else k_weight.data_ptr(), 0 if w is None else dtype_code(w), eps,
+        *((None, 0, 0) if rotary is None else (rotary.data_ptr(), *rotary.shape)), interleaved,
+        *cache._pool_args, table.data_ptr(), table.stride(0), table.shape[1],
+        *cache._bounds_args, cache._status_ptr, _raw_stream(index)))
 
 
 def kv4_read(cache, table, starts, B, S, T, cu, k_out, v_out) -> None:
     """fc_kv4_read into k_out and v_out (of one layout)."""
-    dev = cache.device
-    with _On(dev):
-        rc = _lib.load().fc_kv4_read(
-            cache._pool_ptr, cache.num_pages, cache.num_kv_heads, cache.head_dim, cache.page_size,
-            table.data_ptr(), table.stride(0), table.shape[1], _addr(starts), B, S, T, _addr(cu),
-            k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out),
-            *_token_strides(k_out, cu is not None), cache._status_ptr,
-            torch.cuda.current_stream(dev).cuda_stream)
-    if rc:
-        _lib.check(rc, "kv4_read")
+    index = cache._index
+    _kv4_call(_lib.load().fc_kv4_read, "kv4_read", index, (
+        *cache._pool_args, table.data_ptr(), table.stride(0), table.shape[1],
+        None if starts is None else starts.data_ptr(), B, S, T,
+        None if cu is None else cu.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+        dtype_code(k_out), *_token_strides(k_out, cu is not None), cache._status_ptr,
+        _raw_stream(index)))
 
 
 def kv4_attn(cache, q, table, lengths, selected, scale, out, lse) -> None:
     """fc_kv4_attn; q and out (B, Sq, Hq, D) or (B, Hq, D)."""
-    dev = cache.device
-    lib = _lib.load()
-    B, Hq, D = q.shape[0], q.shape[-2], q.shape[-1]
-    Sq = q.shape[1] if q.dim() == 4 else 1
+    index = cache._index
+    stream = _raw_stream(index)
+    s = q.shape
+    B, Sq, Hq = (s[0], s[1], s[2]) if len(s) == 4 else (s[0], 1, s[1])
     # a selection of no pages is not the same as none: its address is not null
-    sel = None if selected is None else selected.data_ptr() or cache._status_ptr
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    ws = _kv4_workspace("attn", dev, stream,
-                        lib.fc_kv4_attn_workspace_size(B, Sq, Hq, cache.num_kv_heads, D))
-    with _On(dev):
-        rc = lib.fc_kv4_attn(
-            q.data_ptr(), dtype_code(q), B, Sq, Hq, *_token_strides(q, False),
-            cache._pool_ptr, cache.num_pages, cache.num_kv_heads, D, cache.page_size,
-            table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
-            sel, 0 if selected is None else selected.shape[2], scale,
-            out.data_ptr(), *_token_strides(out, False), _addr(lse),
-            ws.data_ptr(), ws.numel(), cache._status_ptr, stream)
-    if rc:
-        ws.zero_()
-        _lib.check(rc, "kv4_attn")
+    sel = (None, 0) if selected is None else (selected.data_ptr() or cache._status_ptr,
+                                              selected.shape[2])
+    ws = _kv4_workspace("attn", (B, Sq, Hq, cache.num_kv_heads, cache.head_dim), index, stream)
+    _kv4_call(_lib.load().fc_kv4_attn, "kv4_attn", index, (
+        q.data_ptr(), dtype_code(q), B, Sq, Hq, *_token_strides(q, False), *cache._pool_args,
+        table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(), *sel, scale,
+        out.data_ptr(), *_token_strides(out, False), None if lse is None else lse.data_ptr(),
+        ws[1], ws[2], cache._status_ptr, stream), ws)
 
 
 def kv4_select(cache, q, table, lengths, count, sink, recent, pages) -> None:
     """fc_kv4_select; q (B, Hq, D), pages (B, Hk, count) int32."""
-    dev = cache.device
-    lib = _lib.load()
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    ws = _kv4_workspace("select", dev, stream, lib.fc_kv4_select_workspace_size(
-        q.shape[0], cache.num_kv_heads, table.shape[1]))
-    with _On(dev):
-        rc = lib.fc_kv4_select(
-            q.data_ptr(), dtype_code(q), q.shape[0], q.shape[1], q.stride(0), q.stride(1),
-            cache._bounds_ptr, cache._exponents_ptr, cache.num_pages, cache.num_kv_heads,
-            cache.head_dim, cache.page_size, table.data_ptr(), table.stride(0), table.shape[1],
-            lengths.data_ptr(), count, sink, recent, pages.data_ptr(), ws.data_ptr(), ws.numel(),
-            cache._status_ptr, stream)
-    if rc:
-        ws.zero_()
-        _lib.check(rc, "kv4_select")
+    index = cache._index
+    stream = _raw_stream(index)
+    B, Hq = q.shape[0], q.shape[1]
+    n = table.shape[1]
+    ws = _kv4_workspace("select", (B, cache.num_kv_heads, n), index, stream)
+    _kv4_call(_lib.load().fc_kv4_select, "kv4_select", index, (
+        q.data_ptr(), dtype_code(q), B, Hq, q.stride(0), q.stride(1), *cache._bounds_args,
+        *cache._pool_args[1:], table.data_ptr(), table.stride(0), n, lengths.data_ptr(), count,
+        sink, recent, pages.data_ptr(), ws[1], ws[2], cache._status_ptr, stream), ws)

@@ -133,33 +133,37 @@ class PagedInt4Cache:
             self.exponents = torch.zeros(self.num_pages, self.num_kv_heads, dtype=torch.int32,
                                          device=dev)
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._pool_ptr, self._status_ptr = self.pool.data_ptr(), self.status.data_ptr()
-        self._bounds_ptr = self.bounds.data_ptr() if bounds else None
-        self._exponents_ptr = self.exponents.data_ptr() if bounds else None
+        self._index, self._scale = dev.index, self.head_dim ** -0.5
+        self._status_ptr = self.status.data_ptr()
+        self._pool_args = (self.pool.data_ptr(), self.num_pages, self.num_kv_heads, self.head_dim,
+                           self.page_size)
+        self._bounds_args = (self.bounds.data_ptr(), self.exponents.data_ptr()) if bounds \
+            else (None, None)
 
     # ------------------------------------------------------------ argument checks
     def _check(self, *tensors):
-        grad = torch.is_grad_enabled()
+        index, grad = self._index, torch.is_grad_enabled()
         for t in tensors:
             if t is None:
                 continue
-            if t.device != self.device:
+            if t.get_device() != index:
                 K.require_cuda(t)
                 raise ValueError(f"a tensor is on {t.device}, the cache on {self.device}")
             if grad and t.requires_grad:
                 raise RuntimeError("the 4-bit cache holds rounded values and has no gradient: "
                                    "call it under torch.no_grad()")
 
-    def _index(self, name, t, shape):
-        if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+    def _ints(self, name, t, shape):
+        if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} "
                              f"(got {t.dtype}, {tuple(t.shape)})")
 
     def _table(self, page_table):
-        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[1] == 0 \
-                or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        s = page_table.shape
+        if page_table.dtype is not torch.int32 or len(s) != 2 or s[1] == 0 \
+                or (s[1] > 1 and page_table.stride(1) != 1):
             raise ValueError("page_table must be an int32 (B, n) tensor with unit stride along n")
-        return page_table.shape[0]
+        return s[0]
 
     def _rows(self, name, t, dims, heads=None):
         s = t.shape
@@ -168,6 +172,7 @@ class PagedInt4Cache:
                              f"{tuple(s)}")
         if t.stride(-1) != 1:
             raise ValueError(f"{name}: the head dim must have unit stride")
+        return s
 
     # ----------------------------------------------------------------- operations
     def append(self, q, k, v, page_table, lengths, *, cu_seqlens=None, q_weight=None,
@@ -196,26 +201,24 @@ class PagedInt4Cache:
         B = self._table(page_table)
         packed = cu_seqlens is not None
         dims = (3,) if packed else (3, 4)
-        self._rows("k", k, dims, self.num_kv_heads)
-        self._rows("v", v, dims, self.num_kv_heads)
-        lead = k.shape[:-2]
-        if v.shape != k.shape or v.dtype != k.dtype:
+        shape = self._rows("k", k, dims, self.num_kv_heads)
+        lead = shape[:-2]
+        if self._rows("v", v, dims) != shape or v.dtype is not k.dtype:
             raise ValueError("k and v must have one shape and dtype")
         if packed:
-            self._index("cu_seqlens", cu_seqlens, (B + 1,))
+            self._ints("cu_seqlens", cu_seqlens, (B + 1,))
             S, T = 0, lead[0]
         else:
             S = lead[1] if len(lead) == 2 else 1
             T = B * S
             if lead[0] != B:
                 raise ValueError(f"k has {lead[0]} sequences, the page table {B}")
-        self._index("lengths", lengths, (B,))
+        self._ints("lengths", lengths, (B,))
         if q is not None:
-            self._rows("q", q, dims)
-            if q.shape[:-2] != lead or q.dtype != k.dtype:
+            if self._rows("q", q, dims)[:-2] != lead or q.dtype is not k.dtype:
                 raise ValueError("q must have the tokens and the dtype of k")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             else:
                 self._rows("q_out", q_out, dims)
                 if q_out.shape != q.shape or q_out.dtype != q.dtype:
@@ -229,7 +232,7 @@ class PagedInt4Cache:
                                    or not rotary.is_contiguous()):
             raise ValueError("rotary must be a contiguous fp32 (positions, R) tensor")
         if positions is not None:
-            self._index("positions", positions, lead if len(lead) == positions.dim() else (T,))
+            self._ints("positions", positions, lead if len(lead) == positions.dim() else (T,))
         K.kv4_append(self, q, k, v, q_out, B, S, T, cu_seqlens, page_table, lengths, positions,
                      q_weight, k_weight, eps, rotary, bool(interleaved))
         return q_out
@@ -250,23 +253,23 @@ class PagedInt4Cache:
         """
         self._check(q, page_table, lengths, selected, out)
         B = self._table(page_table)
-        self._rows("q", q, (3, 4))
-        if q.shape[0] != B:
-            raise ValueError(f"q has {q.shape[0]} sequences, the page table {B}")
-        self._index("lengths", lengths, (B,))
+        shape = self._rows("q", q, (3, 4))
+        if shape[0] != B:
+            raise ValueError(f"q has {shape[0]} sequences, the page table {B}")
+        self._ints("lengths", lengths, (B,))
         if selected is not None:
             if q.dim() == 4 and q.shape[1] != 1:
                 raise ValueError("selected pages go with one query per sequence")
-            self._index("selected", selected, (B, self.num_kv_heads, selected.shape[-1]))
+            self._ints("selected", selected, (B, self.num_kv_heads, selected.shape[-1]))
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             self._rows("out", out, (3, 4))
             if out.shape != q.shape or out.dtype != q.dtype:
                 raise ValueError("out must have the shape and dtype of q")
         lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
         K.kv4_attn(self, q, page_table, lengths, selected,
-                   self.head_dim ** -0.5 if scale is None else scale, out, lse)
+                   self._scale if scale is None else scale, out, lse)
         return (out, lse) if return_lse else out
 
     def select(self, q, page_table, lengths, count, *, sink=1, recent=1):
@@ -285,7 +288,7 @@ class PagedInt4Cache:
         self._rows("q", q, (3,))
         if q.shape[0] != B:
             raise ValueError(f"q has {q.shape[0]} sequences, the page table {B}")
-        self._index("lengths", lengths, (B,))
+        self._ints("lengths", lengths, (B,))
         if count <= 0:
             raise ValueError(f"count must be positive (got {count})")
         pages = torch.empty(B, self.num_kv_heads, count, dtype=torch.int32, device=q.device)
@@ -302,14 +305,15 @@ class PagedInt4Cache:
         if count is None or count < 0:
             raise ValueError("read needs the number of tokens (count)")
         if starts is not None:
-            self._index("starts", starts, (B,))
+            self._ints("starts", starts, (B,))
         if cu_seqlens is not None:
-            self._index("cu_seqlens", cu_seqlens, (B + 1,))
+            self._ints("cu_seqlens", cu_seqlens, (B + 1,))
             shape, S, T = (count,), 0, count
         else:
             shape, S, T = (B, count), count, B * count
-        k, v = torch.empty(2, *shape, self.num_kv_heads, self.head_dim, dtype=dtype,
-                           device=self.device)
+        shape = (*shape, self.num_kv_heads, self.head_dim)
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         K.kv4_read(self, page_table, starts, B, S, T, cu_seqlens, k, v)
         return k, v
 

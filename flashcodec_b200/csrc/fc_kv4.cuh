@@ -130,9 +130,6 @@ __device__ __forceinline__ int warp_find(F key, int n, int64_t x) {
 }
 
 // ------------------------------------------------------------------ host side
-// lanes that hold one head, 8 channels each, as a power of two
-constexpr int lanes_per_head(int W) { return W <= 2 ? 8 : W <= 4 ? 16 : 32; }
-
 template <typename F>
 int by_head_dim(int64_t D, F f) {
     switch (D) {

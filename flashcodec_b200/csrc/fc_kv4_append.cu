@@ -24,6 +24,18 @@ namespace fc {
 namespace kv4 {
 namespace {
 
+// How a head lies over lanes: chunks of 8 channels, one in a lane, or, where the whole
+// head turns by halves (FULL), two, D / 2 channels apart: then a lane holds both channels
+// of its pairs and exchanges only sums, with half as many lanes.  (Two need a power of two
+// of chunks, as the sum of squares goes by halves.)
+template <int W, bool FULL>
+struct Lay {
+    static constexpr int CH = FULL ? 2 : 1, half = 4 * W / CH;
+    static constexpr int LPT = half <= 4 ? 4 : half <= 8 ? 8 : half <= 16 ? 16 : 32;  // lanes of a head
+    static constexpr int TPP = 32 / LPT;                                             // heads of a warp
+};
+constexpr bool can_be_full(int W) { return (W & (W - 1)) == 0; }
+
 // 8 neighbouring channels of a head in one lane, as pairs for the paired fp32
 // instructions: even channels (0, 2), (4, 6) and odd ones (1, 3), (5, 7).
 struct Row {
@@ -137,34 +149,36 @@ struct AppendArgs {
 };
 
 // Cosines and sines of a lane's channels.  Halves: c.e, c.o and s.e, s.o as the
-// channels, the sines negative in the first half; pairs: c.e and s.e for the four pairs.
+// channels, the sines negative in the first half (not where a lane has both halves);
+// pairs: c.e and s.e for the four pairs.
 struct Angles {
     Row c, s;
 };
 
-// What a lane's place in the head makes of the rotation: 0 outside of it, 1 and 2 the
-// halves, 3 pairs; `from`: the lane of the other half.
+// What the place of a chunk in the head makes of the rotation: 0 outside of it, 1 and 2
+// the halves, 3 pairs; the lane of the other half; where its angles are in the table's row.
 struct Place {
-    int part, from, index;
+    int part, lane, index;
 };
 
-template <int LPT>
+template <int W, bool FULL>
 __device__ __forceinline__ Place place_of(const AppendArgs &a, int lane) {
-    const int li = lane % LPT, shift = a.R / 16;
+    const int ci = lane % Lay<W, FULL>::LPT, shift = a.R / 16;
     Place p;
-    p.part = li * 8 >= a.R ? 0 : a.interleaved ? 3 : li < shift ? 1 : 2;
-    p.from = p.part == 1 ? lane + shift : p.part == 2 ? lane - shift : lane;
-    p.index = p.part == 3 ? li * 4 : (p.part == 2 ? li - shift : li) * 8;
+    p.part = ci * 8 >= a.R ? 0 : a.interleaved ? 3 : FULL || ci < shift ? 1 : 2;
+    p.lane = p.part == 1 ? lane + shift : p.part == 2 ? lane - shift : lane;
+    p.index = p.part == 3 ? ci * 4 : (p.part == 2 ? ci - shift : ci) * 8;
     return p;
 }
 
-__device__ __forceinline__ Row load_weights(const AppendArgs &a, const void *w, int li) {
+__device__ __forceinline__ Row load_weights(const AppendArgs &a, const void *w, int ci) {
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = w && li * 8 < a.D ? load_as_f32(w, li * 8 + i, a.w_dtype) : 0.f;
+    for (int i = 0; i < 8; i++) x[i] = w && ci * 8 < a.D ? load_as_f32(w, ci * 8 + i, a.w_dtype) : 0.f;
     return Row{{pair(x[0], x[2]), pair(x[4], x[6])}, {pair(x[1], x[3]), pair(x[5], x[7])}};
 }
 
+template <bool FULL>
 __device__ __forceinline__ void load_angles(Angles &t, const AppendArgs &a, const Place &p, int64_t pos) {
     if (p.part == 0) return;
     if (pos < 0 || pos >= a.rotary_rows) {
@@ -174,7 +188,7 @@ __device__ __forceinline__ void load_angles(Angles &t, const AppendArgs &a, cons
     const float *row = a.rotary + pos * a.R + p.index;
     const float4 c = *reinterpret_cast<const float4 *>(row);
     const float4 s = *reinterpret_cast<const float4 *>(row + a.R / 2);
-    if (p.part == 3) {
+    if (!FULL && p.part == 3) {
         t.c.e[0] = pair(c.x, c.y);
         t.c.e[1] = pair(c.z, c.w);
         t.s.e[0] = pair(s.x, s.y);
@@ -182,7 +196,7 @@ __device__ __forceinline__ void load_angles(Angles &t, const AppendArgs &a, cons
     } else {
         const float4 d = *reinterpret_cast<const float4 *>(row + 4);
         const float4 u = *reinterpret_cast<const float4 *>(row + a.R / 2 + 4);
-        const float2 g = p.part == 1 ? pair(-1.f, -1.f) : pair(1.f, 1.f);
+        const float2 g = !FULL && p.part == 1 ? pair(-1.f, -1.f) : pair(1.f, 1.f);
         t.c = Row{{pair(c.x, c.z), pair(d.x, d.z)}, {pair(c.y, c.w), pair(d.y, d.w)}};
         t.s = Row{{__fmul2_rn(pair(s.x, s.z), g), __fmul2_rn(pair(u.x, u.z), g)},
                   {__fmul2_rn(pair(s.y, s.w), g), __fmul2_rn(pair(u.y, u.w), g)}};
@@ -219,23 +233,28 @@ __device__ __forceinline__ void norm_row(Row &x, float r, const Row &w) {
     }
 }
 
-// Norms of N heads, each held by LPT >= 8 lanes.  All lanes of the warp call it.  The
-// lanes share the heads out while they sum (the two halves of an exchange keep one half
-// of the heads each), so that a lane sums, and takes the root of, one head.
-template <int LPT, int N>
-__device__ __forceinline__ void norm_rows(Row x[N], const Row &w, const AppendArgs &a) {
+// Norms of N heads; `w`: the lane's weights.  All lanes of the warp call it.  The lanes
+// share the sums out while they add (the two halves of an exchange keep one half of them
+// each), so that a lane sums, and takes the root of, one head.
+template <int W, bool FULL, int N, typename Weights>
+__device__ __forceinline__ void norm_rows(Row x[N][Lay<W, FULL>::CH], Weights w, const AppendArgs &a) {
+    using L = Lay<W, FULL>;
+    constexpr int V = N * L::CH;
+    static_assert(V <= L::LPT && (V & (V - 1)) == 0, "every lane ends with one sum");
     const int lane = threadIdx.x & 31;
-    float s[N];
+    float s[V];  // sum k N + p: chunk k of head p
 #pragma unroll
-    for (int p = 0; p < N; p++) s[p] = squares(x[p]);
-    int n = N;  // heads this lane still sums
+    for (int k = 0; k < L::CH; k++)
 #pragma unroll
-    for (int m = 1; m < LPT; m *= 2) {
+        for (int p = 0; p < N; p++) s[k * N + p] = squares(x[p][k]);
+    int n = V;  // sums this lane still adds
+#pragma unroll
+    for (int m = 1; m < L::LPT; m *= 2) {
         if (n > 1) {
             const bool up = lane & m;
             n /= 2;
 #pragma unroll
-            for (int i = 0; i < N / 2; i++) {
+            for (int i = 0; i < V / 2; i++) {
                 if (i >= n) break;
                 const float give = up ? s[i] : s[i + n], mine = up ? s[i + n] : s[i];
                 s[i] = __fadd_rn(mine, __shfl_xor_sync(0xffffffffu, give, m));
@@ -244,35 +263,51 @@ __device__ __forceinline__ void norm_rows(Row x[N], const Row &w, const AppendAr
             s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], m));
         }
     }
+    // the first halving was by chunk
+    if constexpr (L::CH == 2) s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], 1));
     const float r = norm_factor(s[0], a);
-    // head p is with the lane whose low bits, the last halving first, spell p
+    // head p is with the lanes whose next bits, the last halving first, spell p
 #pragma unroll
     for (int p = 0; p < N; p++) {
         int from = 0;
 #pragma unroll
-        for (int m = 1, h = N / 2; h; m *= 2, h /= 2) from += p & h ? m : 0;
-        norm_row(x[p], __shfl_sync(0xffffffffu, r, from, LPT), w);
+        for (int m = L::CH, h = N / 2; h; m *= 2, h /= 2) from += p & h ? m : 0;
+        const float f = __shfl_sync(0xffffffffu, r, from, L::LPT);
+#pragma unroll
+        for (int k = 0; k < L::CH; k++) norm_row(x[p][k], f, w(k));
     }
 }
 
-// Rotation of one head held by LPT lanes.  All lanes of the warp call it.
-__device__ __forceinline__ void rotate_row(Row &x, const Angles &t, const Place &p, const AppendArgs &a) {
-    if (a.interleaved) {
+// Rotation of one head.  All lanes of the warp call it.
+template <int W, bool FULL>
+__device__ __forceinline__ void rotate_row(Row x[Lay<W, FULL>::CH], const Angles &t, const Place &p,
+                                           const AppendArgs &a) {
+    if constexpr (FULL) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float2 e = x[0].e[i], o = x[0].o[i], u = x[1].e[i], v = x[1].o[i];
+            const float2 s = t.s.e[i], r = t.s.o[i];
+            x[0].e[i] = turn2(e, t.c.e[i], u, pair(-s.x, -s.y));
+            x[0].o[i] = turn2(o, t.c.o[i], v, pair(-r.x, -r.y));
+            x[1].e[i] = turn2(u, t.c.e[i], e, s);
+            x[1].o[i] = turn2(v, t.c.o[i], o, r);
+        }
+    } else if (a.interleaved) {
         if (p.part == 3) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float2 e = x.e[i], o = x.o[i], s = t.s.e[i];
-                x.e[i] = turn2(e, t.c.e[i], o, pair(-s.x, -s.y));
-                x.o[i] = turn2(o, t.c.e[i], e, s);
+                const float2 e = x[0].e[i], o = x[0].o[i], s = t.s.e[i];
+                x[0].e[i] = turn2(e, t.c.e[i], o, pair(-s.x, -s.y));
+                x[0].o[i] = turn2(o, t.c.e[i], e, s);
             }
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const float2 e = shfl2(x.e[i], p.from), o = shfl2(x.o[i], p.from);
+            const float2 e = shfl2(x[0].e[i], p.lane), o = shfl2(x[0].o[i], p.lane);
             if (p.part) {
-                x.e[i] = turn2(x.e[i], t.c.e[i], e, t.s.e[i]);
-                x.o[i] = turn2(x.o[i], t.c.o[i], o, t.s.o[i]);
+                x[0].e[i] = turn2(x[0].e[i], t.c.e[i], e, t.s.e[i]);
+                x[0].o[i] = turn2(x[0].o[i], t.c.o[i], o, t.s.o[i]);
             }
         }
     }
@@ -333,12 +368,13 @@ __device__ __forceinline__ uint32_t quantise(Row &x, __half &scale) {
     return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
 }
 
-template <typename T, int W, int LPT>
+template <typename T, int W, bool FULL>
 __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *smem) {
-    constexpr int D = 32 * W, ROW = 4 * W + 4, TPP = 32 / LPT;  // tokens of a pass
+    using L = Lay<W, FULL>;
+    constexpr int D = 32 * W, ROW = 4 * W + 4, CH = L::CH, LPT = L::LPT, TPP = L::TPP;  // TPP tokens a pass
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int g = lane / LPT, li = lane % LPT;
-    const bool live = li * 8 < D;
+    const bool live = li < L::half;
     const int P = 1 << a.table.log_page;
 
     // the page slot: sequence b, its page-th page that gets new tokens
@@ -375,26 +411,23 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
 
     const T *k0 = static_cast<const T *>(a.k) + b * (a.S ? a.k_sb : 0) + h * a.k_sh + li * 8;
     const T *v0 = static_cast<const T *>(a.v) + b * (a.S ? a.v_sb : 0) + h * a.v_sh + li * 8;
-    const Place place = place_of<LPT>(a, lane);
-    Raw<T> kr, vr;   // of the next pass
-    Angles angles;
+    const Place place = place_of<W, FULL>(a, lane);
+    Raw<T> kr[CH], vr[CH];  // of the next pass
     // pass p of a tile at position tb: token p + g of it
     auto load = [&](int tb, int p) {
         const int t = tb + p + g;
-        kr = zero_raw<T>();
-        vr = zero_raw<T>();
-        if (live && t >= lo && t < hi) {
-            const int64_t row = t0 + (t - len);
-            kr = load_raw(k0 + row * a.k_ss, a.vec & 4);
-            vr = load_raw(v0 + row * a.v_ss, a.vec & 8);
-            if (a.R) load_angles(angles, a, place, a.positions ? (int64_t)a.positions[a.S ? b * a.S + row : row] : t);
+        const bool on = live && t >= lo && t < hi;
+        const int64_t row = t0 + (t - len);
+#pragma unroll
+        for (int k = 0; k < CH; k++) {
+            kr[k] = on ? load_raw(k0 + row * a.k_ss + k * L::half * 8, a.vec & 4) : zero_raw<T>();
+            vr[k] = on ? load_raw(v0 + row * a.v_ss + k * L::half * 8, a.vec & 8) : zero_raw<T>();
         }
     };
     // the first tile of this warp that gets tokens
     int tile = max(warp, (lo - base) / 16);
     tile += ((warp - tile) % warps + warps) % warps;
     if (tile < P / 16 && base + tile * 16 < hi) load(base + tile * 16, max(lo - base - tile * 16, 0) / TPP * TPP);
-    const Row kw = load_weights(a, a.norm_k ? a.kw : nullptr, li);
 
     if ((unsigned)id >= (unsigned)a.table.num_pages) {
         if (threadIdx.x == 0) atomicOr(a.table.status, kBadPage);
@@ -403,9 +436,14 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
     const int64_t record = (int64_t)id * a.Hk + h;
     unsigned char *tiles = a.pool + record * (P / 16) * tile_bytes(W);
     const bool older = lo > base;
-    float2 mn[4], mx[4];
+    float2 mn[CH][4], mx[CH][4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) { mn[i] = pair(INFINITY, INFINITY); mx[i] = pair(-INFINITY, -INFINITY); }
+    for (int k = 0; k < CH; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            mn[k][i] = pair(INFINITY, INFINITY);
+            mx[k][i] = pair(-INFINITY, -INFINITY);
+        }
 
     uint32_t *stage = reinterpret_cast<uint32_t *>(smem) + warp * 16 * ROW;
     const int r = lane >> 2, c = lane & 3;
@@ -415,34 +453,52 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
         unsigned char *out = tiles + (int64_t)tile * tile_bytes(W);
         uint32_t *vw = reinterpret_cast<uint32_t *>(out + v_off(W));
         for (int p = tlo / TPP * TPP; p < thi; p += TPP) {
-            Row x = widen(kr), y = widen(vr);
-            const Angles now = angles;
+            Row x[1][CH], y[CH];
+#pragma unroll
+            for (int k = 0; k < CH; k++) {
+                x[0][k] = widen(kr[k]);
+                y[k] = widen(vr[k]);
+            }
+            const int t = p + g;
+            const bool on = live && t >= tlo && t < thi;
             if (p + TPP < thi)
                 load(tb, p + TPP);
             else if (tile + warps < P / 16 && tb + 16 * warps < hi)
                 load(tb + 16 * warps, 0);
-            if (a.norm_k) norm_rows<LPT, 1>(&x, kw, a);
-            if (a.R) rotate_row(x, now, place, a);
-            __half ks, vs;
-            const uint32_t kc = quantise(x, ks), vc = quantise(y, vs);
-            const int t = p + g;
-            if (live && t >= tlo && t < thi) {
-                const int j = li / 4, q = li % 4;
-                reinterpret_cast<uint32_t *>(out)[t * 4 * W + q * W + j] = kc;
-                stage[t * ROW + li] = vc;
-                if (q == 0) {
-                    reinterpret_cast<__half *>(out + ks_off(W))[(2 * (t & 7) + (t >> 3)) * W + j] = ks;
-                    reinterpret_cast<__half *>(out + vs_off(W))[4 * (((t & 7) >> 1) * W + j) +
-                                                                2 * (t >> 3) + (t & 1)] = vs;
+            if (a.norm_k)
+                norm_rows<W, FULL, 1>(x, [&](int k) { return load_weights(a, a.kw, li + k * L::half); }, a);
+            if (a.R) {
+                Angles angles;
+                if (on) {
+                    const int64_t row = t0 + (tb + t - len);
+                    const int64_t pos = a.positions ? (int64_t)a.positions[a.S ? b * a.S + row : row] : tb + t;
+                    load_angles<FULL>(angles, a, place, pos);
                 }
-                if (a.bounds) {
-                    const float s = __half2float(ks);
-                    const float2 z[4] = {__fmul2_rn(x.e[0], pair(s, s)), __fmul2_rn(x.e[1], pair(s, s)),
-                                         __fmul2_rn(x.o[0], pair(s, s)), __fmul2_rn(x.o[1], pair(s, s))};
+                rotate_row<W, FULL>(x[0], angles, place, a);
+            }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        mn[i] = pair(fminf(mn[i].x, z[i].x), fminf(mn[i].y, z[i].y));
-                        mx[i] = pair(fmaxf(mx[i].x, z[i].x), fmaxf(mx[i].y, z[i].y));
+            for (int k = 0; k < CH; k++) {
+                __half ks, vs;
+                const uint32_t kc = quantise(x[0][k], ks), vc = quantise(y[k], vs);
+                if (on) {
+                    const int ci = li + k * L::half, j = ci / 4, q = ci % 4;
+                    reinterpret_cast<uint32_t *>(out)[t * 4 * W + q * W + j] = kc;
+                    stage[t * ROW + ci] = vc;
+                    if (q == 0) {
+                        reinterpret_cast<__half *>(out + ks_off(W))[(2 * (t & 7) + (t >> 3)) * W + j] = ks;
+                        reinterpret_cast<__half *>(out + vs_off(W))[4 * (((t & 7) >> 1) * W + j) +
+                                                                    2 * (t >> 3) + (t & 1)] = vs;
+                    }
+                    if (a.bounds) {
+                        const float s = __half2float(ks);
+                        const Row &u = x[0][k];
+                        const float2 z[4] = {__fmul2_rn(u.e[0], pair(s, s)), __fmul2_rn(u.e[1], pair(s, s)),
+                                             __fmul2_rn(u.o[0], pair(s, s)), __fmul2_rn(u.o[1], pair(s, s))};
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            mn[k][i] = pair(fminf(mn[k][i].x, z[i].x), fminf(mn[k][i].y, z[i].y));
+                            mx[k][i] = pair(fmaxf(mx[k][i].x, z[i].x), fmaxf(mx[k][i].y, z[i].y));
+                        }
                     }
                 }
             }
@@ -482,25 +538,28 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
     if (a.bounds) {
         // the block's tokens: over the lanes that share channels, then over the warps
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int k = 0; k < CH; k++)
 #pragma unroll
-            for (int m = LPT; m < 32; m *= 2) {
-                const float2 u = shfl2(mn[i], lane ^ m), v = shfl2(mx[i], lane ^ m);
-                mn[i] = pair(fminf(mn[i].x, u.x), fminf(mn[i].y, u.y));
-                mx[i] = pair(fmaxf(mx[i].x, v.x), fmaxf(mx[i].y, v.y));
-            }
-        }
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int m = LPT; m < 32; m *= 2) {
+                    const float2 u = shfl2(mn[k][i], lane ^ m), v = shfl2(mx[k][i], lane ^ m);
+                    mn[k][i] = pair(fminf(mn[k][i].x, u.x), fminf(mn[k][i].y, u.y));
+                    mx[k][i] = pair(fmaxf(mx[k][i].x, v.x), fmaxf(mx[k][i].y, v.y));
+                }
         __syncthreads();
         float *lo_s = reinterpret_cast<float *>(smem), *hi_s = lo_s + warps * D;
         if (g == 0 && live) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {  // channels 0 2, 4 6, 1 3, 5 7
-                const int d = warp * D + li * 8 + (i & 1) * 4 + (i >> 1);
-                lo_s[d] = mn[i].x;
-                lo_s[d + 2] = mn[i].y;
-                hi_s[d] = mx[i].x;
-                hi_s[d + 2] = mx[i].y;
-            }
+            for (int k = 0; k < CH; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {  // channels 0 2, 4 6, 1 3, 5 7
+                    const int d = warp * D + (li + k * L::half) * 8 + (i & 1) * 4 + (i >> 1);
+                    lo_s[d] = mn[k][i].x;
+                    lo_s[d + 2] = mn[k][i].y;
+                    hi_s[d] = mx[k][i].x;
+                    hi_s[d + 2] = mx[k][i].y;
+                }
         }
         __syncthreads();
         if (warp == 0) {
@@ -543,14 +602,15 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
 
 // Query heads: one warp for some heads of a token, kQPasses rows of lanes at a time, the
 // next ones on their way while these are turned.
-template <typename T>
-constexpr int kQPasses = sizeof(T) == 4 ? 2 : 4;
+template <typename T, bool FULL>
+constexpr int kQPasses = (sizeof(T) == 4 ? 2 : 4) / (FULL ? 2 : 1);
 
-template <typename T, int W, int LPT>
+template <typename T, int W, bool FULL>
 __device__ __forceinline__ void turn_queries(const AppendArgs &a) {
-    constexpr int D = 32 * W, TPP = 32 / LPT, N = kQPasses<T>;
-    const int lane = threadIdx.x & 31, g = lane / LPT, li = lane % LPT;
-    const bool live = li * 8 < D;
+    using L = Lay<W, FULL>;
+    constexpr int CH = L::CH, TPP = L::TPP, N = kQPasses<T, FULL>;
+    const int lane = threadIdx.x & 31, g = lane / L::LPT, li = lane % L::LPT;
+    const bool live = li < L::half;
     const int64_t unit = ((int64_t)blockIdx.x - (int64_t)a.slots * a.Hk) * (blockDim.x >> 5) +
                          (threadIdx.x >> 5);
     const int64_t t = (uint32_t)unit / (uint32_t)a.q_units;
@@ -568,41 +628,54 @@ __device__ __forceinline__ void turn_queries(const AppendArgs &a) {
     }
     const T *q = static_cast<const T *>(a.q) + (a.S ? b * a.q_sb : 0) + row * a.q_ss + li * 8;
     T *qo = static_cast<T *>(a.qo) + (a.S ? b * a.qo_sb : 0) + row * a.qo_ss + li * 8;
-    Raw<T> raw[N];
+    Raw<T> raw[N][CH];
     auto load = [&](int h0) {
 #pragma unroll
         for (int p = 0; p < N; p++)
-            raw[p] = live && h0 + p * TPP < end ? load_raw(q + (h0 + p * TPP) * a.q_sh, a.vec & 1) : zero_raw<T>();
+#pragma unroll
+            for (int k = 0; k < CH; k++)
+                raw[p][k] = live && h0 + p * TPP < end
+                                ? load_raw(q + (h0 + p * TPP) * a.q_sh + k * L::half * 8, a.vec & 1)
+                                : zero_raw<T>();
     };
     load(h);
-    const Place place = place_of<LPT>(a, lane);
-    const Row w = load_weights(a, a.norm_q ? a.qw : nullptr, li);
+    const Place place = place_of<W, FULL>(a, lane);
+    Row w[CH];
     Angles angles;
+    int64_t pos = 0;
     if (a.R)
-        load_angles(angles, a, place,
-                    a.positions ? (int64_t)a.positions[t]
-                                : (int64_t)max(0, a.lengths[b]) + (a.S ? row : t - a.cu[b]));
-    for (; h - g < end; h += N * TPP) {
-        Row x[N];
+        pos = a.positions ? (int64_t)a.positions[t]
+                          : (int64_t)max(0, a.lengths[b]) + (a.S ? row : t - a.cu[b]);
 #pragma unroll
-        for (int p = 0; p < N; p++) x[p] = widen(raw[p]);
+    for (int k = 0; k < CH; k++) w[k] = load_weights(a, a.norm_q ? a.qw : nullptr, li + k * L::half);
+    if (a.R && live) load_angles<FULL>(angles, a, place, pos);
+    for (; h - g < end; h += N * TPP) {
+        Row x[N][CH];
+#pragma unroll
+        for (int p = 0; p < N; p++)
+#pragma unroll
+            for (int k = 0; k < CH; k++) x[p][k] = widen(raw[p][k]);
         if (h - g + N * TPP < end) load(h + N * TPP);
-        if (a.norm_q) norm_rows<LPT, N>(x, w, a);
+        if (a.norm_q) norm_rows<W, FULL, N>(x, [&](int k) { return w[k]; }, a);
 #pragma unroll
         for (int p = 0; p < N; p++) {
-            if (a.R) rotate_row(x[p], angles, place, a);
-            if (live && h + p * TPP < end) store_row(qo + (h + p * TPP) * a.qo_sh, a.vec & 2, x[p]);
+            if (a.R) rotate_row<W, FULL>(x[p], angles, place, a);
+            if (live && h + p * TPP < end) {
+#pragma unroll
+                for (int k = 0; k < CH; k++)
+                    store_row(qo + (h + p * TPP) * a.qo_sh + k * L::half * 8, a.vec & 2, x[p][k]);
+            }
         }
     }
 }
 
-template <typename T, int W, int LPT>
+template <typename T, int W, bool FULL>
 __global__ void __launch_bounds__(256, 2) append_kernel(const __grid_constant__ AppendArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     if ((int64_t)blockIdx.x < (int64_t)a.slots * a.Hk)
-        write_page<T, W, LPT>(a, smem);
+        write_page<T, W, FULL>(a, smem);
     else
-        turn_queries<T, W, LPT>(a);
+        turn_queries<T, W, FULL>(a);
 }
 
 // ------------------------------------------------------------------------ read
@@ -774,22 +847,29 @@ extern "C" int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t 
     return by_dtype(dtype, [&](auto t) {
         return by_head_dim(D, [&](auto w) {
             using E = decltype(t);
-            constexpr int W = decltype(w)::value, LPT = lanes_per_head(W);
+            constexpr int W = decltype(w)::value;
             a.slots = (int)slots;
-            // heads of a query warp: all of a token's where there are tokens enough for
-            // 32 warps an SM, else fewer, down to one load's worth
-            constexpr int per = kQPasses<E> * (32 / LPT);
-            const int64_t loads = (Hq + per - 1) / per, want = (32 * (int64_t)num_sms() + T - 1) / T;
-            a.q_heads = (int)(per * ((loads + want - 1) / want));
-            a.q_units = a.q_heads ? (int)((Hq + a.q_heads - 1) / a.q_heads) : 0;
-            const int64_t blocks = slots * Hk + (T * a.q_units + warps - 1) / warps;
-            if (slots * Hk > 0x7fffffff || blocks * warps > 0x7fffffff) {
-                set_error("kv4_append: too many tokens for one call");
-                return FC_ENOTSUP;
+            auto launch = [&](auto full) {
+                constexpr bool FULL = decltype(full)::value;
+                // heads of a query warp: all of a token's where there are tokens enough for
+                // 32 warps an SM, else fewer, down to one load's worth
+                constexpr int per = kQPasses<E, FULL> * Lay<W, FULL>::TPP;
+                const int64_t loads = (Hq + per - 1) / per, want = (32 * (int64_t)num_sms() + T - 1) / T;
+                a.q_heads = (int)(per * ((loads + want - 1) / want));
+                a.q_units = a.q_heads ? (int)((Hq + a.q_heads - 1) / a.q_heads) : 0;
+                const int64_t blocks = slots * Hk + (T * a.q_units + warps - 1) / warps;
+                if (slots * Hk > 0x7fffffff || blocks * warps > 0x7fffffff) {
+                    set_error("kv4_append: too many tokens for one call");
+                    return FC_ENOTSUP;
+                }
+                const size_t stage = (size_t)warps * 16 * (4 * W + 4) * 4, red = (size_t)warps * 32 * W * 8;
+                append_kernel<E, W, FULL><<<(unsigned)blocks, warps * 32, stage > red ? stage : red, st>>>(a);
+                return check_launch("kv4_append");
+            };
+            if constexpr (can_be_full(W)) {
+                if (a.R == D && !interleaved) return launch(std::true_type());
             }
-            const size_t stage = (size_t)warps * 16 * (4 * W + 4) * 4, red = (size_t)warps * 32 * W * 8;
-            append_kernel<E, W, LPT><<<(unsigned)blocks, warps * 32, stage > red ? stage : red, st>>>(a);
-            return check_launch("kv4_append");
+            return launch(std::false_type());
         });
     });
 }

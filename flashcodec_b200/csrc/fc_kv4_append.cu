@@ -143,7 +143,7 @@ struct AppendArgs {
     Table table;
     signed char *bounds;
     int *exps;
-    int vec;                         // 1 q, 2 q_out, 4 k, 8 v: rows on 16-byte boundaries
+    int vec;                         // 1 q, 2 q_out, 4 k, 8 v, 16 weights: rows on 16-byte boundaries
     int slots;                       // page slots; blocks < slots * Hk write the cache
     int q_units, q_heads;            // warps of a token, heads of each
 };
@@ -171,11 +171,20 @@ __device__ __forceinline__ Place place_of(const AppendArgs &a, int lane) {
     return p;
 }
 
+// Norm weights of chunk ci.
 __device__ __forceinline__ Row load_weights(const AppendArgs &a, const void *w, int ci) {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = w && ci * 8 < a.D ? load_as_f32(w, ci * 8 + i, a.w_dtype) : 0.f;
     return Row{{pair(x[0], x[2]), pair(x[4], x[6])}, {pair(x[1], x[3]), pair(x[5], x[7])}};
+}
+
+// ... in every pass: those of the tokens' own type come in whole words.
+template <typename T>
+__device__ __forceinline__ Row load_weights_again(const AppendArgs &a, const void *w, int ci) {
+    if (a.w_dtype == Elem<T>::code && ci * 8 < a.D)
+        return widen(load_raw(static_cast<const T *>(w) + ci * 8, a.vec & 16));
+    return load_weights(a, w, ci);
 }
 
 template <bool FULL>
@@ -327,10 +336,16 @@ __device__ __forceinline__ float rcp_fast(float x) {
 
 // Codes of a lane's 8 channels, left in x as whole numbers, and the scale of their group,
 // which 4 lanes share; returns the word of the K layout: channel i in nibble
-// (i >> 1) + 4 (i & 1).  x / scale is taken as a product with 1 / scale, rounded by adding
-// 1.5 * 2^23; where that lies within 1e-5 of a half (its error is under 2e-6), or past 7
-// (scales at either end of fp16's range), divisions decide, so that the codes are those of
-// clamp(rint(x / scale), -7, 7).
+// (i >> 1) + 4 (i & 1).
+//
+// The code is rint(x / scale) of the rounded quotient.  Halves are common (a bf16 input and
+// an fp16 scale have few bits: 1 in 700 quotients is one), so the quotient has to be right
+// there: t = x * inv, inv about 1 / scale, is off by 2^-22; one Newton step for t * scale = x
+// adds (x - t * scale) * inv, whose residual is exact, and leaves 2^-44, so that a half comes
+// out as itself.  No other quotient comes out as a half: (c + 1/2) * scale has at most 15
+// bits, its fp32 neighbours x differ from it by an ulp, and their quotients from the half by
+// more than half an ulp times 1 + 2^-11.  Scales at either end of fp16's range, where codes
+// would pass 7, and groups that are no numbers go the long way.
 __device__ __forceinline__ uint32_t quantise(Row &x, __half &scale) {
     float top = max_nan(max_nan(fabsf(x.e[0].x), fabsf(x.e[0].y)), max_nan(fabsf(x.e[1].x), fabsf(x.e[1].y)));
     top = max_nan(top, max_nan(max_nan(fabsf(x.o[0].x), fabsf(x.o[0].y)), max_nan(fabsf(x.o[1].x), fabsf(x.o[1].y))));
@@ -343,16 +358,13 @@ __device__ __forceinline__ uint32_t quantise(Row &x, __half &scale) {
     float2 y[4];
     const float2 inv2 = pair(inv, inv), up = pair(12582912.f, 12582912.f), down = pair(-12582912.f, -12582912.f);
     float2 *const z[4] = {&x.e[0], &x.e[1], &x.o[0], &x.o[1]};
-    float off = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float2 t = __fmul2_rn(*z[i], inv2);
-        const float2 n = __fadd2_rn(__fadd2_rn(t, up), down);
-        const float2 d = __fadd2_rn(t, pair(-n.x, -n.y));
-        off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
-        y[i] = n;
+        float2 t = __fmul2_rn(*z[i], inv2);
+        t = __ffma2_rn(__ffma2_rn(pair(-t.x, -t.y), pair(s, s), *z[i]), inv2, t);
+        y[i] = __fadd2_rn(__fadd2_rn(t, up), down);  // to the nearest whole number, halves to even
     }
-    if (off > 0.5f - 1e-5f || !(top * inv <= 7.4f)) {
+    if (!(top * inv <= 7.4f)) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             y[i].x = bad ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(z[i]->x, s)), -7.f), 7.f);
@@ -436,6 +448,7 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
     const int64_t record = (int64_t)id * a.Hk + h;
     unsigned char *tiles = a.pool + record * (P / 16) * tile_bytes(W);
     const bool older = lo > base;
+    const int e0 = a.bounds && older ? a.exps[record] : -40;
     float2 mn[CH][4], mx[CH][4];
 #pragma unroll
     for (int k = 0; k < CH; k++)
@@ -466,7 +479,7 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
             else if (tile + warps < P / 16 && tb + 16 * warps < hi)
                 load(tb + 16 * warps, 0);
             if (a.norm_k)
-                norm_rows<W, FULL, 1>(x, [&](int k) { return load_weights(a, a.kw, li + k * L::half); }, a);
+                norm_rows<W, FULL, 1>(x, [&](int k) { return load_weights_again<T>(a, a.kw, li + k * L::half); }, a);
             if (a.R) {
                 Angles angles;
                 if (on) {
@@ -563,7 +576,6 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
         }
         __syncthreads();
         if (warp == 0) {
-            const int e0 = older ? a.exps[record] : -40;
             signed char *out = a.bounds + record * 2 * D;
             float u[W], v[W], top = 0.f;
             int o0[W], o1[W];
@@ -840,7 +852,8 @@ extern "C" int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t 
     a.vec = (Hq && rows_aligned(q, dtype, q_sb, q_ss, q_sh) ? 1 : 0) |
             (Hq && rows_aligned(q_out, dtype, qo_sb, qo_ss, qo_sh) ? 2 : 0) |
             (rows_aligned(k, dtype, k_sb, k_ss, k_sh) ? 4 : 0) |
-            (rows_aligned(v, dtype, v_sb, v_ss, v_sh) ? 8 : 0);
+            (rows_aligned(v, dtype, v_sb, v_ss, v_sh) ? 8 : 0) |
+            (aligned(q_weight, 16) && aligned(k_weight, 16) ? 16 : 0);
     const int64_t slots = a.S ? B * ((S + 2 * page_size - 2) / page_size) : T / page_size + 2 * B;
     const int warps = (int)(page_size / 16 < 8 ? page_size / 16 : 8);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -130,6 +130,12 @@ __device__ __forceinline__ int warp_find(F key, int n, int64_t x) {
 }
 
 // ------------------------------------------------------------------ host side
+// Workspaces begin with a header and arrival counters for this many (sequence, head, ..)
+// units, whatever a call's sizes: what a call writes behind them is never a later call's
+// counters.
+constexpr int64_t kMaxUnits = 1 << 18;
+constexpr int64_t kCounterBytes = 256 + kMaxUnits * 4;
+
 template <typename F>
 int by_head_dim(int64_t D, F f) {
     switch (D) {

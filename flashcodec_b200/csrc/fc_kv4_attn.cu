@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
     }
 }
 
-constexpr int kMaxBlocksPerSm = 8;
+constexpr int kMaxBlocksPerSm = 4;
 
 // Blocks of a wave: what of the kernel fits on the device.
 template <int W, int NT, int LIMBS, bool RUNS>
@@ -944,8 +944,6 @@ int wave() {
     return cache[dev];
 }
 
-int64_t counter_bytes(int64_t units) { return 256 + (units * 4 + 255) / 256 * 256; }
-
 }  // namespace
 }  // namespace kv4
 }  // namespace fc
@@ -954,11 +952,8 @@ using namespace fc;
 using namespace fc::kv4;
 
 extern "C" size_t fc_kv4_attn_workspace_size(int64_t B, int64_t Sq, int64_t Hq, int64_t Hk, int64_t D) {
-    if (B <= 0 || Sq <= 0 || Hk <= 0 || Hq < Hk) return 256;
-    const int64_t rows = Sq * (Hq / Hk);
-    // the smaller of the row blocks the kernels use holds 4 rows; 16 rows are the largest
-    return (size_t)(counter_bytes(B * Hk * ((rows + 3) / 4)) +
-                    (int64_t)num_sms() * kMaxBlocksPerSm * 2 * 16 * (D + 2) * 4);
+    // 16 rows are the largest row block; two parts of a block
+    return (size_t)(kCounterBytes + (int64_t)num_sms() * kMaxBlocksPerSm * 2 * 16 * (D + 2) * 4);
 }
 
 extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int64_t Hq, int64_t q_sb,
@@ -1003,7 +998,7 @@ extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int6
     const int nt = rows * limbs > 8 ? 2 : 1;
     const int rpc = 8 * nt / limbs;
     const int64_t row_blocks = (rows + rpc - 1) / rpc;
-    if (B * Hk * row_blocks > 0x7fffffff) { set_error("kv4_attn: too many rows"); return FC_ENOTSUP; }
+    if (B * Hk * row_blocks > kMaxUnits) { set_error("kv4_attn: too many rows"); return FC_ENOTSUP; }
     char *ws = static_cast<char *>(workspace);
     AttnArgs a{};
     a.q = q; a.q_sb = q_sb; a.q_ss = q_ss; a.q_sh = q_sh;
@@ -1019,7 +1014,7 @@ extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int6
     a.sign = s < 0.f ? -1.f : 1.f;
     a.out = out; a.o_sb = o_sb; a.o_ss = o_ss; a.o_sh = o_sh; a.lse = lse;
     a.counters = reinterpret_cast<int *>(ws + 256);
-    a.parts = reinterpret_cast<float *>(ws + counter_bytes(B * Hk * ((rows + 3) / 4)));
+    a.parts = reinterpret_cast<float *>(ws + kCounterBytes);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return by_head_dim(D, [&](auto w) {
         auto launch = [&](auto n, auto lm, auto runs) {

@@ -270,8 +270,6 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     if (last_s) pick(a, keys, n, out, pick_s);
 }
 
-int64_t counter_bytes(int64_t units) { return 256 + (units * 4 + 255) / 256 * 256; }
-
 }  // namespace
 }  // namespace kv4
 }  // namespace fc
@@ -280,7 +278,7 @@ using namespace fc;
 using namespace fc::kv4;
 
 extern "C" size_t fc_kv4_select_workspace_size(int64_t B, int64_t Hk, int64_t max_pages) {
-    return (size_t)(counter_bytes(B * Hk) + B * Hk * max_pages * 4);
+    return (size_t)(kCounterBytes + B * Hk * max_pages * 4);
 }
 
 extern "C" int fc_kv4_select(const void *q, int dtype, int64_t B, int64_t Hq, int64_t q_sb, int64_t q_sh,
@@ -303,7 +301,10 @@ extern "C" int fc_kv4_select(const void *q, int dtype, int64_t B, int64_t Hq, in
         return FC_EINVAL;
     }
     if (B == 0) return FC_OK;
-    if (B > 65535) { set_error("kv4_select: more than 65535 sequences"); return FC_ENOTSUP; }
+    if (B > 65535 || B * Hk > kMaxUnits) {
+        set_error("kv4_select: more than 65535 sequences, or 2^18 of them and KV heads");
+        return FC_ENOTSUP;
+    }
     if (!q || !exponents || !lengths || !pages || !workspace || !aligned(workspace, 16)) {
         set_error("kv4_select: null pointer or misaligned workspace");
         return FC_EINVAL;
@@ -316,7 +317,7 @@ extern "C" int fc_kv4_select(const void *q, int dtype, int64_t B, int64_t Hq, in
                  Table{page_table, table_stride, (int)max_pages, (int)num_pages, ilog2(page_size), status},
                  lengths, (int)count, (int)sink, (int)recent, pages,
                  reinterpret_cast<int *>(static_cast<char *>(workspace) + 256),
-                 reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + counter_bytes(B * Hk)),
+                 reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + kCounterBytes),
                  Hq / Hk * D > 1024 ? ilog2((Hq / Hk * D + 1023) / 1024) : 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return by_head_dim(D, [&](auto w) {

@@ -442,6 +442,35 @@ def test_select_ties_zeros_and_long_tables():
     cache.check()
 
 
+def test_calls_of_different_sizes_share_a_workspace():
+    """Few long sequences, then many: what a call leaves behind is not the next one's counters."""
+    Hk, G, D, page = 4, 2, 64, 16
+    few, many = [6000, 5000], [300 + 7 * i for i in range(70)]
+    held = [filled(lens, Hk, D, page, seed=s, bounds=True) for s, lens in ((1, few), (2, many))]
+    q = [torch.randn(len(lens), Hk * G, D, generator=torch.Generator().manual_seed(4)).cuda() for lens in (few, many)]
+    first = None
+    for _ in range(2):
+        for order in ((0, 1), (1, 0)):
+            got = {}
+            for i in order:
+                (cache, table, _), lens = held[i], i32((few, many)[i])
+                pages = cache.select(q[i], table, lens, 9)
+                got[i] = (cache.attend(q[i], table, lens), pages, cache.attend(q[i], table, lens, selected=pages))
+            first = first or got
+            assert all(torch.equal(x, y) for i in (0, 1) for x, y in zip(got[i], first[i]))
+    for i, lens in enumerate((few, many)):
+        for b in range(0, len(lens), 13):
+            k, v = held[i][2][b]
+            for h in range(Hk):
+                x = q[i][b, h * G:(h + 1) * G].cpu().numpy()
+                m = -(-lens[b] // page)
+                bd = [kv4.bounds(k[p * page:(p + 1) * page, h]) for p in range(m)]
+                want = kv4.select(x, np.array([y[0] for y in bd]), [y[1] for y in bd], 9, 1, 1)
+                assert first[i][1][b, h].tolist() == want
+                o, _ = kv4.attend(x, k[:, h], v[:, h])
+                near(first[i][0][b, h * G:(h + 1) * G], o, "fp32", np.abs(v).max())
+
+
 def test_selected_in_any_order_and_out_of_range():
     Hk, G, D, page, n = 2, 2, 64, 16, 100
     cache, table, held = filled([n, 0], Hk, D, page)

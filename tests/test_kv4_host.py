@@ -177,7 +177,7 @@ def test_attn_refuses(lib, kw, rc):
     (dict(Hq=1024), 1)])
 def test_select_refuses(lib, kw, rc):
     P = ctypes.c_void_p(0x1000)
-    a = dict(q=P, dtype=1, B=2, Hq=4, bounds=P, exps=P, count=4, sink=1, recent=1, ws=P, ws_bytes=1 << 20) | kw
+    a = dict(q=P, dtype=1, B=2, Hq=4, bounds=P, exps=P, count=4, sink=1, recent=1, ws=P, ws_bytes=1 << 22) | kw
     got = lib.fc_kv4_select(a["q"], a["dtype"], a["B"], a["Hq"], 256, 64, a["bounds"], a["exps"], 8, 2, 64, 16,
                             P, 4, 4, P, a["count"], a["sink"], a["recent"], P, a["ws"], a["ws_bytes"], P, None)
     assert got == rc and lib.fc_last_error_string()

@@ -62,13 +62,13 @@ struct AttnArgs {
     float *parts;   // two per block: [row][D], then the references and the sums
 };
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 3;
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
 // What a segment costs beyond its chunks (queries, the pipeline's start, the joins), in
 // chunks of its block's 4 warps; a block's least piece is a chunk for every warp more.
 // Times in us with 0 / 8 / 16 / 32 (one column block): 16 sequences of 32768 tokens 115 /
 // 113 / 112 / 111, 61 of 1..12000 58 / 23 / 20 / 21; with two column blocks, whose joins
 // are twice as long: 24 sequences of 1..9000 with 16 rows 194 / 52 / 41 / 36.
-constexpr int overhead(int NT) { return NT == 1 ? 16 : 32; }
+constexpr int overhead(int NT, int TILES) { return (NT == 1 ? 32 : 64) / TILES; }
 constexpr float kSlack = 4.f;    // log2 of how far a score may pass the reference
 
 __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
@@ -151,9 +151,10 @@ __device__ __forceinline__ void load_words(const void *p, uint32_t w[N]) {
     }
 }
 
-template <int W, int NT, int LIMBS, bool RUNS>
+template <int W, int NT, int LIMBS, int TILES, bool RUNS>
 struct Attn {
-    static constexpr int D = 32 * W, TILE = tile_bytes(W), STAGE = 2 * TILE;
+    static constexpr int D = 32 * W, TILE = tile_bytes(W), STAGE = TILES * TILE;
+    static constexpr int kStages = TILES == 4 ? 2 : 3;
     static constexpr int RPC = 8 * NT / LIMBS;  // query rows of a block
     static constexpr int H = (W + 1) / 2;       // pairs of groups
     static constexpr bool RAW = LIMBS == 1;     // how codes become operands
@@ -162,7 +163,7 @@ struct Attn {
 
     const AttnArgs &a;
     unsigned char *ring;  // of this warp
-    int *pos_s;           // (kStages, 2) first positions of the staged tiles
+    int *pos_s;           // (kStages, TILES) first positions of the staged tiles
     int warp, lane, r, c;
     // this segment
     int b, h, rb, len, chunk0, chunk1;
@@ -184,7 +185,7 @@ struct Attn {
         r = lane >> 2;
         c = lane & 3;
         ring = smem + warp * RING;
-        pos_s = pos + warp * kStages * 2;
+        pos_s = pos + warp * kStages * TILES;
         log_tpp = a.table.log_page - 4;
     }
 
@@ -313,34 +314,35 @@ struct Attn {
     }
     static constexpr int kNowhere = 0x7fffffff - 64;  // a position past every length
 
-    // The common case: all tokens of the sequence, pages of 32 tokens and more, so that a
-    // chunk is one run of bytes.  `tile`: of the page; n: tokens of the chunk that are held.
+    // The common case: all tokens of the sequence, pages of a chunk's tokens and more, so
+    // that a chunk is one run of bytes.  `tile`: of the page; n: tokens held from there on.
     __device__ __forceinline__ void issue_run(int tile, int id, int n, int stage) const {
         constexpr int N = TILE / 16;  // 36 W pieces of a tile
         unsigned char *dst = ring + stage * STAGE + lane * 16;
         const unsigned char *s =
             base_ptr + lane * 16 + (uint64_t)(uint32_t)id * page_stride + (uint32_t)(tile * TILE);
-        if (n > 16) {
+        const int tiles = (n + 15) / 16;
+        if (tiles >= TILES) {
 #pragma unroll
-            for (int i = 0; i < (2 * N + 31) / 32; i++)
-                if (32 * i + 31 < 2 * N || lane < 2 * N - 32 * i) cp_async16(dst + 512 * i, s + 512 * i);
+            for (int i = 0; i < (TILES * N + 31) / 32; i++)
+                if (32 * i + 31 < TILES * N || lane < TILES * N - 32 * i) cp_async16(dst + 512 * i, s + 512 * i);
         } else {
-#pragma unroll
-            for (int i = 0; i < (N + 31) / 32; i++)
-                if (32 * i + 31 < N || lane < N - 32 * i) cp_async16(dst + 512 * i, s + 512 * i);
+            const int left = tiles * N - lane;
+#pragma unroll 1
+            for (int i = 0; 32 * i < left; i++) cp_async16(dst + 512 * i, s + 512 * i);
         }
     }
 
-    // Any other: lanes 0 and 1 have looked the two tiles up (`page` of the sequence, `id`).
+    // Any other: lane y has looked tile y up (`page` of the sequence, `id`).
     __device__ __forceinline__ void issue_tiles(int chunk, int page, int id, int stage) const {
         constexpr int N = TILE / 16;
-        const int tile = (2 * chunk + (lane & 1)) & ((1 << log_tpp) - 1);
+        const int tile = (TILES * chunk + lane % TILES) & ((1 << log_tpp) - 1);
         const int p = (page << a.table.log_page) + tile * 16;
         if (page < 0 || p >= len) id = -1;
-        if (lane < 2) pos_s[stage * 2 + lane] = id < 0 ? kNowhere : p;
+        if (lane < TILES) pos_s[stage * TILES + lane] = id < 0 ? kNowhere : p;
         const unsigned char *s = base_ptr + (uint64_t)(uint32_t)id * page_stride + (uint32_t)(tile * TILE);
 #pragma unroll
-        for (int y = 0; y < 2; y++) {
+        for (int y = 0; y < TILES; y++) {
             const unsigned char *z = reinterpret_cast<const unsigned char *>(
                 __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(s), y));
             if (__shfl_sync(0xffffffffu, id, y) < 0) continue;
@@ -491,12 +493,12 @@ struct Attn {
         }
     }
 
-    // Both tiles of a chunk.
+    // All tiles of a chunk.
     template <bool MASKED>
-    __device__ __forceinline__ void gather_chunk(const unsigned char *tile, const float S[2][NT][4]) {
+    __device__ __forceinline__ void gather_chunk(const unsigned char *tile, const float S[TILES][NT][4]) {
         if constexpr (RAW) {
-            gather<MASKED>(tile, S[0], acc);
-            gather<MASKED>(tile + TILE, S[1], acc);
+#pragma unroll
+            for (int t = 0; t < TILES; t++) gather<MASKED>(tile + t * TILE, S[t], acc);
         } else {
             // a chunk's sum by itself: the long sum is then in rounded fp32 additions
             float part[NT][2 * W][4];
@@ -506,8 +508,8 @@ struct Attn {
                 for (int m = 0; m < 2 * W; m++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) part[nt][m][i] = 0.f;
-            gather<MASKED>(tile, S[0], part);
-            gather<MASKED>(tile + TILE, S[1], part);
+#pragma unroll
+            for (int t = 0; t < TILES; t++) gather<MASKED>(tile + t * TILE, S[t], part);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -517,35 +519,40 @@ struct Attn {
         }
     }
 
-    // The staged chunk, whose tiles hold the positions from p0 and from p1.
-    __device__ __forceinline__ void chunk(int stage, int p0, int p1) {
+    // The staged chunk, whose tile t holds the positions from p[t].
+    __device__ __forceinline__ void chunk(int stage, const int p[TILES]) {
         unsigned char *tile = ring + stage * STAGE;
-        float S[2][NT][4];
-        score(tile, S[0]);
-        score(tile + TILE, S[1]);
-        const bool masked = max(p0, p1) + 16 > min_seen;
+        float S[TILES][NT][4];
+        int last = p[0];
+#pragma unroll
+        for (int t = 0; t < TILES; t++) {
+            score(tile + t * TILE, S[t]);
+            last = max(last, p[t]);
+        }
+        const bool masked = last + 16 > min_seen;
         if (masked) {
-            mask(tile, p0, S[0]);
-            mask(tile + TILE, p1, S[1]);
+#pragma unroll
+            for (int t = 0; t < TILES; t++) mask(tile + t * TILE, p[t], S[t]);
             __syncwarp();
         }
         // does a score pass its reference, or a scale of the values the running bound?
-        uint32_t sv[W];
-        const int half = lane >> 4;
+        // (this lane's share of the scales: TILES W / 2 of a tile)
+        constexpr int SH = TILES * W / 2, LT = 32 / TILES;
+        uint32_t sv[(SH + 1) / 2];
         {
-            const unsigned char *p = tile + half * TILE + vs_off(W) + (lane & 15) * 2 * W;
-            if constexpr (W % 2 == 0) {
-                load_words<W / 2>(p, sv);
+            const unsigned char *q = tile + lane / LT * TILE + vs_off(W) + lane % LT * 2 * SH;
+            if constexpr (SH % 2 == 0) {
+                load_words<SH / 2>(q, sv);
             } else {
 #pragma unroll
-                for (int i = 0; i < (W + 1) / 2; i++)  // 2 W bytes: W halves, the last word overlaps
-                    sv[i] = reinterpret_cast<const uint16_t *>(p)[2 * i] |
-                            (uint32_t)reinterpret_cast<const uint16_t *>(p)[min(2 * i + 1, W - 1)] << 16;
+                for (int i = 0; i < (SH + 1) / 2; i++)  // an odd number: the last word holds one twice
+                    sv[i] = reinterpret_cast<const uint16_t *>(q)[2 * i] |
+                            (uint32_t)reinterpret_cast<const uint16_t *>(q)[min(2 * i + 1, SH - 1)] << 16;
             }
         }
         __half2 st = h2(sv[0]);
 #pragma unroll
-        for (int i = 1; i < (W + 1) / 2; i++) st = __hmax2(st, h2(sv[i]));
+        for (int i = 1; i < (SH + 1) / 2; i++) st = __hmax2(st, h2(sv[i]));
         const float sm = __half2float(__hmax(__low2half(st), __high2half(st)));
         bool pass = sm > slim;
         float top[NT][2];
@@ -553,7 +560,9 @@ struct Attn {
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int y = 0; y < 2; y++) {
-                top[nt][y] = fmaxf(fmaxf(S[0][nt][y], S[0][nt][y + 2]), fmaxf(S[1][nt][y], S[1][nt][y + 2]));
+                top[nt][y] = fmaxf(S[0][nt][y], S[0][nt][y + 2]);
+#pragma unroll
+                for (int t = 1; t < TILES; t++) top[nt][y] = fmaxf(top[nt][y], fmaxf(S[t][nt][y], S[t][nt][y + 2]));
                 pass = pass || fmaf(top[nt][y], f[nt][y], -M[nt][y]) > lim;
             }
         if (__any_sync(0xffffffffu, pass)) {
@@ -591,7 +600,7 @@ struct Attn {
                 }
         }
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+        for (int t = 0; t < TILES; t++)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -612,8 +621,8 @@ struct Attn {
             gather_chunk<false>(tile, S);
     }
 
-    // This warp's chunks of the segment: chunk0 + warp, + 4, ..., each copied two rounds
-    // before it is used.
+    // This warp's chunks of the segment: chunk0 + warp, + 4, ..., each copied
+    // kStages - 1 rounds before it is used.
     __device__ __forceinline__ void run() {
         pages = (len + (1 << a.table.log_page) - 1) >> a.table.log_page;
         base_ptr = a.pool + ((int64_t)h << log_tpp) * TILE;
@@ -649,7 +658,8 @@ struct Attn {
     __device__ __forceinline__ void run_pages() {
         // lane i holds the page of the chunk i rounds into a window of 32 rounds; the
         // window after it is on its way
-        const int shift = log_tpp - 1;
+        constexpr int LOG = TILES == 4 ? 2 : 1;
+        const int shift = log_tpp - LOG;
         int next = chunk0 + warp, round = 0;
         auto window = [&](int first) {
             const int chunk = first + kWarps * lane;
@@ -659,7 +669,7 @@ struct Attn {
         rounds(
             [&](int stage) {
                 const int id = __shfl_sync(0xffffffffu, ids, round);
-                issue_run(2 * (next & ((1 << shift) - 1)), id, len - 32 * next, stage);
+                issue_run((next & ((1 << shift) - 1)) << LOG, id, len - 16 * TILES * next, stage);
                 next += kWarps;
                 if (++round == 32) {
                     round = 0;
@@ -667,26 +677,36 @@ struct Attn {
                     ids2 = window(next + 32 * kWarps);
                 }
             },
-            [&](int i, int stage) { chunk(stage, 32 * i, 32 * i + 16); });
+            [&](int i, int stage) {
+                int p[TILES];
+#pragma unroll
+                for (int t = 0; t < TILES; t++) p[t] = 16 * (TILES * i + t);
+                chunk(stage, p);
+            });
     }
 
     __device__ __forceinline__ void run_tiles() {
-        const int odd = lane & 1;
+        const int y = lane % TILES;
         int next = chunk0 + warp;  // the next chunk to copy
-        int page = next < chunk1 ? logical(2 * next + odd) : -1;
+        int page = next < chunk1 ? logical(TILES * next + y) : -1;
         int id = physical(page);
-        int page2 = next + kWarps < chunk1 ? logical(2 * (next + kWarps) + odd) : -1;
+        int page2 = next + kWarps < chunk1 ? logical(TILES * (next + kWarps) + y) : -1;
         rounds(
             [&](int stage) {
                 issue_tiles(next, page, id, stage);
                 next += kWarps;
                 page = page2;
                 id = physical(page);
-                page2 = next + kWarps < chunk1 ? logical(2 * (next + kWarps) + odd) : -1;
+                page2 = next + kWarps < chunk1 ? logical(TILES * (next + kWarps) + y) : -1;
             },
             [&](int, int stage) {
-                const int p0 = pos_s[stage * 2], p1 = pos_s[stage * 2 + 1];
-                if (p0 < len || p1 < len) chunk(stage, p0, p1);
+                int p[TILES], least = kNowhere;
+#pragma unroll
+                for (int t = 0; t < TILES; t++) {
+                    p[t] = pos_s[stage * TILES + t];
+                    least = min(least, p[t]);
+                }
+                if (least < len) chunk(stage, p);
             });
     }
 
@@ -808,24 +828,25 @@ struct Attn {
 };
 
 // Chunks of sequence b, 0 where it holds nothing.
+template <int TILES>
 __device__ __forceinline__ int chunks_of(const AttnArgs &a, int64_t b) {
     const int len = a.table.length(a.lengths[b]);
     if (len <= 0) return 0;
-    if (a.selected) return ((a.n_selected << (a.table.log_page - 4)) + 1) / 2;
-    return (len + 31) / 32;
+    if (a.selected) return ((a.n_selected << (a.table.log_page - 4)) + TILES - 1) / TILES;
+    return (len + 16 * TILES - 1) / (16 * TILES);
 }
 
 // The line: unit (sequence, KV head, row block) u of n > 0 chunks is n + OVERHEAD
 // long, the first OVERHEAD standing for what a segment costs beyond its chunks.
 // Block i of `blocks` has the piece [U i / blocks, U (i + 1) / blocks).
-template <int W, int NT, int LIMBS, bool RUNS>
+template <int W, int NT, int LIMBS, int TILES, bool RUNS>
 __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kernel(const __grid_constant__ AttnArgs a) {
-    using A = Attn<W, NT, LIMBS, RUNS>;
-    constexpr int OVERHEAD = overhead(NT), MIN_PIECE = OVERHEAD + kWarps;
+    using A = Attn<W, NT, LIMBS, TILES, RUNS>;
+    constexpr int OVERHEAD = overhead(NT, TILES), MIN_PIECE = OVERHEAD + kWarps;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int64_t sums[kWarps], pre_s;
     __shared__ int b_s, first_s, last_s;
-    __shared__ int pos[kWarps * kStages * 2];
+    __shared__ int pos[kWarps * A::kStages * TILES];
     __shared__ float ml[kWarps * A::RPC * 2];
 
     const int HR = a.Hk * a.row_blocks;
@@ -833,7 +854,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
     const int b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
     int64_t mine = 0;
     for (int b = b0; b < b1; b++) {
-        const int n = chunks_of(a, b);
+        const int n = chunks_of<TILES>(a, b);
         mine += n ? n + OVERHEAD : 0;
     }
     int64_t upto = mine;
@@ -844,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
     }
     if ((threadIdx.x & 31) == 31) sums[threadIdx.x >> 5] = upto;
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {  // nothing held: zeros
-        if (chunks_of(a, b)) continue;
+        if (chunks_of<TILES>(a, b)) continue;
         for (int i = threadIdx.x; i < a.Sq * a.Hq * A::D; i += kThreads) {
             const int row = i / A::D, s = row / a.Hq;
             store_from_f32(a.out, b * a.o_sb + s * a.o_ss + (row - s * a.Hq) * a.o_sh + i % A::D, a.dtype, 0.f);
@@ -868,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
         int64_t at = before * HR;
         int b = b0;
         for (;; b++) {
-            const int n = chunks_of(a, b);
+            const int n = chunks_of<TILES>(a, b);
             const int64_t w = n ? (int64_t)(n + OVERHEAD) * HR : 0;
             if (x < at + w) break;
             at += w;
@@ -879,7 +900,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
     __syncthreads();
     int b = b_s;
     int64_t base = pre_s;  // where the line of sequence b begins
-    int n = chunks_of(a, b);
+    int n = chunks_of<TILES>(a, b);
     int64_t unit = (x - base) / (n + OVERHEAD);
 
     A t(a, smem, pos);
@@ -918,7 +939,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
         if (++unit == HR) {
             unit = 0;
             base = u1;
-            if (x < end) do { n = chunks_of(a, ++b); } while (n == 0);
+            if (x < end) do { n = chunks_of<TILES>(a, ++b); } while (n == 0);
         }
     }
 }
@@ -926,17 +947,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
 constexpr int kMaxBlocksPerSm = 4;
 
 // Blocks of a wave: what of the kernel fits on the device.
-template <int W, int NT, int LIMBS, bool RUNS>
+template <int W, int NT, int LIMBS, int TILES, bool RUNS>
 int wave() {
     static int cache[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
     if (cache[dev] == 0) {
-        constexpr int smem = Attn<W, NT, LIMBS, RUNS>::SMEM;
+        constexpr int smem = Attn<W, NT, LIMBS, TILES, RUNS>::SMEM;
         int n = 0;
-        if (cudaFuncSetAttribute(attn_kernel<W, NT, LIMBS, RUNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+        if (cudaFuncSetAttribute(attn_kernel<W, NT, LIMBS, TILES, RUNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
                 cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_kernel<W, NT, LIMBS, RUNS>, kThreads, smem) !=
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_kernel<W, NT, LIMBS, TILES, RUNS>, kThreads, smem) !=
                 cudaSuccess || n < 1)
             return 0;
         cache[dev] = num_sms() * (n < kMaxBlocksPerSm ? n : kMaxBlocksPerSm);
@@ -1017,20 +1038,27 @@ extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int6
     a.parts = reinterpret_cast<float *>(ws + kCounterBytes);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return by_head_dim(D, [&](auto w) {
-        auto launch = [&](auto n, auto lm, auto runs) {
-            constexpr int W = decltype(w)::value, NT = decltype(n)::value, L = decltype(lm)::value;
+        constexpr int W = decltype(w)::value;
+        using std::integral_constant;
+        auto launch = [&](auto n, auto lm, auto tiles, auto runs) {
+            constexpr int NT = decltype(n)::value, L = decltype(lm)::value, T = decltype(tiles)::value;
             constexpr bool R = decltype(runs)::value;
-            const int blocks = wave<W, NT, L, R>();
+            const int blocks = wave<W, NT, L, T, R>();
             if (!blocks) { set_error("kv4_attn: the kernel does not fit this device"); return FC_ECUDA; }
-            attn_kernel<W, NT, L, R><<<blocks, kThreads, Attn<W, NT, L, R>::SMEM, st>>>(a);
+            attn_kernel<W, NT, L, T, R><<<blocks, kThreads, Attn<W, NT, L, T, R>::SMEM, st>>>(a);
             return check_launch("kv4_attn");
         };
-        using I1 = std::integral_constant<int, 1>;
-        using I2 = std::integral_constant<int, 2>;
-        auto of_kind = [&](auto runs) {
-            if (limbs == 1) return nt == 1 ? launch(I1(), I1(), runs) : launch(I2(), I1(), runs);
-            return nt == 1 ? launch(I1(), I2(), runs) : launch(I2(), I2(), runs);
+        auto of_kind = [&](auto tiles, auto runs) {
+            integral_constant<int, 1> one;
+            integral_constant<int, 2> two;
+            if (limbs == 1) return nt == 1 ? launch(one, one, tiles, runs) : launch(two, one, tiles, runs);
+            return nt == 1 ? launch(one, two, tiles, runs) : launch(two, two, tiles, runs);
         };
-        return page_size >= 32 && !selected ? of_kind(std::true_type()) : of_kind(std::false_type());
+        // Chunks of 64 tokens where pages hold them whole and rings of them fit; of 32 else.
+        if constexpr (W <= 4) {
+            if (page_size >= 64 && !selected) return of_kind(integral_constant<int, 4>(), std::true_type());
+        }
+        return page_size >= 32 && !selected ? of_kind(integral_constant<int, 2>(), std::true_type())
+                                            : of_kind(integral_constant<int, 2>(), std::false_type());
     });
 }

@@ -827,6 +827,9 @@ struct Attn {
     }
 };
 
+// A sequence, in the sums of the line's lengths (at most 2^18 of up to 2^26).
+constexpr int64_t kOne = int64_t(1) << 44;
+
 // Chunks of sequence b, 0 where it holds nothing.
 template <int TILES>
 __device__ __forceinline__ int chunks_of(const AttnArgs &a, int64_t b) {
@@ -845,7 +848,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
     constexpr int OVERHEAD = overhead(NT, TILES), MIN_PIECE = OVERHEAD + kWarps;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int64_t sums[kWarps], pre_s;
-    __shared__ int b_s, first_s, last_s;
+    __shared__ int b_s, first_s, last_s, most[kWarps];
     __shared__ int pos[kWarps * A::kStages * TILES];
     __shared__ float ml[kWarps * A::RPC * 2];
 
@@ -853,9 +856,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
     const int per = (a.B + kThreads - 1) / kThreads;
     const int b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
     int64_t mine = 0;
+    int longest = 0;
     for (int b = b0; b < b1; b++) {
         const int n = chunks_of<TILES>(a, b);
-        mine += n ? n + OVERHEAD : 0;
+        longest = max(longest, n + OVERHEAD);
+        mine += n ? n + OVERHEAD + kOne : 0;
     }
     int64_t upto = mine;
 #pragma unroll
@@ -864,6 +869,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
         if ((threadIdx.x & 31) >= o) upto += v;
     }
     if ((threadIdx.x & 31) == 31) sums[threadIdx.x >> 5] = upto;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = longest;
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {  // nothing held: zeros
         if (chunks_of<TILES>(a, b)) continue;
         for (int i = threadIdx.x; i < a.Sq * a.Hq * A::D; i += kThreads) {
@@ -873,14 +880,20 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
         }
     }
     __syncthreads();
-    int64_t before = upto - mine, all = 0;
+    int64_t before = upto - mine, all = 0;  // lengths, and sequences from kOne on
 #pragma unroll
     for (int w = 0; w < kWarps; w++) {
         if (w < (int)(threadIdx.x >> 5)) before += sums[w];
         all += sums[w];
+        longest = max(longest, most[w]);
     }
-    const int64_t U = all * HR;
-    const int64_t blocks = min((int64_t)gridDim.x, (U + MIN_PIECE - 1) / MIN_PIECE);
+    before &= kOne - 1;
+    mine &= kOne - 1;
+    const int64_t U = (all & (kOne - 1)) * HR, units = (all / kOne) * HR;
+    int64_t blocks = min((int64_t)gridDim.x, (U + MIN_PIECE - 1) / MIN_PIECE);
+    // Equal units that are short: one block for each, no piece crossing from one to the
+    // next (one sequence of 517 tokens: 11.4 us, 12.6 across; 3 of one token: 7.6, 11.4).
+    if (units && units <= gridDim.x && longest < 2 * MIN_PIECE && U == units * longest) blocks = units;
     if ((int64_t)blockIdx.x >= blocks) return;
     int64_t x = U * blockIdx.x / blocks;
     const int64_t end = U * (blockIdx.x + 1) / blocks;

@@ -600,70 +600,52 @@ def _kv4_call(fn, what, index, args, ws=None):
         _lib.check(rc, what)
 
 
-def _token_strides(t, packed):
-    """(sequence, token, head) strides of (B, S, H, D), (B, H, D) or packed (T, H, D)."""
-    s = t.stride()
-    if len(s) == 4:
-        return s[0], s[1], s[2]
-    return (0, s[0], s[1]) if packed else (s[0], 0, s[1])
+def _code(dtype) -> int:
+    code = DTYPE_CODE.get(dtype)
+    if code is None:
+        raise ValueError(f"unsupported dtype {dtype}")
+    return code
 
 
-def kv4_append(cache, q, k, v, q_out, B, S, T, cu, table, lengths, positions, q_weight, k_weight,
-               eps, rotary, interleaved) -> None:
-    """fc_kv4_append on a PagedInt4Cache; shapes are the caller's to check."""
-    packed = cu is not None
-    w = q_weight if q_weight is not None else k_weight
+# `*_at`: addresses and strides of rows, `table`: (address, row stride, columns), as
+# PagedInt4Cache's checks make them; other integers are addresses.
+def kv4_append(cache, rows_at, dtype, B, S, T, cu, lengths, positions, w_at, w_dtype, eps, turn,
+               interleaved, table) -> None:
+    """fc_kv4_append; rows_at: q, q_out, the query heads, k and v; turn: the rotary table."""
     index = cache._index
-    qs = (None, 0, 0, 0, None, 0, 0, 0, 0) if q is None else (
-        q.data_ptr(), *_token_strides(q, packed), q_out.data_ptr(), *_token_strides(q_out, packed),
-        q.shape[-2])
-    _kv4_call(_lib.load().fc_kv4_append, "kv4_append", index, (
-        *qs, k.data_ptr(), *_token_strides(k, packed), v.data_ptr(), *_token_strides(v, packed),
-        dtype_code(k), B, S, T, None if cu is None else cu.data_ptr(), lengths.data_ptr(),
-        None if positions is None else positions.data_ptr(),
-        None if q_weight is None else q_weight.data_ptr(),
-        None if k_weight is None else k_weight.data_ptr(), 0 if w is None else dtype_code(w), eps,
-        *((None, 0, 0) if rotary is None else (rotary.data_ptr(), *rotary.shape)), interleaved,
-        *cache._pool_args, table.data_ptr(), table.stride(0), table.shape[1],
+    _kv4_call(cache._lib.fc_kv4_append, "kv4_append", index, (
+        *rows_at, _code(dtype), B, S, T, cu, lengths, positions, *w_at,
+        0 if w_dtype is None else _code(w_dtype), eps, *turn, interleaved, *cache._pool_args, *table,
         *cache._bounds_args, cache._status_ptr, _raw_stream(index)))
 
 
-def kv4_read(cache, table, starts, B, S, T, cu, k_out, v_out) -> None:
-    """fc_kv4_read into k_out and v_out (of one layout)."""
+def kv4_read(cache, table, starts, B, S, T, cu, k_out, v_out, dtype, strides) -> None:
+    """fc_kv4_read."""
     index = cache._index
-    _kv4_call(_lib.load().fc_kv4_read, "kv4_read", index, (
-        *cache._pool_args, table.data_ptr(), table.stride(0), table.shape[1],
-        None if starts is None else starts.data_ptr(), B, S, T,
-        None if cu is None else cu.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
-        dtype_code(k_out), *_token_strides(k_out, cu is not None), cache._status_ptr,
-        _raw_stream(index)))
+    _kv4_call(cache._lib.fc_kv4_read, "kv4_read", index, (
+        *cache._pool_args, *table, starts, B, S, T, cu, k_out, v_out, _code(dtype), *strides,
+        cache._status_ptr, _raw_stream(index)))
 
 
-def kv4_attn(cache, q, table, lengths, selected, scale, out, lse) -> None:
-    """fc_kv4_attn; q and out (B, Sq, Hq, D) or (B, Hq, D)."""
+def kv4_attn(cache, q_at, dtype, shape, table, lengths, selected, scale, out_at, lse) -> None:
+    """fc_kv4_attn; q of `shape` (B, Sq, Hq, D) or (B, Hq, D)."""
     index = cache._index
     stream = _raw_stream(index)
-    s = q.shape
-    B, Sq, Hq = (s[0], s[1], s[2]) if len(s) == 4 else (s[0], 1, s[1])
+    B, Sq, Hq = shape[:3] if len(shape) == 4 else (shape[0], 1, shape[1])
     # a selection of no pages is not the same as none: its address is not null
     sel = (None, 0) if selected is None else (selected.data_ptr() or cache._status_ptr,
                                               selected.shape[2])
     ws = _kv4_workspace("attn", (B, Sq, Hq, cache.num_kv_heads, cache.head_dim), index, stream)
-    _kv4_call(_lib.load().fc_kv4_attn, "kv4_attn", index, (
-        q.data_ptr(), dtype_code(q), B, Sq, Hq, *_token_strides(q, False), *cache._pool_args,
-        table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(), *sel, scale,
-        out.data_ptr(), *_token_strides(out, False), None if lse is None else lse.data_ptr(),
-        ws[1], ws[2], cache._status_ptr, stream), ws)
+    _kv4_call(cache._lib.fc_kv4_attn, "kv4_attn", index, (
+        q_at[0], _code(dtype), B, Sq, Hq, *q_at[1:], *cache._pool_args, *table, lengths, *sel, scale,
+        *out_at, None if lse is None else lse.data_ptr(), ws[1], ws[2], cache._status_ptr, stream), ws)
 
 
-def kv4_select(cache, q, table, lengths, count, sink, recent, pages) -> None:
+def kv4_select(cache, q_at, dtype, B, Hq, table, lengths, count, sink, recent, pages) -> None:
     """fc_kv4_select; q (B, Hq, D), pages (B, Hk, count) int32."""
     index = cache._index
     stream = _raw_stream(index)
-    B, Hq = q.shape[0], q.shape[1]
-    n = table.shape[1]
-    ws = _kv4_workspace("select", (B, cache.num_kv_heads, n), index, stream)
-    _kv4_call(_lib.load().fc_kv4_select, "kv4_select", index, (
-        q.data_ptr(), dtype_code(q), B, Hq, q.stride(0), q.stride(1), *cache._bounds_args,
-        *cache._pool_args[1:], table.data_ptr(), table.stride(0), n, lengths.data_ptr(), count,
-        sink, recent, pages.data_ptr(), ws[1], ws[2], cache._status_ptr, stream), ws)
+    ws = _kv4_workspace("select", (B, cache.num_kv_heads, table[2]), index, stream)
+    _kv4_call(cache._lib.fc_kv4_select, "kv4_select", index, (
+        q_at[0], _code(dtype), B, Hq, q_at[1], q_at[3], *cache._bounds_args, *cache._pool_args[1:],
+        *table, lengths, count, sink, recent, pages, ws[1], ws[2], cache._status_ptr, stream), ws)

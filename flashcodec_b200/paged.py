@@ -133,7 +133,7 @@ class PagedInt4Cache:
             self.exponents = torch.zeros(self.num_pages, self.num_kv_heads, dtype=torch.int32,
                                          device=dev)
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._index, self._scale = dev.index, self.head_dim ** -0.5
+        self._index, self._scale, self._lib = dev.index, self.head_dim ** -0.5, _lib.load()
         self._status_ptr = self.status.data_ptr()
         self._pool_args = (self.pool.data_ptr(), self.num_pages, self.num_kv_heads, self.head_dim,
                            self.page_size)
@@ -141,7 +141,9 @@ class PagedInt4Cache:
             else (None, None)
 
     # ------------------------------------------------------------ argument checks
-    def _check(self, *tensors):
+    # (a decode step calls these for every layer: each looks at a tensor's attributes once)
+    def _here(self, *tensors):
+        """Tensors (or None) on the cache's device, none asking for a gradient."""
         index, grad = self._index, torch.is_grad_enabled()
         for t in tensors:
             if t is None:
@@ -159,20 +161,29 @@ class PagedInt4Cache:
                              f"(got {t.dtype}, {tuple(t.shape)})")
 
     def _table(self, page_table):
+        """(address, row stride, columns) of a page table, and its rows."""
         s = page_table.shape
-        if page_table.dtype is not torch.int32 or len(s) != 2 or s[1] == 0 \
-                or (s[1] > 1 and page_table.stride(1) != 1):
-            raise ValueError("page_table must be an int32 (B, n) tensor with unit stride along n")
-        return s[0]
+        if page_table.dtype is not torch.int32 or len(s) != 2 or s[1] == 0:
+            raise ValueError("page_table must be an int32 (B, n) tensor")
+        st = page_table.stride()
+        if st[1] != 1 and s[1] > 1:
+            raise ValueError("page_table must have unit stride along n")
+        return s[0], (page_table.data_ptr(), st[0], s[1])
 
-    def _rows(self, name, t, dims, heads=None):
-        s = t.shape
-        if len(s) not in dims or s[-1] != self.head_dim or (heads is not None and s[-2] != heads):
-            raise ValueError(f"{name}: expected (..., {heads or 'heads'}, {self.head_dim}), got "
-                             f"{tuple(s)}")
-        if t.stride(-1) != 1:
+    def _rows(self, name, t, shape=None, packed=False, heads=None):
+        """(address, sequence, token and head strides) of (B, S, H, D), (B, H, D) or packed
+        (T, H, D) rows."""
+        s, st = t.shape, t.stride()
+        n = len(s)
+        if n not in (3, 4) or (packed and n != 3) or s[-1] != self.head_dim \
+                or (heads is not None and s[-2] != heads) or (shape is not None and s != shape):
+            want = tuple(shape) if shape is not None else (..., heads or "heads", self.head_dim)
+            raise ValueError(f"{name}: expected {want}, got {tuple(s)}")
+        if st[-1] != 1:
             raise ValueError(f"{name}: the head dim must have unit stride")
-        return s
+        if n == 4:
+            return t.data_ptr(), st[0], st[1], st[2]
+        return (t.data_ptr(), 0, st[0], st[1]) if packed else (t.data_ptr(), st[0], 0, st[1])
 
     # ----------------------------------------------------------------- operations
     def append(self, q, k, v, page_table, lengths, *, cu_seqlens=None, q_weight=None,
@@ -196,45 +207,57 @@ class PagedInt4Cache:
         Arithmetic is fp32 and rounded in a fixed order, so what is stored does
         not depend on how tokens are split into calls.
         """
-        self._check(q, k, v, page_table, lengths, cu_seqlens, q_weight, k_weight, rotary,
-                    positions, q_out)
-        B = self._table(page_table)
+        self._here(q, k, v, page_table, lengths, cu_seqlens, q_weight, k_weight, rotary, positions,
+                   q_out)
+        B, table = self._table(page_table)
         packed = cu_seqlens is not None
-        dims = (3,) if packed else (3, 4)
-        shape = self._rows("k", k, dims, self.num_kv_heads)
-        lead = shape[:-2]
-        if self._rows("v", v, dims) != shape or v.dtype is not k.dtype:
-            raise ValueError("k and v must have one shape and dtype")
+        k_at = self._rows("k", k, packed=packed, heads=self.num_kv_heads)
+        shape, dtype = k.shape, k.dtype
+        v_at = self._rows("v", v, shape, packed)
+        if v.dtype is not dtype:
+            raise ValueError("k and v must have one dtype")
+        cu = None
         if packed:
             self._ints("cu_seqlens", cu_seqlens, (B + 1,))
-            S, T = 0, lead[0]
+            S, T, cu = 0, shape[0], cu_seqlens.data_ptr()
         else:
-            S = lead[1] if len(lead) == 2 else 1
+            S = shape[1] if len(shape) == 4 else 1
             T = B * S
-            if lead[0] != B:
-                raise ValueError(f"k has {lead[0]} sequences, the page table {B}")
+            if shape[0] != B:
+                raise ValueError(f"k has {shape[0]} sequences, the page table {B}")
         self._ints("lengths", lengths, (B,))
+        q_at, heads = (None, 0, 0, 0, None, 0, 0, 0), 0
         if q is not None:
-            if self._rows("q", q, dims)[:-2] != lead or q.dtype is not k.dtype:
+            q_at, qs = self._rows("q", q, packed=packed), q.shape
+            if qs[:-2] != shape[:-2] or q.dtype is not dtype:
                 raise ValueError("q must have the tokens and the dtype of k")
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            else:
-                self._rows("q_out", q_out, dims)
-                if q_out.shape != q.shape or q_out.dtype != q.dtype:
-                    raise ValueError("q_out must have the shape and dtype of q")
-        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is not None and (w.shape != (self.head_dim,) or w.stride(0) != 1):
-                raise ValueError(f"{name} must be a contiguous ({self.head_dim},) tensor")
-        if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-            raise ValueError("q_weight and k_weight must have one dtype")
-        if rotary is not None and (rotary.dtype != torch.float32 or rotary.dim() != 2
-                                   or not rotary.is_contiguous()):
-            raise ValueError("rotary must be a contiguous fp32 (positions, R) tensor")
+            elif q_out.dtype is not dtype:
+                raise ValueError("q_out must have the dtype of q")
+            heads = qs[-2]
+            q_at += self._rows("q_out", q_out, qs, packed)
+        elif q_out is not None:
+            raise ValueError("q_out goes with q")
+        w_at, w_dtype = [None, None], None
+        for i, w in enumerate((q_weight, k_weight)):
+            if w is None:
+                continue
+            if w.shape != (self.head_dim,) or w.stride(0) != 1:
+                raise ValueError(f"norm weights must be contiguous ({self.head_dim},) tensors")
+            if w_dtype is not None and w.dtype is not w_dtype:
+                raise ValueError("q_weight and k_weight must have one dtype")
+            w_at[i], w_dtype = w.data_ptr(), w.dtype
+        turn = (None, 0, 0)
+        if rotary is not None:
+            if rotary.dtype is not torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous():
+                raise ValueError("rotary must be a contiguous fp32 (positions, R) tensor")
+            turn = (rotary.data_ptr(), *rotary.shape)
         if positions is not None:
-            self._ints("positions", positions, lead if len(lead) == positions.dim() else (T,))
-        K.kv4_append(self, q, k, v, q_out, B, S, T, cu_seqlens, page_table, lengths, positions,
-                     q_weight, k_weight, eps, rotary, bool(interleaved))
+            self._ints("positions", positions, shape[:-2] if positions.dim() == 2 else (T,))
+            positions = positions.data_ptr()
+        K.kv4_append(self, (*q_at, heads, *k_at, *v_at), dtype, B, S, T, cu, lengths.data_ptr(),
+                     positions, w_at, w_dtype, eps, turn, bool(interleaved), table)
         return q_out
 
     def attend(self, q, page_table, lengths, *, scale=None, selected=None, out=None,
@@ -251,25 +274,23 @@ class PagedInt4Cache:
         natural log of the softmax sums, q.shape[:-1] fp32.  A query that sees no
         token gives zeros (and -inf).
         """
-        self._check(q, page_table, lengths, selected, out)
-        B = self._table(page_table)
-        shape = self._rows("q", q, (3, 4))
+        self._here(q, page_table, lengths, selected, out)
+        B, table = self._table(page_table)
+        q_at, shape = self._rows("q", q), q.shape
         if shape[0] != B:
             raise ValueError(f"q has {shape[0]} sequences, the page table {B}")
         self._ints("lengths", lengths, (B,))
         if selected is not None:
-            if q.dim() == 4 and q.shape[1] != 1:
+            if len(shape) == 4 and shape[1] != 1:
                 raise ValueError("selected pages go with one query per sequence")
             self._ints("selected", selected, (B, self.num_kv_heads, selected.shape[-1]))
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        else:
-            self._rows("out", out, (3, 4))
-            if out.shape != q.shape or out.dtype != q.dtype:
-                raise ValueError("out must have the shape and dtype of q")
-        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
-        K.kv4_attn(self, q, page_table, lengths, selected,
-                   self._scale if scale is None else scale, out, lse)
+        elif out.dtype is not q.dtype:
+            raise ValueError("out must have the dtype of q")
+        lse = torch.empty(shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+        K.kv4_attn(self, q_at, q.dtype, shape, table, lengths.data_ptr(), selected,
+                   self._scale if scale is None else scale, self._rows("out", out, shape), lse)
         return (out, lse) if return_lse else out
 
     def select(self, q, page_table, lengths, count, *, sink=1, recent=1):
@@ -283,16 +304,17 @@ class PagedInt4Cache:
         """
         if self.bounds is None:
             raise ValueError("this cache keeps no page bounds (bounds=True)")
-        self._check(q, page_table, lengths)
-        B = self._table(page_table)
-        self._rows("q", q, (3,))
-        if q.shape[0] != B:
-            raise ValueError(f"q has {q.shape[0]} sequences, the page table {B}")
+        self._here(q, page_table, lengths)
+        B, table = self._table(page_table)
+        q_at, shape = self._rows("q", q), q.shape
+        if len(shape) != 3 or shape[0] != B:
+            raise ValueError(f"q must be ({B}, heads, {self.head_dim}) (got {tuple(shape)})")
         self._ints("lengths", lengths, (B,))
         if count <= 0:
             raise ValueError(f"count must be positive (got {count})")
-        pages = torch.empty(B, self.num_kv_heads, count, dtype=torch.int32, device=q.device)
-        K.kv4_select(self, q, page_table, lengths, count, sink, recent, pages)
+        pages = torch.empty((B, self.num_kv_heads, count), dtype=torch.int32, device=self.device)
+        K.kv4_select(self, q_at, q.dtype, B, shape[1], table, lengths.data_ptr(), count, sink, recent,
+                     pages.data_ptr())
         return pages
 
     def read(self, page_table, starts=None, *, count=None, cu_seqlens=None, dtype=torch.bfloat16):
@@ -300,21 +322,24 @@ class PagedInt4Cache:
         position ``starts`` ((B,) int32; None: 0) as (B, count, Hk, D), or, with
         ``cu_seqlens``, cu_seqlens[b + 1] - cu_seqlens[b] of sequence b, ``count``
         in all, packed as (count, Hk, D)."""
-        self._check(page_table, starts, cu_seqlens)
-        B = self._table(page_table)
+        self._here(page_table, starts, cu_seqlens)
+        B, table = self._table(page_table)
         if count is None or count < 0:
             raise ValueError("read needs the number of tokens (count)")
         if starts is not None:
             self._ints("starts", starts, (B,))
+            starts = starts.data_ptr()
+        H, D = self.num_kv_heads, self.head_dim
         if cu_seqlens is not None:
             self._ints("cu_seqlens", cu_seqlens, (B + 1,))
-            shape, S, T = (count,), 0, count
+            cu_seqlens = cu_seqlens.data_ptr()
+            shape, S, T = (count, H, D), 0, count
         else:
-            shape, S, T = (B, count), count, B * count
-        shape = (*shape, self.num_kv_heads, self.head_dim)
+            shape, S, T = (B, count, H, D), count, B * count
         k = torch.empty(shape, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        K.kv4_read(self, page_table, starts, B, S, T, cu_seqlens, k, v)
+        K.kv4_read(self, table, starts, B, S, T, cu_seqlens, k.data_ptr(), v.data_ptr(), dtype,
+                   (count * H * D, H * D, D))
         return k, v
 
     def check(self):

@@ -180,7 +180,7 @@ inline int check_cache(const char *what, int64_t B, int64_t Hk, int64_t D, int64
         return FC_EINVAL;
     }
     if (B < 0 || Hk <= 0 || num_pages <= 0 || max_pages <= 0 || B > (1 << 24) || Hk > 65535 ||
-        num_pages > 0x7fffffff || max_pages * page_size > 0x7fffffff) {
+        num_pages > 0x7fffffff || max_pages > 0x7fffffff || max_pages * page_size > 0x7fffff00) {
         set_error("%s: bad shape", what);
         return FC_EINVAL;
     }

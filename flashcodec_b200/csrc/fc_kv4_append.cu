@@ -819,6 +819,39 @@ __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ ReadA
     }
 }
 
+// Rows (sequence, token, head) of D elements, strides in elements.
+struct Rows {
+    const void *p;
+    int64_t sb, ss, sh, H;
+};
+
+// Whether two sets of B x S rows (packed: 1 x T) can share a byte.  Sets whose spans meet
+// are told apart where they are slices of the heads of one buffer: equal strides from token
+// to token, heads in runs that do not meet within one.
+bool rows_meet(const Rows &x, const Rows &y, int64_t B, int64_t S, int64_t D, int64_t size) {
+    auto span = [&](const Rows &r, int64_t &lo, int64_t &hi) {
+        lo = hi = 0;
+        for (int64_t e : {(B - 1) * r.sb, (S - 1) * r.ss, (r.H - 1) * r.sh}) (e < 0 ? lo : hi) += e;
+        const int64_t base = (int64_t)reinterpret_cast<uintptr_t>(r.p);
+        lo = base + lo * size;
+        hi = base + (hi + D) * size;
+    };
+    int64_t x0, x1, y0, y1;
+    span(x, x0, x1);
+    span(y, y0, y1);
+    if (x0 >= y1 || y0 >= x1) return false;
+    const int64_t step = S > 1 ? x.ss : x.sb;  // from token to token
+    const bool same = (S == 1 || x.ss == y.ss) && (B == 1 || x.sb == y.sb) &&
+                      (S == 1 || B == 1 || x.sb % (step ? step : 1) == 0);
+    if (!same || (S * B > 1 && step <= 0) || x.sh < 0 || y.sh < 0) return true;
+    const int64_t xw = ((x.H - 1) * x.sh + D) * size, yw = ((y.H - 1) * y.sh + D) * size;
+    int64_t d = (int64_t)reinterpret_cast<uintptr_t>(y.p) - (int64_t)reinterpret_cast<uintptr_t>(x.p);
+    if (S * B == 1) return d < xw && -d < yw;
+    const int64_t pitch = step * size;
+    d = (d % pitch + pitch) % pitch;
+    return d < xw || d + yw > pitch;
+}
+
 }  // namespace
 }  // namespace kv4
 }  // namespace fc
@@ -873,6 +906,17 @@ extern "C" int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t 
         }
         if (rotary_rows <= 0 || !aligned(rotary, 16)) {
             set_error("kv4_append: the rotary table must have rows and be 16-byte aligned");
+            return FC_EINVAL;
+        }
+    }
+    if (Hq) {
+        const int64_t nb = cu_seqlens ? 1 : B, ns = cu_seqlens ? T : S, size = dtype_size(dtype);
+        const Rows out{q_out, qo_sb, qo_ss, qo_sh, Hq};
+        const bool in_place = q == q_out && q_sh == qo_sh && (ns == 1 || q_ss == qo_ss) && (nb == 1 || q_sb == qo_sb);
+        if ((!in_place && rows_meet(out, Rows{q, q_sb, q_ss, q_sh, Hq}, nb, ns, D, size)) ||
+            rows_meet(out, Rows{k, k_sb, k_ss, k_sh, Hk}, nb, ns, D, size) ||
+            rows_meet(out, Rows{v, v_sb, v_ss, v_sh, Hk}, nb, ns, D, size)) {
+            set_error("kv4_append: q_out overlaps an input (it may be q itself)");
             return FC_EINVAL;
         }
     }

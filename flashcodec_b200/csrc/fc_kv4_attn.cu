@@ -873,8 +873,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
     if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = longest;
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {  // nothing held: zeros
         if (chunks_of<TILES>(a, b)) continue;
-        for (int i = threadIdx.x; i < a.Sq * a.Hq * A::D; i += kThreads) {
-            const int row = i / A::D, s = row / a.Hq;
+        for (int64_t i = threadIdx.x; i < (int64_t)a.Sq * a.Hq * A::D; i += kThreads) {
+            const int64_t row = i / A::D, s = row / a.Hq;
             store_from_f32(a.out, b * a.o_sb + s * a.o_ss + (row - s * a.Hq) * a.o_sh + i % A::D, a.dtype, 0.f);
             if (a.lse && i % A::D == 0) a.lse[(int64_t)b * a.Sq * a.Hq + row] = -INFINITY;
         }

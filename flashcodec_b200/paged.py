@@ -290,7 +290,7 @@ class PagedInt4Cache:
             raise ValueError("out must have the dtype of q")
         lse = torch.empty(shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
         K.kv4_attn(self, q_at, q.dtype, shape, table, lengths.data_ptr(), selected,
-                   self._scale if scale is None else scale, self._rows("out", out, shape), lse)
+                   self._scale if scale is None else float(scale), self._rows("out", out, shape), lse)
         return (out, lse) if return_lse else out
 
     def select(self, q, page_table, lengths, count, *, sink=1, recent=1):

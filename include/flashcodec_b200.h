@@ -579,7 +579,8 @@ FC_API int64_t fc_kv4_page_bytes(int64_t Hk, int64_t D, int64_t page_size);
  * *_sb strides are not used).  Sequence b's tokens go to positions
  * lengths[b], lengths[b] + 1, ...; a negative length skips the sequence
  * (its queries are still turned).  lengths is not changed.
- * q, q_out  (.., Hq, D) or NULL with Hq = 0.  q_out may be q.
+ * q, q_out  (.., Hq, D) or NULL with Hq = 0.  q_out may be q, but must not overlap
+ *          other inputs (slices of the heads of one buffer do not).
  * q_weight, k_weight  (D) weights of w_dtype of an RMS norm of every head, each
  *          NULL for none:  x * r * w, r = 1 / sqrt(mean(x^2) + eps).
  * rotary   (rotary_rows, rotary_dim) fp32, cosines then sines of the angles of

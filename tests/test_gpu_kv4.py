@@ -236,6 +236,26 @@ def test_values_that_are_not_numbers_stay_in_their_group():
     assert not out.isnan().any()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_values_that_are_not_numbers_do_not_reach_queries_that_do_not_see_them(dtype):
+    """The last of 4 drafted tokens is NaN in keys and values; the earlier queries never see it."""
+    Hk, G, D, page, n, Sq = 2, 2, 64, 32, 45, 4
+    cache, table, held = filled([n - 1], Hk, D, page)
+    table = torch.cat([table, table], 1)[:, :2]
+    bad = torch.full((1, Hk, D), math.nan, device="cuda")
+    cache.append(None, bad, bad, table, i32([n - 1]))
+    q = torch.randn(1, Sq, Hk * G, D, generator=torch.Generator().manual_seed(1)).to(DT[dtype])
+    q[0, 1, 0] = math.nan  # nor does a query that is no number reach its neighbours
+    out = cache.attend(q.cuda(), table, i32([n]))[0]
+    assert out[3].isnan().all() and out[1, 0].isnan().all()
+    for s in range(3):
+        for h in range(Hk):
+            rows = slice(h * G + (s == 1 and h == 0), (h + 1) * G)
+            k, v = (x[: n - Sq + 1 + s, h] for x in held[0])
+            want, _ = kv4.attend(q[0, s, rows].float().numpy(), k, v)
+            near(out[s, rows], want, dtype, np.abs(v).max(), (s, h))
+
+
 # ------------------------------------------------------------------------- attend
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("D,page,Hk,G,Sq", [
@@ -527,6 +547,7 @@ def test_refusals():
     t, n = i32([[0, 1]]), i32([0])
     x = torch.randn(1, Hk, D, device="cuda")
     q = torch.randn(1, 2 * Hk, D, device="cuda")
+    wide = torch.randn(1, 6, D, device="cuda")
     bad = [
         lambda: cache.append(q, x, x.bfloat16(), t, n),
         lambda: cache.append(q, x, x[:, :1], t, n),
@@ -543,6 +564,9 @@ def test_refusals():
         lambda: cache.append(q, x, x, t, n, cu_seqlens=i32([0])),
         lambda: cache.append(q, x, x, t, n, positions=i32([0, 1])),
         lambda: cache.append(q, x, x, t, n, q_out=x),
+        lambda: cache.append(x, x, x + 1, t, n, q_out=x),
+        lambda: cache.append(wide[:, :4], wide[:, 4:6], x, t, n, q_out=wide[:, 1:5]),
+        lambda: cache.append(q, wide[:, 4:6], x, t, n, q_out=wide[:, 1:5]),
         lambda: cache.attend(q[:, :3], t, n),
         lambda: cache.attend(q[..., :32], t, n),
         lambda: cache.attend(q, t, n, selected=i32([[[0]]])),

@@ -1027,9 +1027,13 @@ extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int6
     }
     const int64_t rows = Sq * (Hq / Hk);
     const int limbs = dtype == FC_BF16 ? 1 : 2;
-    // One column block of 8 serves up to 8 (4) rows.  More rows take two: they double
-    // the matrix instructions but share the unpacking, against reading the pages twice.
-    const int nt = rows * limbs > 8 ? 2 : 1;
+    // One column block of 8 serves up to 8 (4) rows.  More rows can take two, which double
+    // the matrix instructions but share the unpacking, against reading the pages again for
+    // the next rows.  Two need 255 registers, 8 warps an SM instead of 12, so they pay where
+    // tables are long: 16 rows, us with two / one: 16 x 32768 tokens, 8 heads 179 / 206;
+    // 24 x 1..9000 36 / 34; 4 x 4096 30 / 22.  At D = 256 they spill (8 x 8192: 62 / 35).
+    const int64_t tokens = B * Hk * (selected ? n_selected : max_pages) * page_size;
+    const int nt = rows * limbs > 8 && D <= 128 && tokens >= 1 << 21 ? 2 : 1;
     const int rpc = 8 * nt / limbs;
     const int64_t row_blocks = (rows + rpc - 1) / rpc;
     if (B * Hk * row_blocks > kMaxUnits) { set_error("kv4_attn: too many rows"); return FC_ENOTSUP; }
@@ -1064,8 +1068,10 @@ extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int6
         auto of_kind = [&](auto tiles, auto runs) {
             integral_constant<int, 1> one;
             integral_constant<int, 2> two;
-            if (limbs == 1) return nt == 1 ? launch(one, one, tiles, runs) : launch(two, one, tiles, runs);
-            return nt == 1 ? launch(one, two, tiles, runs) : launch(two, two, tiles, runs);
+            if constexpr (W <= 4) {
+                if (nt == 2) return limbs == 1 ? launch(two, one, tiles, runs) : launch(two, two, tiles, runs);
+            }
+            return limbs == 1 ? launch(one, one, tiles, runs) : launch(one, two, tiles, runs);
         };
         // Chunks of 64 tokens where pages hold them whole and rings of them fit; of 32 else.
         if constexpr (W <= 4) {

@@ -321,6 +321,27 @@ def test_attend_ranges(dtype, kscale, vscale):
     near(out[0], want, dtype, top)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,page,Hk,G,Sq", [(128, 64, 2, 16, 1), (64, 32, 4, 4, 5), (96, 16, 2, 9, 1)])
+def test_attend_many_rows_over_a_long_table(dtype, D, page, Hk, G, Sq):
+    """Tables that could hold 2^21 tokens and heads: two column blocks serve a head's rows."""
+    lens = [1, page + 3, 900]
+    cache, table, held = filled(lens, Hk, D, page, seed=D)
+    long = torch.full((3, (1 << 21) // (3 * Hk * page) + 1), -1, dtype=torch.int32, device="cuda")
+    long[:, : table.shape[1]] = table
+    q = torch.randn(3, Sq, Hk * G, D, generator=torch.Generator().manual_seed(1)).to(DT[dtype])
+    out = cache.attend(q.cuda(), long, i32(lens))
+    for b, n in enumerate(lens):
+        for s in range(Sq):
+            seen = max(0, n - (Sq - 1 - s))
+            for h in range(Hk):
+                rows = slice(h * G, (h + 1) * G)
+                k, v = (x[:seen, h] for x in held[b])
+                want, _ = kv4.attend(q[b, s, rows].float().numpy(), k, v)
+                near(out[b, s, rows], want, dtype, np.abs(v).max() if seen else 1.0, (b, s, h))
+    cache.check()
+
+
 def test_attend_scale_out_strides_and_shared_pages():
     Hk, G, D, page = 2, 2, 64, 16
     cache, table, held = filled([50], Hk, D, page)

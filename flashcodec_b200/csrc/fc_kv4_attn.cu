@@ -839,6 +839,12 @@ __device__ __forceinline__ int chunks_of(const AttnArgs &a, int64_t b) {
     return (len + 16 * TILES - 1) / (16 * TILES);
 }
 
+// Where a block is on the line.
+struct Plan {
+    int64_t U, blocks, x, end, base;  // base: where the line of sequence b begins
+    int b, n, unit;                   // n: chunks of a unit of b
+};
+
 // The line: unit (sequence, KV head, row block) u of n > 0 chunks is n + OVERHEAD
 // long, the first OVERHEAD standing for what a segment costs beyond its chunks.
 // Block i of `blocks` has the piece [U i / blocks, U (i + 1) / blocks).
@@ -847,8 +853,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
     using A = Attn<W, NT, LIMBS, TILES, RUNS>;
     constexpr int OVERHEAD = overhead(NT, TILES), MIN_PIECE = OVERHEAD + kWarps;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int64_t sums[kWarps], pre_s;
-    __shared__ int b_s, first_s, last_s, most[kWarps];
+    __shared__ int64_t sums[kWarps];
+    __shared__ Plan plan;
+    __shared__ int first_s, last_s, most[kWarps];
     __shared__ int pos[kWarps * A::kStages * TILES];
     __shared__ float ml[kWarps * A::RPC * 2];
 
@@ -895,48 +902,54 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
     // next (one sequence of 517 tokens: 11.4 us, 12.6 across; 3 of one token: 7.6, 11.4).
     if (units && units <= gridDim.x && longest < 2 * MIN_PIECE && U == units * longest) blocks = units;
     if ((int64_t)blockIdx.x >= blocks) return;
-    int64_t x = U * blockIdx.x / blocks;
-    const int64_t end = U * (blockIdx.x + 1) / blocks;
-    // the sequence that x falls in
-    if (x >= before * HR && x < (before + mine) * HR) {
+    const int64_t x0 = U * blockIdx.x / blocks;
+    // the sequence that the piece begins in
+    if (x0 >= before * HR && x0 < (before + mine) * HR) {
         int64_t at = before * HR;
-        int b = b0;
+        int b = b0, n;
         for (;; b++) {
-            const int n = chunks_of<TILES>(a, b);
+            n = chunks_of<TILES>(a, b);
             const int64_t w = n ? (int64_t)(n + OVERHEAD) * HR : 0;
-            if (x < at + w) break;
+            if (x0 < at + w) break;
             at += w;
         }
-        b_s = b;
-        pre_s = at;
+        plan.U = U;
+        plan.blocks = blocks;
+        plan.x = x0;
+        plan.end = U * (blockIdx.x + 1) / blocks;
+        plan.base = at;
+        plan.b = b;
+        plan.n = n;
+        plan.unit = (int)((x0 - at) / (n + OVERHEAD));
     }
     __syncthreads();
-    int b = b_s;
-    int64_t base = pre_s;  // where the line of sequence b begins
-    int n = chunks_of<TILES>(a, b);
-    int64_t unit = (x - base) / (n + OVERHEAD);
 
+    // (the plan stays in shared memory: its registers are the segment's)
     A t(a, smem, pos);
-    while (x < end) {
-        const int64_t u0 = base + unit * (n + OVERHEAD) + OVERHEAD, u1 = u0 + n;  // its chunks
-        t.chunk0 = (int)(max(x, u0) - u0);
-        t.chunk1 = (int)(min(end, u1) - u0);
+    while (plan.x < plan.end) {
+        auto first_chunk = [&] { return plan.base + (int64_t)plan.unit * (plan.n + OVERHEAD) + OVERHEAD; };
+        {
+            const int64_t u0 = first_chunk();
+            t.chunk0 = (int)(max(plan.x, u0) - u0);
+            t.chunk1 = (int)(min(plan.end, u0 + plan.n) - u0);
+        }
         if (t.chunk0 < t.chunk1) {
-            t.b = b;
-            t.h = (int)unit / a.row_blocks;
-            t.rb = (int)unit - t.h * a.row_blocks;
-            t.len = a.table.length(a.lengths[b]);
-            const bool whole = t.chunk0 == 0 && t.chunk1 == n;
+            t.b = plan.b;
+            t.h = plan.unit / a.row_blocks;
+            t.rb = plan.unit - t.h * a.row_blocks;
+            t.len = a.table.length(a.lengths[t.b]);
             t.run();
+            const bool whole = t.chunk0 == 0 && t.chunk1 == plan.n;
             // parts of a block: 0 of a unit that began in an earlier one, 1 of one that ends in a later one
             t.join(smem, ml, whole, a.parts + ((int64_t)blockIdx.x * 2 + (t.chunk0 == 0)) * A::PART);
             if (!whole) {
                 __syncthreads();
                 if (threadIdx.x == 0) {
                     // the blocks with chunks of this unit: i0 (its first chunk) to i1
-                    const int64_t i0 = ((u0 + 1) * blocks - 1) / U, i1 = (u1 * blocks - 1) / U;
+                    const int64_t u0 = first_chunk(), u1 = u0 + plan.n;
+                    const int64_t i0 = ((u0 + 1) * plan.blocks - 1) / plan.U, i1 = (u1 * plan.blocks - 1) / plan.U;
                     __threadfence();
-                    int *counter = a.counters + ((int64_t)b * HR + unit);
+                    int *counter = a.counters + ((int64_t)plan.b * HR + plan.unit);
                     const bool last = atomicAdd(counter, 1) == (int)(i1 - i0);
                     if (last) *counter = 0;
                     __threadfence();
@@ -948,12 +961,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
             }
             __syncthreads();
         }
-        x = max(x, u1);
-        if (++unit == HR) {
-            unit = 0;
-            base = u1;
-            if (x < end) do { n = chunks_of<TILES>(a, ++b); } while (n == 0);
+        if (threadIdx.x == 0) {
+            const int64_t u1 = first_chunk() + plan.n;
+            plan.x = max(plan.x, u1);
+            if (++plan.unit == HR) {
+                plan.unit = 0;
+                plan.base = u1;
+                if (plan.x < plan.end) do { plan.n = chunks_of<TILES>(a, ++plan.b); } while (plan.n == 0);
+            }
         }
+        __syncthreads();
     }
 }
 

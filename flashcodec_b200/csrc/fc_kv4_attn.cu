@@ -35,9 +35,12 @@
 // (sequence, head) are joined by the last block to finish, in order: the result does
 // not depend on timing.  No block waits for another.
 //
-// 16 sequences of 32768 tokens, 32/8 heads, D = 128, bf16 (604 MB): 112 us, 5.4 TB/s, 84 %
-// of the copy rate; the copies alone take 103 us.  3 blocks of 168 registers an SM; 4 of
-// 128 spill (123 us), 5 warps a block too (132).  Copies as bulk copies: 127 us.
+// 16 sequences of 32768 tokens, 32/8 heads, D = 128, bf16 (604 MB): 105 us, 5.7 TB/s, 89 %
+// of the copy rate, in short runs; 122 us under sustained load, where the power cap holds
+// the SMs at 1.75 GHz.  The copies alone take 100 us; the rest is the latency of 12 warps'
+// own instructions (1.8 a cycle and SM, 222 for 16 tokens).  3 blocks of 168 registers an
+// SM; 4 of 128 spill (121 us), 5 warps a block too.  Bulk copies in place of cp.async were
+// slower (127 us against 123 at that time), chunks of 32 tokens are by 6 %.
 #include "fc_attn_common.cuh"
 #include "fc_kv4.cuh"
 
@@ -65,9 +68,10 @@ struct AttnArgs {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 // What a segment costs beyond its chunks (queries, the pipeline's start, the joins), in
 // chunks of its block's 4 warps; a block's least piece is a chunk for every warp more.
-// Times in us with 0 / 8 / 16 / 32 (one column block): 16 sequences of 32768 tokens 115 /
-// 113 / 112 / 111, 61 of 1..12000 58 / 23 / 20 / 21; with two column blocks, whose joins
-// are twice as long: 24 sequences of 1..9000 with 16 rows 194 / 52 / 41 / 36.
+// Times in us for 0 / 8 / 16 / 32 chunks of 32 tokens (one column block): 16 sequences of
+// 32768 tokens 115 / 113 / 112 / 111, 61 of 1..12000 58 / 23 / 20 / 21; with two column
+// blocks, whose joins are twice as long: 24 sequences of 1..9000 with 16 rows 194 / 52 /
+// 41 / 36.
 constexpr int overhead(int NT, int TILES) { return (NT == 1 ? 32 : 64) / TILES; }
 constexpr float kSlack = 4.f;    // log2 of how far a score may pass the reference
 

@@ -16,8 +16,8 @@
 // in unsigned order) are counted in 1024 equal bins between the least and the largest, the
 // bin that holds the last key wanted is counted in the same way, until what is wanted of it
 // is all or one value; one prefix sum over the pages then writes the indices in order.
-// 2048 pages of 4 x 8 (sequence, head)s at D = 128 (17 MB): 13.8 us, of which the choice
-// takes some 8; keys kept in shared memory between its passes did not shorten it (14.3).
+// 2048 pages of 4 x 8 (sequence, head)s at D = 128 (17 MB): 13.0 us, of which the choice
+// takes some 8; keys kept in shared memory between its passes did not shorten it.
 #include "fc_kv4.cuh"
 
 namespace fc {
@@ -238,23 +238,31 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     for (int i = 0; i < 8; i++) zr[i] = live ? reinterpret_cast<const int *>(z)[li * 8 + i] : 0;
     int mine = 0;
     if (p0 + warp * 32 < n) {
-#pragma unroll 4
-        for (int it = 0; it < GRP; it++) {  // PPW pages at a time, one a group
-            const int id = __shfl_sync(0xffffffffu, rec, it * PPW + grp);
-            int4 v = make_int4(0, 0, 0, 0);
-            if (live)
-                v = __ldg(reinterpret_cast<const int4 *>(a.bounds + ((int64_t)id * a.Hk + h) * 2 * D) + li);
-            int sum = 0;
-            const int w[4] = {v.x, v.y, v.z, v.w};
+        constexpr int AHEAD = 8;  // loads on their way at a time
+#pragma unroll 1
+        for (int i0 = 0; i0 < GRP; i0 += AHEAD) {  // PPW pages at a time, one a group
+            int4 v[AHEAD];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                sum = __dp2a_lo(zr[2 * i], w[i], sum);
-                sum = __dp2a_hi(zr[2 * i + 1], w[i], sum);
+            for (int i = 0; i < AHEAD; i++) {
+                const int id = __shfl_sync(0xffffffffu, rec, (i0 + i) * PPW + grp);
+                v[i] = make_int4(0, 0, 0, 0);
+                if (live)
+                    v[i] = __ldg(reinterpret_cast<const int4 *>(a.bounds + ((int64_t)id * a.Hk + h) * 2 * D) + li);
             }
 #pragma unroll
-            for (int o = GRP / 2; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const int s = __shfl_sync(0xffffffffu, sum, (lane % PPW) * GRP);
-            if (lane / PPW == it) mine = s;
+            for (int i = 0; i < AHEAD; i++) {
+                int sum = 0;
+                const int w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    sum = __dp2a_lo(zr[2 * j], w[j], sum);
+                    sum = __dp2a_hi(zr[2 * j + 1], w[j], sum);
+                }
+#pragma unroll
+                for (int o = GRP / 2; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const int s = __shfl_sync(0xffffffffu, sum, (lane % PPW) * GRP);
+                if (lane / PPW == i0 + i) mine = s;
+            }
         }
     }
     uint32_t *keys = a.keys + (b * a.Hk + h) * a.table.max_pages;

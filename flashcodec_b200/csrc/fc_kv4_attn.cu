@@ -17,9 +17,10 @@
 // exact.  What is left is the 8 that is on every stored code: for the scores a product of
 // the tokens' scales with -8 * (sum of q of each group), one more matrix instruction for
 // 16 tokens; for the output the groups' sums of weight * scale, one with an operand of
-// eights for each group.  The tensor cores add subnormal products with about 2^-17 of the
-// largest, enough beside 2^-9 of a bf16 query; fp16 and fp32 queries get codes made exact
-// (fp16 1024 + u, minus 1032) and two fp16 parts in neighbouring columns (22 bits).
+// eights for each group, taken off every 256 tokens.  The tensor cores add subnormal
+// products with about 2^-17 of the largest, enough beside 2^-9 of a bf16 query; fp16 and
+// fp32 queries get codes made exact (fp16 1024 + u, minus 1032) and two fp16 parts in
+// neighbouring columns (22 bits).
 // Queries are scaled by a power of two per row so that fp16 holds them.  A group of 32
 // channels is two matrix instructions; its scale comes in after it, in fp32.
 //
@@ -625,6 +626,27 @@ struct Attn {
             gather_chunk<false>(tile, S);
     }
 
+    // The 8 on every code comes off the sums.  The tensor cores cut what they add to, so a
+    // sum that only grows (8 times the weights, where the codes themselves cancel) would lose
+    // an ulp of itself at every step, always downward: flat weights over 262,144 tokens were
+    // half off.  Centred every 256 tokens, the loss stays below 2^-16 of a code's step.
+    static constexpr int kCentre = 16 / TILES;
+    __device__ __forceinline__ void centre() {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < W; j++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+#pragma unroll
+                    for (int m = 2 * j; m < 2 * j + 2; m++) {
+                        acc[nt][m][y] -= ws[nt][j][y];
+                        acc[nt][m][y + 2] = fmaf(-16.f, ws[nt][j][y], acc[nt][m][y + 2]);  // these came as 16 u
+                    }
+                    ws[nt][j][y] = 0.f;
+                }
+    }
+
     // This warp's chunks of the segment: chunk0 + warp, + 4, ..., each copied
     // kStages - 1 rounds before it is used.
     __device__ __forceinline__ void run() {
@@ -653,6 +675,9 @@ struct Attn {
             if (i + (kStages - 1) * kWarps < chunk1) fetch(stage == 0 ? kStages - 1 : stage - 1);
             cp_async_commit();
             use(i, stage);
+            if constexpr (RAW) {
+                if (i / kWarps % kCentre == kCentre - 1) centre();
+            }
             __syncwarp();
             stage = stage == kStages - 1 ? 0 : stage + 1;
         }

@@ -301,6 +301,28 @@ def test_attend_many_splits(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("D,G,page", [(128, 2, 64), (64, 2, 32), (128, 12, 64)])
+def test_flat_attention_over_long_sequences(dtype, D, G, page):
+    """Equal weights over 131072 tokens in a batch so large that a warp takes 32768 of them:
+    the output is a mean, 1 / 360 of the values.  Beside its rounding it may be off by what
+    the sums lose (2^-16 of a code's step, at most M / 7), by the roundings of the weights
+    times scales (2^-11 each, 6 standard deviations of their mean) and by those of the fp32
+    sums of the weights (2^-20)."""
+    n, B = 131072, 450
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda")[None].contiguous()
+    cache = fc().PagedInt4Cache(n // page, 1, D, page_size=page)
+    v = torch.randn(1, n, 1, D, generator=torch.Generator().manual_seed(5)).cuda()
+    cache.append(None, torch.zeros_like(v), v, table, i32([0]))
+    held = cache.read(table, count=n, dtype=torch.float32)[1][0, :, 0].double()
+    want, top = held.mean(0).cpu().numpy(), float(held.abs().max())
+    out = cache.attend(torch.zeros(B, G, D, dtype=DT[dtype], device="cuda"), table.repeat(B, 1).contiguous(),
+                       torch.full((B,), n, dtype=torch.int32, device="cuda"))
+    err = np.abs(out.double().cpu().numpy() - want).max((0, 1))
+    lim = 2 * UNIT[dtype] * np.abs(want) + 2.0 ** -16 * top / 7 + 6 * 2.0 ** -11 / n ** 0.5 + 2.0 ** -20 * top
+    assert (err <= lim).all(), f"{err.max():.2e} over {lim[err.argmax()]:.2e}"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("kscale,vscale", [(1e-4, 1e-4), (40.0, 1e-3), (1.0, 3e3), (30.0, 1e4)])
 def test_attend_ranges(dtype, kscale, vscale):
     """Tiny and huge keys and values: a sharp softmax, scales near both ends of fp16."""

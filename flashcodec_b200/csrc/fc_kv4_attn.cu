@@ -36,8 +36,8 @@
 // (sequence, head) are joined by the last block to finish, in order: the result does
 // not depend on timing.  No block waits for another.
 //
-// 16 sequences of 32768 tokens, 32/8 heads, D = 128, bf16 (604 MB): 105 us, 5.7 TB/s, 89 %
-// of the copy rate, in short runs; 122 us under sustained load, where the power cap holds
+// 16 sequences of 32768 tokens, 32/8 heads, D = 128, bf16 (604 MB): 107 us, 5.6 TB/s, 87 %
+// of the copy rate, in short runs; 124 us under sustained load, where the power cap holds
 // the SMs at 1.75 GHz.  The copies alone take 100 us; the rest is the latency of 12 warps'
 // own instructions (1.8 a cycle and SM, 222 for 16 tokens).  3 blocks of 168 registers an
 // SM; 4 of 128 spill (121 us), 5 warps a block too.  Bulk copies in place of cp.async were

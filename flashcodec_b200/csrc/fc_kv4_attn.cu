@@ -988,8 +988,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
                 __syncthreads();
                 if (last_s) t.merge(first_s, last_s);
             }
-            __syncthreads();
         }
+        // Every thread has read the plan, and left shared memory, before the next unit is
+        // planned: also where the piece ends among the chunks that stand for this unit's
+        // overhead, and so has none of its chunks.
+        __syncthreads();
         if (threadIdx.x == 0) {
             const int64_t u1 = first_chunk() + plan.n;
             plan.x = max(plan.x, u1);

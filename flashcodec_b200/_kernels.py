@@ -562,7 +562,21 @@ except ImportError:
 
     _current_device = torch.cuda.current_device
 
+# (entry point, device, stream) -> workspace of the eager calls there, and of the calls of the
+# capture that was last under way there
 _kv4_workspaces: dict = {}
+_kv4_captured: dict = {}
+
+
+class _Kv4Workspace:
+    __slots__ = ("buffer", "address", "bytes", "units", "capture")
+
+    def __init__(self, capture):
+        self.buffer, self.address, self.bytes, self.units, self.capture = None, None, 0, -1, capture
+
+    def clear(self):
+        """Zero the arrival counters, the size of a workspace for no sequence; the rest needs none."""
+        self.buffer[:_lib.load().fc_kv4_select_workspace_size(0, 0, 0)].zero_()
 
 
 def kv4_page_bytes(Hk: int, D: int, page_size: int) -> int:
@@ -572,20 +586,29 @@ def kv4_page_bytes(Hk: int, D: int, page_size: int) -> int:
     return n
 
 
-def _kv4_workspace(what, sizes, index, stream):
-    """(address, bytes) of the zero-initialised workspace of one entry point, shared by the
-    calls of a (device, stream); `sizes` are the arguments of its size function."""
-    key = (what, index, stream)
-    held = _kv4_workspaces.get(key)
-    if held is None:
-        held = _kv4_workspaces[key] = [None, 0, 0, set()]
-    if sizes not in held[3]:
+def _kv4_workspace(what, sizes, units, index, stream):
+    """The workspace of one entry point, its counters zeroed: one for the eager calls of a (device,
+    stream), one for each capture there.  `sizes` are the arguments of its size function, which
+    grows with `units` alone.
+
+    A captured graph keeps the address of its workspace, and what zeroes a buffer that a
+    capture allocates is a node of that graph.  So a capture shares its buffer with nothing: not
+    with eager calls, whose buffer is replaced when a larger call comes, and not with the next
+    capture, whose graph may be replayed first or on another stream.  The buffer is a graph's own
+    (it comes from the capture's memory pool, which lives as long as the graph does)."""
+    capture = _lib.load().fc_capture_id(stream)
+    workspaces, key = _kv4_captured if capture else _kv4_workspaces, (what, index, stream)
+    ws = workspaces.get(key)
+    if ws is None or ws.capture != capture:
+        ws = workspaces[key] = _Kv4Workspace(capture)
+    if units > ws.units:
         nbytes = getattr(_lib.load(), f"fc_kv4_{what}_workspace_size")(*sizes)
-        if nbytes > held[2]:
-            held[0] = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-            held[1], held[2] = held[0].data_ptr(), nbytes
-        held[3].add(sizes)
-    return held
+        if nbytes > ws.bytes:
+            ws.buffer = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+            ws.address, ws.bytes = ws.buffer.data_ptr(), nbytes
+            ws.clear()
+        ws.units = units
+    return ws
 
 
 def _kv4_call(fn, what, index, args, ws=None):
@@ -596,7 +619,7 @@ def _kv4_call(fn, what, index, args, ws=None):
             rc = fn(*args)
     if rc:
         if ws is not None:
-            ws[0].zero_()
+            ws.clear()
         _lib.check(rc, what)
 
 
@@ -635,17 +658,19 @@ def kv4_attn(cache, q_at, dtype, shape, table, lengths, selected, scale, out_at,
     # a selection of no pages is not the same as none: its address is not null
     sel = (None, 0) if selected is None else (selected.data_ptr() or cache._status_ptr,
                                               selected.shape[2])
-    ws = _kv4_workspace("attn", (B, Sq, Hq, cache.num_kv_heads, cache.head_dim), index, stream)
+    ws = _kv4_workspace("attn", (B, Sq, Hq, cache.num_kv_heads, cache.head_dim), cache.head_dim, index,
+                        stream)
     _kv4_call(cache._lib.fc_kv4_attn, "kv4_attn", index, (
         q_at[0], _code(dtype), B, Sq, Hq, *q_at[1:], *cache._pool_args, *table, lengths, *sel, scale,
-        *out_at, None if lse is None else lse.data_ptr(), ws[1], ws[2], cache._status_ptr, stream), ws)
+        *out_at, None if lse is None else lse.data_ptr(), ws.address, ws.bytes, cache._status_ptr, stream), ws)
 
 
 def kv4_select(cache, q_at, dtype, B, Hq, table, lengths, count, sink, recent, pages) -> None:
     """fc_kv4_select; q (B, Hq, D), pages (B, Hk, count) int32."""
     index = cache._index
     stream = _raw_stream(index)
-    ws = _kv4_workspace("select", (B, cache.num_kv_heads, table[2]), index, stream)
+    sizes = (B, cache.num_kv_heads, table[2])
+    ws = _kv4_workspace("select", sizes, math.prod(sizes), index, stream)
     _kv4_call(cache._lib.fc_kv4_select, "kv4_select", index, (
         q_at[0], _code(dtype), B, Hq, q_at[1], q_at[3], *cache._bounds_args, *cache._pool_args[1:],
-        *table, lengths, count, sink, recent, pages, ws[1], ws[2], cache._status_ptr, stream), ws)
+        *table, lengths, count, sink, recent, pages, ws.address, ws.bytes, cache._status_ptr, stream), ws)

@@ -18,7 +18,7 @@ FC_OK, FC_EINVAL, FC_ECUDA, FC_ERANGE, FC_ENOTSUP = 0, 1, 2, 3, 4
 FC_F32, FC_BF16, FC_F16, FC_I8 = 0, 1, 2, 3
 
 # exported symbols, in header order (tests check the library exports them all)
-SYMBOLS = ("fc_version", "fc_last_error_string", "fc_jpeg_encode", "fc_jpeg_decode",
+SYMBOLS = ("fc_version", "fc_last_error_string", "fc_capture_id", "fc_jpeg_encode", "fc_jpeg_decode",
            "fc_jpeg_encode_grouped", "fc_jpeg_decode_grouped", "fc_png_encode", "fc_png_decode", "fc_decode_attn_workspace_size",
            "fc_decode_attn", "fc_decode_attn_grouped", "fc_decode_attn_png",
            "fc_decode_attn_noalloc",
@@ -51,6 +51,7 @@ class AppendStream(ctypes.Structure):
 _SIGS = {
     "fc_version": ([], ctypes.c_char_p),
     "fc_last_error_string": ([], ctypes.c_char_p),
+    "fc_capture_id": ([_P], ctypes.c_uint64),
     "fc_jpeg_encode": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I32, _I32,
                         _P, _I64, _I64, _I64, _I64, _P, _I32, _I64, _I64, _I64, _P, _P], _I32),
     "fc_jpeg_decode": ([_P, _I32, _I64, _I64, _I64, _I64, _I32, _I64, _I64, _I64, _I64,

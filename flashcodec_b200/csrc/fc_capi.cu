@@ -51,3 +51,13 @@ int num_sms() {
 extern "C" const char *fc_version(void) { return FC_VERSION_STRING; }
 
 extern "C" const char *fc_last_error_string(void) { return fc::g_err; }
+
+extern "C" unsigned long long fc_capture_id(void *stream) {
+    cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &state, &id) != cudaSuccess) {
+        cudaGetLastError();  // the legacy stream while another one captures: not part of it
+        return 0;
+    }
+    return state == cudaStreamCaptureStatusNone ? 0 : id;
+}

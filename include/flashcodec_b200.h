@@ -54,6 +54,12 @@ FC_API const char *fc_version(void);
 /* Message of the last failed call on this thread ("" if none). */
 FC_API const char *fc_last_error_string(void);
 
+/* The id of the capture that `stream` is part of, unique in the process; 0 where
+ * none is under way.  A workspace that a captured graph uses must live as long as
+ * the graph and, unless replays and other calls are kept apart by stream order,
+ * be its alone: callers that keep workspaces by stream tell captures apart by it. */
+FC_API unsigned long long fc_capture_id(void *stream);
+
 /*
  * jpeg archive / compress.
  * Replaces flashcodec/codecs/jpeg.py:55-67 (dct_compress) followed by
@@ -617,8 +623,9 @@ FC_API int fc_kv4_read(const void *pool, int64_t num_pages, int64_t Hk, int64_t 
                        int64_t o_ss, int64_t o_sh, int *status, void *stream);
 
 /* Bytes of workspace that fc_kv4_attn needs for these sizes (any lengths),
- * zero-filled before its first use and left with zeroed counters by every call.
- * Calls sharing one must not overlap on the GPU. */
+ * zero-filled before its first use (the first fc_kv4_select_workspace_size(0, 0, 0)
+ * bytes of it, the arrival counters, suffice) and left with zeroed counters by
+ * every call.  Calls sharing one must not overlap on the GPU. */
 FC_API size_t fc_kv4_attn_workspace_size(int64_t B, int64_t Sq, int64_t Hq, int64_t Hk, int64_t D);
 
 /* Attention of the last Sq tokens of every sequence over the cache:

@@ -26,8 +26,12 @@
 //
 // Weights.  Base-2 softmax with a running reference per row, moved only when a score
 // passes it by 2^4, and a running power of two above the values' scales, so that
-// weight * scale, an fp16 operand, stays in 2^-14 .. 2^15.  One rounding of the weight
-// and one of the product for bf16 queries (2^-11 each), two fp16 parts otherwise.
+// weight * scale, an fp16 operand, is at most 2^15.  fp16 and fp32 queries: the product is
+// rounded once, to two fp16 parts; the power of two follows the scales from fp16's least on,
+// so that the largest weight and scale make 2^10 or more.  bf16 queries: the weight is
+// rounded to fp16 and the product again (2^-11 each); a weight has to fit fp16 by itself, so
+// the power of two is 1 at least, and where all scales are below 2^-10 the products of
+// weights under 2^-14 of the largest are subnormal.
 //
 // Work.  The chunks (32 tokens) of all (sequence, KV head, row block) are one line,
 // cut into equal pieces for one wave of blocks, whatever the lengths; the lengths are
@@ -169,6 +173,11 @@ struct Attn {
     const AttnArgs &a;
     unsigned char *ring;  // of this warp
     int *pos_s;           // (kStages, TILES) first positions of the staged tiles
+    // Where the bound above the values' scales begins: weight * scale <= kSlim * 2^kLim = 2^15.
+    // Two fp16 parts of a product hold 22 bits of it down to about 2^-2, so the bound follows the
+    // scales from the least there is; from 1 on, values near 1e-4 lost half of those bits and
+    // values near 1e-5 all but a few.  A weight that is an fp16 operand itself stays below 2^15.
+    static constexpr float kLim = LIMBS == 2 ? 39.f : 15.f, kSlim = LIMBS == 2 ? 0x1p-24f : 1.f;
     int warp, lane, r, c;
     // this segment
     int b, h, rb, len, chunk0, chunk1;
@@ -299,8 +308,8 @@ struct Attn {
                 for (int j = 0; j < W; j++) ws[nt][j][0] = ws[nt][j][1] = 0.f;
             }
         }
-        lim = 15.f;
-        slim = 1.f;
+        lim = kLim;
+        slim = kSlim;
     }
 
     // ------------------------------------------------------------------ copies

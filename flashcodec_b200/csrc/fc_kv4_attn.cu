@@ -68,6 +68,7 @@ struct AttnArgs {
     float *lse;
     int *counters;  // one per (sequence, KV head, row block), zero between calls
     float *parts;   // two per block: [row][D], then the references and the sums
+    float *aside;   // one per warp: the state of its earlier spans
 };
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
@@ -638,7 +639,7 @@ struct Attn {
     // The 8 on every code comes off the sums.  The tensor cores cut what they add to, so a
     // sum that only grows (8 times the weights, where the codes themselves cancel) would lose
     // an ulp of itself at every step, always downward: flat weights over 262,144 tokens were
-    // half off.  Centred every 256 tokens, the loss stays below 2^-16 of a code's step.
+    // half off.  Centred every 256 tokens, it loses below 2^-16 of a code's step.
     static constexpr int kCentre = 16 / TILES;
     __device__ __forceinline__ void centre() {
 #pragma unroll
@@ -654,6 +655,45 @@ struct Attn {
                     }
                     ws[nt][j][y] = 0.f;
                 }
+    }
+
+    // Centred sums still grow where the values have a mean, and lose to the same cut: values
+    // around 3, then around -3, over 262,144 tokens of a warp were 2e-3 off.  So a segment is
+    // run in spans of 4096 tokens a warp (256 steps: below 2^-16 of the sum on average), whose
+    // states are joined in rounded fp32 in the workspace, as the registers are the loop's and the
+    // rings fill shared memory.  200 x 65536 tokens of one head (two spans a segment): 285 us
+    // with and without.
+    static constexpr int kSpan = 4096 / (16 * TILES) * kWarps;  // chunks
+    static constexpr int ASIDE = (4 + 8 * W) * NT * 32;  // floats of a warp: references, sums, outputs
+    // Joins the state with the one put aside (`more`: there is one); `last`: stays in registers.
+    __device__ __forceinline__ void put_aside(bool more, bool last) {
+        centre();
+        float *z = a.aside + ((int64_t)blockIdx.x * kWarps + warp) * ASIDE + lane;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            float g[2], h[2];
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const float held = more ? z[32 * y] : M[nt][y], m = fmaxf(held, M[nt][y]);
+                g[y] = exp2_fast(M[nt][y] - m);
+                h[y] = exp2_fast(held - m);
+                M[nt][y] = m;
+                l[nt][y] = fmaf(l[nt][y], g[y], more ? z[32 * (2 + y)] * h[y] : 0.f);
+                if (!last) {
+                    z[32 * y] = m;
+                    z[32 * (2 + y)] = l[nt][y];
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 2 * W; m++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float *v = z + 32 * (4 + 4 * m + i);
+                    acc[nt][m][i] = fmaf(acc[nt][m][i], g[i & 1], more ? *v * h[i & 1] : 0.f);
+                    if (!last) *v = acc[nt][m][i];
+                }
+            z += 32 * (4 + 8 * W);
+        }
     }
 
     // This warp's chunks of the segment: chunk0 + warp, + 4, ..., each copied
@@ -966,20 +1006,29 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
     A t(a, smem, pos);
     while (plan.x < plan.end) {
         auto first_chunk = [&] { return plan.base + (int64_t)plan.unit * (plan.n + OVERHEAD) + OVERHEAD; };
-        {
-            const int64_t u0 = first_chunk();
-            t.chunk0 = (int)(max(plan.x, u0) - u0);
-            t.chunk1 = (int)(min(plan.end, u0 + plan.n) - u0);
-        }
-        if (t.chunk0 < t.chunk1) {
+        auto begin = [&] { return (int)max(plan.x - first_chunk(), (int64_t)0); };
+        auto end = [&] { return (int)min(plan.end - first_chunk(), (int64_t)plan.n); };
+        if (begin() < end()) {
             t.b = plan.b;
             t.h = plan.unit / a.row_blocks;
             t.rb = plan.unit - t.h * a.row_blocks;
             t.len = a.table.length(a.lengths[t.b]);
-            t.run();
-            const bool whole = t.chunk0 == 0 && t.chunk1 == plan.n;
+            if constexpr (A::RAW) {
+                t.chunk1 = begin();
+                do {
+                    t.chunk0 = t.chunk1;
+                    t.chunk1 = min(t.chunk0 + A::kSpan, end());
+                    t.run();
+                    if (end() - begin() > A::kSpan) t.put_aside(t.chunk0 > begin(), t.chunk1 == end());
+                } while (t.chunk1 < end());
+            } else {
+                t.chunk0 = begin();
+                t.chunk1 = end();
+                t.run();
+            }
+            const bool whole = begin() == 0 && end() == plan.n;
             // parts of a block: 0 of a unit that began in an earlier one, 1 of one that ends in a later one
-            t.join(smem, ml, whole, a.parts + ((int64_t)blockIdx.x * 2 + (t.chunk0 == 0)) * A::PART);
+            t.join(smem, ml, whole, a.parts + ((int64_t)blockIdx.x * 2 + (begin() == 0)) * A::PART);
             if (!whole) {
                 __syncthreads();
                 if (threadIdx.x == 0) {
@@ -1016,6 +1065,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && W <= 4 ? 3 : 2) attn_kern
 }
 
 constexpr int kMaxBlocksPerSm = 4;
+// Floats that a launch can need of the workspace: 16 rows are the largest row block, two parts of
+// a block; two column blocks (up to D = 128) put aside as much as one of twice the head dim.
+inline int64_t parts_floats(int64_t D) { return (int64_t)num_sms() * kMaxBlocksPerSm * 2 * 16 * (D + 2); }
+inline int64_t aside_floats(int64_t D) {
+    return (int64_t)num_sms() * kMaxBlocksPerSm * kWarps * 32 * (4 + D / 4) * (D <= 128 ? 2 : 1);
+}
 
 // Blocks of a wave: what of the kernel fits on the device.
 template <int W, int NT, int LIMBS, int TILES, bool RUNS>
@@ -1044,8 +1099,7 @@ using namespace fc;
 using namespace fc::kv4;
 
 extern "C" size_t fc_kv4_attn_workspace_size(int64_t B, int64_t Sq, int64_t Hq, int64_t Hk, int64_t D) {
-    // 16 rows are the largest row block; two parts of a block
-    return (size_t)(kCounterBytes + (int64_t)num_sms() * kMaxBlocksPerSm * 2 * 16 * (D + 2) * 4);
+    return (size_t)(kCounterBytes + (parts_floats(D) + aside_floats(D)) * 4);
 }
 
 extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int64_t Hq, int64_t q_sb,
@@ -1111,6 +1165,7 @@ extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int6
     a.out = out; a.o_sb = o_sb; a.o_ss = o_ss; a.o_sh = o_sh; a.lse = lse;
     a.counters = reinterpret_cast<int *>(ws + 256);
     a.parts = reinterpret_cast<float *>(ws + kCounterBytes);
+    a.aside = a.parts + parts_floats(D);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return by_head_dim(D, [&](auto w) {
         constexpr int W = decltype(w)::value;

@@ -46,3 +46,29 @@ def test_small_values(dtype, vscale, alike):
         assert (err <= lim).all(), f"{err.max():.3e} over {lim.flat[err.argmax()]:.3e}"
     else:
         near(out, want, dtype, top)
+
+
+# --------------------------------------------------------------- values with a mean
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("halves", [False, True])
+def test_flat_attention_over_values_with_a_mean(dtype, halves):
+    """Equal weights over 2^20 tokens, 2^18 of them a warp's, of values around 3, or around 3 and
+    then around -3: the sums grow with the mean.  Beside its rounding the output may be off by
+      * what sums lose that are cut at each of 256 steps of 16 tokens before they are added up
+        in rounded fp32: growing from zero, 256 / 2 ulps (2^-23) of the mean, 2^-16 * 3;
+      * the cuts of the codes' offset between two centrings, 2^-16 of a code's step (M / 7);
+      * the fp32 sums' roundings, 2^-20 M, as in the test of values without a mean."""
+    n, D, B, page, G = 1 << 20, 128, 450, 64, 2
+    cache = fc().PagedInt4Cache(n // page, 1, D, page_size=page)
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda")[None].contiguous()
+    v = torch.randn(1, n, 1, D, generator=torch.Generator("cuda").manual_seed(5), device="cuda") + 3
+    if halves:
+        v[:, n // 2:] -= 6
+    cache.append(None, torch.zeros_like(v), v, table, i32([0]))
+    held = cache.read(table, count=n, dtype=torch.float32)[1][0, :, 0].double()
+    want, top = held.mean(0).cpu().numpy(), float(held.abs().max())
+    out = cache.attend(torch.zeros(B, G, D, dtype=DT[dtype], device="cuda"), table.repeat(B, 1).contiguous(),
+                       torch.full((B,), n, dtype=torch.int32, device="cuda"))
+    err = np.abs(out.double().cpu().numpy() - want).max((0, 1))
+    lim = 2 * UNIT[dtype] * np.abs(want) + 2.0 ** -16 * 3 + 2.0 ** -16 * top / 7 + 2.0 ** -20 * top
+    assert (err <= lim).all(), f"{err.max():.2e} over {lim[err.argmax()]:.2e}"

@@ -72,3 +72,25 @@ def test_flat_attention_over_values_with_a_mean(dtype, halves):
     err = np.abs(out.double().cpu().numpy() - want).max((0, 1))
     lim = 2 * UNIT[dtype] * np.abs(want) + 2.0 ** -16 * 3 + 2.0 ** -16 * top / 7 + 2.0 ** -20 * top
     assert (err <= lim).all(), f"{err.max():.2e} over {lim[err.argmax()]:.2e}"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,page,G,Sq", [(64, 64, 2, 1), (96, 16, 4, 1), (128, 64, 16, 1), (256, 32, 2, 1),
+                                         (128, 128, 2, 3), (192, 64, 3, 1)])
+@pytest.mark.parametrize("rise", [-1.0, 1.0])
+def test_segments_of_several_spans(dtype, D, page, G, Sq, rise):
+    """70001 tokens a sequence in batches so large that a warp takes 17500 of them, with scores that
+    rise or fall by 80 on the way: the references of a warp's spans lie far apart."""
+    n, B = 70001, 450
+    g = torch.Generator().manual_seed(D)
+    way = torch.linspace(0, 80 * rise, n)[:, None] / D ** 0.5
+    cache, table, hk, hv = held_by(torch.randn(n, D, generator=g) + way, torch.randn(n, D, generator=g), page)
+    q = (1 + 0.2 * torch.randn(1, Sq, G, D, generator=g)).to(DT[dtype])
+    out, lse = cache.attend(q.cuda().expand(B, Sq, G, D).contiguous(), table.repeat(B, 1),
+                            torch.full((B,), n, dtype=torch.int32, device="cuda"), return_lse=True)
+    for s in range(Sq):
+        m = n - Sq + 1 + s
+        want, wl = kv4.attend(q[0, s].float().numpy(), hk[:m], hv[:m])
+        near(out[:, s], np.broadcast_to(want, out[:, s].shape), dtype, np.abs(hv).max(), s)
+        assert (np.abs(lse[:, s].double().cpu().numpy() - wl) <= 2.0 ** -9 * (1 + np.abs(wl))).all()
+    cache.check()

@@ -80,6 +80,11 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 // 41 / 36.
 constexpr int overhead(int NT, int TILES) { return (NT == 1 ? 32 : 64) / TILES; }
 constexpr float kSlack = 4.f;    // log2 of how far a score may pass the reference
+constexpr float kNone = -3e38f;  // the reference of a row that has seen no token
+// Beyond this a reference 2^11 (2^35) below a score and the score cannot both be told from their
+// neighbours: scores of 2^27 and more came out as zeros or NaN.  The reference is then the
+// largest rounded score itself and weights are at most 1, which fits fp16 with every scale.
+constexpr float kLarge = 0x1p22f;
 
 __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -192,6 +197,7 @@ struct Attn {
     // running state: references, sums, outputs, sums of weight * scale of each group
     float M[NT][2], l[NT][2], acc[NT][2 * W][4], ws[RAW ? NT : 1][W][2];
     float lim, slim;
+    bool large;  // a row of this warp has a reference beyond kLarge
 
     __device__ __forceinline__ Attn(const AttnArgs &args, unsigned char *smem, int *pos)
         : a(args) {
@@ -289,7 +295,11 @@ struct Attn {
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 const int from = (2 * c + y) * 4;
+                // neither zero, which would make a masked score a NaN, nor infinity, which would a
+                // score of zero: scores beyond those are ones that round to zero, and ones whose
+                // weights are one and zeros at this factor too (their logarithm is not kept)
                 f[nt][y] = __shfl_sync(0xffffffffu, down, from) * a.scale * (RAW ? 0x1p24f : 1.f);
+                f[nt][y] = fminf(fmaxf(f[nt][y], 1e-37f), 3.4028234e38f);
                 const int sq = min(row_of(nt, 2 * c + y), a.rows - 1) / a.G;
                 seen[nt][y] = len - (a.Sq - 1 - sq);
             }
@@ -299,7 +309,7 @@ struct Attn {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-            for (int y = 0; y < 2; y++) { M[nt][y] = -1e30f; l[nt][y] = 0.f; }
+            for (int y = 0; y < 2; y++) { M[nt][y] = kNone; l[nt][y] = 0.f; }
 #pragma unroll
             for (int m = 0; m < 2 * W; m++)
 #pragma unroll
@@ -311,6 +321,7 @@ struct Attn {
         }
         lim = kLim;
         slim = kSlim;
+        large = false;
     }
 
     // ------------------------------------------------------------------ copies
@@ -569,7 +580,7 @@ struct Attn {
 #pragma unroll
         for (int i = 1; i < (SH + 1) / 2; i++) st = __hmax2(st, h2(sv[i]));
         const float sm = __half2float(__hmax(__low2half(st), __high2half(st)));
-        bool pass = sm > slim;
+        bool pass = sm > slim || large;
         float top[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -585,6 +596,7 @@ struct Attn {
 #pragma unroll
             for (int o = 16; o; o /= 2) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
             const float old = lim;
+            bool far = false;
             if (s > slim && s <= 65504.f) {
                 const uint32_t u = __float_as_uint(s);
                 const int e = (int)(u >> 23) - 127 + ((u & 0x7fffffu) != 0);  // s <= 2^e
@@ -598,8 +610,14 @@ struct Attn {
                     float t = top[nt][y];
 #pragma unroll
                     for (int o = 4; o < 32; o *= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+                    const bool any = t > -INFINITY;
                     float m = M[nt][y] + (old - lim);
-                    if (t > -INFINITY) m = fmaxf(m, fmaf(t, f[nt][y], -(lim - kSlack)));
+                    if (any) m = fmaxf(m, fmaf(t, f[nt][y], -(lim - kSlack)));
+                    if (fabsf(m) > kLarge) {  // a number that no score is above
+                        m = fabsf(M[nt][y]) > kLarge ? M[nt][y] : M[nt][y] + fmaxf(old, 0.f);
+                        if (any) m = fmaxf(m, __fmul_rn(t, f[nt][y]));
+                        far = far || m > kNone;
+                    }
                     const float g = exp2_fast(M[nt][y] - m);
                     M[nt][y] = m;
                     l[nt][y] *= g;
@@ -613,23 +631,33 @@ struct Attn {
                         acc[nt][i][y + 2] *= g;
                     }
                 }
+            large = __any_sync(0xffffffffu, far);
         }
+        auto weights = [&](auto exponents) {
 #pragma unroll
-        for (int t = 0; t < TILES; t++)
+            for (int t = 0; t < TILES; t++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    const float2 x = __ffma2_rn(make_float2(S[t][nt][i], S[t][nt][i + 1]),
-                                                make_float2(f[nt][0], f[nt][1]),
-                                                make_float2(-M[nt][0], -M[nt][1]));
-                    S[t][nt][i] = exp2_fast(x.x);
-                    S[t][nt][i + 1] = exp2_fast(x.y);
-                    const float2 s = __fadd2_rn(make_float2(l[nt][0], l[nt][1]),
-                                                make_float2(S[t][nt][i], S[t][nt][i + 1]));
-                    l[nt][0] = s.x;
-                    l[nt][1] = s.y;
-                }
+                    for (int i = 0; i < 4; i += 2) {
+                        const float2 x = exponents(make_float2(S[t][nt][i], S[t][nt][i + 1]), nt);
+                        S[t][nt][i] = exp2_fast(x.x);
+                        S[t][nt][i + 1] = exp2_fast(x.y);
+                        const float2 s = __fadd2_rn(make_float2(l[nt][0], l[nt][1]),
+                                                    make_float2(S[t][nt][i], S[t][nt][i + 1]));
+                        l[nt][0] = s.x;
+                        l[nt][1] = s.y;
+                    }
+        };
+        if (large)
+            weights([&](float2 x, int nt) {
+                return make_float2(__fsub_rn(__fmul_rn(x.x, f[nt][0]), M[nt][0]),
+                                   __fsub_rn(__fmul_rn(x.y, f[nt][1]), M[nt][1]));
+            });
+        else
+            weights([&](float2 x, int nt) {
+                return __ffma2_rn(x, make_float2(f[nt][0], f[nt][1]), make_float2(-M[nt][0], -M[nt][1]));
+            });
         if (masked)
             gather_chunk<true>(tile, S);
         else

@@ -94,3 +94,40 @@ def test_segments_of_several_spans(dtype, D, page, G, Sq, rise):
         near(out[:, s], np.broadcast_to(want, out[:, s].shape), dtype, np.abs(hv).max(), s)
         assert (np.abs(lse[:, s].double().cpu().numpy() - wl) <= 2.0 ** -9 * (1 + np.abs(wl))).all()
     cache.check()
+
+
+# ------------------------------------------------------------------ ends of the range
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("log2q", [20, 26, 33, 50, 100, 118, 125])
+@pytest.mark.parametrize("best", [0.0, 2.0 ** -12, -2.0 ** -12])
+def test_queries_and_scores_at_the_ends_of_fp32(dtype, log2q, best):
+    """Queries near the largest number: the weights are one and zeros, whether the largest score
+    is zero, far above it or far below -1e30 (the other keys' scores are far below it)."""
+    n, D = 200, 64
+    g = torch.Generator().manual_seed(13)
+    q = 2.0 ** log2q * (1 + torch.rand(2, D, generator=g)).to(DT[dtype])
+    v = torch.randn(n, D, generator=g)
+    k = -(1 + torch.rand(n, 1, generator=g)).expand(n, D) * 2.0 ** -9
+    k = k.contiguous()
+    k[77] = best
+    cache, table, hk, hv = held_by(k, v)
+    want, wl = kv4.attend(q.double().numpy(), hk, hv)
+    assert (want == hv[77]).all()
+    out, lse = cache.attend(q[None].cuda(), table, i32([n]), return_lse=True)
+    near(out[0], want, dtype, np.abs(hv).max())
+    if log2q < 120 or dtype == "fp32":  # bf16 queries beyond: the logarithm itself is not kept
+        assert (np.abs(lse[0].double().cpu().numpy() - wl) <= 2.0 ** -9 * np.abs(wl)).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("scale", [0.0, 1e-30, None])
+def test_tiny_queries_and_scales(dtype, scale):
+    """Scores that round to zero, next to tokens that the first of two queries does not see."""
+    n, D = 77, 64
+    g = torch.Generator().manual_seed(14)
+    cache, table, hk, hv = held_by(torch.randn(n, D, generator=g), torch.randn(n, D, generator=g))
+    q = (1e-25 * torch.randn(1, 2, 2, D, generator=g)).to(DT[dtype])
+    out = cache.attend(q.cuda(), table, i32([n]), scale=scale)[0]
+    for s in range(2):
+        want, _ = kv4.attend(q[0, s].float().numpy(), hk[: n - 1 + s], hv[: n - 1 + s], scale=scale)
+        near(out[s], want, dtype, np.abs(hv).max(), s)

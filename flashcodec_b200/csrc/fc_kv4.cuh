@@ -29,8 +29,9 @@
 // Optional page bounds: for every page and KV head the least and the largest
 // value of every key channel, as int8 multiples of one power of two 2^e (least
 // rounded down, largest up; e the smallest integer >= -40 for which all fit in
-// -127..127).  Rounding by powers of two nests exactly, so the bounds of a page do
-// not depend on how its tokens were split into calls.
+// -127..127); a group whose scale is NaN counts as zeros.  Rounding by powers of two
+// nests exactly, so the bounds of a page do not depend on how its tokens were split
+// into calls.
 #pragma once
 
 #include "fc_common.cuh"

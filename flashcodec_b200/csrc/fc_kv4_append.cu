@@ -505,7 +505,7 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
                                                                     2 * (t >> 3) + (t & 1)] = vs;
                     }
                     if (a.bounds) {
-                        const float s = __half2float(ks);
+                        const float s = __hisnan(ks) ? 0.f : __half2float(ks);  // no numbers: zeros
                         const Row &u = x[0][k];
                         const float2 z[4] = {__fmul2_rn(u.e[0], pair(s, s)), __fmul2_rn(u.e[1], pair(s, s)),
                                              __fmul2_rn(u.o[0], pair(s, s)), __fmul2_rn(u.o[1], pair(s, s))};
@@ -592,7 +592,6 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
                     u[i] = fminf(u[i], lo_s[w * D + d]);
                     v[i] = fmaxf(v[i], hi_s[w * D + d]);
                 }
-                if (u[i] > v[i]) u[i] = v[i] = 0.f;  // no number among them
                 top = fmaxf(top, fmaxf(fabsf(u[i]), fabsf(v[i])));
             }
 #pragma unroll

@@ -596,7 +596,8 @@ FC_API int64_t fc_kv4_page_bytes(int64_t Hk, int64_t D, int64_t page_size);
  * positions (T) int32 rows of the table, or NULL for the cache positions.
  * bounds, exponents  (num_pages, Hk, 2, D) int8 and (num_pages, Hk) int32: the
  *          least and the largest value held of every key channel of a page, as
- *          multiples of 2^exponent, rounded outward; or NULL, NULL.
+ *          multiples of 2^exponent, rounded outward (a group with a NaN scale
+ *          counts as zeros); or NULL, NULL.
  * Arithmetic is fp32, every product and sum rounded by itself; the stored bits
  * do not depend on how tokens are split into calls. */
 FC_API int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t q_sh, void *q_out,

@@ -1,0 +1,64 @@
+"""What the paged 4-bit cache says of inputs at the edge: groups that are no numbers, positions
+outside the rotary table, padded packed batches, rows that are not held, fused buffers."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4
+from test_gpu_kv4 import fc, i32, table_of
+
+pytestmark = pytest.mark.gpu
+
+
+def tokens(n, H, D, seed, lead=()):
+    return torch.randn(*lead, n, H, D, generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+# ----------------------------------------------------------------------- page bounds
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("cuts", [[1] * 20, [7, 1, 12], [3, 5, 12], [8, 12]])
+@pytest.mark.parametrize("first", [0, 7])
+def test_bounds_with_groups_that_are_no_numbers_do_not_depend_on_the_split(what, cuts, first):
+    """A key token's group that is NaN counts as zeros, alone in its call or not; the bounds of
+    channels of one sign that have none keep the sign."""
+    Hk, D, page, n = 2, 64, 32, 20
+    k = tokens(n, Hk, D, 1, (1,)).abs() + 0.5
+    k[:, :, 1] *= -1
+    k[0, first, :, 3], k[0, 8, 0, 40] = what, what
+    table, pages = table_of([n], page)
+    got = []
+    for parts in ([n], cuts):
+        cache, at = fc().PagedInt4Cache(pages, Hk, D, page_size=page, bounds=True), 0
+        cache.pool.zero_()
+        for c in parts:
+            cache.append(None, k[:, at:at + c], k[:, at:at + c], table, i32([at]))
+            at += c
+        got.append((cache.pool, cache.bounds, cache.exponents))
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    held = kv4.values(*kv4.quantise(k[0].cpu().numpy()))
+    for h in range(Hk):
+        want, e = kv4.bounds(np.nan_to_num(held[:, h]))
+        assert np.array_equal(got[0][1][table[0, 0], h].cpu().numpy(), want)
+        assert int(got[0][2][table[0, 0], h]) == e
+    assert (want[1, 32:] < 0).all()  # the last head's second group has none
+
+
+def test_bounds_of_a_page_without_numbers():
+    """Bounds of zero; keys of numbers that come later are within them all the same."""
+    Hk, D, page = 1, 64, 16
+    k = torch.full((1, 4, Hk, D), math.nan, device="cuda")
+    k[0, 2:] = tokens(2, Hk, D, 2) + 5
+    table, pages = table_of([4], page)
+    cache = fc().PagedInt4Cache(pages, Hk, D, page_size=page, bounds=True)
+    for at in (0, 2):
+        cache.append(None, k[:, at:at + 2], k[:, at:at + 2], table, i32([at]))
+        lo, hi = cache.bounds[table[0, 0], 0].double().cpu().numpy()
+        unit = 2.0 ** int(cache.exponents[table[0, 0], 0])
+        if at == 0:
+            assert not lo.any() and not hi.any()
+    held = kv4.values(*kv4.quantise(k[0, 2:, 0].cpu().numpy()))
+    assert (lo * unit <= held.min(0)).all() and (hi * unit >= held.max(0)).all()

@@ -24,8 +24,9 @@ operations on it:
 ``page_table`` (B, n) and ``lengths`` (B,) are int32 CUDA tensors which the
 kernels read when they run: a captured CUDA graph follows their contents.  The
 caller owns page allocation; entries past a sequence's pages are never read.
-Kernels check pages, lengths and positions against the buffers: what does not
-fit is skipped or clamped and noted in ``status`` (see ``check``).  The
+Kernels check pages, lengths and positions against the buffers: tokens without a
+page are skipped, positions outside the rotary table take its nearest row, and
+either is noted in ``status`` (see ``check``).  The
 reference has no paged cache; its notes on 4-bit K/V quantisation
 (docs/llama-cpp-kv-quantization.md) are the nearest it has.
 """

@@ -567,8 +567,10 @@ FC_API int fc_ipc_close_handle(void *base);
  *          outside the pool (FC_KV4_BAD_PAGE), a length or position past what
  *          the table can hold (FC_KV4_BAD_LENGTH) or a position outside the
  *          rotary table (FC_KV4_BAD_POSITION).  No kernel accesses memory
- *          outside the buffers then; the output rows concerned are not valid
- *          and appends skip the tokens.
+ *          outside the buffers then: appends skip the tokens that have no page;
+ *          heads whose position has no row of the rotary table are turned by
+ *          the nearest one, and stored; attention over such pages or lengths
+ *          gives rows that are not valid.
  * All entry points are asynchronous on `stream` and can be captured. */
 #define FC_KV4_BAD_PAGE 1
 #define FC_KV4_BAD_LENGTH 2

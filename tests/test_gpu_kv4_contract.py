@@ -62,3 +62,22 @@ def test_bounds_of_a_page_without_numbers():
             assert not lo.any() and not hi.any()
     held = kv4.values(*kv4.quantise(k[0, 2:, 0].cpu().numpy()))
     assert (lo * unit <= held.min(0)).all() and (hi * unit >= held.max(0)).all()
+
+
+# ------------------------------------------------------------------- rotary positions
+def test_a_position_outside_the_rotary_table_takes_its_nearest_row():
+    Hk, D, page = 1, 64, 16
+    table, pages = table_of([4], page)
+    q, k = tokens(4, 2, D, 3, (1,)), tokens(4, Hk, D, 4, (1,))
+    tab = fc().rotary_table(3, D)
+    got = []
+    for pos in ([[-5, 1, 7, 2 ** 31 - 1]], [[0, 1, 2, 2]]):
+        cache = fc().PagedInt4Cache(pages, Hk, D, page_size=page)
+        cache.pool.zero_()
+        out = cache.append(q, k, k, table, i32([0]), rotary=tab, positions=i32(pos))
+        got.append((out, cache.pool))
+        if pos[0][0] < 0:
+            with pytest.raises(fc()._lib.FlashCodecError, match="rotary table"):
+                cache.check()
+        cache.check()
+    assert all(torch.equal(x, y) for x, y in zip(*got))

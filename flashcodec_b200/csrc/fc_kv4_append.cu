@@ -409,6 +409,7 @@ __device__ __forceinline__ void write_page(const AppendArgs &a, unsigned char *s
         first = (int64_t)(c0 >> lp) + 2 * b;
         n = max(0, (int)min((int64_t)c1, a.T) - max(0, c0));
         t0 = max(0, c0);
+        if ((c0 < 0 || c1 > a.T) && threadIdx.x == 0) atomicOr(a.table.status, kBadLength);  // tokens that are not there
     }
     const int len = a.lengths[b];
     if (len < 0 || n <= 0 || slot < first) return;
@@ -631,6 +632,7 @@ __device__ __forceinline__ void turn_queries(const AppendArgs &a) {
     int h = (int)((uint32_t)unit - (uint32_t)t * a.q_units) * a.q_heads + g;
     const int end = min(h - g + a.q_heads, a.Hq);
     int64_t b, row;
+    bool none = false;  // a row of no sequence
     if (a.S) {
         b = (uint32_t)t / (uint32_t)a.S;
         row = t - b * a.S;
@@ -638,9 +640,18 @@ __device__ __forceinline__ void turn_queries(const AppendArgs &a) {
         const int *cu = a.cu;
         b = warp_find([=](int i) { return (int64_t)cu[i]; }, a.B, t);
         row = t;
+        none = t < cu[b] || t >= cu[b + 1];
     }
     const T *q = static_cast<const T *>(a.q) + (a.S ? b * a.q_sb : 0) + row * a.q_ss + li * 8;
     T *qo = static_cast<T *>(a.qo) + (a.S ? b * a.qo_sb : 0) + row * a.qo_ss + li * 8;
+    if (none) {
+        const float2 o = pair(0.f, 0.f);
+        for (; live && h < end; h += TPP)
+#pragma unroll
+            for (int k = 0; k < CH; k++)
+                store_row(qo + h * a.qo_sh + k * L::half * 8, a.vec & 2, Row{{o, o}, {o, o}});
+        return;
+    }
     Raw<T> raw[N][CH];
     auto load = [&](int h0) {
 #pragma unroll

@@ -41,7 +41,7 @@ from . import _kernels as K
 from . import _lib
 
 _STATUS = ((1, "a page outside the pool"),
-           (2, "a length or position past what the page table holds"),
+           (2, "a length or position past what the page table holds, or cu_seqlens past the rows given"),
            (4, "a position outside the rotary table"))
 
 
@@ -194,7 +194,9 @@ class PagedInt4Cache:
 
         q, k, v: (B, S, H, D), (B, H, D) for one token each, or packed (T, H, D)
             with ``cu_seqlens`` (B + 1,) int32; fp32, bf16 or fp16, any strides
-            with unit stride along D.  q may be None.
+            with unit stride along D.  q may be None.  Packed rows of no sequence
+            (from cu_seqlens[B] on: a captured batch has a fixed number) are not
+            stored, and their queries come out as zeros.
         lengths: (B,) int32, tokens held before the call (unchanged by it); a
             negative one skips the sequence.
         q_weight, k_weight: (D,) weights of a per-head RMS norm (``eps``), or None.

@@ -565,9 +565,11 @@ FC_API int fc_ipc_close_handle(void *base);
  *
  * status   device int, required: bits are OR-ed in when a kernel meets a page
  *          outside the pool (FC_KV4_BAD_PAGE), a length or position past what
- *          the table can hold (FC_KV4_BAD_LENGTH) or a position outside the
- *          rotary table (FC_KV4_BAD_POSITION).  No kernel accesses memory
- *          outside the buffers then: appends skip the tokens that have no page;
+ *          the table can hold, or cu_seqlens past the rows that there are
+ *          (FC_KV4_BAD_LENGTH), or a position outside the rotary table
+ *          (FC_KV4_BAD_POSITION).  No kernel accesses memory
+ *          outside the buffers then: appends skip the tokens that have no page
+ *          or no row;
  *          heads whose position has no row of the rotary table are turned by
  *          the nearest one, and stored; attention over such pages or lengths
  *          gives rows that are not valid.
@@ -584,7 +586,9 @@ FC_API int64_t fc_kv4_page_bytes(int64_t Hk, int64_t D, int64_t page_size);
  * pages, and write the queries back.
  * Tokens come as (B, S, H, D) with strides *_sb, *_ss, *_sh (cu_seqlens NULL,
  * T = B * S), or packed as (T, H, D) with cu_seqlens (B + 1) int32 (S and the
- * *_sb strides are not used).  Sequence b's tokens go to positions
+ * *_sb strides are not used); rows before cu_seqlens[0] and from cu_seqlens[B] on
+ * belong to no sequence (a captured batch of fixed size), nothing is stored of
+ * them and their queries are zeros.  Sequence b's tokens go to positions
  * lengths[b], lengths[b] + 1, ...; a negative length skips the sequence
  * (its queries are still turned).  lengths is not changed.
  * q, q_out  (.., Hq, D) or NULL with Hq = 0.  q_out may be q, but must not overlap

@@ -81,3 +81,53 @@ def test_a_position_outside_the_rotary_table_takes_its_nearest_row():
                 cache.check()
         cache.check()
     assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+# -------------------------------------------------------------- padded packed batches
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("front,new,T", [(0, [3, 1, 20], 64), (0, [5, 0, 11], 16), (0, [0, 0, 0], 40), (21, [3, 0, 19], 50),
+                                         (16, [1, 15, 16], 48), (3, [2, 2, 2], 9), (0, [16, 16, 0], 33)])
+def test_rows_of_no_sequence_in_a_packed_batch(dtype, front, new, T):
+    """A captured prefill has a fixed number of rows, more than its sequences need: the others'
+    queries are zeros and they ask for no position."""
+    Hq, Hk, D, page, ctx = 4, 2, 64, 16, [5, 16, 31]
+    cu = np.concatenate([[front], front + np.cumsum(new)]).astype(int)
+    q, k, v = (tokens(T, H, D, 5 + i).to(dtype) for i, H in enumerate((Hq, Hk, Hk)))
+    table, pages = table_of([a + b for a, b in zip(new, ctx)], page)
+    tab = fc().rotary_table(max(a + b for a, b in zip(new, ctx)), D)  # no row beyond what is held
+    pools = []
+    for padded in (True, False):
+        rows = slice(0, T) if padded else slice(front, int(cu[-1]))
+        cache = fc().PagedInt4Cache(pages, Hk, D, page_size=page)
+        cache.pool.zero_()
+        at = i32((cu if padded else cu - front).tolist())
+        if padded or cu[-1] > front:
+            out = cache.append(q[rows], k[rows], v[rows], table, i32(ctx), cu_seqlens=at, rotary=tab,
+                               q_weight=torch.ones(D, device="cuda", dtype=dtype))
+        else:
+            out = q[rows]
+        cache.check()
+        pools.append((cache.pool, out))
+        if padded:
+            got = out
+            gk, gv = cache.read(table, i32(ctx), count=T, cu_seqlens=at, dtype=dtype)
+            assert (out[: front] == 0).all() and (out[int(cu[-1]):] == 0).all()
+            mine = slice(front, int(cu[-1]))
+            held = kv4.values(*kv4.quantise(v[mine].float().cpu().numpy()))
+            assert torch.equal(gv[mine].cpu(), torch.from_numpy(held).to(dtype))
+    cache.check()
+    assert torch.equal(pools[0][0], pools[1][0])
+    assert torch.equal(got[front:int(cu[-1])], pools[1][1])
+
+
+def test_tokens_that_a_packed_batch_cuts_off_are_reported():
+    Hk, D, page, T = 1, 64, 16, 12
+    k = tokens(T, Hk, D, 9)
+    table, pages = table_of([40, 40], page)
+    cache = fc().PagedInt4Cache(pages, Hk, D, page_size=page)
+    for cu in ([0, 5, 13], [0, 40, 41], [0, 12, 13]):
+        cache.append(None, k, k, table, i32([0, 0]), cu_seqlens=i32(cu))
+        with pytest.raises(fc()._lib.FlashCodecError, match="past what"):
+            cache.check()
+    cache.append(None, k, k, table, i32([0, 0]), cu_seqlens=i32([0, 5, 12]))
+    cache.check()

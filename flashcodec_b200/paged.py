@@ -256,11 +256,12 @@ class PagedInt4Cache:
             if rotary.dtype is not torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous():
                 raise ValueError("rotary must be a contiguous fp32 (positions, R) tensor")
             turn = (rotary.data_ptr(), *rotary.shape)
+        pos = None
         if positions is not None:
             self._ints("positions", positions, shape[:-2] if positions.dim() == 2 else (T,))
-            positions = positions.data_ptr()
+            pos = positions.data_ptr()
         K.kv4_append(self, (*q_at, heads, *k_at, *v_at), dtype, B, S, T, cu, lengths.data_ptr(),
-                     positions, w_at, w_dtype, eps, turn, bool(interleaved), table)
+                     pos, w_at, w_dtype, eps, turn, bool(interleaved), table)
         return q_out
 
     def attend(self, q, page_table, lengths, *, scale=None, selected=None, out=None,
@@ -329,19 +330,21 @@ class PagedInt4Cache:
         B, table = self._table(page_table)
         if count is None or count < 0:
             raise ValueError("read needs the number of tokens (count)")
+        # (the tensors stay named: a caller's temporary would be freed, and the outputs be put there)
+        at = cu = None
         if starts is not None:
             self._ints("starts", starts, (B,))
-            starts = starts.data_ptr()
+            at = starts.data_ptr()
         H, D = self.num_kv_heads, self.head_dim
         if cu_seqlens is not None:
             self._ints("cu_seqlens", cu_seqlens, (B + 1,))
-            cu_seqlens = cu_seqlens.data_ptr()
+            cu = cu_seqlens.data_ptr()
             shape, S, T = (count, H, D), 0, count
         else:
             shape, S, T = (B, count, H, D), count, B * count
         k = torch.empty(shape, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        K.kv4_read(self, table, starts, B, S, T, cu_seqlens, k.data_ptr(), v.data_ptr(), dtype,
+        K.kv4_read(self, table, at, B, S, T, cu, k.data_ptr(), v.data_ptr(), dtype,
                    (count * H * D, H * D, D))
         return k, v
 

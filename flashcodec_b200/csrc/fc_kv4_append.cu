@@ -748,6 +748,18 @@ __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ ReadA
     const int lane = threadIdx.x & 31;
     if (unit >= (int64_t)a.slots * a.Hk) return;
     const int slot = (int)(unit / a.Hk), h = (int)(unit % a.Hk);
+    T *ko = static_cast<T *>(a.k) + h * a.o_sh;
+    T *vo = static_cast<T *>(a.v) + h * a.o_sh;
+    auto clear = [&](int64_t row, int64_t end) {  // rows that nothing is read for
+        const float2 o = pair(0.f, 0.f);
+        const Row zero{{o, o}, {o, o}};
+        const int n = (int)(end - row) * 4 * W;
+        for (int u = lane; u < n; u += 32) {
+            const int64_t at = (row + u / (4 * W)) * a.o_ss + u % (4 * W) * 8;
+            store_row(ko + at, a.vec & 1, zero);
+            store_row(vo + at, a.vec & 2, zero);
+        }
+    };
     int b, n;
     int64_t first, t0;
     if (a.S) {
@@ -756,31 +768,51 @@ __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ ReadA
         first = (int64_t)b * per;
         n = (int)a.S;
         t0 = 0;
+        ko += b * a.o_sb;
+        vo += b * a.o_sb;
     } else {
         const int *cu = a.cu;
+        // slots before and behind the sequences' are for the rows of none
+        const int64_t c0 = min((int64_t)max(cu[0], 0), a.T), cB = max(cu[a.B], 0);
+        const int64_t behind = (cB >> 4) + 2 * a.B;
+        if (slot < c0 >> 4) return clear((int64_t)slot * 16, (int64_t)slot * 16 + 16);
+        if (slot == a.slots - 1) return clear(c0 & ~15, c0);
+        if (slot >= behind) {
+            const int64_t row = cB + (slot - behind) * 16;
+            if (row < a.T) clear(row, min(row + 16, a.T));
+            return;
+        }
         b = warp_find([=](int i) { return (int64_t)(cu[i] >> 4) + 2 * i; }, a.B, slot);
         first = (int64_t)(cu[b] >> 4) + 2 * b;
         n = max(0, (int)min((int64_t)cu[b + 1], a.T) - max(0, cu[b]));
         t0 = max(0, cu[b]);
+        if ((cu[b] < 0 || cu[b + 1] > a.T) && lane == 0) atomicOr(a.table.status, kBadLength);
     }
-    const int start = a.starts ? a.starts[b] : 0;
-    if (start < 0 || n <= 0 || slot < first) return;
-    const int64_t tile64 = (start >> 4) + (slot - first), end = (int64_t)start + n;
-    if (tile64 * 16 >= end) return;
-    if (tile64 * 16 >= (int64_t)a.table.max_pages << a.table.log_page) {
-        if (lane == 0) atomicOr(a.table.status, kBadLength);
-        return;
-    }
-    const int tile = (int)tile64, tb = tile * 16;
-    const int lo = max(start, tb) - tb, hi = (int)min(end - tb, (int64_t)16);
-    if (lo >= hi) return;
+    int start = a.starts ? a.starts[b] : 0;
+    const bool skipped = start < 0;
+    if (skipped) start = 0;
+    if (n <= 0 || slot < first) return;
+    const int64_t tile64 = (start >> 4) + (slot - first), tb = tile64 * 16, end = (int64_t)start + n;
+    if (tb >= end) return;
+    const int lo = (int)(max((int64_t)start, tb) - tb), hi = (int)min(end - tb, (int64_t)16);
+    const int64_t row0 = t0 + (tb - start);
+    if (skipped) return clear(row0 + lo, row0 + hi);
+    int bad = 0, id = 0;
     const int tpp = a.table.log_page - 4;
-    const int id = a.table.page(b, tile >> tpp);
+    const int64_t page = tile64 >> tpp;
+    if (page >= a.table.max_pages) {
+        bad = kBadLength;
+    } else {
+        id = a.table.pages[b * a.table.stride + page];
+        if ((unsigned)id >= (unsigned)a.table.num_pages) bad = kBadPage;
+    }
+    if (bad) {
+        if (lane == 0) atomicOr(a.table.status, bad);
+        return clear(row0 + lo, row0 + hi);
+    }
+    const int tile = (int)tile64;
     const unsigned char *in = a.pool + ((((int64_t)id * a.Hk + h) << tpp) + (tile & ((1 << tpp) - 1))) *
                                            tile_bytes(W);
-    T *ko = static_cast<T *>(a.k) + (a.S ? b * a.o_sb : 0) + h * a.o_sh;
-    T *vo = static_cast<T *>(a.v) + (a.S ? b * a.o_sb : 0) + h * a.o_sh;
-    const int64_t row0 = t0 + (tb - start);
     // values: to shared memory while the keys are turned
     uint32_t *vs = values[threadIdx.x >> 5];
     {
@@ -1011,7 +1043,7 @@ extern "C" int fc_kv4_read(const void *pool, int64_t num_pages, int64_t Hk, int6
     a.k = k_out; a.v = v_out; a.o_sb = o_sb; a.o_ss = o_ss; a.o_sh = o_sh;
     a.vec = (rows_aligned(k_out, dtype, o_sb, o_ss, o_sh) ? 1 : 0) |
             (rows_aligned(v_out, dtype, o_sb, o_ss, o_sh) ? 2 : 0);
-    const int64_t slots = a.S ? B * ((S + 30) / 16) : T / 16 + 2 * B;
+    const int64_t slots = a.S ? B * ((S + 30) / 16) : T / 16 + 2 * B + 2;
     const int64_t blocks = (slots * Hk + 3) / 4;
     if (slots > 0x7fffffff || blocks > 0x7fffffff) {
         set_error("kv4_read: too many tokens for one call");

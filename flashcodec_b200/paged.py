@@ -325,7 +325,9 @@ class PagedInt4Cache:
         """The values held, as (k, v): ``count`` tokens of every sequence from
         position ``starts`` ((B,) int32; None: 0) as (B, count, Hk, D), or, with
         ``cu_seqlens``, cu_seqlens[b + 1] - cu_seqlens[b] of sequence b, ``count``
-        in all, packed as (count, Hk, D)."""
+        in all, packed as (count, Hk, D).  Zeros for sequences with a negative
+        start, for packed rows of no sequence, and where no page can be read
+        (which ``check`` reports)."""
         self._here(page_table, starts, cu_seqlens)
         B, table = self._table(page_table)
         if count is None or count < 0:

@@ -622,7 +622,8 @@ FC_API int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t q_sh
 /* The values held, code * scale rounded to dtype: positions starts[b] + i
  * (starts NULL: from 0) of every sequence, i < S, into k_out and v_out
  * (B, S, Hk, D), or packed (T, Hk, D) with cu_seqlens; both of strides o_sb,
- * o_ss, o_sh. */
+ * o_ss, o_sh.  Every row is written: those of sequences with a negative start,
+ * packed rows of no sequence, and rows that `status` reports, with zeros. */
 FC_API int fc_kv4_read(const void *pool, int64_t num_pages, int64_t Hk, int64_t D,
                        int64_t page_size, const int *page_table, int64_t table_stride,
                        int64_t max_pages, const int *starts, int64_t B, int64_t S, int64_t T,

@@ -89,7 +89,7 @@ def test_a_position_outside_the_rotary_table_takes_its_nearest_row():
                                          (16, [1, 15, 16], 48), (3, [2, 2, 2], 9), (0, [16, 16, 0], 33)])
 def test_rows_of_no_sequence_in_a_packed_batch(dtype, front, new, T):
     """A captured prefill has a fixed number of rows, more than its sequences need: the others'
-    queries are zeros and they ask for no position."""
+    queries are zeros, they ask for no position, and reading gives zeros there."""
     Hq, Hk, D, page, ctx = 4, 2, 64, 16, [5, 16, 31]
     cu = np.concatenate([[front], front + np.cumsum(new)]).astype(int)
     q, k, v = (tokens(T, H, D, 5 + i).to(dtype) for i, H in enumerate((Hq, Hk, Hk)))
@@ -110,8 +110,11 @@ def test_rows_of_no_sequence_in_a_packed_batch(dtype, front, new, T):
         pools.append((cache.pool, out))
         if padded:
             got = out
+            junk = [torch.full((T, Hk, D), math.nan, device="cuda", dtype=dtype) for _ in range(4)]
+            del junk  # what an output of this size may be made of
             gk, gv = cache.read(table, i32(ctx), count=T, cu_seqlens=at, dtype=dtype)
-            assert (out[: front] == 0).all() and (out[int(cu[-1]):] == 0).all()
+            for x in (gk, gv, out):
+                assert (x[: front] == 0).all() and (x[int(cu[-1]):] == 0).all()
             mine = slice(front, int(cu[-1]))
             held = kv4.values(*kv4.quantise(v[mine].float().cpu().numpy()))
             assert torch.equal(gv[mine].cpu(), torch.from_numpy(held).to(dtype))
@@ -129,5 +132,45 @@ def test_tokens_that_a_packed_batch_cuts_off_are_reported():
         cache.append(None, k, k, table, i32([0, 0]), cu_seqlens=i32(cu))
         with pytest.raises(fc()._lib.FlashCodecError, match="past what"):
             cache.check()
+        cache.read(table, count=T, cu_seqlens=i32(cu))
+        with pytest.raises(fc()._lib.FlashCodecError, match="past what"):
+            cache.check()
     cache.append(None, k, k, table, i32([0, 0]), cu_seqlens=i32([0, 5, 12]))
+    cache.check()
+
+
+# ------------------------------------------------------------------ rows that are not held
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,page", [(64, 16), (96, 32), (128, 64)])
+def test_read_gives_zeros_where_nothing_can_be_read(dtype, D, page):
+    """Sequences that are skipped (a negative start), positions past the page table, pages outside
+    the pool: zeros, and a bit of the status for the last two."""
+    Hk, n = 2, 3 * page
+    table, pages = table_of([n] * 4, page)
+    cache = fc().PagedInt4Cache(pages, Hk, D, page_size=page)
+    x = tokens(n, Hk, D, 10, (4,))
+    cache.append(None, x, x, table, i32([0] * 4))
+    want = torch.from_numpy(kv4.values(*kv4.quantise(x.cpu().numpy()))).to(dtype).cuda()
+    junk = [torch.full((4, n, Hk, D), math.nan, device="cuda", dtype=dtype) for _ in range(4)]
+    del junk
+    for y in cache.read(table, i32([-1, 0, -2 ** 31, 0]), count=n, dtype=dtype):
+        assert (y[[0, 2]] == 0).all() and torch.equal(y[[1, 3]], want[[1, 3]])
+    cache.check()
+    start = page + 5  # past the last page from token n - start on
+    for y in cache.read(table, i32([start, 0, 2 ** 31 - 1, 0]), count=n, dtype=dtype):
+        assert torch.equal(y[0, : n - start], want[0, start:]) and (y[0, n - start:] == 0).all()
+        assert (y[2] == 0).all() and torch.equal(y[[1, 3]], want[[1, 3]])
+    with pytest.raises(fc()._lib.FlashCodecError, match="past what"):
+        cache.check()
+    bad = table.clone()
+    bad[1, 1] = pages
+    for y in cache.read(bad, None, count=n, dtype=dtype):
+        assert (y[1, page:2 * page] == 0).all() and torch.equal(y[1, :page], want[1, :page])
+    with pytest.raises(fc()._lib.FlashCodecError, match="page outside"):
+        cache.check()
+    # packed, with a sequence that is skipped in the middle
+    cu = i32([0, 7, 30, 30 + page, 40 + page])
+    for y in cache.read(table, i32([3, -1, 0, 1]), count=40 + page, cu_seqlens=cu, dtype=dtype):
+        assert torch.equal(y[:7], want[0, 3:10]) and (y[7:30] == 0).all()
+        assert torch.equal(y[30:30 + page], want[2, :page]) and torch.equal(y[30 + page:], want[3, 1:11])
     cache.check()

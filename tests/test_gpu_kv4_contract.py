@@ -174,3 +174,47 @@ def test_read_gives_zeros_where_nothing_can_be_read(dtype, D, page):
         assert torch.equal(y[:7], want[0, 3:10]) and (y[7:30] == 0).all()
         assert torch.equal(y[30:30 + page], want[2, :page]) and torch.equal(y[30 + page:], want[3, 1:11])
     cache.check()
+
+
+# ------------------------------------------------------------------------ fused buffers
+@pytest.mark.parametrize("order", ["bshd", "bhsd", "hbsd", "sbhd"])
+@pytest.mark.parametrize("B,S", [(2, 3), (1, 5), (3, 1)])
+def test_queries_written_over_themselves_in_a_fused_buffer(order, B, S):
+    """One buffer holds the heads of queries, keys and values, in whatever order of its dims."""
+    Hq, Hk, D, page = 4, 2, 64, 16
+    H = Hq + 2 * Hk
+    x = tokens(S, H, D, 11, (B,)).bfloat16()
+    perm = ["bshd".index(c) for c in order]
+    back = [order.index(c) for c in "bshd"]
+    table, pages = table_of([S] * B, page)
+    tab = fc().rotary_table(16, D)
+    got = []
+    for fused in (False, True):
+        y = x.permute(perm).contiguous().permute(back)
+        assert y.shape == x.shape
+        q, k, v = (y if fused else x.clone()).split([Hq, Hk, Hk], 2)
+        cache = fc().PagedInt4Cache(pages, Hk, D, page_size=page)
+        cache.pool.zero_()
+        out = cache.append(q, k, v, table, i32([0] * B), rotary=tab, q_out=q if fused else None)
+        got.append((out.contiguous(), cache.pool))
+        assert torch.equal(y[:, :, Hq:], x[:, :, Hq:])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_fused_buffers_that_overlap_are_still_refused():
+    Hq, Hk, D, page, B, S = 4, 2, 64, 16, 2, 3
+    table, pages = table_of([S] * B, page)
+    cache = fc().PagedInt4Cache(pages, Hk, D, page_size=page)
+    for perm in ([0, 1, 2, 3], [0, 2, 1, 3]):
+        y = tokens(S, 9, D, 12, (B,)).permute(perm).contiguous().permute(perm)
+        q, out, k = y[:, :, :Hq], y[:, :, 1:1 + Hq], y[:, :, 7:9]
+        for a, b, c in ((q, k, out), (y[:, :, 5:9], y[:, :, 3:5], q), (q, y[:, :, 3:5], q)):
+            with pytest.raises(ValueError, match="overlaps"):
+                cache.append(a, b, k.clone(), table, i32([0] * B), q_out=c)
+        cache.append(q, k, k.clone(), table, i32([0] * B), q_out=q)
+    # two sets of rows of one buffer that lie between each other in no such order
+    y = torch.zeros(4096, device="cuda")
+    a = y.as_strided((2, 3, 2, D), (300, 70, 1000, 1))
+    b = y.as_strided((2, 3, 2, D), (310, 70, 1000, 1), 5)
+    with pytest.raises(ValueError, match="overlaps"):
+        cache.append(a, b, b.clone(), table, i32([0] * B), q_out=a)

@@ -36,6 +36,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _kernels as K
 from . import _lib
@@ -144,8 +145,9 @@ class PagedInt4Cache:
     # ------------------------------------------------------------ argument checks
     # (a decode step calls these for every layer: each looks at a tensor's attributes once)
     def _here(self, *tensors):
-        """Tensors (or None) on the cache's device, none asking for a gradient."""
+        """Tensors (or None) on the cache's device, none asking for a gradient or with a tangent."""
         index, grad = self._index, torch.is_grad_enabled()
+        dual = getattr(forward_ad, "_current_level", 0) >= 0  # inside a dual level
         for t in tensors:
             if t is None:
                 continue
@@ -155,6 +157,9 @@ class PagedInt4Cache:
             if grad and t.requires_grad:
                 raise RuntimeError("the 4-bit cache holds rounded values and has no gradient: "
                                    "call it under torch.no_grad()")
+            if dual and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the 4-bit cache holds rounded values and has no tangent: "
+                                   "pass the primal of a dual tensor")
 
     def _ints(self, name, t, shape):
         if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():

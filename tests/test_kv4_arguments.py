@@ -66,3 +66,20 @@ def test_arguments_live_until_the_launch(cache, monkeypatch, call):
     else:
         cache.select(rows(3, heads=4), table(), tmp(i32(1, 1, 2)), 3)
     assert tmp.launched
+
+
+def test_dual_tensors_are_refused(cache, monkeypatch):
+    """A tangent would be dropped: forward-mode differentiation is refused like reverse mode."""
+    from torch.autograd import forward_ad
+    monkeypatch.setattr(K, "kv4_attn", lambda *args: None)
+    q, table, lengths = torch.zeros(3, 4, D), torch.zeros(3, 4, dtype=torch.int32), i32(1, 1, 2)
+    with forward_ad.dual_level():
+        cache.attend(q, table, lengths)
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        for guard in (torch.no_grad(), torch.enable_grad()):
+            with guard, pytest.raises(RuntimeError, match="tangent"):
+                cache.attend(dual, table, lengths)
+        cache.attend(forward_ad.unpack_dual(dual).primal, table, lengths)
+    cache.attend(q, table, lengths)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        cache.attend(q.clone().requires_grad_(), table, lengths)

@@ -111,6 +111,8 @@ class PagedInt4Cache:
 
     Attributes: ``pool`` (num_pages, bytes) uint8; ``bounds`` (num_pages, Hk, 2,
     D) int8 and ``exponents`` (num_pages, Hk) int32, or None; ``status`` int32.
+    They cannot be replaced, only written to (a cache restored from a file:
+    ``cache.pool.copy_(saved)``).
     """
 
     def __init__(self, num_pages, num_kv_heads, head_dim, page_size=64, bounds=False,
@@ -127,20 +129,27 @@ class PagedInt4Cache:
         self.num_pages, self.num_kv_heads = int(num_pages), int(num_kv_heads)
         self.head_dim, self.page_size = int(head_dim), int(page_size)
         self.page_bytes = K.kv4_page_bytes(self.num_kv_heads, self.head_dim, self.page_size)
-        self.pool = torch.empty(self.num_pages, self.page_bytes, dtype=torch.uint8, device=dev)
-        self.bounds = self.exponents = None
+        self._pool = torch.empty(self.num_pages, self.page_bytes, dtype=torch.uint8, device=dev)
+        self._bounds = self._exponents = None
         if bounds:
-            self.bounds = torch.zeros(self.num_pages, self.num_kv_heads, 2, self.head_dim,
-                                      dtype=torch.int8, device=dev)
-            self.exponents = torch.zeros(self.num_pages, self.num_kv_heads, dtype=torch.int32,
-                                         device=dev)
-        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+            self._bounds = torch.zeros(self.num_pages, self.num_kv_heads, 2, self.head_dim,
+                                       dtype=torch.int8, device=dev)
+            self._exponents = torch.zeros(self.num_pages, self.num_kv_heads, dtype=torch.int32,
+                                          device=dev)
+        self._status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._index, self._scale, self._lib = dev.index, self.head_dim ** -0.5, _lib.load()
-        self._status_ptr = self.status.data_ptr()
-        self._pool_args = (self.pool.data_ptr(), self.num_pages, self.num_kv_heads, self.head_dim,
+        self._status_ptr = self._status.data_ptr()
+        self._pool_args = (self._pool.data_ptr(), self.num_pages, self.num_kv_heads, self.head_dim,
                            self.page_size)
-        self._bounds_args = (self.bounds.data_ptr(), self.exponents.data_ptr()) if bounds \
+        self._bounds_args = (self._bounds.data_ptr(), self._exponents.data_ptr()) if bounds \
             else (None, None)
+
+    # The calls pass these tensors' addresses, taken once: their contents may be written, they
+    # themselves stay.
+    pool = property(lambda self: self._pool)
+    bounds = property(lambda self: self._bounds)
+    exponents = property(lambda self: self._exponents)
+    status = property(lambda self: self._status)
 
     # ------------------------------------------------------------ argument checks
     # (a decode step calls these for every layer: each looks at a tensor's attributes once)

@@ -17,7 +17,7 @@ def cache(monkeypatch):
     cache = object.__new__(PagedInt4Cache)
     cache.device, cache._index, cache._scale = torch.device("cpu"), -1, 1.0  # a CPU tensor's index
     cache.num_kv_heads, cache.head_dim, cache.page_size = HK, D, PAGE
-    cache.bounds = cache.exponents = torch.zeros(1)
+    cache._bounds = cache._exponents = torch.zeros(1)
     return cache
 
 
@@ -83,3 +83,14 @@ def test_dual_tensors_are_refused(cache, monkeypatch):
     cache.attend(q, table, lengths)
     with pytest.raises(RuntimeError, match="no gradient"):
         cache.attend(q.clone().requires_grad_(), table, lengths)
+
+
+@pytest.mark.parametrize("name", ["pool", "bounds", "exponents", "status"])
+def test_the_caches_tensors_cannot_be_replaced(cache, name):
+    """Launches go by their addresses: the kernels would write to what was freed."""
+    cache._pool = cache._status = torch.zeros(1)
+    held = getattr(cache, name)
+    with pytest.raises(AttributeError):
+        setattr(cache, name, held.clone())
+    getattr(cache, name).fill_(3)
+    assert getattr(cache, name) is held and held.item() == 3

@@ -34,6 +34,8 @@
 // into calls.
 #pragma once
 
+#include <algorithm>
+
 #include "fc_common.cuh"
 
 namespace fc {
@@ -192,6 +194,73 @@ inline int check_cache(const char *what, int64_t B, int64_t Hk, int64_t D, int64
     return FC_OK;
 }
 
+// Rows (sequence, token, head) of D elements, strides in elements.
+struct Rows {
+    const void *p;
+    int64_t sb, ss, sh, H;
+};
+
+// The same rows in the same places.
+inline bool same_rows(const Rows &x, const Rows &y, int64_t B, int64_t S) {
+    return x.p == y.p && (x.H == 1 || x.sh == y.sh) && (S == 1 || x.ss == y.ss) && (B == 1 || x.sb == y.sb);
+}
+
+// Rows of an expanded tensor: several in one place.
+inline bool rows_repeat(const Rows &x, int64_t B, int64_t S) {
+    return (B > 1 && x.sb == 0) || (S > 1 && x.ss == 0) || (x.H > 1 && x.sh == 0);
+}
+
+// For slices of the heads of one buffer, its dims in any order: whether they have heads in
+// common (0, 1), or -1 for sets that are no such slices.
+inline int heads_meet(const Rows &x, const Rows &y, int64_t B, int64_t S, int64_t D, int64_t size) {
+    const int64_t sh = x.H > 1 ? x.sh : y.sh;
+    const int64_t d = (int64_t)reinterpret_cast<uintptr_t>(y.p) - (int64_t)reinterpret_cast<uintptr_t>(x.p);
+    if ((B > 1 && x.sb != y.sb) || (S > 1 && x.ss != y.ss) || (y.H > 1 && y.sh != sh) || sh <= 0 ||
+        d % (sh * size))
+        return -1;
+    const int64_t h = d / (sh * size);  // of x, where y begins
+    // their rows lie apart when each dim's stride passes all that the ones inside it reach
+    struct { int64_t n, stride; } dim[3] = {{B, x.sb}, {S, x.ss}, {(x.H > h + y.H ? x.H : h + y.H) - (h < 0 ? h : 0), sh}};
+    for (auto &z : dim)
+        if (z.n <= 1) z.stride = 0;
+    std::sort(dim, dim + 3, [](const auto &a, const auto &b) { return a.stride < b.stride; });
+    int64_t reach = D;
+    for (const auto &z : dim) {
+        if (z.n <= 1) continue;
+        if (z.stride < reach) return -1;
+        reach += (z.n - 1) * z.stride;
+    }
+    return h < x.H && h + y.H > 0;
+}
+
+// Whether two sets of B x S rows (packed: 1 x T) can share a byte.  Sets whose spans meet
+// are told apart where they are slices of the heads of one buffer, or have equal strides from
+// token to token and heads in runs that do not meet within one.
+inline bool rows_meet(const Rows &x, const Rows &y, int64_t B, int64_t S, int64_t D, int64_t size) {
+    auto span = [&](const Rows &r, int64_t &lo, int64_t &hi) {
+        lo = hi = 0;
+        for (int64_t e : {(B - 1) * r.sb, (S - 1) * r.ss, (r.H - 1) * r.sh}) (e < 0 ? lo : hi) += e;
+        const int64_t base = (int64_t)reinterpret_cast<uintptr_t>(r.p);
+        lo = base + lo * size;
+        hi = base + (hi + D) * size;
+    };
+    int64_t x0, x1, y0, y1;
+    span(x, x0, x1);
+    span(y, y0, y1);
+    if (x0 >= y1 || y0 >= x1) return false;
+    const int slices = heads_meet(x, y, B, S, D, size);
+    if (slices >= 0) return slices;
+    const int64_t step = S > 1 ? x.ss : x.sb;  // from token to token
+    const bool same = (S == 1 || x.ss == y.ss) && (B == 1 || x.sb == y.sb) &&
+                      (S == 1 || B == 1 || x.sb % (step ? step : 1) == 0);
+    if (!same || (S * B > 1 && step <= 0) || x.sh < 0 || y.sh < 0) return true;
+    const int64_t xw = ((x.H - 1) * x.sh + D) * size, yw = ((y.H - 1) * y.sh + D) * size;
+    int64_t d = (int64_t)reinterpret_cast<uintptr_t>(y.p) - (int64_t)reinterpret_cast<uintptr_t>(x.p);
+    if (S * B == 1) return d < xw && -d < yw;
+    const int64_t pitch = step * size;
+    d = (d % pitch + pitch) % pitch;
+    return d < xw || d + yw > pitch;
+}
 
 }  // namespace kv4
 }  // namespace fc

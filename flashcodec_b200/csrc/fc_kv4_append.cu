@@ -20,8 +20,6 @@
 // it writes: codes that share a word with older tokens and the page bounds are
 // read, merged and written without atomics.  The other blocks take query heads,
 // one warp for one token's heads.
-#include <algorithm>
-
 #include "fc_kv4.cuh"
 
 namespace fc {
@@ -865,64 +863,6 @@ __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ ReadA
     }
 }
 
-// Rows (sequence, token, head) of D elements, strides in elements.
-struct Rows {
-    const void *p;
-    int64_t sb, ss, sh, H;
-};
-
-// For slices of the heads of one buffer, its dims in any order: whether they have heads in
-// common (0, 1), or -1 for sets that are no such slices.
-int heads_meet(const Rows &x, const Rows &y, int64_t B, int64_t S, int64_t D, int64_t size) {
-    const int64_t sh = x.H > 1 ? x.sh : y.sh;
-    const int64_t d = (int64_t)reinterpret_cast<uintptr_t>(y.p) - (int64_t)reinterpret_cast<uintptr_t>(x.p);
-    if ((B > 1 && x.sb != y.sb) || (S > 1 && x.ss != y.ss) || (y.H > 1 && y.sh != sh) || sh <= 0 ||
-        d % (sh * size))
-        return -1;
-    const int64_t h = d / (sh * size);  // of x, where y begins
-    // their rows lie apart when each dim's stride passes all that the ones inside it reach
-    struct { int64_t n, stride; } dim[3] = {{B, x.sb}, {S, x.ss}, {(x.H > h + y.H ? x.H : h + y.H) - (h < 0 ? h : 0), sh}};
-    for (auto &z : dim)
-        if (z.n <= 1) z.stride = 0;
-    std::sort(dim, dim + 3, [](const auto &a, const auto &b) { return a.stride < b.stride; });
-    int64_t reach = D;
-    for (const auto &z : dim) {
-        if (z.n <= 1) continue;
-        if (z.stride < reach) return -1;
-        reach += (z.n - 1) * z.stride;
-    }
-    return h < x.H && h + y.H > 0;
-}
-
-// Whether two sets of B x S rows (packed: 1 x T) can share a byte.  Sets whose spans meet
-// are told apart where they are slices of the heads of one buffer, or have equal strides from
-// token to token and heads in runs that do not meet within one.
-bool rows_meet(const Rows &x, const Rows &y, int64_t B, int64_t S, int64_t D, int64_t size) {
-    auto span = [&](const Rows &r, int64_t &lo, int64_t &hi) {
-        lo = hi = 0;
-        for (int64_t e : {(B - 1) * r.sb, (S - 1) * r.ss, (r.H - 1) * r.sh}) (e < 0 ? lo : hi) += e;
-        const int64_t base = (int64_t)reinterpret_cast<uintptr_t>(r.p);
-        lo = base + lo * size;
-        hi = base + (hi + D) * size;
-    };
-    int64_t x0, x1, y0, y1;
-    span(x, x0, x1);
-    span(y, y0, y1);
-    if (x0 >= y1 || y0 >= x1) return false;
-    const int slices = heads_meet(x, y, B, S, D, size);
-    if (slices >= 0) return slices;
-    const int64_t step = S > 1 ? x.ss : x.sb;  // from token to token
-    const bool same = (S == 1 || x.ss == y.ss) && (B == 1 || x.sb == y.sb) &&
-                      (S == 1 || B == 1 || x.sb % (step ? step : 1) == 0);
-    if (!same || (S * B > 1 && step <= 0) || x.sh < 0 || y.sh < 0) return true;
-    const int64_t xw = ((x.H - 1) * x.sh + D) * size, yw = ((y.H - 1) * y.sh + D) * size;
-    int64_t d = (int64_t)reinterpret_cast<uintptr_t>(y.p) - (int64_t)reinterpret_cast<uintptr_t>(x.p);
-    if (S * B == 1) return d < xw && -d < yw;
-    const int64_t pitch = step * size;
-    d = (d % pitch + pitch) % pitch;
-    return d < xw || d + yw > pitch;
-}
-
 }  // namespace
 }  // namespace kv4
 }  // namespace fc
@@ -983,13 +923,14 @@ extern "C" int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t 
     if (Hq) {
         const int64_t nb = cu_seqlens ? 1 : B, ns = cu_seqlens ? T : S, size = dtype_size(dtype);
         const Rows out{q_out, qo_sb, qo_ss, qo_sh, Hq};
-        const bool in_place = q == q_out && q_sh == qo_sh && (ns == 1 || q_ss == qo_ss) && (nb == 1 || q_sb == qo_sb);
-        if ((!in_place && rows_meet(out, Rows{q, q_sb, q_ss, q_sh, Hq}, nb, ns, D, size)) ||
+        const Rows in{q, q_sb, q_ss, q_sh, Hq};
+        if ((!same_rows(out, in, nb, ns) && rows_meet(out, in, nb, ns, D, size)) ||
             rows_meet(out, Rows{k, k_sb, k_ss, k_sh, Hk}, nb, ns, D, size) ||
             rows_meet(out, Rows{v, v_sb, v_ss, v_sh, Hk}, nb, ns, D, size)) {
             set_error("kv4_append: q_out overlaps an input (it may be q itself)");
             return FC_EINVAL;
         }
+        if (rows_repeat(out, nb, ns)) { set_error("kv4_append: q_out has rows in one place"); return FC_EINVAL; }
     }
     AppendArgs a{};
     a.q = q; a.k = k; a.v = v; a.qo = q_out;

@@ -1152,6 +1152,12 @@ extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int6
     }
     if (B == 0 || Sq == 0) return FC_OK;
     if (!q || !out || !lengths) { set_error("kv4_attn: null pointer"); return FC_EINVAL; }
+    const Rows to{out, o_sb, o_ss, o_sh, Hq}, from{q, q_sb, q_ss, q_sh, Hq};
+    if (!same_rows(to, from, B, Sq) && rows_meet(to, from, B, Sq, D, dtype_size(dtype))) {
+        set_error("kv4_attn: out overlaps q (it may be q itself)");
+        return FC_EINVAL;
+    }
+    if (rows_repeat(to, B, Sq)) { set_error("kv4_attn: out has rows in one place"); return FC_EINVAL; }
     if (Hk * page_size * (tile_bytes((int)(D / 32)) / 16) > 0x7fffffff) {
         set_error("kv4_attn: pages over 2 GiB");
         return FC_ENOTSUP;

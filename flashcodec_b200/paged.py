@@ -288,6 +288,7 @@ class PagedInt4Cache:
         scale: of the scores (default D ** -0.5).
         selected: (B, Hk, n) int32 from ``select`` (one query per sequence): only
             the tokens of these pages, each named once, count.
+        out: where the outputs go (default: a new tensor; may be q).
         Returns the outputs in q's shape and dtype, and with ``return_lse`` the
         natural log of the softmax sums, q.shape[:-1] fp32.  A query that sees no
         token gives zeros (and -inf).

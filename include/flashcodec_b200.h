@@ -638,7 +638,8 @@ FC_API size_t fc_kv4_attn_workspace_size(int64_t B, int64_t Sq, int64_t Hq, int6
 
 /* Attention of the last Sq tokens of every sequence over the cache:
  *     out = softmax(softmax_scale * q . K^T) . V
- * q (B, Sq, Hq, D), out likewise (its dtype is q's).  Query i of sequence b sees
+ * q (B, Sq, Hq, D), out likewise (its dtype is q's; it may be q itself, but must
+ * not overlap it otherwise).  Query i of sequence b sees
  * positions 0 .. lengths[b] - Sq + i (lengths counts the Sq tokens); one that
  * sees none, and every query of a sequence with lengths[b] <= 0, gets zeros.
  * selected (B, Hk, n_selected) int32, or NULL: only the tokens of these pages

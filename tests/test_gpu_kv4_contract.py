@@ -218,3 +218,30 @@ def test_fused_buffers_that_overlap_are_still_refused():
     b = y.as_strided((2, 3, 2, D), (310, 70, 1000, 1), 5)
     with pytest.raises(ValueError, match="overlaps"):
         cache.append(a, b, b.clone(), table, i32([0] * B), q_out=a)
+
+
+def test_outputs_of_attend_over_the_queries():
+    """Over the queries themselves is fine, whatever pieces the work is cut into; partly over them,
+    or rows in one place, is refused."""
+    Hk, G, D, page, B = 2, 2, 64, 16, 3
+    lens = [9000, 0, 700]
+    table, pages = table_of(lens, page)
+    cache = fc().PagedInt4Cache(pages, Hk, D, page_size=page)
+    for b, n in enumerate(lens):
+        if n:
+            x = tokens(n, Hk, D, 20 + b, (1,))
+            cache.append(None, x, x, table[b:b + 1], i32([0]))
+    for S in (1, 4, 9):
+        y = tokens(S, 6, D, 13, (B,))
+        q = y[:, :, : Hk * G]
+        want = cache.attend(q.clone(), table, i32(lens))
+        for out in (y[:, :, 1:1 + Hk * G], y[:, :, 2:], q[:1].expand(B, -1, -1, -1) if S == 1 else y[:, :1, :4].expand_as(q)):
+            with pytest.raises(ValueError, match="overlaps|one place"):
+                cache.attend(q, table, i32(lens), out=out)
+        with pytest.raises(ValueError, match="one place"):
+            cache.attend(q, table, i32(lens), out=torch.empty(1, S, 1, D, device="cuda").expand_as(q))
+        with pytest.raises(ValueError, match="one place"):
+            cache.append(q, q[:, :, :Hk], q[:, :, :Hk], table, i32([0] * B),
+                         q_out=torch.empty(1, S, 4, D, device="cuda").expand_as(q))
+        assert cache.attend(q, table, i32(lens), out=q).data_ptr() == y.data_ptr()
+        assert torch.equal(q, want)

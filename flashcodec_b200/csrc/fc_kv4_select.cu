@@ -1,7 +1,7 @@
 // Paged 4-bit KV cache: the pages of each sequence and KV head worth attending to.
 //
-// A page's bounds give an upper bound of q . k over its keys: the sum over channels
-// of max(q * least, q * largest).  Summed over the heads of a group this is linear
+// A page's bounds give an upper bound of z . k over its keys, z the rounded queries:
+// the sum over channels of max(z * least, z * largest).  Summed over the heads of a group this is linear
 // in the positive and the negative parts of the queries, so a page costs one dot
 // product of 2 D bytes with two vectors, P = sum_heads max(z, 0) and N = sum_heads
 // min(z, 0), whatever the number of heads:

@@ -11,7 +11,7 @@ operations on it:
   positions, quantisation and the page write, one launch;
 * ``attend``  -- attention of the newest token(s) of every sequence, one launch;
 * ``select``  -- the pages of a long context worth attending to, by a bound on
-  their scores; ``attend(..., selected=pages)`` reads only those;
+  the scores of the rounded queries; ``attend(..., selected=pages)`` reads only those;
 * ``read``    -- the values held, gathered back (the prefix of a prompt's next
   chunk).
 
@@ -316,9 +316,15 @@ class PagedInt4Cache:
         """(B, Hk, count) int32: for every KV head the pages to attend to, ascending,
         then -1.
 
-        A page's score bounds the sum over the group's query heads of q . k for
-        every key in it; the first ``sink`` and last ``recent`` pages of a sequence
-        are always taken, the rest by score (ties: the lower index).  q (B, Hq, D).
+        A page's score bounds the sum over the group's query heads of z . k for
+        every key in it, z being the group's queries in whole numbers up to 127 of
+        one power of two (with 1024 channels of queries and more, of fewer bits).
+        The queries themselves may pass it by half a unit of z times the sum of
+        the page's largest |keys|: small channels beside one far larger count for
+        little.  What the chosen pages hold of the softmax is not bounded.
+
+        The first ``sink`` and last ``recent`` pages of a sequence are always taken,
+        the rest by score (ties: the lower index).  q (B, Hq, D).
         The cache needs ``bounds=True``.
         """
         if self.bounds is None:

@@ -663,11 +663,12 @@ FC_API size_t fc_kv4_select_workspace_size(int64_t B, int64_t Hk, int64_t max_pa
  * smallest integer >= -100 with |q| <= 127 * 2^s, plus ceil(log2(Hq/Hk * D /
  * 1024)) where that is positive), a page scores
  *     sum over heads and channels of max(z * least, z * largest) * 2^exponent,
- * an upper bound of the sum of the heads' scores of any of its keys.  The first
- * `sink` and the last `recent` pages of a sequence stay; the others follow by
+ * an upper bound of the sum of the heads' z . k of any of its keys (that of q . k
+ * may pass it by 2^(s-1) times the sum over heads and channels of max(|least|,
+ * |largest|) * 2^exponent).  The first `sink` and the last `recent` pages of a sequence stay; the others follow by
  * score, equal ones by index, to `count` pages.  pages (B, Hk, count) int32 gets
  * their indices in ascending order, then -1.  Scores are whole numbers below
- * 2^24 times powers of two, so the choice is exact. */
+ * 2^24 times powers of two, so the choice by them is exact. */
 FC_API int fc_kv4_select(const void *q, int dtype, int64_t B, int64_t Hq, int64_t q_sb, int64_t q_sh,
                          const signed char *bounds, const int *exponents, int64_t num_pages,
                          int64_t Hk, int64_t D, int64_t page_size, const int *page_table,

@@ -867,11 +867,24 @@ attn_kernel(AttnArgs a) {
 // ---------------------------------------------------------------- planning
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
+// Bytes of the arrival counters: the same for all calls of up to kWsUnits units, so that the
+// partials of one are never the counters of another that shares the workspace.
+size_t counter_bytes(int64_t units) {
+    return align_up((size_t)std::max<int64_t>(units, kWsUnits) * 4, 256);
+}
+
+// Beyond kWsUnits they may be: such a call clears its own.
+int clear_counters(int *counters, int64_t units, int n_split, cudaStream_t st) {
+    if (n_split <= 1 || units <= kWsUnits) return FC_OK;
+    if (cudaMemsetAsync(counters, 0, (size_t)units * 4, st) == cudaSuccess) return FC_OK;
+    set_error("decode_attn: clearing the arrival counters failed");
+    return FC_ECUDA;
+}
+
 size_t workspace_for(int64_t units, int n_split, int GT, int64_t D) {
     if (n_split <= 1) return kWsHeader;
     const size_t slots = (size_t)units * n_split;
-    size_t w = kWsHeader;
-    w = align_up(w + (size_t)units * 4, 256);
+    size_t w = kWsHeader + counter_bytes(units);
     w = align_up(w + slots * GT * 4, 256);
     w = align_up(w + slots * GT * 4, 256);
     w = align_up(w + slots * GT * D * 4, 256);
@@ -1175,8 +1188,9 @@ static int decode_attn_impl(const void *q, int q_dtype, int64_t B, int64_t Hq, i
             t.epoch = next_epoch();
             size_t off = kWsHeader;
             t.cnt = reinterpret_cast<int *>(wsb + off);
-            off = align_up(off + (size_t)B * Hk * 4, 256);
+            off += counter_bytes(B * Hk);
             const size_t slots = (size_t)B * Hk * ns;
+            if (int rc = clear_counters(t.cnt, B * Hk, ns, static_cast<cudaStream_t>(stream))) return rc;
             t.pm = reinterpret_cast<float *>(wsb + off);
             off = align_up(off + slots * GT * 4, 256);
             t.pl = reinterpret_cast<float *>(wsb + off);
@@ -1252,8 +1266,9 @@ static int decode_attn_impl(const void *q, int q_dtype, int64_t B, int64_t Hq, i
     const int64_t units = B * Hk * p.n_groups;
     size_t off = kWsHeader;
     a.cnt = reinterpret_cast<int *>(ws + off);
-    off = align_up(off + (size_t)units * 4, 256);
+    off += counter_bytes(units);
     const size_t slots = (size_t)units * p.n_split;
+    if (int rc = clear_counters(a.cnt, units, p.n_split, static_cast<cudaStream_t>(stream))) return rc;
     a.pm = reinterpret_cast<float *>(ws + off);
     off = align_up(off + slots * p.GT * 4, 256);
     a.pl = reinterpret_cast<float *>(ws + off);

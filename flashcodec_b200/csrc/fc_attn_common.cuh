@@ -12,6 +12,7 @@ namespace fc {
 
 constexpr uint64_t kWaitNs = 100000000ull;  // 100 ms bound on any wait
 constexpr int kWsHeader = 256;              // workspace bytes before the counters
+constexpr int kWsUnits = 1 << 14;           // units that every workspace has counters for
 
 // Launch epochs: a positive, increasing tag per call (wraps after 2^31 - 1).
 int next_epoch();

@@ -23,12 +23,13 @@
 
 #include <mutex>
 
-#include "fc_common.cuh"
+#include "fc_attn_common.cuh"
 
 namespace {
 
-constexpr size_t kScratchBytes = FC_NOALLOC_SCRATCH_BYTES;
-constexpr size_t kHeaderBytes = 256;  // the workspace header (status word first)
+constexpr size_t kHeaderBytes = fc::kWsHeader;  // the workspace header (status word first)
+// the counters that every workspace has come on top
+constexpr size_t kScratchBytes = FC_NOALLOC_SCRATCH_BYTES + fc::kWsUnits * 4;
 constexpr int kMaxDevices = 64;
 
 static __device__ __align__(256) unsigned char g_attn_scratch[kScratchBytes];

@@ -187,8 +187,9 @@ FC_API int fc_png_decode(const float *deltas, int64_t d_sb, int64_t d_sh, int64_
  * the workspace was zeroed produced invalid output.  The rest holds the
  * split partials and per-(batch, KV head) arrival counters.  The workspace
  * must be zero-filled before its first use; a completed call leaves its
- * counters at zero again.  Calls sharing one workspace must not overlap on
- * the GPU (issue them on one stream).
+ * counters at zero again.  Calls of any sizes may share one workspace that is
+ * large enough for each, but must not overlap on the GPU (issue them on one
+ * stream).
  */
 FC_API size_t fc_decode_attn_workspace_size(int64_t B, int64_t Hq, int64_t Hk, int64_t D,
                                      int64_t n_blocks, int s, int r, int64_t n_raw);
@@ -292,8 +293,8 @@ FC_API int fc_decode_attn_png(const void *q, int q_dtype, int64_t B, int64_t Hq,
  * an FFI that may not call cudaMalloc and cannot reach their host framework's
  * allocator.  Same arguments and result as fc_decode_attn, without the
  * workspace: the split partials live in a scratch array compiled into the
- * library, FC_NOALLOC_SCRATCH_BYTES per GPU, held on every GPU that loads the
- * library's kernels until the process exits.
+ * library, FC_NOALLOC_SCRATCH_BYTES per GPU (and 64 KiB for the arrival counters),
+ * held on every GPU that loads the library's kernels until the process exits.
  *
  * - Calls whose plan needs more scratch than that return FC_ERANGE (use
  *   fc_decode_attn with a workspace).  The check is made against the plan

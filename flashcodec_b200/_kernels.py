@@ -135,7 +135,9 @@ def png_decode(deltas: torch.Tensor, anchors: torch.Tensor, out: torch.Tensor,
 
 
 # ------------------------------------------------------------------ attention
+# (device, stream, capture: 0 for eager calls) -> workspace
 _workspaces: dict = {}
+KEPT_CAPTURES = 16
 
 
 def attn_workspace_bytes(B, Hq, Hk, D, n_blocks, s, r, n_raw) -> int:
@@ -143,30 +145,53 @@ def attn_workspace_bytes(B, Hq, Hk, D, n_blocks, s, r, n_raw) -> int:
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Zero-initialised workspace cached per (device, stream).  The kernel
-    leaves its counters at zero, so the buffer is reused across calls issued
-    on the same stream."""
-    stream = torch.cuda.current_stream(device)
-    key = (device.index, stream.cuda_stream)
+    """Zero-initialised workspace of the current stream: one for its eager
+    calls, one for each capture of a CUDA graph there.  The kernel leaves its
+    counters at zero, so the buffer is reused across calls.
+
+    A capture shares its buffer with nothing else: a graph keeps the address,
+    while eager calls replace theirs when a larger one comes, and what zeroes
+    a buffer allocated in a capture is a node of that graph alone.  The last
+    KEPT_CAPTURES captures of a stream stay known to attn_status; a graph's
+    memory pool keeps its buffer in any case."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    key = (device.index, stream, _lib.load().fc_capture_id(stream))
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(max(nbytes, 4096), dtype=torch.uint8, device=device)
         _workspaces[key] = ws
+        captures = [k for k in _workspaces if k[:2] == key[:2] and k[2]]
+        for k in captures[:-KEPT_CAPTURES]:
+            del _workspaces[k]
     return ws
 
 
 def reset_workspace(device: torch.device) -> None:
     """Zero the cached workspace of the current stream (after a failed call)."""
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    if key in _workspaces:
-        _workspaces[key].zero_()
+    stream = torch.cuda.current_stream(device).cuda_stream
+    ws = _workspaces.get((device.index, stream, _lib.load().fc_capture_id(stream)))
+    if ws is not None:
+        ws.zero_()
+
+
+def _held_workspaces(device: torch.device) -> list:
+    """(workspace, whether of a capture) of the current stream."""
+    at = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    return [(ws, k[2] != 0) for k, ws in list(_workspaces.items()) if k[:2] == at]
+
+
+def _status_word(ws: torch.Tensor, captured: bool) -> torch.Tensor:
+    """The status word of a workspace.  Kernels write nothing else of the
+    header (256 bytes), so one that is not zero behind the word is of a graph
+    that has not run yet: its word is no status."""
+    word = ws[:4].view(torch.int32)
+    return torch.where(ws[4:256].any(), torch.zeros_like(word), word) if captured else word
 
 
 def attn_status(device: torch.device) -> int:
-    """The workspace status word of the current stream (synchronises)."""
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    ws = _workspaces.get(key)
-    return 0 if ws is None else int(ws[:4].view(torch.int32).item())
+    """The workspace status word of the current stream, of its eager calls and
+    its last captures (synchronises)."""
+    return max((int(_status_word(*w).item()) for w in _held_workspaces(device)), default=0)
 
 
 class StatusProbe:
@@ -203,14 +228,15 @@ def attn_status_async(device: torch.device, reset: bool = False) -> StatusProbe:
     host memory, in stream order, without synchronising; reset=True clears the
     word after the copy.  Poll the probe after a model step."""
     stream = torch.cuda.current_stream(device)
-    ws = _workspaces.get((device.index, stream.cuda_stream))
+    held = _held_workspaces(device)
     host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-    if ws is None:
+    if not held:
         return StatusProbe(host, None)
-    word = ws[:4].view(torch.int32)
-    host.copy_(word, non_blocking=True)
+    words = [_status_word(*w) for w in held]
+    host.copy_(words[0] if len(words) == 1 else torch.stack(words).amax(0), non_blocking=True)
     if reset:
-        word.zero_()
+        for ws, _ in held:
+            ws[:4].zero_()
     ev = torch.cuda.Event()
     ev.record(stream)
     return StatusProbe(host, ev)

@@ -187,7 +187,7 @@ inline int check_cache(const char *what, int64_t B, int64_t Hk, int64_t D, int64
         set_error("%s: bad shape", what);
         return FC_EINVAL;
     }
-    if (!pool || !page_table || !status || !aligned(pool, 16)) {
+    if (!pool || (!page_table && B) || !status || !aligned(pool, 16)) {
         set_error("%s: the pool (16-byte aligned), the page table and the status word are required", what);
         return FC_EINVAL;
     }

@@ -640,7 +640,7 @@ __device__ __forceinline__ void turn_queries(const AppendArgs &a) {
         const int *cu = a.cu;
         b = warp_find([=](int i) { return (int64_t)cu[i]; }, a.B, t);
         row = t;
-        none = t < cu[b] || t >= cu[b + 1];
+        none = a.B == 0 || t < cu[b] || t >= cu[b + 1];
     }
     const T *q = static_cast<const T *>(a.q) + (a.S ? b * a.q_sb : 0) + row * a.q_ss + li * 8;
     T *qo = static_cast<T *>(a.qo) + (a.S ? b * a.qo_sb : 0) + row * a.qo_ss + li * 8;
@@ -900,8 +900,8 @@ extern "C" int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t 
         set_error("kv4_append: bad token counts");
         return FC_EINVAL;
     }
-    if (T == 0 || B == 0) return FC_OK;
-    if (!k || !v || !lengths || (Hq && (!q || !q_out))) { set_error("kv4_append: null pointer"); return FC_EINVAL; }
+    if (T == 0 || (B == 0 && !cu_seqlens)) return FC_OK;
+    if (!k || !v || (!lengths && B) || (Hq && (!q || !q_out))) { set_error("kv4_append: null pointer"); return FC_EINVAL; }
     if ((bounds == nullptr) != (exponents == nullptr)) {
         set_error("kv4_append: bounds and their exponents go together");
         return FC_EINVAL;
@@ -954,7 +954,7 @@ extern "C" int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t 
             (rows_aligned(k, dtype, k_sb, k_ss, k_sh) ? 4 : 0) |
             (rows_aligned(v, dtype, v_sb, v_ss, v_sh) ? 8 : 0) |
             (aligned(q_weight, 16) && aligned(k_weight, 16) ? 16 : 0);
-    const int64_t slots = a.S ? B * ((S + 2 * page_size - 2) / page_size) : T / page_size + 2 * B;
+    const int64_t slots = a.S ? B * ((S + 2 * page_size - 2) / page_size) : B ? T / page_size + 2 * B : 0;
     const int warps = (int)(page_size / 16 < 8 ? page_size / 16 : 8);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return by_dtype(dtype, [&](auto t) {
@@ -975,6 +975,7 @@ extern "C" int fc_kv4_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t 
                     set_error("kv4_append: too many tokens for one call");
                     return FC_ENOTSUP;
                 }
+                if (blocks == 0) return FC_OK;
                 const size_t stage = (size_t)warps * 16 * (4 * W + 4) * 4, red = (size_t)warps * 32 * W * 8;
                 append_kernel<E, W, FULL><<<(unsigned)blocks, warps * 32, stage > red ? stage : red, st>>>(a);
                 return check_launch("kv4_append");
@@ -1000,7 +1001,7 @@ extern "C" int fc_kv4_read(const void *pool, int64_t num_pages, int64_t Hk, int6
         set_error("kv4_read: bad token counts");
         return FC_EINVAL;
     }
-    if (T == 0 || B == 0) return FC_OK;
+    if (T == 0 || (B == 0 && !cu_seqlens)) return FC_OK;
     if (!k_out || !v_out) { set_error("kv4_read: null pointer"); return FC_EINVAL; }
     ReadArgs a{};
     a.pool = static_cast<const unsigned char *>(pool);

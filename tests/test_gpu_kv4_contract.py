@@ -245,3 +245,26 @@ def test_outputs_of_attend_over_the_queries():
                          q_out=torch.empty(1, S, 4, D, device="cuda").expand_as(q))
         assert cache.attend(q, table, i32(lens), out=q).data_ptr() == y.data_ptr()
         assert torch.equal(q, want)
+
+
+def test_batches_of_no_sequence():
+    """Nothing to do, and packed rows of no sequence come out as zeros."""
+    Hq, Hk, D, page = 4, 2, 64, 16
+    cache = fc().PagedInt4Cache(3, Hk, D, page_size=page, bounds=True)
+    cache.pool.zero_()
+    table, none = i32([]).view(0, 5), i32([])
+    q, k = tokens(1, Hq, D, 1, (0,)), tokens(1, Hk, D, 1, (0,))
+    assert cache.append(q, k, k, table, none).shape == q.shape
+    out, lse = cache.attend(q, table, none, return_lse=True)
+    assert out.shape == q.shape and lse.shape == q.shape[:-1]
+    assert cache.select(q[:, 0], table, none, 2).shape == (0, Hk, 2)
+    assert cache.read(table, none, count=3)[0].shape == (0, 3, Hk, D)
+    q, k = tokens(21, Hq, D, 2), tokens(21, Hk, D, 3)
+    tab = fc().rotary_table(4, D)
+    assert (cache.append(q, k, k, table, none, cu_seqlens=i32([0]), rotary=tab) == 0).all()
+    cache.append(None, k, k, table, none, cu_seqlens=i32([0]))
+    junk = [torch.full((21, Hk, D), math.nan, device="cuda", dtype=torch.bfloat16) for _ in range(4)]
+    del junk
+    assert all((x == 0).all() for x in cache.read(table, none, count=21, cu_seqlens=i32([0])))
+    assert not cache.pool.any()
+    cache.check()

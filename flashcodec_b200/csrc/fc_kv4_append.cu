@@ -644,14 +644,6 @@ __device__ __forceinline__ void turn_queries(const AppendArgs &a) {
     }
     const T *q = static_cast<const T *>(a.q) + (a.S ? b * a.q_sb : 0) + row * a.q_ss + li * 8;
     T *qo = static_cast<T *>(a.qo) + (a.S ? b * a.qo_sb : 0) + row * a.qo_ss + li * 8;
-    if (none) {
-        const float2 o = pair(0.f, 0.f);
-        for (; live && h < end; h += TPP)
-#pragma unroll
-            for (int k = 0; k < CH; k++)
-                store_row(qo + h * a.qo_sh + k * L::half * 8, a.vec & 2, Row{{o, o}, {o, o}});
-        return;
-    }
     Raw<T> raw[N][CH];
     auto load = [&](int h0) {
 #pragma unroll
@@ -663,6 +655,14 @@ __device__ __forceinline__ void turn_queries(const AppendArgs &a) {
                                 : zero_raw<T>();
     };
     load(h);
+    if (none) {
+        const float2 o = pair(0.f, 0.f);
+        for (; live && h < end; h += TPP)
+#pragma unroll
+            for (int k = 0; k < CH; k++)
+                store_row(qo + h * a.qo_sh + k * L::half * 8, a.vec & 2, Row{{o, o}, {o, o}});
+        return;
+    }
     const Place place = place_of<W, FULL>(a, lane);
     Row w[CH];
     Angles angles;

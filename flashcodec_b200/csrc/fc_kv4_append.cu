@@ -13,10 +13,10 @@
 // and bounds are the same bits for every way of splitting tokens into calls.
 //
 // The launch moves each input and output byte once.  8191 packed tokens of 32/8 heads of
-// 128, bf16 (177 MB, 27.5 us at the copy rate), take 55 us: the queries 22 us, at the rate of
-// memory, keys and values 32 us, bound by issue (2.2 instructions a cycle and SM).  A decode
-// step's 64 tokens take 8.3 us, one 7.0: a chain of dependent loads.  Its blocks
-// have two roles.  One block per (page that gets tokens, KV head) owns everything
+// 128, bf16 (177 MB, 27.5 us at the copy rate), take 56 us: the queries 22 us, at the rate of
+// memory, keys and values 32 us, bound by the latency of the instructions and loads of 16
+// warps an SM (2.2 of 4 instructions a cycle).  A decode step's 64 tokens take 8.0 us, one
+// 6.6: a chain of dependent loads.  Its blocks have two roles.  One block per (page that gets tokens, KV head) owns everything
 // it writes: codes that share a word with older tokens and the page bounds are
 // read, merged and written without atomics.  The other blocks take query heads,
 // one warp for one token's heads.

@@ -2,9 +2,10 @@
 //
 //   out = softmax(scale * q . K^T) . V,  K = code * scale per group of 32 channels
 //
-// Every held byte is read once per KV head (4.5 bits a value, so HBM bounds it from
-// below at 144 bytes a token and head at D = 128), and each value takes part in
-// Hq / Hk products on each side.  What competes with HBM is the issue rate: at
+// Every held byte is read once per KV head and block of 8 query rows (4 of fp16 or fp32;
+// twice that with two column blocks): 4.5 bits a value, so HBM bounds it from below at 144
+// bytes a token and head at D = 128, and each value takes part in Hq / Hk products on each
+// side.  What competes with HBM is the issue rate: at
 // 6.4 TB/s an SM receives 46 values a cycle to unpack.  So the pages are stored in
 // the operand order of mma.m16n8k16 (fc_kv4.cuh): tokens (K) or channels (V) in the 16
 // rows, the group's query rows in the 8 columns, and nothing is exchanged between lanes
@@ -33,17 +34,17 @@
 // the power of two is 1 at least, and where all scales are below 2^-10 the products of
 // weights under 2^-14 of the largest are subnormal.
 //
-// Work.  The chunks (32 tokens) of all (sequence, KV head, row block) are one line,
-// cut into equal pieces for one wave of blocks, whatever the lengths; the lengths are
+// Work.  The chunks (64 tokens; 32 where pages are smaller, heads wider than 128 or pages
+// selected) of all (sequence, KV head, row block) are one line, cut into equal pieces for one wave of blocks, whatever the lengths; the lengths are
 // read on the device.  A block's 4 warps take the chunks of its piece in turn, each
 // with its own ring of asynchronous copies and its own running state.  Pieces of one
 // (sequence, head) are joined by the last block to finish, in order: the result does
 // not depend on timing.  No block waits for another.
 //
-// 16 sequences of 32768 tokens, 32/8 heads, D = 128, bf16 (604 MB): 107 us, 5.6 TB/s, 87 %
-// of the copy rate, in short runs; 124 us under sustained load, where the power cap holds
-// the SMs at 1.75 GHz.  The copies alone take 100 us; the rest is the latency of 12 warps'
-// own instructions (1.8 a cycle and SM, 222 for 16 tokens).  3 blocks of 168 registers an
+// 16 sequences of 32768 tokens, 32/8 heads, D = 128, bf16 (604 MB): 124 us under sustained
+// load, 4.9 TB/s, 76 % of the copy rate, where the power cap holds the SMs at 1.75 GHz; 107.5
+// us, 87 %, in short runs (fp16 queries 125).  The copies alone take 100 us; the rest is the
+// latency of 12 warps' own instructions (1.9 of 4 a cycle and SM, 228 for 16 tokens).  3 blocks of 168 registers an
 // SM; 4 of 128 spill (121 us), 5 warps a block too.  Bulk copies in place of cp.async were
 // slower (127 us against 123 at that time), chunks of 32 tokens are by 6 %.
 #include "fc_attn_common.cuh"
@@ -1176,8 +1177,9 @@ extern "C" int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int6
     // One column block of 8 serves up to 8 (4) rows.  More rows can take two, which double
     // the matrix instructions but share the unpacking, against reading the pages again for
     // the next rows.  Two need 255 registers, 8 warps an SM instead of 12, so they pay where
-    // tables are long: 16 rows, us with two / one: 16 x 32768 tokens, 8 heads 179 / 206;
-    // 24 x 1..9000 36 / 34; 4 x 4096 30 / 22.  At D = 256 they spill (8 x 8192: 62 / 35).
+    // sequences are long.  The host knows the table's width alone, so short sequences get two
+    // as well where the table could hold long ones.  16 rows, us with two / one: 16 x 32768
+    // tokens, 8 heads 179 / 206; 24 x 1..9000 36 / 34; 4 x 4096 30 / 22.  At D = 256 they spill (8 x 8192: 62 / 35).
     const int64_t tokens = B * Hk * (selected ? n_selected : max_pages) * page_size;
     const int nt = rows * limbs > 8 && D <= 128 && tokens >= 1 << 21 ? 2 : 1;
     const int rpc = 8 * nt / limbs;

@@ -16,7 +16,7 @@
 // in unsigned order) are counted in 1024 equal bins between the least and the largest, the
 // bin that holds the last key wanted is counted in the same way, until what is wanted of it
 // is all or one value; one prefix sum over the pages then writes the indices in order.
-// 2048 pages of 4 x 8 (sequence, head)s at D = 128 (17 MB): 13.0 us, of which the choice
+// 2048 pages of 4 x 8 (sequence, head)s at D = 128 (17 MB): 13.6 us, of which the choice
 // takes some 8; keys kept in shared memory between its passes did not shorten it.
 #include "fc_kv4.cuh"
 

@@ -51,7 +51,7 @@ def rotary_table(max_positions, rotary_dim, base=10000.0, *, scaling=None, facto
                  beta_fast=32.0, beta_slow=1.0, attention_factor=None, device="cuda"):
     """(max_positions, rotary_dim) fp32: the cosines, then the sines, of every
     position's angles ``position * base ** (-2 i / rotary_dim)``, evaluated in
-    fp64 and rounded once.
+    fp64 and rounded once.  (``append`` takes multiples of 16 as rotary_dim.)
 
     scaling: how the frequencies are stretched for contexts ``factor`` times
     ``original_max_positions``:

@@ -185,7 +185,7 @@ def _status_word(ws: torch.Tensor, captured: bool) -> torch.Tensor:
     header (256 bytes), so one that is not zero behind the word is of a graph
     that has not run yet: its word is no status."""
     word = ws[:4].view(torch.int32)
-    return torch.where(ws[4:256].any(), torch.zeros_like(word), word) if captured else word
+    return torch.where((ws[4:256] != 0).any(), torch.zeros_like(word), word) if captured else word
 
 
 def attn_status(device: torch.device) -> int:

@@ -647,7 +647,8 @@ FC_API size_t fc_kv4_attn_workspace_size(int64_t B, int64_t Sq, int64_t Hq, int6
  * (indices into the sequence's row of the page table, each at most once;
  * negative or past the sequence's pages: none); Sq = 1 with it.
  * lse (B, Sq, Hq) fp32 or NULL: the natural logarithm of the softmax sums, -inf
- * where a query sees nothing.  Scores, sums and accumulation are fp32. */
+ * where a query sees nothing (with bf16 queries of 2^120 and more it is not the
+ * logarithm; out holds).  Scores, sums and accumulation are fp32. */
 FC_API int fc_kv4_attn(const void *q, int dtype, int64_t B, int64_t Sq, int64_t Hq, int64_t q_sb,
                        int64_t q_ss, int64_t q_sh, const void *pool, int64_t num_pages, int64_t Hk,
                        int64_t D, int64_t page_size, const int *page_table, int64_t table_stride,

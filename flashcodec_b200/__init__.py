@@ -16,11 +16,12 @@ from .attention import attention_status, block_basis, codec_decode_attention
 from .cache import CodecKVCache, _CodecStream, make_codec
 from .codecs import (JPEGCodec, PNGCodec, dct_basis, dct_compress, dct_decompress,
                      dequantize_coeffs, png_filter, png_reconstruct, quantize_coeffs)
-from .paged import PagedInt4Cache, rotary_table
+from .paged import PagedInt4Cache, PagedInt8Cache, rotary_axes, rotary_table
 from .patch import (apply_flash_codec, find_attention_modules, remove_flash_codec,
                     undo_flash_codec)
 from .patch_attention import (apply_codec_attention, codec_attention_stats,
                               remove_codec_attention)
+from .prompt import prompt_attention
 
 __version__ = "0.1.0"
 
@@ -46,6 +47,6 @@ __all__ = [
     "dct_basis", "dct_compress", "dct_decompress",
     "quantize_coeffs", "dequantize_coeffs",
     "png_filter", "png_reconstruct",
-    "PagedInt4Cache", "rotary_table",
+    "PagedInt4Cache", "PagedInt8Cache", "rotary_table", "rotary_axes", "prompt_attention",
     "__version__",
 ]

@@ -588,7 +588,7 @@ except ImportError:
 
     _current_device = torch.cuda.current_device
 
-# (entry point, device, stream) -> workspace of the eager calls there, and of the calls of the
+# (cache, entry point, device, stream) -> workspace of the eager calls there, and of the calls of the
 # capture that was last under way there
 _kv4_workspaces: dict = {}
 _kv4_captured: dict = {}
@@ -612,10 +612,10 @@ def kv4_page_bytes(Hk: int, D: int, page_size: int) -> int:
     return n
 
 
-def _kv4_workspace(what, sizes, units, index, stream):
+def _kv4_workspace(what, sizes, units, index, stream, cache="kv4"):
     """The workspace of one entry point, its counters zeroed: one for the eager calls of a (device,
     stream), one for each capture there.  `sizes` are the arguments of its size function, which
-    grows with `units` alone.
+    grows with `units` alone.  (The 8-bit cache's have the same counters in front.)
 
     A captured graph keeps the address of its workspace, and what zeroes a buffer that a
     capture allocates is a node of that graph.  So a capture shares its buffer with nothing: not
@@ -623,12 +623,12 @@ def _kv4_workspace(what, sizes, units, index, stream):
     capture, whose graph may be replayed first or on another stream.  The buffer is a graph's own
     (it comes from the capture's memory pool, which lives as long as the graph does)."""
     capture = _lib.load().fc_capture_id(stream)
-    workspaces, key = _kv4_captured if capture else _kv4_workspaces, (what, index, stream)
+    workspaces, key = _kv4_captured if capture else _kv4_workspaces, (cache, what, index, stream)
     ws = workspaces.get(key)
     if ws is None or ws.capture != capture:
         ws = workspaces[key] = _Kv4Workspace(capture)
     if units > ws.units:
-        nbytes = getattr(_lib.load(), f"fc_kv4_{what}_workspace_size")(*sizes)
+        nbytes = getattr(_lib.load(), f"fc_{cache}_{what}_workspace_size")(*sizes)
         if nbytes > ws.bytes:
             ws.buffer = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
             ws.address, ws.bytes = ws.buffer.data_ptr(), nbytes
@@ -700,3 +700,58 @@ def kv4_select(cache, q_at, dtype, B, Hq, table, lengths, count, sink, recent, p
     _kv4_call(cache._lib.fc_kv4_select, "kv4_select", index, (
         q_at[0], _code(dtype), B, Hq, q_at[1], q_at[3], *cache._bounds_args, *cache._pool_args[1:],
         *table, lengths, count, sink, recent, pages, ws.address, ws.bytes, cache._status_ptr, stream), ws)
+
+
+# --------------------------------------------------------- paged 8-bit KV cache
+def kv8_append(cache, rows_at, dtype, B, S, T, cu, lengths, positions, axes, n_axes, w_at, w_dtype,
+               eps, turn, interleaved, table) -> None:
+    """fc_kv8_append; arguments as of kv4_append."""
+    index = cache._index
+    _kv4_call(cache._lib.fc_kv8_append, "kv8_append", index, (
+        *rows_at, _code(dtype), B, S, T, cu, lengths, positions, axes, n_axes, *w_at,
+        0 if w_dtype is None else _code(w_dtype), eps, *turn, interleaved, *cache._pool_args, *table,
+        cache._status_ptr, _raw_stream(index)))
+
+
+def kv8_read(cache, table, starts, B, S, T, cu, k_out, v_out, dtype, strides) -> None:
+    """fc_kv8_read."""
+    index = cache._index
+    _kv4_call(cache._lib.fc_kv8_read, "kv8_read", index, (
+        *cache._pool_args, *table, starts, B, S, T, cu, k_out, v_out, _code(dtype), *strides,
+        cache._status_ptr, _raw_stream(index)))
+
+
+def kv8_attn(cache, q_at, dtype, shape, table, lengths, scale, out_at, lse) -> None:
+    """fc_kv8_attn; q of `shape` (B, Sq, Hq, D) or (B, Hq, D)."""
+    index = cache._index
+    stream = _raw_stream(index)
+    B, Sq, Hq = shape[:3] if len(shape) == 4 else (shape[0], 1, shape[1])
+    ws = _kv4_workspace("attn", (B, Sq, Hq, cache.num_kv_heads, cache.head_dim), cache.head_dim, index,
+                        stream, cache="kv8")
+    _kv4_call(cache._lib.fc_kv8_attn, "kv8_attn", index, (
+        q_at[0], _code(dtype), B, Sq, Hq, *q_at[1:], *cache._pool_args, *table, lengths, scale,
+        *out_at, None if lse is None else lse.data_ptr(), ws.address, ws.bytes, cache._status_ptr, stream), ws)
+
+
+# ------------------------------------------------------- attention over prompts
+def prompt_attn(q, k, v, cu_q, cu_k, causal, scale, out, lse) -> None:
+    """fc_prompt_attn; q, out (T, Hq, D) and k, v (T, Hk, D) packed, or (B, S, H, D) without cu's."""
+    def at(t):
+        return (t.data_ptr(), *((0, *t.stride()[:2]) if t.dim() == 3 else t.stride()[:3]))
+    dev, D = q.device, q.shape[-1]
+    if cu_q is None:
+        B, Sq, Sk = q.shape[0], q.shape[1], k.shape[1]
+        Tq, Tk = B * Sq, B * Sk
+    else:
+        B, Sq, Sk, Tq, Tk = cu_q.shape[0] - 1, 0, 0, q.shape[0], k.shape[0]
+    Hq, Hk = q.shape[-2], k.shape[-2]
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        ws = workspace(dev, lib.fc_prompt_attn_workspace_size(B, Tq, Hq, Hk, D))
+        rc = lib.fc_prompt_attn(*at(q), *at(k), *at(v), _code(q.dtype), B, Sq, Sk, Tq, Tk, Hq, Hk, D,
+                                None if cu_q is None else cu_q.data_ptr(),
+                                None if cu_k is None else cu_k.data_ptr(), bool(causal), scale,
+                                *at(out), _p(lse), _p(ws), ws.numel(), _stream(dev))
+    if rc != _lib.FC_OK:
+        reset_workspace(dev)
+    _lib.check(rc, "prompt_attn")

@@ -1,4 +1,4 @@
-"""A paged 4-bit KV cache for batches of sequences that come and go.
+"""Paged KV caches, in 4 and in 8 bits, for batches of sequences that come and go.
 
 The codec streams (``cache.py``) hold one batch that grows in step.  A serving
 engine instead keeps one pool of pages per layer and a table that says which
@@ -26,8 +26,13 @@ kernels read when they run: a captured CUDA graph follows their contents.  The
 caller owns page allocation; entries past a sequence's pages are never read.
 Kernels check pages, lengths and positions against the buffers: tokens without a
 page are skipped, positions outside the rotary table take its nearest row, and
-either is noted in ``status`` (see ``check``).  The
-reference has no paged cache; its notes on 4-bit K/V quantisation
+either is noted in ``status`` (see ``check``).
+
+``PagedInt8Cache`` is the same pool with int8 codes and one scale for every 16
+tokens of a head (8 bits a value): ``append``, ``attend`` and ``read`` as above;
+its ``append`` also takes positions of several axes (time, height, width).
+
+The reference has no paged cache; its notes on 4-bit K/V quantisation
 (docs/llama-cpp-kv-quantization.md) are the nearest it has.
 """
 
@@ -98,25 +103,33 @@ def rotary_table(max_positions, rotary_dim, base=10000.0, *, scaling=None, facto
     return (torch.cat([angle.cos(), angle.sin()], 1) * gain).float()
 
 
-class PagedInt4Cache:
-    """One layer's pool of 4-bit K/V pages.
+def rotary_axes(sections, alternate=False, device="cuda"):
+    """(sum(sections),) int32: the axis (time, height, width, ...) by whose position each
+    rotary pair turns.  ``sections``: pairs of every axis, rotary_dim / 2 in all; in runs,
+    or with ``alternate`` dealt out in turn, an axis dropping out when it has its pairs
+    ((3, 2, 2): 0 1 2 0 1 2 0)."""
+    left = [int(n) for n in sections]
+    if not left or min(left) < 0 or sum(left) == 0:
+        raise ValueError(f"sections must be numbers of pairs, some in all (got {sections})")
+    axes = []
+    if alternate:
+        while any(left):
+            for axis, n in enumerate(left):
+                if n:
+                    axes.append(axis)
+                    left[axis] -= 1
+    else:
+        for axis, n in enumerate(left):
+            axes += [axis] * n
+    return torch.tensor(axes, dtype=torch.int32, device=device)
 
-    Args:
-        num_pages: pages of the pool.
-        num_kv_heads, head_dim: of the model (head_dim 64, 96, 128, 192 or 256).
-        page_size: tokens of a page, a power of two from 16 to 1024.
-        bounds: keep every page's least and largest key values per channel,
-            which ``select`` needs (2 * head_dim + 4 bytes per page and KV head).
-        device: a CUDA device.
 
-    Attributes: ``pool`` (num_pages, bytes) uint8; ``bounds`` (num_pages, Hk, 2,
-    D) int8 and ``exponents`` (num_pages, Hk) int32, or None; ``status`` int32.
-    They cannot be replaced, only written to (a cache restored from a file:
-    ``cache.pool.copy_(saved)``).
-    """
+class _PagedCache:
+    """What the paged caches share: their pool's sizes, and the checks of arguments."""
 
-    def __init__(self, num_pages, num_kv_heads, head_dim, page_size=64, bounds=False,
-                 device="cuda"):
+    _bits = 0
+
+    def __init__(self, num_pages, num_kv_heads, head_dim, page_size, device):
         dev = torch.device(device)
         if dev.type != "cuda":
             raise RuntimeError("flashcodec_b200 runs on CUDA devices only (got "
@@ -129,26 +142,12 @@ class PagedInt4Cache:
         self.num_pages, self.num_kv_heads = int(num_pages), int(num_kv_heads)
         self.head_dim, self.page_size = int(head_dim), int(page_size)
         self.page_bytes = K.kv4_page_bytes(self.num_kv_heads, self.head_dim, self.page_size)
-        self._pool = torch.empty(self.num_pages, self.page_bytes, dtype=torch.uint8, device=dev)
-        self._bounds = self._exponents = None
-        if bounds:
-            self._bounds = torch.zeros(self.num_pages, self.num_kv_heads, 2, self.head_dim,
-                                       dtype=torch.int8, device=dev)
-            self._exponents = torch.zeros(self.num_pages, self.num_kv_heads, dtype=torch.int32,
-                                          device=dev)
         self._status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._index, self._scale, self._lib = dev.index, self.head_dim ** -0.5, _lib.load()
         self._status_ptr = self._status.data_ptr()
-        self._pool_args = (self._pool.data_ptr(), self.num_pages, self.num_kv_heads, self.head_dim,
-                           self.page_size)
-        self._bounds_args = (self._bounds.data_ptr(), self._exponents.data_ptr()) if bounds \
-            else (None, None)
 
-    # The calls pass these tensors' addresses, taken once: their contents may be written, they
+    # The calls pass the tensors' addresses, taken once: their contents may be written, they
     # themselves stay.
-    pool = property(lambda self: self._pool)
-    bounds = property(lambda self: self._bounds)
-    exponents = property(lambda self: self._exponents)
     status = property(lambda self: self._status)
 
     # ------------------------------------------------------------ argument checks
@@ -164,10 +163,10 @@ class PagedInt4Cache:
                 K.require_cuda(t)
                 raise ValueError(f"a tensor is on {t.device}, the cache on {self.device}")
             if grad and t.requires_grad:
-                raise RuntimeError("the 4-bit cache holds rounded values and has no gradient: "
+                raise RuntimeError(f"the {self._bits}-bit cache holds rounded values and has no gradient: "
                                    "call it under torch.no_grad()")
             if dual and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError("the 4-bit cache holds rounded values and has no tangent: "
+                raise RuntimeError(f"the {self._bits}-bit cache holds rounded values and has no tangent: "
                                    "pass the primal of a dual tensor")
 
     def _ints(self, name, t, shape):
@@ -200,32 +199,12 @@ class PagedInt4Cache:
             return t.data_ptr(), st[0], st[1], st[2]
         return (t.data_ptr(), 0, st[0], st[1]) if packed else (t.data_ptr(), st[0], 0, st[1])
 
-    # ----------------------------------------------------------------- operations
-    def append(self, q, k, v, page_table, lengths, *, cu_seqlens=None, q_weight=None,
-               k_weight=None, eps=1e-6, rotary=None, interleaved=False, positions=None,
-               q_out=None):
-        """Put new tokens at the ends of their sequences; returns the queries.
-
-        q, k, v: (B, S, H, D), (B, H, D) for one token each, or packed (T, H, D)
-            with ``cu_seqlens`` (B + 1,) int32; fp32, bf16 or fp16, any strides
-            with unit stride along D.  q may be None.  Packed rows of no sequence
-            (from cu_seqlens[B] on: a captured batch has a fixed number) are not
-            stored, and their queries come out as zeros.
-        lengths: (B,) int32, tokens held before the call (unchanged by it); a
-            negative one skips the sequence.
-        q_weight, k_weight: (D,) weights of a per-head RMS norm (``eps``), or None.
-        rotary: ``rotary_table``'s (positions, R) fp32, R a multiple of 16, or
-            None; its first R channels turn, in pairs (i, i + R/2), or (2i, 2i+1)
-            with ``interleaved``.
-        positions: (B, S) or (T,) int32 rows of the table (default: the cache
-            positions, lengths + i).
-        q_out: where the queries go (default: a new tensor; may be q).
-
-        Arithmetic is fp32 and rounded in a fixed order, so what is stored does
-        not depend on how tokens are split into calls.
-        """
+    def _append_args(self, q, k, v, page_table, lengths, cu_seqlens, q_weight, k_weight, rotary,
+                     positions, axes, q_out):
+        """An append's arguments, checked: rows and tokens, axes, norm weights, rotary table, page
+        table, and where the queries go."""
         self._here(q, k, v, page_table, lengths, cu_seqlens, q_weight, k_weight, rotary, positions,
-                   q_out)
+                   axes, q_out)
         B, table = self._table(page_table)
         packed = cu_seqlens is not None
         k_at = self._rows("k", k, packed=packed, heads=self.num_kv_heads)
@@ -270,12 +249,120 @@ class PagedInt4Cache:
             if rotary.dtype is not torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous():
                 raise ValueError("rotary must be a contiguous fp32 (positions, R) tensor")
             turn = (rotary.data_ptr(), *rotary.shape)
-        pos = None
-        if positions is not None:
+        pos, turns = None, (None, 0)
+        if axes is not None:
+            if rotary is None or positions is None or positions.dim() == 0:
+                raise ValueError("axes go with a rotary table and positions of every axis")
+            self._ints("axes", axes, (rotary.shape[1] // 2,))
+            self._ints("positions", positions, (positions.shape[0], *shape[:-2]))
+            if positions.shape[0] == 0:
+                raise ValueError("positions have no axis")
+            turns = (axes.data_ptr(), positions.shape[0])
+        elif positions is not None:
             self._ints("positions", positions, shape[:-2] if positions.dim() == 2 else (T,))
+        if positions is not None:
             pos = positions.data_ptr()
-        K.kv4_append(self, (*q_at, heads, *k_at, *v_at), dtype, B, S, T, cu, lengths.data_ptr(),
-                     pos, w_at, w_dtype, eps, turn, bool(interleaved), table)
+        return ((*q_at, heads, *k_at, *v_at), dtype, B, S, T, cu, lengths.data_ptr(), pos), turns, \
+            (w_at, w_dtype), turn, table, q_out
+
+    def _read(self, kernel, page_table, starts, count, cu_seqlens, dtype):
+        self._here(page_table, starts, cu_seqlens)
+        B, table = self._table(page_table)
+        if count is None or count < 0:
+            raise ValueError("read needs the number of tokens (count)")
+        # (the tensors stay named: a caller's temporary would be freed, and the outputs be put there)
+        at = cu = None
+        if starts is not None:
+            self._ints("starts", starts, (B,))
+            at = starts.data_ptr()
+        H, D = self.num_kv_heads, self.head_dim
+        if cu_seqlens is not None:
+            self._ints("cu_seqlens", cu_seqlens, (B + 1,))
+            cu = cu_seqlens.data_ptr()
+            shape, S, T = (count, H, D), 0, count
+        else:
+            shape, S, T = (B, count, H, D), count, B * count
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        kernel(self, table, at, B, S, T, cu, k.data_ptr(), v.data_ptr(), dtype,
+               (count * H * D, H * D, D))
+        return k, v
+
+    def check(self):
+        """Raise if a kernel met a bad page, length or position since the last
+        check, and clear the word (synchronises)."""
+        word = int(self.status.item())
+        if word:
+            self.status.zero_()
+            raise _lib.FlashCodecError(_lib.FC_ERANGE, "paged cache: " + "; ".join(
+                text for bit, text in _STATUS if word & bit))
+
+
+class PagedInt4Cache(_PagedCache):
+    """One layer's pool of 4-bit K/V pages.
+
+    Args:
+        num_pages: pages of the pool.
+        num_kv_heads, head_dim: of the model (head_dim 64, 96, 128, 192 or 256).
+        page_size: tokens of a page, a power of two from 16 to 1024.
+        bounds: keep every page's least and largest key values per channel,
+            which ``select`` needs (2 * head_dim + 4 bytes per page and KV head).
+        device: a CUDA device.
+
+    Attributes: ``pool`` (num_pages, bytes) uint8; ``bounds`` (num_pages, Hk, 2,
+    D) int8 and ``exponents`` (num_pages, Hk) int32, or None; ``status`` int32.
+    They cannot be replaced, only written to (a cache restored from a file:
+    ``cache.pool.copy_(saved)``).
+    """
+
+    _bits = 4
+
+    def __init__(self, num_pages, num_kv_heads, head_dim, page_size=64, bounds=False,
+                 device="cuda"):
+        super().__init__(num_pages, num_kv_heads, head_dim, page_size, device)
+        self._pool = torch.empty(self.num_pages, self.page_bytes, dtype=torch.uint8, device=self.device)
+        self._bounds = self._exponents = None
+        if bounds:
+            self._bounds = torch.zeros(self.num_pages, self.num_kv_heads, 2, self.head_dim,
+                                       dtype=torch.int8, device=self.device)
+            self._exponents = torch.zeros(self.num_pages, self.num_kv_heads, dtype=torch.int32,
+                                          device=self.device)
+        self._pool_args = (self._pool.data_ptr(), self.num_pages, self.num_kv_heads, self.head_dim,
+                           self.page_size)
+        self._bounds_args = (self._bounds.data_ptr(), self._exponents.data_ptr()) if bounds \
+            else (None, None)
+
+    pool = property(lambda self: self._pool)
+    bounds = property(lambda self: self._bounds)
+    exponents = property(lambda self: self._exponents)
+
+    # ----------------------------------------------------------------- operations
+    def append(self, q, k, v, page_table, lengths, *, cu_seqlens=None, q_weight=None,
+               k_weight=None, eps=1e-6, rotary=None, interleaved=False, positions=None,
+               q_out=None):
+        """Put new tokens at the ends of their sequences; returns the queries.
+
+        q, k, v: (B, S, H, D), (B, H, D) for one token each, or packed (T, H, D)
+            with ``cu_seqlens`` (B + 1,) int32; fp32, bf16 or fp16, any strides
+            with unit stride along D.  q may be None.  Packed rows of no sequence
+            (from cu_seqlens[B] on: a captured batch has a fixed number) are not
+            stored, and their queries come out as zeros.
+        lengths: (B,) int32, tokens held before the call (unchanged by it); a
+            negative one skips the sequence.
+        q_weight, k_weight: (D,) weights of a per-head RMS norm (``eps``), or None.
+        rotary: ``rotary_table``'s (positions, R) fp32, R a multiple of 16, or
+            None; its first R channels turn, in pairs (i, i + R/2), or (2i, 2i+1)
+            with ``interleaved``.
+        positions: (B, S) or (T,) int32 rows of the table (default: the cache
+            positions, lengths + i).
+        q_out: where the queries go (default: a new tensor; may be q).
+
+        Arithmetic is fp32 and rounded in a fixed order, so what is stored does
+        not depend on how tokens are split into calls.
+        """
+        rows, _, weights, turn, table, q_out = self._append_args(
+            q, k, v, page_table, lengths, cu_seqlens, q_weight, k_weight, rotary, positions, None, q_out)
+        K.kv4_append(self, *rows, *weights, eps, turn, bool(interleaved), table)
         return q_out
 
     def attend(self, q, page_table, lengths, *, scale=None, selected=None, out=None,
@@ -349,36 +436,78 @@ class PagedInt4Cache:
         in all, packed as (count, Hk, D).  Zeros for sequences with a negative
         start, for packed rows of no sequence, and where no page can be read
         (which ``check`` reports)."""
-        self._here(page_table, starts, cu_seqlens)
+        return self._read(K.kv4_read, page_table, starts, count, cu_seqlens, dtype)
+
+
+class PagedInt8Cache(_PagedCache):
+    """One layer's pool of 8-bit K/V pages.
+
+    Args as for ``PagedInt4Cache`` (without bounds).
+
+    Attributes: ``codes`` (num_pages, 2, Hk, page_size, D) int8, keys and values;
+    ``scales`` (num_pages, 2, Hk, page_size / 16) fp32, one for every 16 tokens of a
+    head; ``status`` int32.  They cannot be replaced, only written to.
+
+    A code stands for (code + 1/2) * scale, a power of two with the run's largest
+    |value| below 128 scales: values are off by half a scale at most, 1/128 of that
+    largest value.  While a run of 16 tokens fills, a larger value may raise its scale;
+    the codes held are then shifted, and equal those of the run quantised at once: what
+    is stored does not depend on how tokens are split into calls.  A run with an infinity
+    or a NaN reads as NaN.  A run whose tokens were dropped keeps its scale until its
+    first position is appended anew.
+    """
+
+    _bits = 8
+
+    def __init__(self, num_pages, num_kv_heads, head_dim, page_size=64, device="cuda"):
+        super().__init__(num_pages, num_kv_heads, head_dim, page_size, device)
+        self.page_bytes = 2 * self.num_kv_heads * self.page_size * (4 * self.head_dim + 1) // 4
+        at = (self.num_pages, 2, self.num_kv_heads)
+        self._codes = torch.empty(*at, self.page_size, self.head_dim, dtype=torch.int8, device=self.device)
+        self._scales = torch.zeros(*at, self.page_size // 16, dtype=torch.float32, device=self.device)
+        self._pool_args = (self._codes.data_ptr(), self._scales.data_ptr(), self.num_pages,
+                           self.num_kv_heads, self.head_dim, self.page_size)
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+
+    # ----------------------------------------------------------------- operations
+    def append(self, q, k, v, page_table, lengths, *, cu_seqlens=None, q_weight=None,
+               k_weight=None, eps=1e-6, rotary=None, interleaved=False, positions=None,
+               axes=None, q_out=None):
+        """Put new tokens at the ends of their sequences; returns the queries.
+
+        Arguments as for ``PagedInt4Cache.append``, and
+        axes: (R / 2,) int32 from ``rotary_axes``: pair i turns by the angle of
+            ``positions[axes[i]]``, positions then being (A, B, S), (A, B) or (A, T)
+            int32 (time, height and width of the tokens of images and video).
+        """
+        rows, turns, weights, turn, table, q_out = self._append_args(
+            q, k, v, page_table, lengths, cu_seqlens, q_weight, k_weight, rotary, positions, axes, q_out)
+        K.kv8_append(self, *rows, *turns, *weights, eps, turn, bool(interleaved), table)
+        return q_out
+
+    def attend(self, q, page_table, lengths, *, scale=None, out=None, return_lse=False):
+        """Attention of every sequence's newest tokens over what the cache holds:
+        ``PagedInt4Cache.attend`` without selected pages."""
+        self._here(q, page_table, lengths, out)
         B, table = self._table(page_table)
-        if count is None or count < 0:
-            raise ValueError("read needs the number of tokens (count)")
-        # (the tensors stay named: a caller's temporary would be freed, and the outputs be put there)
-        at = cu = None
-        if starts is not None:
-            self._ints("starts", starts, (B,))
-            at = starts.data_ptr()
-        H, D = self.num_kv_heads, self.head_dim
-        if cu_seqlens is not None:
-            self._ints("cu_seqlens", cu_seqlens, (B + 1,))
-            cu = cu_seqlens.data_ptr()
-            shape, S, T = (count, H, D), 0, count
-        else:
-            shape, S, T = (B, count, H, D), count, B * count
-        k = torch.empty(shape, dtype=dtype, device=self.device)
-        v = torch.empty_like(k)
-        K.kv4_read(self, table, at, B, S, T, cu, k.data_ptr(), v.data_ptr(), dtype,
-                   (count * H * D, H * D, D))
-        return k, v
+        q_at, shape = self._rows("q", q), q.shape
+        if shape[0] != B:
+            raise ValueError(f"q has {shape[0]} sequences, the page table {B}")
+        self._ints("lengths", lengths, (B,))
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.dtype is not q.dtype:
+            raise ValueError("out must have the dtype of q")
+        lse = torch.empty(shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+        K.kv8_attn(self, q_at, q.dtype, shape, table, lengths.data_ptr(),
+                   self._scale if scale is None else float(scale), self._rows("out", out, shape), lse)
+        return (out, lse) if return_lse else out
 
-    def check(self):
-        """Raise if a kernel met a bad page, length or position since the last
-        check, and clear the word (synchronises)."""
-        word = int(self.status.item())
-        if word:
-            self.status.zero_()
-            raise _lib.FlashCodecError(_lib.FC_ERANGE, "paged cache: " + "; ".join(
-                text for bit, text in _STATUS if word & bit))
+    def read(self, page_table, starts=None, *, count=None, cu_seqlens=None, dtype=torch.bfloat16):
+        """The values held, as (k, v): ``PagedInt4Cache.read``."""
+        return self._read(K.kv8_read, page_table, starts, count, cu_seqlens, dtype)
 
 
-__all__ = ["PagedInt4Cache", "rotary_table"]
+__all__ = ["PagedInt4Cache", "PagedInt8Cache", "rotary_axes", "rotary_table"]

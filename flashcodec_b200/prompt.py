@@ -1,0 +1,91 @@
+"""Attention over whole prompts, before decoding goes on from a cache.
+
+Decode steps attend to a compressed cache one token at a time; a prompt's own
+attention has many queries for every key and runs here: packed sequences of
+different lengths, causal, grouped heads.  With ``cu_seqlens_k`` the keys of a
+sequence may begin before its queries: the next chunk of a long prompt, over the
+values that a paged cache's ``read`` gives.  One launch (csrc/fc_prompt.cu).
+The reference leaves prompts to the model's own attention.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd import forward_ad
+
+from . import _kernels as K
+
+
+def _rows(name, t):
+    if t.stride(-1) != 1:
+        raise ValueError(f"{name}: the head dim must have unit stride")
+    if t.shape[-2] == 0:
+        raise ValueError(f"{name} has no heads")
+
+
+def prompt_attention(q, k, v, cu_seqlens=None, cu_seqlens_k=None, *, causal=True, scale=None, out=None,
+                     return_lse=False):
+    """softmax(scale * q . K^T) . V of every sequence.
+
+    q: packed (T, Hq, D) with ``cu_seqlens``, or (B, S, Hq, D) without; bf16 or
+        fp16, any strides with unit stride along D; D 64, 96, 128, 192 or 256.
+    k, v: (Tk, Hk, D) or (B, Sk, Hk, D) of q's dtype; Hq a multiple of Hk.
+    cu_seqlens: (B + 1,) int32 CUDA tensor, sequence b being rows cu_seqlens[b] to
+        cu_seqlens[b + 1].  Rows of no sequence (a captured batch of fixed size)
+        get zeros.
+    cu_seqlens_k: the same for k and v (default: ``cu_seqlens``).  Both are read
+        when the kernel runs, and cut to the rows that there are.
+    causal: query i of n sees the keys up to its own, the last query being at the
+        last key; else all keys.  A query that sees none gives zeros (and -inf).
+    scale: of the scores (default D ** -0.5).
+    out: where the outputs go (default: a new tensor; may be q).
+    Returns the outputs in q's shape and dtype, and with ``return_lse`` the natural
+    log of the softmax sums, q.shape[:-1] fp32.
+
+    Scores, softmax and sums are fp32; weights are rounded to q's dtype before they
+    meet the values.  It serves and has no gradient.
+    """
+    K.require_cuda(q, k, v, cu_seqlens, cu_seqlens_k, out)
+    dual = getattr(forward_ad, "_current_level", 0) >= 0  # inside a dual level
+    for t in (q, k, v, out):
+        if t is None:
+            continue
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError("prompt_attention has no gradient: call it under torch.no_grad()")
+        if dual and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("prompt_attention has no tangent: pass the primal of a dual tensor")
+    for name, t in (("k", k), ("v", v), ("cu_seqlens", cu_seqlens), ("cu_seqlens_k", cu_seqlens_k), ("out", out)):
+        if t is not None and t.device != q.device:
+            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+    packed = cu_seqlens is not None
+    if q.dim() != (3 if packed else 4):
+        raise ValueError("q must be (T, heads, D) with cu_seqlens or (B, S, heads, D) without "
+                         f"(got {tuple(q.shape)})")
+    if k.dim() != q.dim() or k.shape != v.shape or k.shape[-1] != q.shape[-1] \
+            or (not packed and k.shape[0] != q.shape[0]):
+        raise ValueError(f"k and v must be alike and go with q (got {tuple(k.shape)}, {tuple(v.shape)} "
+                         f"and {tuple(q.shape)})")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must have one dtype")
+    if cu_seqlens_k is not None and not packed:
+        raise ValueError("cu_seqlens_k goes with cu_seqlens")
+    if packed and cu_seqlens_k is None and k.shape[0] != q.shape[0]:
+        raise ValueError(f"{k.shape[0]} keys for {q.shape[0]} queries need cu_seqlens_k")
+    for name, t in (("cu_seqlens", cu_seqlens), ("cu_seqlens_k", cu_seqlens_k)):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < 1
+                              or t.shape != cu_seqlens.shape or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int32 tensor of one entry more than sequences "
+                             f"(got {t.dtype}, {tuple(t.shape)})")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must have the shape and dtype of q")
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        _rows(name, t)
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+    K.prompt_attn(q, k, v, cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, causal,
+                  q.shape[-1] ** -0.5 if scale is None else float(scale), out, lse)
+    return (out, lse) if return_lse else out
+
+
+__all__ = ["prompt_attention"]

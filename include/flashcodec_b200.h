@@ -678,6 +678,86 @@ FC_API int fc_kv4_select(const void *q, int dtype, int64_t B, int64_t Hq, int64_
                          int64_t sink, int64_t recent, int *pages, void *workspace,
                          size_t workspace_bytes, int *status, void *stream);
 
+/* ---- paged 8-bit KV cache --------------------------------------------------
+ *
+ * The paged cache in 8 bits: `codes` int8 (num_pages, 2, Hk, page_size, D), keys and
+ * values, and `scales` fp32 (num_pages, 2, Hk, page_size / 16), one for every 16 tokens
+ * of a head, both contiguous.  With amax over the tokens that such a run holds so far
+ * and all channels,
+ *     scale = 2^e, e the smallest integer >= -126 with amax < 128 * 2^e (0 for amax = 0),
+ *     code  = floor(x / scale), standing for (code + 1/2) * scale,
+ * and a run with an infinity or a NaN gets a NaN scale: all 16 tokens of it read as NaN.
+ * When an append raises the scale of a run that holds tokens already, their codes are
+ * shifted and equal those of the run quantised at once.  Tokens before lengths[b] count
+ * as held; a run begun anew (its first position appended) forgets its scale.
+ * Page tables, lengths, status bits, head dims and page sizes as for the 4-bit cache.
+ * A page that two sequences share may be read by both, but no append may write it. */
+
+/* As fc_kv4_append, without bounds.  With `axes` (rotary_dim / 2) int32 the positions
+ * are (n_axes, T) and pair i turns by the angle of positions[axes[i]] (entries outside
+ * 0 .. n_axes - 1 count as the nearest); axes NULL: n_axes is not used. */
+FC_API int fc_kv8_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t q_sh, void *q_out,
+                         int64_t qo_sb, int64_t qo_ss, int64_t qo_sh, int64_t Hq,
+                         const void *k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                         const void *v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int dtype,
+                         int64_t B, int64_t S, int64_t T, const int *cu_seqlens,
+                         const int *lengths, const int *positions, const int *axes, int n_axes,
+                         const void *q_weight, const void *k_weight, int w_dtype, float eps,
+                         const float *rotary, int64_t rotary_rows, int rotary_dim,
+                         int interleaved, signed char *codes, float *scales, int64_t num_pages,
+                         int64_t Hk, int64_t D, int64_t page_size, const int *page_table,
+                         int64_t table_stride, int64_t max_pages, int *status, void *stream);
+
+/* As fc_kv4_read: (code + 1/2) * scale rounded to dtype. */
+FC_API int fc_kv8_read(const signed char *codes, const float *scales, int64_t num_pages,
+                       int64_t Hk, int64_t D, int64_t page_size, const int *page_table,
+                       int64_t table_stride, int64_t max_pages, const int *starts, int64_t B,
+                       int64_t S, int64_t T, const int *cu_seqlens, void *k_out, void *v_out,
+                       int dtype, int64_t o_sb, int64_t o_ss, int64_t o_sh, int *status,
+                       void *stream);
+
+/* Bytes of workspace of fc_kv8_attn, as for fc_kv4_attn. */
+FC_API size_t fc_kv8_attn_workspace_size(int64_t B, int64_t Sq, int64_t Hq, int64_t Hk, int64_t D);
+
+/* As fc_kv4_attn, without selected pages. */
+FC_API int fc_kv8_attn(const void *q, int dtype, int64_t B, int64_t Sq, int64_t Hq, int64_t q_sb,
+                       int64_t q_ss, int64_t q_sh, const signed char *codes, const float *scales,
+                       int64_t num_pages, int64_t Hk, int64_t D, int64_t page_size,
+                       const int *page_table, int64_t table_stride, int64_t max_pages,
+                       const int *lengths, float softmax_scale, void *out, int64_t o_sb,
+                       int64_t o_ss, int64_t o_sh, float *lse, void *workspace,
+                       size_t workspace_bytes, int *status, void *stream);
+
+/* ---- attention over whole prompts -------------------------------------------
+ *
+ *     out = softmax(softmax_scale * q . K^T) . V
+ * of sequences of different lengths, Hq a multiple of Hk, bf16 or fp16, head dims 64, 96,
+ * 128, 192 and 256.  No counterpart in the reference, whose prompts run through the
+ * model's own attention.
+ * Packed (Sq = Sk = 0): q, out (Tq, Hq, D) and k, v (Tk, Hk, D) with strides *_ss, *_sh in
+ * elements (*_sb not used), sequence b being rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] of
+ * q and cu_seqlens_k[b] .. of k; both are device memory, read when the kernel runs, and cut
+ * to the rows that there are.  Rows of no sequence get zeros.  Else (B, Sq, Hq, D) and
+ * (B, Sk, Hk, D), Tq = B Sq, Tk = B Sk, cu_seqlens NULL.
+ * Query i of n_q sees the keys 0 .. n_k - n_q + i with `causal` (the last query sees all),
+ * else all n_k; one that sees none gets zeros.  A key or value that a query does not see
+ * does not touch its output, whatever it holds.
+ * lse (as q without D) fp32 or NULL: the natural logarithm of the softmax sums, -inf
+ * where a query sees nothing.  out must not overlap k or v; it may be q itself, but
+ * must not overlap it otherwise.
+ * workspace: of fc_prompt_attn_workspace_size bytes, zero-filled before its first use and
+ * shared with no call that may overlap; its first int is a status word as of the decode
+ * attention (a bounded wait that gave up records the launch there, outputs are invalid then). */
+FC_API size_t fc_prompt_attn_workspace_size(int64_t B, int64_t Tq, int64_t Hq, int64_t Hk, int64_t D);
+FC_API int fc_prompt_attn(const void *q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                          const void *k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                          const void *v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int dtype,
+                          int64_t B, int64_t Sq, int64_t Sk, int64_t Tq, int64_t Tk, int64_t Hq,
+                          int64_t Hk, int64_t D, const int *cu_seqlens_q, const int *cu_seqlens_k,
+                          int causal, float softmax_scale, void *out, int64_t o_sb, int64_t o_ss,
+                          int64_t o_sh, float *lse, void *workspace, size_t workspace_bytes,
+                          void *stream);
+
 #ifdef __cplusplus
 }
 #endif

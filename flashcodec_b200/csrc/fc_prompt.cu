@@ -4,6 +4,36 @@
 //
 // Query i of a sequence of n_q queries and n_k keys is at position n_k - n_q + i and sees the
 // keys up to it (all of them where not causal).
+//
+// 4 D operations a visible pair and head, on tcgen05; what competes with the matrix unit is
+// the softmax: at D = 128 a 128 x 128 tile takes it 512 cycles, and 16384 exponentials take the
+// 16 lanes of the special function units 1024.
+//
+// Tiles.  The heads of a group share their keys, so a tile's 128 rows are TQ = 128 / G tokens
+// times the G heads (row = token * G + head; one TMA box of a 4- or 5-dimensional map): fewer
+// partly filled tiles in short prompts, and less of the diagonal computed in vain.  A block
+// holds one or two query tiles ("streams") and walks the keys in tiles of 128:
+//
+//   warp   TMA: queries, then K and V tiles through a ring
+//   warp   MMA: S = Q K^T into TMEM; O += P V with P read from TMEM, where it replaces S
+//   group of 4 warps a stream: a thread a row; S to registers, running maximum, exp2, P back
+//          in 16 bits; O scaled by it only when the maximum grows by more than 2^8
+//   2 warps: the next item of work, and the V tiles of the diagonal (below)
+//
+// With two streams (D <= 128) one's softmax runs while the other's products do; with wider
+// heads O leaves room for one, whose scores are in two buffers instead.
+//
+// What is masked.  Scores are replaced, not added to, so a NaN there is gone.  A value that no
+// weight but zero meets could still turn a sum into a NaN, so the tiles that hold masked keys
+// (one or two of an item) are looked through in shared memory: what is no number becomes zero
+// there, and is added in plain arithmetic to the rows that do see it.
+//
+// Work.  Items (sequence, KV head, TQ or 2 TQ tokens) are dealt out to one block an SM, the
+// longest first, back and forth; every block finds its own from the lengths, which are on the
+// device, by counting the items of more than a number of tiles.  No block waits for another.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "fc_attn_common.cuh"
 #include "fc_kv4.cuh"
 
@@ -12,10 +42,10 @@ namespace prompt {
 namespace {
 
 using kv4::Rows;
+using kv4::rows_aligned;
 using kv4::rows_meet;
 using kv4::rows_repeat;
 using kv4::same_rows;
-using kv4::warp_find;
 
 // Whether n x Sx rows x and n x Sy rows y can share a byte.
 inline bool meets(const Rows &x, int64_t Sx, const Rows &y, int64_t Sy, int64_t n, int64_t D, int64_t size) {
@@ -32,63 +62,768 @@ inline bool meets(const Rows &x, int64_t Sx, const Rows &y, int64_t Sy, int64_t 
 }
 
 struct Args {
-    const void *q, *k, *v;
+    const void *v;
     void *out;
     float *lse;
-    int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh;
-    int64_t Sq, Sk, Tq, Tk;
-    int B, Hq, Hk, G, causal;
+    int64_t v_sb, v_ss, v_sh, o_sb, o_ss, o_sh;
+    int Sq, Sk, Tq, Tk;
+    int B, D, Hq, Hk, G, TQ, causal, o_vec;
     const int *cu_q, *cu_k;
-    float scale;  // softmax_scale * log2(e)
+    float scale;  // |softmax_scale| * log2(e), > 0
+    int negative;
+    int *status;
+    int epoch;
 };
 
-// One warp a query and head.
-template <typename T, int W>
-__global__ void __launch_bounds__(256) prompt_simple_kernel(const __grid_constant__ Args a) {
-    const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), t = unit / a.Hq;
-    if (t >= a.Tq) return;
-    const int lane = threadIdx.x & 31, h = (int)(unit - t * a.Hq), hk = h / a.G;
-    int64_t k0 = 0, n = 0, b = 0, i = t;
-    if (!a.cu_q) {
-        b = t / a.Sq;
-        i = t - b * a.Sq;
-        n = a.Sk;
-        if (a.causal) n = max(n - a.Sq + i + 1, (int64_t)0);
-    } else if (a.B) {
-        const int *cu = a.cu_q;
-        const int w = warp_find([=](int j) { return (int64_t)cu[j]; }, a.B, t);
-        if (t >= cu[w] && t < cu[w + 1]) {
-            k0 = max(a.cu_k[w], 0);
-            n = max(min((int64_t)a.cu_k[w + 1], a.Tk) - k0, (int64_t)0);
-            if (a.causal) n = max(n - (min((int64_t)cu[w + 1], a.Tq) - 1 - t), (int64_t)0);
+constexpr int kTile = 128;          // rows of a query tile, keys of a tile
+constexpr int kBox = kTile * 128;   // bytes of 128 rows of 64 channels
+constexpr int kItems = 3;           // items known ahead
+
+template <int DP> struct Cfg {
+    static constexpr int NQ = DP <= 128 ? 2 : 1;         // streams
+    static constexpr int LA = NQ == 2 ? 1 : 2;           // score tiles ahead of the softmax
+    static constexpr int UC = DP == 256 ? 128 : DP;      // channels of a ring stage
+    static constexpr int NU = DP / UC;                   // stages of a tile
+    static constexpr int STAGE = kTile * UC * 2;
+    static constexpr int NST = DP == 64 ? 8 : DP == 192 ? 3 : 5;
+    static constexpr int QB = kTile * DP * 2;            // bytes of a query tile
+    static constexpr int SMEM = 1024 + NQ * QB + NST * STAGE;
+    static constexpr int THREADS = 128 * NQ + 128;
+    static constexpr int O_COL = 256;                    // TMEM: scores at 0 and 128, outputs from here
+    static_assert(O_COL + NQ * DP <= 512, "TMEM");
+};
+
+// ------------------------------------------------------------------------ PTX
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, int v,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(smem_addr(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Shared-memory matrix descriptor, 128-byte swizzle; 1024 bytes between groups of 8 rows, and,
+// where the operand is wider than 64 elements along its contiguous dim, 16 KB from box to box.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(kBox >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// M = 128, N = n, fp32 sums; bf16 (or fp16) operands, B K-major or MN-major.
+__host__ __device__ constexpr uint32_t idesc(int n, bool f16, int b_mn) {
+    return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+#define FC_R16(v, o) "=f"(v[o]), "=f"(v[o + 1]), "=f"(v[o + 2]), "=f"(v[o + 3]), "=f"(v[o + 4]), "=f"(v[o + 5]), \
+    "=f"(v[o + 6]), "=f"(v[o + 7]), "=f"(v[o + 8]), "=f"(v[o + 9]), "=f"(v[o + 10]), "=f"(v[o + 11]),           \
+    "=f"(v[o + 12]), "=f"(v[o + 13]), "=f"(v[o + 14]), "=f"(v[o + 15])
+#define FC_W16(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]),      \
+    "r"(v[o + 6]), "r"(v[o + 7]), "r"(v[o + 8]), "r"(v[o + 9]), "r"(v[o + 10]), "r"(v[o + 11]),                 \
+    "r"(v[o + 12]), "r"(v[o + 13]), "r"(v[o + 14]), "r"(v[o + 15])
+// 32 columns of the warp's 32 TMEM lanes, one lane a thread.
+__device__ __forceinline__ void tmem_ld32(uint32_t at, float *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : FC_R16(v, 0), FC_R16(v, 16) : "r"(at));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::FC_W16(v, 0), FC_W16(v, 16), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::FC_W16(v, 0),
+        "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (F16) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+// ------------------------------------------------------------------------ work
+struct Sequence {
+    int q0, nq, k0, nk;  // rows, cut to those that there are
+};
+
+__device__ __forceinline__ Sequence sequence(const Args &a, int b) {
+    Sequence s;
+    if (!a.cu_q) return Sequence{0, a.Sq, 0, a.Sk};
+    s.q0 = min(max(a.cu_q[b], 0), a.Tq);
+    s.nq = max(min(a.cu_q[b + 1], a.Tq) - s.q0, 0);
+    s.k0 = min(max(a.cu_k[b], 0), a.Tk);
+    s.nk = max(min(a.cu_k[b + 1], a.Tk) - s.k0, 0);
+    return s;
+}
+
+struct Item {
+    int b, h, t;         // sequence, KV head, first token
+    Sequence s;
+    int nt[2];           // key tiles of the streams
+    int tiles, first;    // key tiles; the first that holds masked keys
+    int valid;           // 0: no more work
+};
+
+// Keys that token i sees.
+__device__ __forceinline__ int visible(const Args &a, const Sequence &s, int i) {
+    return a.causal ? max(min(s.nk - s.nq + i + 1, s.nk), 0) : s.nk;
+}
+
+__device__ __forceinline__ int tiles_of(int keys) { return (int)(((unsigned)keys + kTile - 1) / kTile); }
+
+// Items of a sequence with at least w > 0 key tiles, TP tokens each: those from a token on.
+__device__ __forceinline__ int items_from(const Args &a, const Sequence &s, int w, int TP) {
+    const int n = (s.nq + TP - 1) / TP;
+    if (!a.causal) return tiles_of(s.nk) >= w ? n : 0;
+    if (tiles_of(s.nk) < w) return 0;
+    // item t's last token sees min(nk, nk - nq + (t + 1) TP) keys: more than (w - 1) kTile
+    const int64_t need = (int64_t)(w - 1) * kTile - ((int64_t)s.nk - s.nq);  // (t + 1) TP > need
+    const int64_t t = need < 0 ? 0 : need / TP;
+    return (int)max((int64_t)0, n - t);
+}
+
+// Item number `rank` of the line of all (sequence, tokens), the ones of most tiles first.  A
+// warp calls it.  Items of no tiles come last.
+__device__ __forceinline__ bool find_item(const Args &a, int64_t rank, int TP, int most, Item &x) {
+    const int lane = threadIdx.x & 31;
+    auto count = [&](int w) {  // items of at least w tiles
+        int64_t n = 0;
+        for (int b = lane; b < a.B; b += 32) {
+            const Sequence s = sequence(a, b);
+            n += w ? items_from(a, s, w, TP) : (s.nq + TP - 1) / TP;
+        }
+#pragma unroll
+        for (int o = 16; o; o /= 2) n += __shfl_xor_sync(0xffffffffu, n, o);
+        return n;
+    };
+    if (count(0) <= rank) return false;
+    int lo = 0, hi = most + 1;  // count(lo) > rank >= count(hi)
+    while (hi - lo > 1) {
+        const int mid = lo + (hi - lo) / 2;
+        (count(mid) > rank ? lo : hi) = mid;
+    }
+    int64_t left = rank - count(lo + 1);  // among the items of lo tiles, by sequence
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        const int b = b0 + lane;
+        int n = 0, t0 = 0;
+        if (b < a.B) {
+            const Sequence s = sequence(a, b);
+            const int all = (s.nq + TP - 1) / TP, ge = lo ? items_from(a, s, lo, TP) : all;
+            n = ge - items_from(a, s, lo + 1, TP);
+            t0 = a.causal ? all - ge : 0;
+        }
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, left < upto);
+        if (here) {
+            const int l = __ffs(here) - 1;
+            x.b = b0 + l;
+            x.t = (__shfl_sync(0xffffffffu, t0, l) + (int)left - __shfl_sync(0xffffffffu, upto - n, l)) * TP;
+            return true;
+        }
+        left -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;  // cu_seqlens changed under way
+}
+
+template <int DP, bool F16>
+struct Block {
+    using C = Cfg<DP>;
+    static constexpr int NQ = C::NQ, LA = C::LA, NU = C::NU, UC = C::UC, NST = C::NST;
+
+    const Args &a;
+    unsigned char *q_s, *ring;
+    uint64_t *kv_full, *kv_empty, *v_raw, *v_half, *q_full, *q_free, *s_full, *p_full, *o_done, *item_full, *item_empty;
+    Item *items;
+    volatile int *abort_s;
+    int *bad;  // by item: its number + 1 if a value was no number
+    uint32_t tmem;
+
+    __device__ __forceinline__ explicit Block(const Args &args) : a(args) {}
+
+    // Every wait is bounded; one that gives up records the launch and ends the block's work.
+    __device__ __forceinline__ bool wait(uint64_t *bar, unsigned parity) const {
+        if (mbar_try_wait(bar, parity)) return true;
+        const uint64_t t0 = global_ns();
+        for (;;) {
+            if (mbar_try_wait_sleep(bar, parity, 20000)) return true;
+            if (*abort_s) return false;
+            if (global_ns() - t0 > kWaitNs) {
+                atomicMax(a.status, a.epoch);
+                *abort_s = 1;
+                return false;
+            }
         }
     }
-    const T *q = static_cast<const T *>(a.q) + b * a.q_sb + i * a.q_ss + h * a.q_sh;
-    float x[W], o[W], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; w++) {
-        x[w] = Elem<T>::to_f32(q[lane + 32 * w]) * a.scale;
-        o[w] = 0.f;
+
+    // The same for a whole warp, which goes on or gives up together.
+    __device__ __forceinline__ bool wait_warp(uint64_t *bar, unsigned parity) const {
+        return __all_sync(0xffffffffu, wait(bar, parity));
     }
-    for (int64_t j = k0; j < k0 + n; j++) {
-        const T *k = static_cast<const T *>(a.k) + b * a.k_sb + j * a.k_ss + hk * a.k_sh;
-        const T *v = static_cast<const T *>(a.v) + b * a.v_sb + j * a.v_ss + hk * a.v_sh;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < W; i++) s = fmaf(x[i], Elem<T>::to_f32(k[lane + 32 * i]), s);
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-        const float top = fmaxf(m, s), ref = top == -INFINITY ? 0.f : top;
-        const float f = exp2f(m - ref), p = exp2f(s - ref);
-        m = top;
-        l = l * f + p;
-#pragma unroll
-        for (int i = 0; i < W; i++) o[i] = fmaf(o[i], f, p * Elem<T>::to_f32(v[lane + 32 * i]));
+
+    // Stage position, from an item's first one on, of V tile j.  Order: K0 .. K(LA - 1), then
+    // V(j), K(j + LA) for every j.
+    __device__ __forceinline__ static int64_t v_pos(int j, int tiles) {
+        return NU * ((int64_t)min(LA, tiles) + j + min(j, max(tiles - LA, 0)));
     }
-    T *out = static_cast<T *>(a.out) + b * a.o_sb + i * a.o_ss + h * a.o_sh;
+
+    // Reads item `it` out of the ring of items: a warp, or one thread.
+    template <bool WARP>
+    __device__ __forceinline__ bool next(int it, Item &x) const {
+        const int slot = it % kItems;
+        if (!(WARP ? wait_warp(item_full + slot, (it / kItems) & 1) : wait(item_full + slot, (it / kItems) & 1))) return false;
+        x = items[slot];
+        if constexpr (WARP) __syncwarp();
+        if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(item_empty + slot);
+        return x.valid;
+    }
+
+    // ---------------------------------------------------------------- TMA warp
+    __device__ __forceinline__ void load(const CUtensorMap *mq, const CUtensorMap *mk, const CUtensorMap *mv) {
+        int64_t pos = 0;
+        unsigned q_uses[2] = {0, 0};
+        Item x;
+        for (int it = 0; next<false>(it, x); it++) {
+            if (!x.tiles) continue;
+            const int bb = a.cu_q ? 0 : x.b;
+            auto queries = [&](int s) {
+                if (!x.nt[s]) return true;
+                if (q_uses[s] && !wait(q_free + s, (q_uses[s] - 1) & 1)) return false;
+                q_uses[s]++;
+                mbar_expect_tx(q_full + s, a.TQ * a.G * 128 * (DP / 64));
 #pragma unroll
-    for (int i = 0; i < W; i++) store_from_f32(out, lane + 32 * i, Elem<T>::code, l == 0.f ? 0.f : o[i] / l);
-    if (a.lse && lane == 0) a.lse[t * a.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
+                for (int c = 0; c < DP / 64; c++)
+                    tma_load_5d(smem_addr(q_s) + s * C::QB + c * kBox, mq, 64 * c, 0, x.h, x.s.q0 + x.t + s * a.TQ, bb, q_full + s);
+                return true;
+            };
+            // (a tile that is looked through first arrives there instead)
+            auto tile = [&](const CUtensorMap *m, int j, uint64_t *full) {
+#pragma unroll
+                for (int u = 0; u < NU; u++, pos++) {
+                    const int st = (int)(pos % NST);
+                    if (pos >= NST && !wait(kv_empty + st, (pos / NST - 1) & 1)) return false;
+                    mbar_expect_tx(full + st, C::STAGE);
+#pragma unroll
+                    for (int c = 0; c < UC / 64; c++)
+                        tma_load_4d(smem_addr(ring) + st * C::STAGE + c * kBox, m, u * UC + 64 * c, x.h, x.s.k0 + j * kTile, bb, full + st);
+                }
+                return true;
+            };
+            if (!queries(0) || !tile(mk, 0, kv_full)) return;
+            if (NQ == 2 && !queries(1)) return;
+            for (int j = 1; j < min(LA, x.tiles); j++)
+                if (!tile(mk, j, kv_full)) return;
+            for (int j = 0; j < x.tiles; j++) {
+                if (!tile(mv, j, j >= x.first ? v_raw : kv_full)) return;
+                if (j + LA < x.tiles && !tile(mk, j + LA, kv_full)) return;
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- MMA warp
+    __device__ __forceinline__ void multiply() {
+        int64_t pos = 0;
+        unsigned q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
+        constexpr uint32_t id_s = idesc(kTile, F16, 0), id_o = idesc(UC, F16, 1);
+        Item x;
+        for (int it = 0; next<false>(it, x); it++) {
+            if (!x.tiles) continue;
+            auto full = [&](int64_t p) {
+#pragma unroll
+                for (int u = 0; u < NU; u++)
+                    if (!wait(kv_full + (p + u) % NST, ((p + u) / NST) & 1)) return false;
+                return true;
+            };
+            auto release = [&](int64_t p) {
+#pragma unroll
+                for (int u = 0; u < NU; u++) mma_commit(kv_empty + (p + u) % NST);
+            };
+            auto scores = [&](int s, int j, int64_t p) {  // K tile j is at p
+                if (j >= x.nt[s]) return true;
+                if (j == 0 && !wait(q_full + s, q_uses[s]++ & 1)) return false;
+                tc_fence_after();
+                const int slot = NQ == 2 ? s : j & 1;
+#pragma unroll
+                for (int u = 0; u < NU; u++) {
+                    const uint32_t kt = smem_addr(ring) + (uint32_t)((p + u) % NST) * C::STAGE;
+                    const uint32_t qt = smem_addr(q_s) + s * C::QB + u * (UC / 64) * kBox;
+#pragma unroll
+                    for (int k = 0; k < UC / 16; k++) {
+                        const uint32_t at = (k >> 2) * kBox + (k & 3) * 32;
+                        mma_ss(tmem + slot * kTile, sw128_desc(qt + at), sw128_desc(kt + at), id_s, u + k > 0);
+                    }
+                }
+                mma_commit(s_full + slot);
+                if (j == x.nt[s] - 1) mma_commit(q_free + s);
+                return true;
+            };
+            for (int j = 0; j < min(LA, x.tiles); j++) {
+                if (!full(pos)) return;
+                for (int s = 0; s < NQ; s++)
+                    if (!scores(s, j, pos)) return;
+                release(pos);
+                pos += NU;
+            }
+            for (int j = 0; j < x.tiles; j++) {
+                const int64_t vp = pos, kp = pos + NU;
+                const bool more = j + LA < x.tiles;
+                pos += more ? 2 * NU : NU;
+                if (!full(vp)) return;
+#pragma unroll
+                for (int s = 0; s < NQ; s++) {
+                    if (j < x.nt[s]) {
+                        const int slot = NQ == 2 ? s : j & 1;
+                        if (!wait(p_full + slot, p_uses[slot]++ & 1)) return;
+                        tc_fence_after();
+#pragma unroll
+                        for (int u = 0; u < NU; u++) {
+                            const uint32_t vt = smem_addr(ring) + (uint32_t)((vp + u) % NST) * C::STAGE;
+#pragma unroll
+                            for (int k = 0; k < kTile / 16; k++)
+                                mma_ts(tmem + C::O_COL + s * DP + u * UC, tmem + slot * kTile + k * 8, sw128_desc(vt + k * 2048),
+                                       id_o, j > 0 || k > 0);
+                        }
+                        mma_commit(o_done + s);
+                    }
+                    if (s == NQ - 1) release(vp);
+                    if (more) {
+                        if (s == 0 && !full(kp)) return;
+                        if (!scores(s, j + LA, kp)) return;
+                        if (s == NQ - 1) release(kp);
+                    }
+                }
+            }
+        }
+    }
+
+    // ------------------------------------------------------------ softmax warps
+    __device__ __forceinline__ void softmax(int s) {
+        const int row = threadIdx.x & 127, lane = threadIdx.x & 31;
+        const uint32_t lanes = (uint32_t)(row & ~31) << 16;  // of this warp
+        const int tok = row / a.G, head = row - tok * a.G;
+        unsigned s_uses[2] = {0, 0}, o_count = 0;
+        Item x;
+        for (int it = 0; next<true>(it, x); it++) {
+            const int i = x.t + s * a.TQ + tok;
+            const bool on = tok < a.TQ && i < x.s.nq;
+            // (rows of no query need no mask: their results go nowhere)
+            const int vis = on ? visible(a, x.s, i) : 0x7fffffff;
+            float ref = -INFINITY, l = 0.f;  // reference, in scores; sum
+            const int nt = NQ == 2 && s ? x.nt[1] : x.nt[0];
+            for (int j = 0; j < nt; j++) {
+                const int slot = NQ == 2 ? s : j & 1;
+                const uint32_t at = tmem + lanes + slot * kTile;
+                if (!wait_warp(s_full + slot, s_uses[NQ == 2 ? 0 : slot]++ & 1)) return;
+                tc_fence_after();
+                float z[kTile];
+#pragma unroll
+                for (int c = 0; c < kTile; c += 32) tmem_ld32(at + c, z + c);
+                tmem_wait_ld();
+                if (a.negative) {
+#pragma unroll
+                    for (int c = 0; c < kTile; c++) z[c] = -z[c];
+                }
+                const int lim = vis - j * kTile;
+                if (__any_sync(0xffffffffu, lim < kTile)) {
+#pragma unroll
+                    for (int c = 0; c < kTile; c++) z[c] = c < lim ? z[c] : -INFINITY;
+                }
+                float t[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+                for (int c = 4; c < kTile; c += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) t[k] = fmaxf(fmaxf(t[k], z[c + k]), c + 4 + k < kTile ? z[c + 4 + k] : t[k]);
+                const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+                // the reference follows only a maximum that is 2^8 above it: weights stay below 2^8
+                if (__any_sync(0xffffffffu, (top - ref) * a.scale > 8.f)) {
+                    const float m = fmaxf(ref, top);
+                    const float f = ref == -INFINITY ? 0.f : exp2_fast((ref - m) * a.scale);
+                    ref = m;
+                    l *= f;
+                    if (j > 0) {
+                        if (!wait_warp(o_done + s, (o_count - 1) & 1)) return;
+                        tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < DP; c += 32) {
+                            float o[32];
+                            uint32_t w[32];
+                            const uint32_t oat = tmem + lanes + C::O_COL + s * DP + c;
+                            tmem_ld32(oat, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; k++) w[k] = __float_as_uint(o[k] * f);
+                            tmem_st32(oat, w);
+                        }
+                    }
+                }
+                const float off = ref == -INFINITY ? 0.f : -ref * a.scale;
+                float sum[4] = {};
+#pragma unroll
+                for (int c = 0; c < kTile; c += 32) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const float u = exp2_fast(fmaf(z[c + 2 * k], a.scale, off));
+                        const float v = exp2_fast(fmaf(z[c + 2 * k + 1], a.scale, off));
+                        sum[2 * k & 3] += u;
+                        sum[2 * k + 1 & 3] += v;
+                        w[k] = pack2<F16>(u, v);
+                    }
+                    tmem_st16(at + c / 2, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + slot);
+                o_count++;
+            }
+            // scores that come two tiles ahead leave two products open: a parity tells one phase from the next only
+            if (NQ == 1 && nt > 1 && !wait_warp(o_done + s, o_count & 1)) return;
+            if (nt && !wait_warp(o_done + s, (o_count - 1) & 1)) return;
+            tc_fence_after();
+            if (!write(x, it, s, i, head, on, vis, nt, ref, l, lanes)) return;
+        }
+    }
+
+    // Outputs of one row.
+    __device__ __forceinline__ bool write(const Item &x, int it, int s, int i, int head, bool on, int vis, int nt, float ref,
+                                          float l, uint32_t lanes) const {
+        using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
+        const int h = x.h * a.G + head;
+        const int64_t row = a.cu_q ? x.s.q0 + i : i;
+        T *out = static_cast<T *>(a.out) + (a.cu_q ? 0 : x.b * a.o_sb) + row * a.o_ss + h * a.o_sh;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const bool fix = nt && *reinterpret_cast<volatile int *>(bad + (it & 1)) == it + 1;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+            if (c >= a.D) break;
+            float o[32];
+            if (nt) {
+                tmem_ld32(tmem + lanes + C::O_COL + s * DP + c, o);
+                tmem_wait_ld();
+            }
+            if (fix && on) {  // values of the masked tiles that are no numbers
+                const T *v = static_cast<const T *>(a.v) + (a.cu_q ? 0 : x.b * a.v_sb) + x.h * a.v_sh + c;
+                for (int j = x.first * kTile; j < vis; j++)
+#pragma unroll
+                    for (int k = 0; k < 32; k++) {
+                        const float y = Elem<T>::to_f32(v[(int64_t)(x.s.k0 + j) * a.v_ss + k]);
+                        if (!(fabsf(y) < INFINITY)) o[k] += y;
+                    }
+            }
+            if (on) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        w[e] = l == 0.f ? 0u : pack2<F16>(o[k + 2 * e] * inv, o[k + 2 * e + 1] * inv);
+                    if (a.o_vec) {
+                        *reinterpret_cast<uint4 *>(out + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            reinterpret_cast<uint16_t *>(out)[c + k + 2 * e] = (uint16_t)w[e];
+                            reinterpret_cast<uint16_t *>(out)[c + k + 2 * e + 1] = (uint16_t)(w[e] >> 16);
+                        }
+                    }
+                }
+            }
+        }
+        tc_fence_before();
+        if (on && a.lse) {
+            const int64_t at = ((a.cu_q ? row : (int64_t)x.b * a.Sq + i)) * a.Hq + h;
+            a.lse[at] = l == 0.f ? -INFINITY : fmaf(ref, a.scale, log2f(l)) * 0.693147180559945309f;
+        }
+        return true;
+    }
+
+    // ------------------------------------------------------------- helper warps
+    // Warp 0 of the two also finds the items, one ahead of the values that it looks through.
+    __device__ __forceinline__ void help(int w) {
+        const int lane = threadIdx.x & 31;
+        int64_t pos = 0;
+        const int TP = NQ * a.TQ;
+        int most = 0;
+        if (w == 0) {
+            for (int b = lane; b < a.B; b += 32) most = max(most, tiles_of(sequence(a, b).nk));
+            most = __reduce_max_sync(0xffffffffu, most);
+        }
+        auto publish = [&](int it) {
+            const int slot = it % kItems;
+            if (it >= kItems && !wait_warp(item_empty + slot, (it / kItems - 1) & 1)) return false;
+            const int64_t n = gridDim.x, c = blockIdx.x, rank = it * n + (it & 1 ? n - 1 - c : c);
+            Item x{};
+            x.valid = find_item(a, rank / a.Hk, TP, most, x);
+            if (x.valid) {
+                x.h = (int)(rank % a.Hk);
+                x.s = sequence(a, x.b);
+                for (int s = 0; s < NQ; s++) {
+                    const int t0 = x.t + s * a.TQ;
+                    x.nt[s] = t0 < x.s.nq ? tiles_of(visible(a, x.s, min(t0 + a.TQ, x.s.nq) - 1)) : 0;
+                }
+                x.tiles = max(x.nt[0], x.nt[1]);
+                x.first = visible(a, x.s, x.t) / kTile;
+            }
+            if (lane == 0) {
+                items[slot] = x;
+                mbar_arrive(item_full + slot);
+            }
+            return true;
+        };
+        if (w == 0 && !publish(0)) return;
+        unsigned seen = 0;  // by stage: the parity of the tiles looked through
+        Item x;
+        for (int it = 0; next<true>(it, x); it++) {
+            if (w == 0 && !publish(it + 1)) return;
+            bool any = false;
+            for (int j = x.first; j < x.tiles; j++)
+                for (int u = 0; u < NU; u++) {
+                    const int64_t p = pos + v_pos(j, x.tiles) + u;
+                    const int st = (int)(p % NST);
+                    // (A barrier for these tiles alone: their next use waits for this one, so no phase of
+                    // it can be missed, and none passed by a warp that is ahead.)
+                    const unsigned parity = seen >> st & 1;
+                    seen ^= 1u << st;
+                    if (!wait_warp(v_raw + st, parity)) return;
+                    uint4 *v = reinterpret_cast<uint4 *>(ring + st * C::STAGE) + w * 32 + lane;
+                    constexpr uint32_t E = F16 ? 0x7c007c00u : 0x7f807f80u, ONE = F16 ? 0x04000400u : 0x00800080u;
+#pragma unroll 4
+                    for (int i = 0; i < C::STAGE / 16 / 64; i++) {
+                        uint4 y = v[i * 64];
+                        // an exponent of all ones carries into the sign bit
+                        auto odd = [](uint32_t z) { return ((z & E) + ONE) & 0x80008000u; };
+                        if (odd(y.x) | odd(y.y) | odd(y.z) | odd(y.w)) {
+                            any = true;
+                            auto zero = [&](uint32_t z) {
+                                const uint32_t m = odd(z);
+                                return z & ~((m >> 15) * 0xffffu);
+                            };
+                            v[i * 64] = make_uint4(zero(y.x), zero(y.y), zero(y.z), zero(y.w));
+                        }
+                    }
+                    if (any) *reinterpret_cast<volatile int *>(bad + (it & 1)) = it + 1;
+                    fence_async_smem();
+                    __syncwarp();
+                    if (w == 0 && !wait_warp(v_half + st, parity)) return;
+                    if (lane == 0) mbar_arrive(w == 0 ? kv_full + st : v_half + st);
+                }
+            pos += 2 * (int64_t)NU * x.tiles;
+        }
+    }
+};
+
+template <int DP, bool F16>
+__global__ void __launch_bounds__(Cfg<DP>::THREADS, 1)
+prompt_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+              const __grid_constant__ CUtensorMap mv, const __grid_constant__ Args a) {
+    using C = Cfg<DP>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ uint64_t bars[4 * C::NST + 2 + 2 + 2 + 2 + 2 + 2 * kItems];
+    __shared__ Item items[kItems];
+    __shared__ int abort_s, bad[2];
+    __shared__ uint32_t tmem_s;
+    Block<DP, F16> k(a);
+    k.q_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    k.ring = k.q_s + C::NQ * C::QB;
+    uint64_t *p = bars;
+    k.kv_full = p; p += C::NST;
+    k.kv_empty = p; p += C::NST;
+    k.v_raw = p; p += C::NST;
+    k.v_half = p; p += C::NST;
+    k.q_full = p; p += 2;
+    k.q_free = p; p += 2;
+    k.s_full = p; p += 2;
+    k.p_full = p; p += 2;
+    k.o_done = p; p += 2;
+    k.item_full = p; p += kItems;
+    k.item_empty = p;
+    k.items = items;
+    k.abort_s = &abort_s;
+    k.bad = bad;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int SW = 4 * C::NQ;  // softmax warps
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::NST; i++) {
+            mbar_init(k.kv_full + i, 1);
+            mbar_init(k.kv_empty + i, 1);
+            mbar_init(k.v_raw + i, 1);
+            mbar_init(k.v_half + i, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(k.q_full + i, 1);
+            mbar_init(k.q_free + i, 1);
+            mbar_init(k.s_full + i, 1);
+            mbar_init(k.p_full + i, 4);
+            mbar_init(k.o_done + i, 1);
+            bad[i] = 0;
+        }
+        for (int i = 0; i < kItems; i++) {
+            mbar_init(k.item_full + i, 1);
+            mbar_init(k.item_empty + i, SW + 4);
+        }
+        abort_s = 0;
+        fence_mbar_init();
+    }
+    if (warp == SW + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // rows of no sequence: zeros
+    if (a.cu_q) {
+        const int lo = a.B ? min(max(a.cu_q[0], 0), a.Tq) : a.Tq, hi = a.B ? min(max(a.cu_q[a.B], 0), a.Tq) : a.Tq;
+        const int64_t n = (int64_t)(lo + a.Tq - hi) * a.Hq;
+        for (int64_t r = (int64_t)blockIdx.x * (C::THREADS / 32) + warp; r < n; r += (int64_t)gridDim.x * (C::THREADS / 32)) {
+            const int64_t t = r / a.Hq, row = t < lo ? t : t - lo + hi, h = r - t * a.Hq;
+            uint16_t *out = static_cast<uint16_t *>(a.out) + row * a.o_ss + h * a.o_sh;
+            for (int d = lane; d < a.D; d += 32) out[d] = 0;
+            if (a.lse && lane == 0) a.lse[row * a.Hq + h] = -INFINITY;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    k.tmem = tmem_s;
+    // two streams: 384 threads of 168 registers, shared out as 256 of 200 and 128 of 104
+    if (warp < SW) {
+        if constexpr (C::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        k.softmax(warp >> 2);
+    } else if (warp == SW) {
+        if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+            k.load(&mq, &mk, &mv);
+        }
+    } else if (warp == SW + 1) {
+        if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (lane == 0) k.multiply();
+    } else {
+        if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        k.help(warp - SW - 2);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (abort_s) {  // copies and products in flight end (within microseconds) before their memory is given back
+        const uint64_t t0 = global_ns();
+        while (global_ns() - t0 < 2000000) {}
+    }
+    if (warp == SW + 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_s));
+    }
+}
+
+// ------------------------------------------------------------------ host side
+PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+
+// A map of `rank` dims, the channels first; boxes of 64 of them.
+bool encode(CUtensorMap *map, bool f16, const void *p, int rank, const int64_t *dims, const int64_t *strides, const int64_t *box) {
+    cuuint64_t d[5], s[4];
+    cuuint32_t b[5], e[5];
+    for (int i = 0; i < rank; i++) {
+        d[i] = (cuuint64_t)dims[i];
+        b[i] = (cuuint32_t)box[i];
+        e[i] = 1;
+        if (i) s[i - 1] = (cuuint64_t)(dims[i] > 1 ? strides[i] * 2 : 16);
+    }
+    auto fn = get_encode();
+    return fn && fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void *>(p),
+                    d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What a map can walk: rows on 16-byte boundaries, apart from one another.
+bool walkable(const void *p, int64_t sb, int64_t nb, int64_t ss, int64_t ns, int64_t sh, int64_t nh) {
+    auto ok = [](int64_t s, int64_t n) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (int64_t(1) << 38)); };
+    return aligned(p, 16) && ok(sb, nb) && ok(ss, ns) && ok(sh, nh);
+}
+
+template <int DP, bool F16>
+int launch(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const Args &a, int64_t items, cudaStream_t st) {
+    using C = Cfg<DP>;
+    static bool ready[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { set_error("prompt_attn: no device"); return FC_ECUDA; }
+    if (!ready[dev]) {
+        if (cudaFuncSetAttribute(prompt_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
+            set_error("prompt_attn: the kernel does not fit this device");
+            return FC_ECUDA;
+        }
+        // the warps that ask for more registers wait for what the others give back: never launch
+        // a kernel that was built with too few to share out
+        cudaFuncAttributes attr;
+        if (cudaFuncGetAttributes(&attr, prompt_kernel<DP, F16>) != cudaSuccess || (C::NQ == 2 && attr.numRegs != 168)) {
+            set_error("prompt_attn: the kernel was built with another number of registers");
+            return FC_ECUDA;
+        }
+        ready[dev] = true;
+    }
+    const int64_t blocks = items < num_sms() ? items : num_sms();
+    prompt_kernel<DP, F16><<<(unsigned)blocks, C::THREADS, C::SMEM, st>>>(mq, mk, mv, a);
+    return check_launch("prompt_attn");
 }
 
 }  // namespace
@@ -124,6 +859,7 @@ extern "C" int fc_prompt_attn(const void *q, int64_t q_sb, int64_t q_ss, int64_t
         set_error("prompt_attn: query heads (%lld) must be a multiple of kv heads (%lld)", (long long)Hq, (long long)Hk);
         return FC_EINVAL;
     }
+    if (Hq / Hk > kTile) { set_error("prompt_attn: more than %d query heads to a kv head", kTile); return FC_ENOTSUP; }
     if (!(softmax_scale == softmax_scale) || softmax_scale - softmax_scale != 0.f) {
         set_error("prompt_attn: the softmax scale must be finite");
         return FC_EINVAL;
@@ -148,22 +884,50 @@ extern "C" int fc_prompt_attn(const void *q, int64_t q_sb, int64_t q_ss, int64_t
         set_error("prompt_attn: workspace of %zu bytes is too small", workspace_bytes);
         return FC_ERANGE;
     }
+    if (!walkable(q, q_sb, nb, q_ss, nq, q_sh, Hq) ||
+        (Tk && (!walkable(k, k_sb, nb, k_ss, nk, k_sh, Hk) || !walkable(v, v_sb, nb, v_ss, nk, v_sh, Hk)))) {
+        set_error("prompt_attn: rows of q, k and v must lie on 16-byte boundaries, with positive strides");
+        return FC_EINVAL;
+    }
+    const bool f16 = dtype == FC_F16;
     Args a{};
-    a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse;
-    a.q_sb = q_sb; a.q_ss = q_ss; a.q_sh = q_sh;
-    a.k_sb = k_sb; a.k_ss = k_ss; a.k_sh = k_sh;
+    a.v = v; a.out = out; a.lse = lse;
     a.v_sb = v_sb; a.v_ss = v_ss; a.v_sh = v_sh;
     a.o_sb = o_sb; a.o_ss = o_ss; a.o_sh = o_sh;
-    a.Sq = Sq; a.Sk = Sk; a.Tq = Tq; a.Tk = Tk; a.B = (int)B; a.Hq = (int)Hq; a.Hk = (int)Hk; a.G = (int)(Hq / Hk); a.causal = causal;
+    a.Sq = (int)Sq; a.Sk = (int)Sk; a.Tq = (int)Tq; a.Tk = (int)Tk;
+    a.B = (int)B; a.D = (int)D; a.Hq = (int)Hq; a.Hk = (int)Hk; a.G = (int)(Hq / Hk); a.TQ = kTile / a.G;
+    a.causal = causal;
+    a.o_vec = rows_aligned(out, dtype, o_sb, o_ss, o_sh);
     a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k;
-    a.scale = softmax_scale * 1.44269504088896341f;
-    const int64_t blocks = (Tq * Hq + 7) / 8;
-    if (blocks > 0x7fffffff) { set_error("prompt_attn: too many rows"); return FC_ENOTSUP; }
+    const float s = softmax_scale * 1.44269504088896341f;
+    a.negative = s < 0.f;
+    // a factor of zero would turn a masked score into a NaN; this one rounds every score to zero
+    a.scale = s < 0.f ? -s : s > 1e-30f ? s : 1e-30f;
+    a.status = static_cast<int *>(workspace);
+    a.epoch = next_epoch();
+    const int64_t one = 1;
+    CUtensorMap mq, mk, mv;
+    {
+        const int64_t dims[5] = {D, a.G, Hk, nq, nb}, st[5] = {1, q_sh, a.G * q_sh, q_ss, q_sb}, box[5] = {64, a.G, 1, a.TQ, 1};
+        bool ok = encode(&mq, f16, q, 5, dims, st, box);
+        const int64_t kd[4] = {D, Hk, nk > one ? nk : one, nb}, kb[4] = {64, 1, kTile, 1};
+        const int64_t ks[4] = {1, k_sh, k_ss, k_sb}, vs[4] = {1, v_sh, v_ss, v_sb};
+        ok = ok && encode(&mk, f16, Tk ? k : q, 4, kd, ks, kb) && encode(&mv, f16, Tk ? v : q, 4, kd, vs, kb);
+        if (!ok) { set_error("prompt_attn: the tensor maps cannot be made"); return FC_ECUDA; }
+    }
+    // no more items than this, whatever the lengths
+    auto items = [&](int nqt) {
+        const int64_t TP = (int64_t)nqt * a.TQ;
+        const int64_t n = (cu_seqlens_q ? Tq / TP + B : B * ((Sq + TP - 1) / TP)) * Hk;
+        return n > 0 ? n : one;
+    };
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return kv4::by_head_dim(D, [&](auto w) {
-        constexpr int W = decltype(w)::value;
-        if (dtype == FC_BF16) prompt_simple_kernel<__nv_bfloat16, W><<<(unsigned)blocks, 256, 0, st>>>(a);
-        else prompt_simple_kernel<__half, W><<<(unsigned)blocks, 256, 0, st>>>(a);
-        return check_launch("prompt_attn");
-    });
+    auto go = [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        return f16 ? launch<DP, true>(mq, mk, mv, a, items(Cfg<DP>::NQ), st) : launch<DP, false>(mq, mk, mv, a, items(Cfg<DP>::NQ), st);
+    };
+    if (D == 64) return go(std::integral_constant<int, 64>());
+    if (D <= 128) return go(std::integral_constant<int, 128>());
+    if (D == 192) return go(std::integral_constant<int, 192>());
+    return go(std::integral_constant<int, 256>());
 }

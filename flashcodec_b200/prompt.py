@@ -16,11 +16,15 @@ from torch.autograd import forward_ad
 from . import _kernels as K
 
 
-def _rows(name, t):
+def _walkable(name, t):
+    """t, or a copy where its rows are not on 16-byte boundaries or not apart from one another:
+    the kernel walks them by tensor maps."""
     if t.stride(-1) != 1:
         raise ValueError(f"{name}: the head dim must have unit stride")
-    if t.shape[-2] == 0:
-        raise ValueError(f"{name} has no heads")
+    step = 16 // t.element_size()
+    if t.data_ptr() % 16 or any(n > 1 and (st <= 0 or st % step) for n, st in zip(t.shape[:-1], t.stride()[:-1])):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
 
 
 def prompt_attention(q, k, v, cu_seqlens=None, cu_seqlens_k=None, *, causal=True, scale=None, out=None,
@@ -61,7 +65,7 @@ def prompt_attention(q, k, v, cu_seqlens=None, cu_seqlens_k=None, *, causal=True
     if q.dim() != (3 if packed else 4):
         raise ValueError("q must be (T, heads, D) with cu_seqlens or (B, S, heads, D) without "
                          f"(got {tuple(q.shape)})")
-    if k.dim() != q.dim() or k.shape != v.shape or k.shape[-1] != q.shape[-1] \
+    if k.dim() != q.dim() or k.shape != v.shape or k.shape[-1] != q.shape[-1] or 0 in (q.shape[-2], k.shape[-2]) \
             or (not packed and k.shape[0] != q.shape[0]):
         raise ValueError(f"k and v must be alike and go with q (got {tuple(k.shape)}, {tuple(v.shape)} "
                          f"and {tuple(q.shape)})")
@@ -80,8 +84,9 @@ def prompt_attention(q, k, v, cu_seqlens=None, cu_seqlens_k=None, *, causal=True
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("out must have the shape and dtype of q")
-    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
-        _rows(name, t)
+    if out.stride(-1) != 1:
+        raise ValueError("out: the head dim must have unit stride")
+    q, k, v = _walkable("q", q), _walkable("k", k), _walkable("v", v)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
     K.prompt_attn(q, k, v, cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, causal,
                   q.shape[-1] ** -0.5 if scale is None else float(scale), out, lse)

@@ -310,29 +310,44 @@ struct Block {
         return __all_sync(0xffffffffu, wait(bar, parity));
     }
 
-    // Stage position, from an item's first one on, of V tile j.  Order: K0 .. K(LA - 1), then
-    // V(j), K(j + LA) for every j.
-    __device__ __forceinline__ static int64_t v_pos(int j, int tiles) {
-        return NU * ((int64_t)min(LA, tiles) + j + min(j, max(tiles - LA, 0)));
+    // Item `it`, in the ring of items until its readers are done with it; null: no more work, or given up.
+    template <bool WARP>
+    __device__ __forceinline__ const Item *next(int it) const {
+        const int slot = it % kItems;
+        if (!(WARP ? wait_warp(item_full + slot, (it / kItems) & 1) : wait(item_full + slot, (it / kItems) & 1))) return nullptr;
+        return items[slot].valid ? items + slot : nullptr;
+    }
+    template <bool WARP>
+    __device__ __forceinline__ void done(int it) const {
+        if constexpr (WARP) __syncwarp();
+        if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(item_empty + it % kItems);
     }
 
-    // Reads item `it` out of the ring of items: a warp, or one thread.
-    template <bool WARP>
-    __device__ __forceinline__ bool next(int it, Item &x) const {
-        const int slot = it % kItems;
-        if (!(WARP ? wait_warp(item_full + slot, (it / kItems) & 1) : wait(item_full + slot, (it / kItems) & 1))) return false;
-        x = items[slot];
-        if constexpr (WARP) __syncwarp();
-        if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(item_empty + slot);
-        return x.valid;
-    }
+    // A place in the ring: its stage and the parity of its use.
+    struct Place {
+        int st = 0;
+        unsigned phase = 0;
+        __device__ __forceinline__ void next() {
+            if (++st == NST) {
+                st = 0;
+                phase ^= 1;
+            }
+        }
+        __device__ __forceinline__ void skip(int n) {
+            for (int i = 0; i < n; i++) next();
+        }
+    };
 
     // ---------------------------------------------------------------- TMA warp
     __device__ __forceinline__ void load(const CUtensorMap *mq, const CUtensorMap *mk, const CUtensorMap *mv) {
-        int64_t pos = 0;
+        Place at;
+        bool round = false;  // the ring has been filled once
         unsigned q_uses[2] = {0, 0};
-        Item x;
-        for (int it = 0; next<false>(it, x); it++) {
+        const uint32_t ring_a = smem_addr(ring), q_a = smem_addr(q_s);
+        const Item *item;
+        for (int it = 0; (item = next<false>(it)); it++) {
+            const Item x = *item;
+            done<false>(it);
             if (!x.tiles) continue;
             const int bb = a.cu_q ? 0 : x.b;
             auto queries = [&](int s) {
@@ -342,19 +357,20 @@ struct Block {
                 mbar_expect_tx(q_full + s, a.TQ * a.G * 128 * (DP / 64));
 #pragma unroll
                 for (int c = 0; c < DP / 64; c++)
-                    tma_load_5d(smem_addr(q_s) + s * C::QB + c * kBox, mq, 64 * c, 0, x.h, x.s.q0 + x.t + s * a.TQ, bb, q_full + s);
+                    tma_load_5d(q_a + s * C::QB + c * kBox, mq, 64 * c, 0, x.h, x.s.q0 + x.t + s * a.TQ, bb, q_full + s);
                 return true;
             };
             // (a tile that is looked through first arrives there instead)
             auto tile = [&](const CUtensorMap *m, int j, uint64_t *full) {
 #pragma unroll
-                for (int u = 0; u < NU; u++, pos++) {
-                    const int st = (int)(pos % NST);
-                    if (pos >= NST && !wait(kv_empty + st, (pos / NST - 1) & 1)) return false;
-                    mbar_expect_tx(full + st, C::STAGE);
+                for (int u = 0; u < NU; u++) {
+                    if (round && !wait(kv_empty + at.st, at.phase ^ 1)) return false;
+                    mbar_expect_tx(full + at.st, C::STAGE);
 #pragma unroll
                     for (int c = 0; c < UC / 64; c++)
-                        tma_load_4d(smem_addr(ring) + st * C::STAGE + c * kBox, m, u * UC + 64 * c, x.h, x.s.k0 + j * kTile, bb, full + st);
+                        tma_load_4d(ring_a + at.st * C::STAGE + c * kBox, m, u * UC + 64 * c, x.h, x.s.k0 + j * kTile, bb, full + at.st);
+                    at.next();
+                    round = round || at.st == 0;
                 }
                 return true;
             };
@@ -371,35 +387,38 @@ struct Block {
 
     // ---------------------------------------------------------------- MMA warp
     __device__ __forceinline__ void multiply() {
-        int64_t pos = 0;
+        Place at;
         unsigned q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
         constexpr uint32_t id_s = idesc(kTile, F16, 0), id_o = idesc(UC, F16, 1);
-        Item x;
-        for (int it = 0; next<false>(it, x); it++) {
+        const uint64_t ring_d = sw128_desc(smem_addr(ring)), q_d = sw128_desc(smem_addr(q_s));
+        const Item *item;
+        for (int it = 0; (item = next<false>(it)); it++) {
+            const Item x = *item;
+            done<false>(it);
             if (!x.tiles) continue;
-            auto full = [&](int64_t p) {
+            auto full = [&](Place p) {
 #pragma unroll
-                for (int u = 0; u < NU; u++)
-                    if (!wait(kv_full + (p + u) % NST, ((p + u) / NST) & 1)) return false;
+                for (int u = 0; u < NU; u++, p.next())
+                    if (!wait(kv_full + p.st, p.phase)) return false;
                 return true;
             };
-            auto release = [&](int64_t p) {
+            auto release = [&](Place p) {
 #pragma unroll
-                for (int u = 0; u < NU; u++) mma_commit(kv_empty + (p + u) % NST);
+                for (int u = 0; u < NU; u++, p.next()) mma_commit(kv_empty + p.st);
             };
-            auto scores = [&](int s, int j, int64_t p) {  // K tile j is at p
+            auto scores = [&](int s, int j, Place p) {  // K tile j is at p
                 if (j >= x.nt[s]) return true;
                 if (j == 0 && !wait(q_full + s, q_uses[s]++ & 1)) return false;
                 tc_fence_after();
                 const int slot = NQ == 2 ? s : j & 1;
 #pragma unroll
-                for (int u = 0; u < NU; u++) {
-                    const uint32_t kt = smem_addr(ring) + (uint32_t)((p + u) % NST) * C::STAGE;
-                    const uint32_t qt = smem_addr(q_s) + s * C::QB + u * (UC / 64) * kBox;
+                for (int u = 0; u < NU; u++, p.next()) {
+                    const uint64_t kd = ring_d + p.st * (C::STAGE >> 4), qd = q_d + ((s * C::QB + u * (UC / 64) * kBox) >> 4);
 #pragma unroll
                     for (int k = 0; k < UC / 16; k++) {
-                        const uint32_t at = (k >> 2) * kBox + (k & 3) * 32;
-                        mma_ss(tmem + slot * kTile, sw128_desc(qt + at), sw128_desc(kt + at), id_s, u + k > 0);
+                        constexpr int step = 32 >> 4;
+                        const int off = (k >> 2) * (kBox >> 4) + (k & 3) * step;
+                        mma_ss(tmem + slot * kTile, qd + off, kd + off, id_s, u + k > 0);
                     }
                 }
                 mma_commit(s_full + slot);
@@ -407,16 +426,18 @@ struct Block {
                 return true;
             };
             for (int j = 0; j < min(LA, x.tiles); j++) {
-                if (!full(pos)) return;
+                if (!full(at)) return;
                 for (int s = 0; s < NQ; s++)
-                    if (!scores(s, j, pos)) return;
-                release(pos);
-                pos += NU;
+                    if (!scores(s, j, at)) return;
+                release(at);
+                at.skip(NU);
             }
             for (int j = 0; j < x.tiles; j++) {
-                const int64_t vp = pos, kp = pos + NU;
+                const Place vp = at;
+                at.skip(NU);
+                const Place kp = at;
                 const bool more = j + LA < x.tiles;
-                pos += more ? 2 * NU : NU;
+                if (more) at.skip(NU);
                 if (!full(vp)) return;
 #pragma unroll
                 for (int s = 0; s < NQ; s++) {
@@ -424,12 +445,13 @@ struct Block {
                         const int slot = NQ == 2 ? s : j & 1;
                         if (!wait(p_full + slot, p_uses[slot]++ & 1)) return;
                         tc_fence_after();
+                        Place p = vp;
 #pragma unroll
-                        for (int u = 0; u < NU; u++) {
-                            const uint32_t vt = smem_addr(ring) + (uint32_t)((vp + u) % NST) * C::STAGE;
+                        for (int u = 0; u < NU; u++, p.next()) {
+                            const uint64_t vd = ring_d + p.st * (C::STAGE >> 4);
 #pragma unroll
                             for (int k = 0; k < kTile / 16; k++)
-                                mma_ts(tmem + C::O_COL + s * DP + u * UC, tmem + slot * kTile + k * 8, sw128_desc(vt + k * 2048),
+                                mma_ts(tmem + C::O_COL + s * DP + u * UC, tmem + slot * kTile + k * 8, vd + k * (2048 >> 4),
                                        id_o, j > 0 || k > 0);
                         }
                         mma_commit(o_done + s);
@@ -451,14 +473,13 @@ struct Block {
         const uint32_t lanes = (uint32_t)(row & ~31) << 16;  // of this warp
         const int tok = row / a.G, head = row - tok * a.G;
         unsigned s_uses[2] = {0, 0}, o_count = 0;
-        Item x;
-        for (int it = 0; next<true>(it, x); it++) {
-            const int i = x.t + s * a.TQ + tok;
-            const bool on = tok < a.TQ && i < x.s.nq;
+        const Item *item;
+        for (int it = 0; (item = next<true>(it)); it++) {
             // (rows of no query need no mask: their results go nowhere)
-            const int vis = on ? visible(a, x.s, i) : 0x7fffffff;
+            const int i = item->t + s * a.TQ + tok;
+            const int vis = tok < a.TQ && i < item->s.nq ? visible(a, item->s, i) : 0x7fffffff;
             float ref = -INFINITY, l = 0.f;  // reference, in scores; sum
-            const int nt = NQ == 2 && s ? x.nt[1] : x.nt[0];
+            const int nt = item->nt[s];
             for (int j = 0; j < nt; j++) {
                 const int slot = NQ == 2 ? s : j & 1;
                 const uint32_t at = tmem + lanes + slot * kTile;
@@ -484,43 +505,46 @@ struct Block {
                     for (int k = 0; k < 4; k++) t[k] = fmaxf(fmaxf(t[k], z[c + k]), c + 4 + k < kTile ? z[c + 4 + k] : t[k]);
                 const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
                 // the reference follows only a maximum that is 2^8 above it: weights stay below 2^8
-                if (__any_sync(0xffffffffu, (top - ref) * a.scale > 8.f)) {
+                const bool move = __any_sync(0xffffffffu, (top - ref) * a.scale > 8.f);
+                float f = 1.f;
+                if (move) {
                     const float m = fmaxf(ref, top);
-                    const float f = ref == -INFINITY ? 0.f : exp2_fast((ref - m) * a.scale);
+                    f = ref == -INFINITY ? 0.f : exp2_fast((ref - m) * a.scale);
                     ref = m;
                     l *= f;
-                    if (j > 0) {
-                        if (!wait_warp(o_done + s, (o_count - 1) & 1)) return;
-                        tc_fence_after();
-#pragma unroll
-                        for (int c = 0; c < DP; c += 32) {
-                            float o[32];
-                            uint32_t w[32];
-                            const uint32_t oat = tmem + lanes + C::O_COL + s * DP + c;
-                            tmem_ld32(oat, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int k = 0; k < 32; k++) w[k] = __float_as_uint(o[k] * f);
-                            tmem_st32(oat, w);
-                        }
-                    }
                 }
                 const float off = ref == -INFINITY ? 0.f : -ref * a.scale;
-                float sum[4] = {};
+                const float2 scale2 = make_float2(a.scale, a.scale), off2 = make_float2(off, off);
+                float2 sum[2] = {};
 #pragma unroll
                 for (int c = 0; c < kTile; c += 32) {
                     uint32_t w[16];
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
-                        const float u = exp2_fast(fmaf(z[c + 2 * k], a.scale, off));
-                        const float v = exp2_fast(fmaf(z[c + 2 * k + 1], a.scale, off));
-                        sum[2 * k & 3] += u;
-                        sum[2 * k + 1 & 3] += v;
-                        w[k] = pack2<F16>(u, v);
+                        float2 u = __ffma2_rn(make_float2(z[c + 2 * k], z[c + 2 * k + 1]), scale2, off2);
+                        u.x = exp2_fast(u.x);
+                        u.y = exp2_fast(u.y);
+                        sum[k & 1] = __fadd2_rn(sum[k & 1], u);
+                        w[k] = pack2<F16>(u.x, u.y);
                     }
                     tmem_st16(at + c / 2, w);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (move && j > 0) {
+                    // (after the weights: their registers are free)
+                    if (!wait_warp(o_done + s, (o_count - 1) & 1)) return;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < DP; c += 32) {
+                        float o[32];
+                        const uint32_t oat = tmem + lanes + C::O_COL + s * DP + c;
+                        tmem_ld32(oat, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; k++) o[k] *= f;
+                        tmem_st32(oat, reinterpret_cast<const uint32_t *>(o));
+                    }
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -531,14 +555,17 @@ struct Block {
             if (NQ == 1 && nt > 1 && !wait_warp(o_done + s, o_count & 1)) return;
             if (nt && !wait_warp(o_done + s, (o_count - 1) & 1)) return;
             tc_fence_after();
-            if (!write(x, it, s, i, head, on, vis, nt, ref, l, lanes)) return;
+            write(*item, it, s, tok, head, nt, ref, l, lanes);
+            done<true>(it);
         }
     }
 
     // Outputs of one row.
-    __device__ __forceinline__ bool write(const Item &x, int it, int s, int i, int head, bool on, int vis, int nt, float ref,
-                                          float l, uint32_t lanes) const {
+    __device__ __forceinline__ void write(const Item &x, int it, int s, int tok, int head, int nt, float ref, float l,
+                                          uint32_t lanes) const {
         using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
+        const int i = x.t + s * a.TQ + tok;
+        const bool on = tok < a.TQ && i < x.s.nq;
         const int h = x.h * a.G + head;
         const int64_t row = a.cu_q ? x.s.q0 + i : i;
         T *out = static_cast<T *>(a.out) + (a.cu_q ? 0 : x.b * a.o_sb) + row * a.o_ss + h * a.o_sh;
@@ -554,7 +581,7 @@ struct Block {
             }
             if (fix && on) {  // values of the masked tiles that are no numbers
                 const T *v = static_cast<const T *>(a.v) + (a.cu_q ? 0 : x.b * a.v_sb) + x.h * a.v_sh + c;
-                for (int j = x.first * kTile; j < vis; j++)
+                for (int j = x.first * kTile, n = visible(a, x.s, i); j < n; j++)
 #pragma unroll
                     for (int k = 0; k < 32; k++) {
                         const float y = Elem<T>::to_f32(v[(int64_t)(x.s.k0 + j) * a.v_ss + k]);
@@ -585,14 +612,13 @@ struct Block {
             const int64_t at = ((a.cu_q ? row : (int64_t)x.b * a.Sq + i)) * a.Hq + h;
             a.lse[at] = l == 0.f ? -INFINITY : fmaf(ref, a.scale, log2f(l)) * 0.693147180559945309f;
         }
-        return true;
     }
 
     // ------------------------------------------------------------- helper warps
     // Warp 0 of the two also finds the items, one ahead of the values that it looks through.
     __device__ __forceinline__ void help(int w) {
         const int lane = threadIdx.x & 31;
-        int64_t pos = 0;
+        int64_t pos = 0;  // where the item's tiles begin
         const int TP = NQ * a.TQ;
         int most = 0;
         if (w == 0) {
@@ -623,14 +649,16 @@ struct Block {
         };
         if (w == 0 && !publish(0)) return;
         unsigned seen = 0;  // by stage: the parity of the tiles looked through
-        Item x;
-        for (int it = 0; next<true>(it, x); it++) {
+        const Item *item;
+        for (int it = 0; (item = next<true>(it)); it++) {
+            const Item x = *item;
+            done<true>(it);
             if (w == 0 && !publish(it + 1)) return;
             bool any = false;
             for (int j = x.first; j < x.tiles; j++)
                 for (int u = 0; u < NU; u++) {
-                    const int64_t p = pos + v_pos(j, x.tiles) + u;
-                    const int st = (int)(p % NST);
+                    // order: K0 .. K(LA - 1), then V(j), K(j + LA) for every j
+                    const int st = (int)((pos + NU * (min(LA, x.tiles) + j + min(j, max(x.tiles - LA, 0))) + u) % NST);
                     // (A barrier for these tiles alone: their next use waits for this one, so no phase of
                     // it can be missed, and none passed by a warp that is ahead.)
                     const unsigned parity = seen >> st & 1;
@@ -734,12 +762,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     __syncthreads();
     tc_fence_after();
     k.tmem = tmem_s;
-    // two streams: 384 threads of 168 registers, shared out as 256 of 200 and 128 of 104
     if (warp < SW) {
-        if constexpr (C::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         k.softmax(warp >> 2);
     } else if (warp == SW) {
-        if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (lane == 0) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
@@ -747,10 +772,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             k.load(&mq, &mk, &mv);
         }
     } else if (warp == SW + 1) {
-        if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (lane == 0) k.multiply();
     } else {
-        if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         k.help(warp - SW - 2);
     }
     __syncwarp();
@@ -810,13 +833,6 @@ int launch(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, 
     if (!ready[dev]) {
         if (cudaFuncSetAttribute(prompt_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
             set_error("prompt_attn: the kernel does not fit this device");
-            return FC_ECUDA;
-        }
-        // the warps that ask for more registers wait for what the others give back: never launch
-        // a kernel that was built with too few to share out
-        cudaFuncAttributes attr;
-        if (cudaFuncGetAttributes(&attr, prompt_kernel<DP, F16>) != cudaSuccess || (C::NQ == 2 && attr.numRegs != 168)) {
-            set_error("prompt_attn: the kernel was built with another number of registers");
             return FC_ECUDA;
         }
         ready[dev] = true;

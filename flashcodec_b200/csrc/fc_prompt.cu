@@ -78,6 +78,7 @@ struct Args {
 constexpr int kTile = 128;          // rows of a query tile, keys of a tile
 constexpr int kBox = kTile * 128;   // bytes of 128 rows of 64 channels
 constexpr int kItems = 3;           // items known ahead
+constexpr int kPolyStep = 4;        // every kPolyStep-th pair of weights is a polynomial
 
 template <int DP> struct Cfg {
     static constexpr int NQ = DP <= 128 ? 2 : 1;         // streams
@@ -119,26 +120,37 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 // M = 128, N = n, fp32 sums; bf16 (or fp16) operands, B K-major or MN-major.
-__host__ __device__ constexpr uint32_t idesc(int n, bool f16, int b_mn) {
+__host__ __device__ constexpr uint32_t idesc(int n, bool f16, int b_mn) {  // (bit 13: -A)
     return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
            ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+// Issued by the one lane whose `lead` is not 0, in code that the whole warp runs: operands stay in
+// uniform registers (from a branch of one lane every one of them had to be moved there first, and
+// issuing took as long as the products: 3100 cycles for the 32 of two tiles).
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p;
+}
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(id), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(acc), "r"(lead)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(id), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(acc), "r"(lead)
         : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+__device__ __forceinline__ void mma_commit(uint32_t lead, uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)), "r"(lead)
+        : "memory");
 }
 
 #define FC_R16(v, o) "=f"(v[o]), "=f"(v[o + 1]), "=f"(v[o + 2]), "=f"(v[o + 3]), "=f"(v[o + 4]), "=f"(v[o + 5]), \
@@ -153,6 +165,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, float *v) {
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
         : FC_R16(v, 0), FC_R16(v, 16) : "r"(at));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t at, float *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : FC_R16(v, 0) : "r"(at));
 }
 __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t *v) {
     asm volatile(
@@ -173,6 +190,51 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// 2^x without the special function units, whose 16 lanes would otherwise take as long as both
+// products of a tile: 2^round(x) put into the exponent, 2^f on [-1/2, 1/2] as a polynomial
+// (least largest relative error, by reweighted least squares: 2^-13.7 of degree 3 for bf16
+// weights, 2^-18.5 of degree 4 for fp16 ones).  From -125 down the result is no weight any more;
+// a NaN stays one.  x is at most 8 or no number.
+template <bool F16>
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    auto low = [](float v) {
+        float y;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(v), "f"(-125.f));
+        return y;
+    };
+    x = make_float2(low(x.x), low(x.y));
+    const float2 magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f);
+    const float2 t = __fadd2_rn(x, magic), n = __fadd2_rn(t, minus);
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    auto c2 = [](float v) { return make_float2(v, v); };
+    float2 p;
+    if constexpr (F16) {
+        p = __ffma2_rn(f, c2(0.009570101276040077f), c2(0.05591785907745361f));
+        p = __ffma2_rn(f, p, c2(0.240247443318367f));
+        p = __ffma2_rn(f, p, c2(0.6931217908859253f));
+        p = __ffma2_rn(f, p, c2(0.9999992847442627f));
+    } else {
+        p = __ffma2_rn(f, c2(0.0551716685295105f), c2(0.2426111251115799f));
+        p = __ffma2_rn(f, p, c2(0.6932609677314758f));
+        p = __ffma2_rn(f, p, c2(0.9999280571937561f));
+    }
+    p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
+    p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
+    return p;
+}
+
+// A pair of 16-bit floats times f, a power of two.
+template <bool F16>
+__device__ __forceinline__ uint32_t scale2(uint32_t w, float f) {
+    if constexpr (F16) {
+        const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&w), __float2half2_rn(f));
+        return *reinterpret_cast<const uint32_t *>(&y);
+    } else {
+        const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&w), __float2bfloat162_rn(f));
+        return *reinterpret_cast<const uint32_t *>(&y);
+    }
 }
 
 template <bool F16>
@@ -388,27 +450,30 @@ struct Block {
     // ---------------------------------------------------------------- MMA warp
     __device__ __forceinline__ void multiply() {
         Place at;
+        const uint32_t lead = elect();
         unsigned q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
-        constexpr uint32_t id_s = idesc(kTile, F16, 0), id_o = idesc(UC, F16, 1);
+        constexpr uint32_t id_o = idesc(UC, F16, 1);
+        const uint32_t id_s = idesc(kTile, F16, 0) | (uint32_t)a.negative << 13;
         const uint64_t ring_d = sw128_desc(smem_addr(ring)), q_d = sw128_desc(smem_addr(q_s));
         const Item *item;
-        for (int it = 0; (item = next<false>(it)); it++) {
-            const Item x = *item;
-            done<false>(it);
-            if (!x.tiles) continue;
+        for (int it = 0; (item = next<true>(it)); it++) {
+            auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+            const int tiles = uniform(item->tiles), nt[2] = {uniform(item->nt[0]), uniform(item->nt[1])};
+            done<true>(it);
+            if (!tiles) continue;
             auto full = [&](Place p) {
 #pragma unroll
                 for (int u = 0; u < NU; u++, p.next())
-                    if (!wait(kv_full + p.st, p.phase)) return false;
+                    if (!wait_warp(kv_full + p.st, p.phase)) return false;
                 return true;
             };
             auto release = [&](Place p) {
 #pragma unroll
-                for (int u = 0; u < NU; u++, p.next()) mma_commit(kv_empty + p.st);
+                for (int u = 0; u < NU; u++, p.next()) mma_commit(lead, kv_empty + p.st);
             };
             auto scores = [&](int s, int j, Place p) {  // K tile j is at p
-                if (j >= x.nt[s]) return true;
-                if (j == 0 && !wait(q_full + s, q_uses[s]++ & 1)) return false;
+                if (j >= nt[s]) return true;
+                if (j == 0 && !wait_warp(q_full + s, q_uses[s]++ & 1)) return false;
                 tc_fence_after();
                 const int slot = NQ == 2 ? s : j & 1;
 #pragma unroll
@@ -418,32 +483,32 @@ struct Block {
                     for (int k = 0; k < UC / 16; k++) {
                         constexpr int step = 32 >> 4;
                         const int off = (k >> 2) * (kBox >> 4) + (k & 3) * step;
-                        mma_ss(tmem + slot * kTile, qd + off, kd + off, id_s, u + k > 0);
+                        mma_ss(lead, tmem + slot * kTile, qd + off, kd + off, id_s, u + k > 0);
                     }
                 }
-                mma_commit(s_full + slot);
-                if (j == x.nt[s] - 1) mma_commit(q_free + s);
+                mma_commit(lead, s_full + slot);
+                if (j == nt[s] - 1) mma_commit(lead, q_free + s);
                 return true;
             };
-            for (int j = 0; j < min(LA, x.tiles); j++) {
+            for (int j = 0; j < min(LA, tiles); j++) {
                 if (!full(at)) return;
                 for (int s = 0; s < NQ; s++)
                     if (!scores(s, j, at)) return;
                 release(at);
                 at.skip(NU);
             }
-            for (int j = 0; j < x.tiles; j++) {
+            for (int j = 0; j < tiles; j++) {
                 const Place vp = at;
                 at.skip(NU);
                 const Place kp = at;
-                const bool more = j + LA < x.tiles;
+                const bool more = j + LA < tiles;
                 if (more) at.skip(NU);
                 if (!full(vp)) return;
 #pragma unroll
                 for (int s = 0; s < NQ; s++) {
-                    if (j < x.nt[s]) {
+                    if (j < nt[s]) {
                         const int slot = NQ == 2 ? s : j & 1;
-                        if (!wait(p_full + slot, p_uses[slot]++ & 1)) return;
+                        if (!wait_warp(p_full + slot, p_uses[slot]++ & 1)) return;
                         tc_fence_after();
                         Place p = vp;
 #pragma unroll
@@ -451,10 +516,10 @@ struct Block {
                             const uint64_t vd = ring_d + p.st * (C::STAGE >> 4);
 #pragma unroll
                             for (int k = 0; k < kTile / 16; k++)
-                                mma_ts(tmem + C::O_COL + s * DP + u * UC, tmem + slot * kTile + k * 8, vd + k * (2048 >> 4),
+                                mma_ts(lead, tmem + C::O_COL + s * DP + u * UC, tmem + slot * kTile + k * 8, vd + k * (2048 >> 4),
                                        id_o, j > 0 || k > 0);
                         }
-                        mma_commit(o_done + s);
+                        mma_commit(lead, o_done + s);
                     }
                     if (s == NQ - 1) release(vp);
                     if (more) {
@@ -468,6 +533,86 @@ struct Block {
     }
 
     // ------------------------------------------------------------ softmax warps
+    // A row's reference and factors are powers of two: P and O are scaled without rounding.
+    struct Row {
+        float ref, l;  // log2 of the reference (a whole number; -inf: nothing seen), sum of weights
+    };
+
+    // One tile of scores into weights.  Returns what O has to be scaled by, 0 if no row of the warp
+    // moved its reference.  In four steps of 32 keys; while one is exponentiated the next one's
+    // maximum is found and the one after it is on its way from TMEM.
+    template <bool MASK>
+    __device__ __forceinline__ float weights(Row &r, uint32_t at, int lim) const {
+        float z[3][32], moved = 0.f;
+        float2 sum[2] = {};
+        const float2 scale = make_float2(a.scale, a.scale);
+        auto largest = [&](float *v, int c) {
+            if constexpr (MASK) {
+#pragma unroll
+                for (int k = 0; k < 32; k++) v[k] = c * 32 + k < lim ? v[k] : -INFINITY;
+            }
+            float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+            for (int k = 4; k < 28; k += 8)
+#pragma unroll
+                for (int e = 0; e < 4; e++) m[e] = fmaxf(fmaxf(m[e], v[k + e]), v[k + 4 + e]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) m[e] = fmaxf(m[e], v[28 + e]);
+            return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        };
+        tmem_ld32(at, z[0]);
+        tmem_ld32(at + 32, z[1]);
+        tmem_wait_ld();
+        float top = largest(z[0], 0);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            // the reference follows only a maximum that is 2^8 above it: weights stay below 2^8
+            if (__any_sync(0xffffffffu, fmaf(top, a.scale, -r.ref) > 8.f)) {
+                const float m = fmaxf(r.ref, ceilf(top * a.scale));
+                const float d = r.ref - m;  // <= 0, no number where both are infinite
+                const float f = d == 0.f ? 1.f : d > -126.f ? __int_as_float(((int)d + 127) << 23) : 0.f;
+                r.ref = m;
+                r.l *= f;
+                moved = moved == 0.f ? (f == 0.f ? 0x1p-126f : f) : fmaxf(moved * f, 0x1p-126f);
+                sum[0].x *= f; sum[0].y *= f; sum[1].x *= f; sum[1].y *= f;
+                if (c) {  // weights of this tile that are there already
+                    tmem_wait_st();
+#pragma unroll
+                    for (int e = 0; e < 16 * c; e += 16) {
+                        float w[16];
+                        tmem_ld16(at + e, w);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 16; k++) w[k] = __uint_as_float(scale2<F16>(__float_as_uint(w[k]), f));
+                        tmem_st16(at + e, reinterpret_cast<const uint32_t *>(w));
+                    }
+                }
+            }
+            if (c < 2) tmem_ld32(at + 32 * c + 64, z[(c + 2) % 3]);
+            const float off = r.ref == -INFINITY ? 0.f : -r.ref;
+            const float2 off2 = make_float2(off, off);
+            if (c < 3) top = largest(z[(c + 1) % 3], c + 1);
+            float *v = z[c % 3];
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                float2 u = __ffma2_rn(make_float2(v[2 * k], v[2 * k + 1]), scale, off2);
+                if (!MASK && k % kPolyStep == kPolyStep - 1) {
+                    u = exp2_poly<F16>(u);
+                } else {
+                    u.x = exp2_fast(u.x);
+                    u.y = exp2_fast(u.y);
+                }
+                sum[k & 1] = __fadd2_rn(sum[k & 1], u);
+                w[k] = pack2<F16>(u.x, u.y);
+            }
+            tmem_st16(at + 16 * c, w);
+            if (c < 2) tmem_wait_ld();
+        }
+        r.l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        return moved;
+    }
+
     __device__ __forceinline__ void softmax(int s) {
         const int row = threadIdx.x & 127, lane = threadIdx.x & 31;
         const uint32_t lanes = (uint32_t)(row & ~31) << 16;  // of this warp
@@ -478,59 +623,16 @@ struct Block {
             // (rows of no query need no mask: their results go nowhere)
             const int i = item->t + s * a.TQ + tok;
             const int vis = tok < a.TQ && i < item->s.nq ? visible(a, item->s, i) : 0x7fffffff;
-            float ref = -INFINITY, l = 0.f;  // reference, in scores; sum
+            Row r{-INFINITY, 0.f};
             const int nt = item->nt[s];
             for (int j = 0; j < nt; j++) {
                 const int slot = NQ == 2 ? s : j & 1;
                 const uint32_t at = tmem + lanes + slot * kTile;
                 if (!wait_warp(s_full + slot, s_uses[NQ == 2 ? 0 : slot]++ & 1)) return;
                 tc_fence_after();
-                float z[kTile];
-#pragma unroll
-                for (int c = 0; c < kTile; c += 32) tmem_ld32(at + c, z + c);
-                tmem_wait_ld();
-                if (a.negative) {
-#pragma unroll
-                    for (int c = 0; c < kTile; c++) z[c] = -z[c];
-                }
                 const int lim = vis - j * kTile;
-                if (__any_sync(0xffffffffu, lim < kTile)) {
-#pragma unroll
-                    for (int c = 0; c < kTile; c++) z[c] = c < lim ? z[c] : -INFINITY;
-                }
-                float t[4] = {z[0], z[1], z[2], z[3]};
-#pragma unroll
-                for (int c = 4; c < kTile; c += 8)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) t[k] = fmaxf(fmaxf(t[k], z[c + k]), c + 4 + k < kTile ? z[c + 4 + k] : t[k]);
-                const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-                // the reference follows only a maximum that is 2^8 above it: weights stay below 2^8
-                const bool move = __any_sync(0xffffffffu, (top - ref) * a.scale > 8.f);
-                float f = 1.f;
-                if (move) {
-                    const float m = fmaxf(ref, top);
-                    f = ref == -INFINITY ? 0.f : exp2_fast((ref - m) * a.scale);
-                    ref = m;
-                    l *= f;
-                }
-                const float off = ref == -INFINITY ? 0.f : -ref * a.scale;
-                const float2 scale2 = make_float2(a.scale, a.scale), off2 = make_float2(off, off);
-                float2 sum[2] = {};
-#pragma unroll
-                for (int c = 0; c < kTile; c += 32) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        float2 u = __ffma2_rn(make_float2(z[c + 2 * k], z[c + 2 * k + 1]), scale2, off2);
-                        u.x = exp2_fast(u.x);
-                        u.y = exp2_fast(u.y);
-                        sum[k & 1] = __fadd2_rn(sum[k & 1], u);
-                        w[k] = pack2<F16>(u.x, u.y);
-                    }
-                    tmem_st16(at + c / 2, w);
-                }
-                if (move && j > 0) {
-                    // (after the weights: their registers are free)
+                const float f = __any_sync(0xffffffffu, lim < kTile) ? weights<true>(r, at, lim) : weights<false>(r, at, lim);
+                if (j > 0 && __any_sync(0xffffffffu, f != 0.f)) {
                     if (!wait_warp(o_done + s, (o_count - 1) & 1)) return;
                     tc_fence_after();
 #pragma unroll
@@ -544,7 +646,6 @@ struct Block {
                         tmem_st32(oat, reinterpret_cast<const uint32_t *>(o));
                     }
                 }
-                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -555,7 +656,7 @@ struct Block {
             if (NQ == 1 && nt > 1 && !wait_warp(o_done + s, o_count & 1)) return;
             if (nt && !wait_warp(o_done + s, (o_count - 1) & 1)) return;
             tc_fence_after();
-            write(*item, it, s, tok, head, nt, ref, l, lanes);
+            write(*item, it, s, tok, head, nt, r.ref, r.l, lanes);
             done<true>(it);
         }
     }
@@ -610,7 +711,7 @@ struct Block {
         tc_fence_before();
         if (on && a.lse) {
             const int64_t at = ((a.cu_q ? row : (int64_t)x.b * a.Sq + i)) * a.Hq + h;
-            a.lse[at] = l == 0.f ? -INFINITY : fmaf(ref, a.scale, log2f(l)) * 0.693147180559945309f;
+            a.lse[at] = l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.693147180559945309f;
         }
     }
 
@@ -772,7 +873,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             k.load(&mq, &mk, &mv);
         }
     } else if (warp == SW + 1) {
-        if (lane == 0) k.multiply();
+        k.multiply();
     } else {
         k.help(warp - SW - 2);
     }

@@ -88,7 +88,7 @@ template <int DP> struct Cfg {
     static constexpr int STAGE = kTile * UC * 2;
     static constexpr int NST = DP == 64 ? 8 : DP == 192 ? 3 : 5;
     static constexpr int QB = kTile * DP * 2;            // bytes of a query tile
-    static constexpr int SMEM = 1024 + NQ * QB + NST * STAGE;
+    
     static constexpr int THREADS = 128 * NQ + 128;
     static constexpr int O_COL = 256;                    // TMEM: scores at 0 and 128, outputs from here
     static_assert(O_COL + NQ * DP <= 512, "TMEM");
@@ -183,7 +183,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t *v) {
         "r"(at)
         : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for this thread's loads from TMEM.  N registers that they write are named, so that no use of
+// them moves in front of it: to the compiler a load is done where it stands.
+#define FC_U16(v, o) "+f"(v[o]), "+f"(v[o + 1]), "+f"(v[o + 2]), "+f"(v[o + 3]), "+f"(v[o + 4]), "+f"(v[o + 5]),   \
+    "+f"(v[o + 6]), "+f"(v[o + 7]), "+f"(v[o + 8]), "+f"(v[o + 9]), "+f"(v[o + 10]), "+f"(v[o + 11]),           \
+    "+f"(v[o + 12]), "+f"(v[o + 13]), "+f"(v[o + 14]), "+f"(v[o + 15])
+template <int N>
+__device__ __forceinline__ void tmem_landed(float *v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i += 16) asm volatile("" : FC_U16(v, i));
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -223,18 +233,6 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
     p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
     p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
     return p;
-}
-
-// A pair of 16-bit floats times f, a power of two.
-template <bool F16>
-__device__ __forceinline__ uint32_t scale2(uint32_t w, float f) {
-    if constexpr (F16) {
-        const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&w), __float2half2_rn(f));
-        return *reinterpret_cast<const uint32_t *>(&y);
-    } else {
-        const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&w), __float2bfloat162_rn(f));
-        return *reinterpret_cast<const uint32_t *>(&y);
-    }
 }
 
 template <bool F16>
@@ -337,20 +335,34 @@ __device__ __forceinline__ bool find_item(const Args &a, int64_t rank, int TP, i
     return false;  // cu_seqlens changed under way
 }
 
+// What of shared memory is not tiles.
+template <int DP> struct Small {
+    using C = Cfg<DP>;
+    // tile copies landed, stages free; tiles to be looked through landed, half of one is done
+    uint64_t kv_full[C::NST], kv_empty[C::NST], v_raw[C::NST], v_half[C::NST];
+    uint64_t q_full[2], q_free[2];  // by stream
+    uint64_t s_full[2], p_full[4];  // by score buffer: scores; either half of the weights are there
+    uint64_t o_done[2];             // by stream: a product P V is done
+    uint64_t item_full[kItems], item_empty[kItems];
+    Item items[kItems];
+    int abort_s, bad[2];            // bad: by item, its number + 1 if a value was no number
+    uint32_t tmem;
+};
+
 template <int DP, bool F16>
 struct Block {
     using C = Cfg<DP>;
     static constexpr int NQ = C::NQ, LA = C::LA, NU = C::NU, UC = C::UC, NST = C::NST;
 
     const Args &a;
-    unsigned char *q_s, *ring;
-    uint64_t *kv_full, *kv_empty, *v_raw, *v_half, *q_full, *q_free, *s_full, *p_full, *o_done, *item_full, *item_empty;
-    Item *items;
-    volatile int *abort_s;
-    int *bad;  // by item: its number + 1 if a value was no number
+    const uint32_t q_a, ring_a;  // shared memory: queries, ring
+    unsigned char *ring;
+    Small<DP> *small;
     uint32_t tmem;
 
-    __device__ __forceinline__ explicit Block(const Args &args) : a(args) {}
+    __device__ __forceinline__ Block(const Args &args, unsigned char *smem)
+        : a(args), q_a(smem_addr(smem)), ring_a(smem_addr(smem) + NQ * C::QB), ring(smem + NQ * C::QB),
+          small(reinterpret_cast<Small<DP> *>(smem + NQ * C::QB + NST * C::STAGE)) {}
 
     // Every wait is bounded; one that gives up records the launch and ends the block's work.
     __device__ __forceinline__ bool wait(uint64_t *bar, unsigned parity) const {
@@ -358,10 +370,10 @@ struct Block {
         const uint64_t t0 = global_ns();
         for (;;) {
             if (mbar_try_wait_sleep(bar, parity, 20000)) return true;
-            if (*abort_s) return false;
+            if (*static_cast<volatile int *>(&small->abort_s)) return false;
             if (global_ns() - t0 > kWaitNs) {
                 atomicMax(a.status, a.epoch);
-                *abort_s = 1;
+                *static_cast<volatile int *>(&small->abort_s) = 1;
                 return false;
             }
         }
@@ -376,13 +388,13 @@ struct Block {
     template <bool WARP>
     __device__ __forceinline__ const Item *next(int it) const {
         const int slot = it % kItems;
-        if (!(WARP ? wait_warp(item_full + slot, (it / kItems) & 1) : wait(item_full + slot, (it / kItems) & 1))) return nullptr;
-        return items[slot].valid ? items + slot : nullptr;
+        if (!(WARP ? wait_warp(small->item_full + slot, (it / kItems) & 1) : wait(small->item_full + slot, (it / kItems) & 1))) return nullptr;
+        return small->items[slot].valid ? small->items + slot : nullptr;
     }
     template <bool WARP>
     __device__ __forceinline__ void done(int it) const {
         if constexpr (WARP) __syncwarp();
-        if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(item_empty + it % kItems);
+        if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(small->item_empty + it % kItems);
     }
 
     // A place in the ring: its stage and the parity of its use.
@@ -405,7 +417,6 @@ struct Block {
         Place at;
         bool round = false;  // the ring has been filled once
         unsigned q_uses[2] = {0, 0};
-        const uint32_t ring_a = smem_addr(ring), q_a = smem_addr(q_s);
         const Item *item;
         for (int it = 0; (item = next<false>(it)); it++) {
             const Item x = *item;
@@ -414,19 +425,19 @@ struct Block {
             const int bb = a.cu_q ? 0 : x.b;
             auto queries = [&](int s) {
                 if (!x.nt[s]) return true;
-                if (q_uses[s] && !wait(q_free + s, (q_uses[s] - 1) & 1)) return false;
+                if (q_uses[s] && !wait(small->q_free + s, (q_uses[s] - 1) & 1)) return false;
                 q_uses[s]++;
-                mbar_expect_tx(q_full + s, a.TQ * a.G * 128 * (DP / 64));
+                mbar_expect_tx(small->q_full + s, a.TQ * a.G * 128 * (DP / 64));
 #pragma unroll
                 for (int c = 0; c < DP / 64; c++)
-                    tma_load_5d(q_a + s * C::QB + c * kBox, mq, 64 * c, 0, x.h, x.s.q0 + x.t + s * a.TQ, bb, q_full + s);
+                    tma_load_5d(q_a + s * C::QB + c * kBox, mq, 64 * c, 0, x.h, x.s.q0 + x.t + s * a.TQ, bb, small->q_full + s);
                 return true;
             };
             // (a tile that is looked through first arrives there instead)
             auto tile = [&](const CUtensorMap *m, int j, uint64_t *full) {
 #pragma unroll
                 for (int u = 0; u < NU; u++) {
-                    if (round && !wait(kv_empty + at.st, at.phase ^ 1)) return false;
+                    if (round && !wait(small->kv_empty + at.st, at.phase ^ 1)) return false;
                     mbar_expect_tx(full + at.st, C::STAGE);
 #pragma unroll
                     for (int c = 0; c < UC / 64; c++)
@@ -436,13 +447,13 @@ struct Block {
                 }
                 return true;
             };
-            if (!queries(0) || !tile(mk, 0, kv_full)) return;
+            if (!queries(0) || !tile(mk, 0, small->kv_full)) return;
             if (NQ == 2 && !queries(1)) return;
             for (int j = 1; j < min(LA, x.tiles); j++)
-                if (!tile(mk, j, kv_full)) return;
+                if (!tile(mk, j, small->kv_full)) return;
             for (int j = 0; j < x.tiles; j++) {
-                if (!tile(mv, j, j >= x.first ? v_raw : kv_full)) return;
-                if (j + LA < x.tiles && !tile(mk, j + LA, kv_full)) return;
+                if (!tile(mv, j, j >= x.first ? small->v_raw : small->kv_full)) return;
+                if (j + LA < x.tiles && !tile(mk, j + LA, small->kv_full)) return;
             }
         }
     }
@@ -454,7 +465,7 @@ struct Block {
         unsigned q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
         constexpr uint32_t id_o = idesc(UC, F16, 1);
         const uint32_t id_s = idesc(kTile, F16, 0) | (uint32_t)a.negative << 13;
-        const uint64_t ring_d = sw128_desc(smem_addr(ring)), q_d = sw128_desc(smem_addr(q_s));
+        const uint64_t ring_d = sw128_desc(ring_a), q_d = sw128_desc(q_a);
         const Item *item;
         for (int it = 0; (item = next<true>(it)); it++) {
             auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
@@ -464,16 +475,16 @@ struct Block {
             auto full = [&](Place p) {
 #pragma unroll
                 for (int u = 0; u < NU; u++, p.next())
-                    if (!wait_warp(kv_full + p.st, p.phase)) return false;
+                    if (!wait_warp(small->kv_full + p.st, p.phase)) return false;
                 return true;
             };
             auto release = [&](Place p) {
 #pragma unroll
-                for (int u = 0; u < NU; u++, p.next()) mma_commit(lead, kv_empty + p.st);
+                for (int u = 0; u < NU; u++, p.next()) mma_commit(lead, small->kv_empty + p.st);
             };
             auto scores = [&](int s, int j, Place p) {  // K tile j is at p
                 if (j >= nt[s]) return true;
-                if (j == 0 && !wait_warp(q_full + s, q_uses[s]++ & 1)) return false;
+                if (j == 0 && !wait_warp(small->q_full + s, q_uses[s]++ & 1)) return false;
                 tc_fence_after();
                 const int slot = NQ == 2 ? s : j & 1;
 #pragma unroll
@@ -486,8 +497,8 @@ struct Block {
                         mma_ss(lead, tmem + slot * kTile, qd + off, kd + off, id_s, u + k > 0);
                     }
                 }
-                mma_commit(lead, s_full + slot);
-                if (j == nt[s] - 1) mma_commit(lead, q_free + s);
+                mma_commit(lead, small->s_full + slot);
+                if (j == nt[s] - 1) mma_commit(lead, small->q_free + s);
                 return true;
             };
             for (int j = 0; j < min(LA, tiles); j++) {
@@ -508,18 +519,22 @@ struct Block {
                 for (int s = 0; s < NQ; s++) {
                     if (j < nt[s]) {
                         const int slot = NQ == 2 ? s : j & 1;
-                        if (!wait_warp(p_full + slot, p_uses[slot]++ & 1)) return;
-                        tc_fence_after();
-                        Place p = vp;
 #pragma unroll
-                        for (int u = 0; u < NU; u++, p.next()) {
-                            const uint64_t vd = ring_d + p.st * (C::STAGE >> 4);
+                        for (int half = 0; half < 2; half++) {
+                            if (!wait_warp(small->p_full + 2 * slot + half, p_uses[slot] & 1)) return;
+                            tc_fence_after();
+                            Place p = vp;
 #pragma unroll
-                            for (int k = 0; k < kTile / 16; k++)
-                                mma_ts(lead, tmem + C::O_COL + s * DP + u * UC, tmem + slot * kTile + k * 8, vd + k * (2048 >> 4),
-                                       id_o, j > 0 || k > 0);
+                            for (int u = 0; u < NU; u++, p.next()) {
+                                const uint64_t vd = ring_d + p.st * (C::STAGE >> 4);
+#pragma unroll
+                                for (int k = 4 * half; k < 4 * half + 4; k++)
+                                    mma_ts(lead, tmem + C::O_COL + s * DP + u * UC, tmem + slot * kTile + k * 8, vd + k * (2048 >> 4),
+                                           id_o, j > 0 || k > 0);
+                            }
                         }
-                        mma_commit(lead, o_done + s);
+                        p_uses[slot]++;
+                        mma_commit(lead, small->o_done + s);
                     }
                     if (s == NQ - 1) release(vp);
                     if (more) {
@@ -533,88 +548,97 @@ struct Block {
     }
 
     // ------------------------------------------------------------ softmax warps
-    // A row's reference and factors are powers of two: P and O are scaled without rounding.
+    // A thread has a row.  Its reference and the factors are powers of two: O is scaled without rounding.
     struct Row {
         float ref, l;  // log2 of the reference (a whole number; -inf: nothing seen), sum of weights
     };
 
-    // One tile of scores into weights.  Returns what O has to be scaled by, 0 if no row of the warp
-    // moved its reference.  In four steps of 32 keys; while one is exponentiated the next one's
-    // maximum is found and the one after it is on its way from TMEM.
-    template <bool MASK>
-    __device__ __forceinline__ float weights(Row &r, uint32_t at, int lim) const {
-        float z[3][32], moved = 0.f;
-        float2 sum[2] = {};
+    // Weights of 64 scores, packed; POLY: some as polynomials.
+    template <bool POLY>
+    __device__ __forceinline__ void weigh(const float *z, float2 off, uint32_t *w, float2 sum[2]) const {
         const float2 scale = make_float2(a.scale, a.scale);
-        auto largest = [&](float *v, int c) {
-            if constexpr (MASK) {
 #pragma unroll
-                for (int k = 0; k < 32; k++) v[k] = c * 32 + k < lim ? v[k] : -INFINITY;
+        for (int k = 0; k < 32; k++) {
+            float2 u = __ffma2_rn(make_float2(z[2 * k], z[2 * k + 1]), scale, off);
+            if (POLY && k % kPolyStep == kPolyStep - 1) {
+                u = exp2_poly<F16>(u);
+            } else {
+                u.x = exp2_fast(u.x);
+                u.y = exp2_fast(u.y);
             }
-            float m[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-            for (int k = 4; k < 28; k += 8)
-#pragma unroll
-                for (int e = 0; e < 4; e++) m[e] = fmaxf(fmaxf(m[e], v[k + e]), v[k + 4 + e]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) m[e] = fmaxf(m[e], v[28 + e]);
-            return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-        };
-        tmem_ld32(at, z[0]);
-        tmem_ld32(at + 32, z[1]);
-        tmem_wait_ld();
-        float top = largest(z[0], 0);
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            // the reference follows only a maximum that is 2^8 above it: weights stay below 2^8
-            if (__any_sync(0xffffffffu, fmaf(top, a.scale, -r.ref) > 8.f)) {
-                const float m = fmaxf(r.ref, ceilf(top * a.scale));
-                const float d = r.ref - m;  // <= 0, no number where both are infinite
-                const float f = d == 0.f ? 1.f : d > -126.f ? __int_as_float(((int)d + 127) << 23) : 0.f;
-                r.ref = m;
-                r.l *= f;
-                moved = moved == 0.f ? (f == 0.f ? 0x1p-126f : f) : fmaxf(moved * f, 0x1p-126f);
-                sum[0].x *= f; sum[0].y *= f; sum[1].x *= f; sum[1].y *= f;
-                if (c) {  // weights of this tile that are there already
-                    tmem_wait_st();
-#pragma unroll
-                    for (int e = 0; e < 16 * c; e += 16) {
-                        float w[16];
-                        tmem_ld16(at + e, w);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int k = 0; k < 16; k++) w[k] = __uint_as_float(scale2<F16>(__float_as_uint(w[k]), f));
-                        tmem_st16(at + e, reinterpret_cast<const uint32_t *>(w));
-                    }
-                }
-            }
-            if (c < 2) tmem_ld32(at + 32 * c + 64, z[(c + 2) % 3]);
-            const float off = r.ref == -INFINITY ? 0.f : -r.ref;
-            const float2 off2 = make_float2(off, off);
-            if (c < 3) top = largest(z[(c + 1) % 3], c + 1);
-            float *v = z[c % 3];
-            uint32_t w[16];
-#pragma unroll
-            for (int k = 0; k < 16; k++) {
-                float2 u = __ffma2_rn(make_float2(v[2 * k], v[2 * k + 1]), scale, off2);
-                if (!MASK && k % kPolyStep == kPolyStep - 1) {
-                    u = exp2_poly<F16>(u);
-                } else {
-                    u.x = exp2_fast(u.x);
-                    u.y = exp2_fast(u.y);
-                }
-                sum[k & 1] = __fadd2_rn(sum[k & 1], u);
-                w[k] = pack2<F16>(u.x, u.y);
-            }
-            tmem_st16(at + 16 * c, w);
-            if (c < 2) tmem_wait_ld();
+            sum[k & 1] = __fadd2_rn(sum[k & 1], u);
+            w[k] = pack2<F16>(u.x, u.y);
         }
+    }
+
+    // One tile of scores into weights.  The scores are read once, in one go: a load from TMEM takes 300
+    // cycles while products are running (four of 32 keys, each waited for: 1800 cycles a tile instead of
+    // 1400).  The product with V begins when the first 64 keys' weights are there.
+    template <bool MASK>
+    __device__ __forceinline__ bool tile(Row &r, int s, int slot, uint32_t lanes, int lim, bool first, unsigned o_count) const {
+        const uint32_t at = tmem + lanes + slot * kTile;
+        float z[kTile];
+#pragma unroll
+        for (int c = 0; c < kTile; c += 32) tmem_ld32(at + c, z + c);
+        tmem_landed<kTile>(z);
+        if constexpr (MASK) {
+#pragma unroll
+            for (int k = 0; k < kTile; k++) z[k] = k < lim ? z[k] : -INFINITY;
+        }
+        float m[8] = {z[0], z[1], z[2], z[3], z[4], z[5], z[6], z[7]};
+#pragma unroll
+        for (int k = 8; k < 120; k += 16)
+#pragma unroll
+            for (int e = 0; e < 8; e++) m[e] = fmaxf(fmaxf(m[e], z[k + e]), z[k + 8 + e]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) m[e] = fmaxf(m[e], z[120 + e]);
+        const float top = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
+        // the reference follows only a maximum that is 2^8 above it: weights stay below 2^8
+        float f = 1.f;
+        const bool moved = __any_sync(0xffffffffu, fmaf(top, a.scale, -r.ref) > 8.f);
+        if (moved) {
+            const float n = fmaxf(r.ref, ceilf(top * a.scale)), d = r.ref - n;  // d <= 0, no number where both are infinite
+            f = d == 0.f ? 1.f : d > -126.f ? __int_as_float(((int)d + 127) << 23) : 0.f;
+            r.ref = n;
+            r.l *= f;
+        }
+        const float off = r.ref == -INFINITY ? 0.f : -r.ref;
+        const float2 off2 = make_float2(off, off);
+        float2 sum[2] = {};
+        uint32_t w[32];
+        weigh<!MASK>(z, off2, w, sum);
+        tmem_st32(at, w);
+        if (moved && !first) {  // O waits for the last product
+            if (!wait_warp(small->o_done + s, (o_count - 1) & 1)) return false;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 16) {
+                float o[16];
+                const uint32_t oat = tmem + lanes + C::O_COL + s * DP + c;
+                tmem_ld16(oat, o);
+                tmem_landed<16>(o);
+#pragma unroll
+                for (int k = 0; k < 16; k++) o[k] *= f;
+                tmem_st16(oat, reinterpret_cast<const uint32_t *>(o));
+            }
+        }
+        ready(slot, 0);
+        weigh<!MASK>(z + 64, off2, w, sum);
+        tmem_st32(at + 32, w);
         r.l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        return moved;
+        ready(slot, 1);
+        return true;
+    }
+    // Half a tile's weights are there.
+    __device__ __forceinline__ void ready(int slot, int half) const {
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(small->p_full + 2 * slot + half);
     }
 
     __device__ __forceinline__ void softmax(int s) {
-        const int row = threadIdx.x & 127, lane = threadIdx.x & 31;
+        const int row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(row & ~31) << 16;  // of this warp
         const int tok = row / a.G, head = row - tok * a.G;
         unsigned s_uses[2] = {0, 0}, o_count = 0;
@@ -627,58 +651,39 @@ struct Block {
             const int nt = item->nt[s];
             for (int j = 0; j < nt; j++) {
                 const int slot = NQ == 2 ? s : j & 1;
-                const uint32_t at = tmem + lanes + slot * kTile;
-                if (!wait_warp(s_full + slot, s_uses[NQ == 2 ? 0 : slot]++ & 1)) return;
+                if (!wait_warp(small->s_full + slot, s_uses[NQ == 2 ? 0 : slot]++ & 1)) return;
                 tc_fence_after();
                 const int lim = vis - j * kTile;
-                const float f = __any_sync(0xffffffffu, lim < kTile) ? weights<true>(r, at, lim) : weights<false>(r, at, lim);
-                if (j > 0 && __any_sync(0xffffffffu, f != 0.f)) {
-                    if (!wait_warp(o_done + s, (o_count - 1) & 1)) return;
-                    tc_fence_after();
-#pragma unroll
-                    for (int c = 0; c < DP; c += 32) {
-                        float o[32];
-                        const uint32_t oat = tmem + lanes + C::O_COL + s * DP + c;
-                        tmem_ld32(oat, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int k = 0; k < 32; k++) o[k] *= f;
-                        tmem_st32(oat, reinterpret_cast<const uint32_t *>(o));
-                    }
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + slot);
+                if (__any_sync(0xffffffffu, lim < kTile) ? !tile<true>(r, s, slot, lanes, lim, j == 0, o_count)
+                                                         : !tile<false>(r, s, slot, lanes, lim, j == 0, o_count))
+                    return;
                 o_count++;
             }
             // scores that come two tiles ahead leave two products open: a parity tells one phase from the next only
-            if (NQ == 1 && nt > 1 && !wait_warp(o_done + s, o_count & 1)) return;
-            if (nt && !wait_warp(o_done + s, (o_count - 1) & 1)) return;
+            if (NQ == 1 && nt > 1 && !wait_warp(small->o_done + s, o_count & 1)) return;
+            if (nt && !wait_warp(small->o_done + s, (o_count - 1) & 1)) return;
             tc_fence_after();
-            write(*item, it, s, tok, head, nt, r.ref, r.l, lanes);
+            write(*item, it, s, tok, head, nt, r, lanes);
             done<true>(it);
         }
     }
 
     // Outputs of one row.
-    __device__ __forceinline__ void write(const Item &x, int it, int s, int tok, int head, int nt, float ref, float l,
-                                          uint32_t lanes) const {
+    __device__ __forceinline__ void write(const Item &x, int it, int s, int tok, int head, int nt, const Row &r, uint32_t lanes) const {
         using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
-        const int i = x.t + s * a.TQ + tok;
+        const int i = x.t + s * a.TQ + tok, h = x.h * a.G + head;
         const bool on = tok < a.TQ && i < x.s.nq;
-        const int h = x.h * a.G + head;
         const int64_t row = a.cu_q ? x.s.q0 + i : i;
         T *out = static_cast<T *>(a.out) + (a.cu_q ? 0 : x.b * a.o_sb) + row * a.o_ss + h * a.o_sh;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const bool fix = nt && *reinterpret_cast<volatile int *>(bad + (it & 1)) == it + 1;
+        const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
+        const bool fix = nt && *reinterpret_cast<volatile int *>(small->bad + (it & 1)) == it + 1;
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
             if (c >= a.D) break;
             float o[32];
             if (nt) {
                 tmem_ld32(tmem + lanes + C::O_COL + s * DP + c, o);
-                tmem_wait_ld();
+                tmem_landed<32>(o);
             }
             if (fix && on) {  // values of the masked tiles that are no numbers
                 const T *v = static_cast<const T *>(a.v) + (a.cu_q ? 0 : x.b * a.v_sb) + x.h * a.v_sh + c;
@@ -695,7 +700,7 @@ struct Block {
                     uint32_t w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        w[e] = l == 0.f ? 0u : pack2<F16>(o[k + 2 * e] * inv, o[k + 2 * e + 1] * inv);
+                        w[e] = r.l == 0.f ? 0u : pack2<F16>(o[k + 2 * e] * inv, o[k + 2 * e + 1] * inv);
                     if (a.o_vec) {
                         *reinterpret_cast<uint4 *>(out + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
                     } else {
@@ -711,7 +716,7 @@ struct Block {
         tc_fence_before();
         if (on && a.lse) {
             const int64_t at = ((a.cu_q ? row : (int64_t)x.b * a.Sq + i)) * a.Hq + h;
-            a.lse[at] = l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.693147180559945309f;
+            a.lse[at] = r.l == 0.f ? -INFINITY : (r.ref + log2f(r.l)) * 0.693147180559945309f;
         }
     }
 
@@ -728,7 +733,7 @@ struct Block {
         }
         auto publish = [&](int it) {
             const int slot = it % kItems;
-            if (it >= kItems && !wait_warp(item_empty + slot, (it / kItems - 1) & 1)) return false;
+            if (it >= kItems && !wait_warp(small->item_empty + slot, (it / kItems - 1) & 1)) return false;
             const int64_t n = gridDim.x, c = blockIdx.x, rank = it * n + (it & 1 ? n - 1 - c : c);
             Item x{};
             x.valid = find_item(a, rank / a.Hk, TP, most, x);
@@ -743,8 +748,8 @@ struct Block {
                 x.first = visible(a, x.s, x.t) / kTile;
             }
             if (lane == 0) {
-                items[slot] = x;
-                mbar_arrive(item_full + slot);
+                small->items[slot] = x;
+                mbar_arrive(small->item_full + slot);
             }
             return true;
         };
@@ -764,7 +769,7 @@ struct Block {
                     // it can be missed, and none passed by a warp that is ahead.)
                     const unsigned parity = seen >> st & 1;
                     seen ^= 1u << st;
-                    if (!wait_warp(v_raw + st, parity)) return;
+                    if (!wait_warp(small->v_raw + st, parity)) return;
                     uint4 *v = reinterpret_cast<uint4 *>(ring + st * C::STAGE) + w * 32 + lane;
                     constexpr uint32_t E = F16 ? 0x7c007c00u : 0x7f807f80u, ONE = F16 ? 0x04000400u : 0x00800080u;
 #pragma unroll 4
@@ -781,11 +786,11 @@ struct Block {
                             v[i * 64] = make_uint4(zero(y.x), zero(y.y), zero(y.z), zero(y.w));
                         }
                     }
-                    if (any) *reinterpret_cast<volatile int *>(bad + (it & 1)) = it + 1;
+                    if (any) *reinterpret_cast<volatile int *>(small->bad + (it & 1)) = it + 1;
                     fence_async_smem();
                     __syncwarp();
-                    if (w == 0 && !wait_warp(v_half + st, parity)) return;
-                    if (lane == 0) mbar_arrive(w == 0 ? kv_full + st : v_half + st);
+                    if (w == 0 && !wait_warp(small->v_half + st, parity)) return;
+                    if (lane == 0) mbar_arrive(w == 0 ? small->kv_full + st : small->v_half + st);
                 }
             pos += 2 * (int64_t)NU * x.tiles;
         }
@@ -797,55 +802,40 @@ __global__ void __launch_bounds__(Cfg<DP>::THREADS, 1)
 prompt_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
               const __grid_constant__ CUtensorMap mv, const __grid_constant__ Args a) {
     using C = Cfg<DP>;
-    extern __shared__ unsigned char smem_raw[];
-    __shared__ uint64_t bars[4 * C::NST + 2 + 2 + 2 + 2 + 2 + 2 * kItems];
-    __shared__ Item items[kItems];
-    __shared__ int abort_s, bad[2];
-    __shared__ uint32_t tmem_s;
-    Block<DP, F16> k(a);
-    k.q_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    k.ring = k.q_s + C::NQ * C::QB;
-    uint64_t *p = bars;
-    k.kv_full = p; p += C::NST;
-    k.kv_empty = p; p += C::NST;
-    k.v_raw = p; p += C::NST;
-    k.v_half = p; p += C::NST;
-    k.q_full = p; p += 2;
-    k.q_free = p; p += 2;
-    k.s_full = p; p += 2;
-    k.p_full = p; p += 2;
-    k.o_done = p; p += 2;
-    k.item_full = p; p += kItems;
-    k.item_empty = p;
-    k.items = items;
-    k.abort_s = &abort_s;
-    k.bad = bad;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    Block<DP, F16> k(a, smem);
+    Small<DP> &m = *k.small;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int SW = 4 * C::NQ;  // softmax warps
+    if (k.q_a & 1023) {  // tiles of 128-byte swizzle begin at multiples of 1024
+        if (threadIdx.x == 0) atomicMax(a.status, a.epoch);
+        return;
+    }
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::NST; i++) {
-            mbar_init(k.kv_full + i, 1);
-            mbar_init(k.kv_empty + i, 1);
-            mbar_init(k.v_raw + i, 1);
-            mbar_init(k.v_half + i, 1);
+            mbar_init(m.kv_full + i, 1);
+            mbar_init(m.kv_empty + i, 1);
+            mbar_init(m.v_raw + i, 1);
+            mbar_init(m.v_half + i, 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(k.q_full + i, 1);
-            mbar_init(k.q_free + i, 1);
-            mbar_init(k.s_full + i, 1);
-            mbar_init(k.p_full + i, 4);
-            mbar_init(k.o_done + i, 1);
-            bad[i] = 0;
+            mbar_init(m.q_full + i, 1);
+            mbar_init(m.q_free + i, 1);
+            mbar_init(m.s_full + i, 1);
+            mbar_init(m.p_full + 2 * i, 4);
+            mbar_init(m.p_full + 2 * i + 1, 4);
+            mbar_init(m.o_done + i, 1);
+            m.bad[i] = 0;
         }
         for (int i = 0; i < kItems; i++) {
-            mbar_init(k.item_full + i, 1);
-            mbar_init(k.item_empty + i, SW + 4);
+            mbar_init(m.item_full + i, 1);
+            mbar_init(m.item_empty + i, SW + 4);
         }
-        abort_s = 0;
+        m.abort_s = 0;
         fence_mbar_init();
     }
     if (warp == SW + 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)));
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&m.tmem)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     // rows of no sequence: zeros
@@ -862,31 +852,36 @@ prompt_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    k.tmem = tmem_s;
+    k.tmem = m.tmem;
+    // Two streams: 384 threads of 168 registers, shared out as 256 of 208 and 128 of 88.
     if (warp < SW) {
+        if constexpr (C::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         k.softmax(warp >> 2);
-    } else if (warp == SW) {
-        if (lane == 0) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
-            k.load(&mq, &mk, &mv);
-        }
-    } else if (warp == SW + 1) {
-        k.multiply();
     } else {
-        k.help(warp - SW - 2);
+        if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == SW) {
+            if (lane == 0) {
+                asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
+                asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+                asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+                k.load(&mq, &mk, &mv);
+            }
+        } else if (warp == SW + 1) {
+            k.multiply();
+        } else {
+            k.help(warp - SW - 2);
+        }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (abort_s) {  // copies and products in flight end (within microseconds) before their memory is given back
+    if (m.abort_s) {  // copies and products in flight end (within microseconds) before their memory is given back
         const uint64_t t0 = global_ns();
         while (global_ns() - t0 < 2000000) {}
     }
     if (warp == SW + 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_s));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(k.tmem));
     }
 }
 
@@ -928,18 +923,27 @@ bool walkable(const void *p, int64_t sb, int64_t nb, int64_t ss, int64_t ns, int
 template <int DP, bool F16>
 int launch(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const Args &a, int64_t items, cudaStream_t st) {
     using C = Cfg<DP>;
+    constexpr int smem = C::NQ * C::QB + C::NST * C::STAGE + (int)sizeof(Small<DP>);
+    static_assert(smem <= 232448, "shared memory");
     static bool ready[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { set_error("prompt_attn: no device"); return FC_ECUDA; }
     if (!ready[dev]) {
-        if (cudaFuncSetAttribute(prompt_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
+        if (cudaFuncSetAttribute(prompt_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
             set_error("prompt_attn: the kernel does not fit this device");
+            return FC_ECUDA;
+        }
+        // warps that ask for more registers wait for what others give back: a kernel that was built
+        // with too few to share out is never launched
+        cudaFuncAttributes attr;
+        if (cudaFuncGetAttributes(&attr, prompt_kernel<DP, F16>) != cudaSuccess || (C::NQ == 2 && attr.numRegs != 168)) {
+            set_error("prompt_attn: the kernel was built with another number of registers");
             return FC_ECUDA;
         }
         ready[dev] = true;
     }
     const int64_t blocks = items < num_sms() ? items : num_sms();
-    prompt_kernel<DP, F16><<<(unsigned)blocks, C::THREADS, C::SMEM, st>>>(mq, mk, mv, a);
+    prompt_kernel<DP, F16><<<(unsigned)blocks, C::THREADS, smem, st>>>(mq, mk, mv, a);
     return check_launch("prompt_attn");
 }
 

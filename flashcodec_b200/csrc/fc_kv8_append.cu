@@ -20,14 +20,14 @@ namespace kv8 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kQPasses = 4;  // passes of a query warp: that many loads of 8 channels on their way in a lane
+constexpr int kQPasses = 4;  // passes of a query warp, at most: that many loads on their way in a lane
 
 struct AppendArgs {
     const void *q, *k, *v;
     void *qo;
     int64_t q_sb, q_ss, q_sh, qo_sb, qo_ss, qo_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
     int64_t T, S;  // tokens in all; tokens of each sequence (0: ragged, by cu)
-    int B, Hq, Hk, D, per, slots, q_units;  // per: runs of a sequence; q_units: warps of a token
+    int B, Hq, Hk, D, per, slots, q_units, q_passes, heads;  // per: runs of a sequence; q_units: warps of a token; heads: of a block
     const int *cu, *lengths, *positions, *axes;
     int n_axes, axes_vec;
     const void *qw, *kw;
@@ -41,22 +41,46 @@ struct AppendArgs {
     int vec;  // bits: q, q_out, k, v rows and norm weights can be read in 16-byte words
 };
 
-template <int W> struct Lay {
-    static constexpr int D = 32 * W;
-    static constexpr int LPR = W == 2 ? 8 : W <= 4 ? 16 : 32;  // lanes of a row (of D = 96 and 192 some idle)
-    static constexpr int RP = 32 / LPR;                        // rows of a warp's pass
+// A lane has 8 channels of a row; FULL, where the whole head turns by halves, 16: both channels of
+// its pairs, so that none go from lane to lane.
+template <int W, bool FULL> struct Lay {
+    static constexpr int D = 32 * W, CH = FULL ? 2 : 1;
+    static constexpr int LPR = FULL ? D / 16 : W == 2 ? 8 : W <= 4 ? 16 : 32;  // lanes of a row (of D = 96 and 192 some idle)
+    static constexpr int RP = 32 / LPR;                                        // rows of a warp's pass
+    static constexpr int HALF = FULL ? D / 2 : 0;                              // from a lane's first channels to its second ones
+};
+
+// 8 elements as they came.
+template <typename T> struct Raw {
+    uint4 w[sizeof(T) == 4 ? 2 : 1];
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, bool vec, float x[8]) {
-    if (!vec) {
+__device__ __forceinline__ Raw<T> load_raw(const T *p, bool vec) {
+    Raw<T> r;
+    if (vec) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = Elem<T>::to_f32(p[i]);
-    } else if constexpr (sizeof(T) == 4) {
-        load_vec_f32<T, 4>(p, x);
-        load_vec_f32<T, 4>(p + 4, x + 4);
+        for (int i = 0; i < (int)(sizeof(Raw<T>) / 16); i++) r.w[i] = reinterpret_cast<const uint4 *>(p)[i];
     } else {
-        load_vec_f32<T, 8>(p, x);
+        using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+        const U *u = reinterpret_cast<const U *>(p);
+        uint32_t *w = reinterpret_cast<uint32_t *>(&r);
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(Raw<T>) / 4); i++) {
+            if constexpr (sizeof(T) == 4) w[i] = u[i];
+            else w[i] = u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
+        }
+    }
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void widen(const Raw<T> &r, float x[8]) {
+    if constexpr (sizeof(T) == 4) {
+        load_vec_f32<T, 4>(reinterpret_cast<const T *>(&r.w[0]), x);
+        load_vec_f32<T, 4>(reinterpret_cast<const T *>(&r.w[1]), x + 4);
+    } else {
+        load_vec_f32<T, 8>(reinterpret_cast<const T *>(&r.w[0]), x);
     }
 }
 
@@ -91,10 +115,11 @@ struct Place {
     int part, lane, pair;
 };
 
-template <int W>
+template <int W, bool FULL>
 __device__ __forceinline__ Place place_of(const AppendArgs &a, int lane) {
-    const int ci = lane % Lay<W>::LPR, shift = a.R / 16;
+    const int ci = lane % Lay<W, FULL>::LPR, shift = a.R / 16;
     Place p;
+    if constexpr (FULL) return Place{1, lane, ci * 8};
     p.part = ci * 8 >= a.R ? 0 : a.interleaved ? 3 : ci < shift ? 1 : 2;
     p.lane = p.part == 1 ? lane + shift : p.part == 2 ? lane - shift : lane;
     p.pair = p.part == 3 ? ci * 4 : (p.part == 2 ? ci - shift : ci) * 8;
@@ -155,7 +180,7 @@ template <typename T>
 __device__ __forceinline__ void load_weights(const AppendArgs &a, const void *w, int ch, bool on, float x[8]) {
     if (!w || !on) return;
     if (a.w_dtype == Elem<T>::code) {
-        load8(static_cast<const T *>(w) + ch, a.vec & 16, x);
+        widen(load_raw(static_cast<const T *>(w) + ch, a.vec & 16), x);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = load_as_f32(w, ch + i, a.w_dtype);
@@ -163,20 +188,38 @@ __device__ __forceinline__ void load_weights(const AppendArgs &a, const void *w,
 }
 
 // x r w of one head.  All lanes of the warp call it (those without channels hold zeros).
-template <int W>
-__device__ __forceinline__ void norm_row(float x[8], const float w[8], const AppendArgs &a) {
-    float s[8];
+template <int W, bool FULL>
+__device__ __forceinline__ void norm_row(float x[][8], const float w[][8], const AppendArgs &a) {
+    using L = Lay<W, FULL>;
+    float sum[L::CH];
 #pragma unroll
-    for (int i = 0; i < 8; i++) s[i] = __fmul_rn(x[i], x[i]);
+    for (int c = 0; c < L::CH; c++) {
+        float s[8];
 #pragma unroll
-    for (int n = 4; n; n /= 2)
+        for (int i = 0; i < 8; i++) s[i] = __fmul_rn(x[c][i], x[c][i]);
 #pragma unroll
-        for (int i = 0; i < n; i++) s[i] = __fadd_rn(s[2 * i], s[2 * i + 1]);
+        for (int n = 4; n; n /= 2)
 #pragma unroll
-    for (int m = 1; m < Lay<W>::LPR; m *= 2) s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], m));
-    const float r = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(s[0], a.inv_d), a.eps)));
+            for (int i = 0; i < n; i++) s[i] = __fadd_rn(s[2 * i], s[2 * i + 1]);
+        sum[c] = s[0];
+    }
+    if constexpr (FULL) {
+        // the two halves' sums: each lane of a pair goes on with one of them
+        const bool up = threadIdx.x & 1;
+        const float give = up ? sum[0] : sum[1], mine = up ? sum[1] : sum[0];
+        float s = __fadd_rn(mine, __shfl_xor_sync(0xffffffffu, give, 1));
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
+        for (int m = 2; m < L::LPR; m *= 2) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, m));
+        sum[0] = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 1));
+    } else {
+#pragma unroll
+        for (int m = 1; m < L::LPR; m *= 2) sum[0] = __fadd_rn(sum[0], __shfl_xor_sync(0xffffffffu, sum[0], m));
+    }
+    const float r = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(sum[0], a.inv_d), a.eps)));
+#pragma unroll
+    for (int c = 0; c < L::CH; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[c][i] = __fmul_rn(__fmul_rn(x[c][i], r), w[c][i]);
 }
 
 __device__ __forceinline__ float turn(float x, float c, float y, float s) {  // x c + y s
@@ -184,21 +227,29 @@ __device__ __forceinline__ float turn(float x, float c, float y, float s) {  // 
 }
 
 // Rotation of one head.  All lanes of the warp call it.
-__device__ __forceinline__ void rotate_row(float x[8], const Angles &g, const Place &p, const AppendArgs &a) {
-    if (a.interleaved) {
+template <bool FULL>
+__device__ __forceinline__ void rotate_row(float x[][8], const Angles &g, const Place &p, const AppendArgs &a) {
+    if constexpr (FULL) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float u = x[0][i], v = x[1][i];
+            x[0][i] = turn(u, g.c[i], v, -g.s[i]);
+            x[1][i] = turn(v, g.c[i], u, g.s[i]);
+        }
+    } else if (a.interleaved) {
         if (p.part) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float u = x[2 * i], v = x[2 * i + 1];
-                x[2 * i] = turn(u, g.c[i], v, -g.s[i]);
-                x[2 * i + 1] = turn(v, g.c[i], u, g.s[i]);
+                const float u = x[0][2 * i], v = x[0][2 * i + 1];
+                x[0][2 * i] = turn(u, g.c[i], v, -g.s[i]);
+                x[0][2 * i + 1] = turn(v, g.c[i], u, g.s[i]);
             }
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float y = __shfl_sync(0xffffffffu, x[i], p.lane);
-            if (p.part) x[i] = turn(x[i], g.c[i], y, p.part == 1 ? -g.s[i] : g.s[i]);
+            const float y = __shfl_sync(0xffffffffu, x[0][i], p.lane);
+            if (p.part) x[0][i] = turn(x[0][i], g.c[i], y, p.part == 1 ? -g.s[i] : g.s[i]);
         }
     }
 }
@@ -216,147 +267,207 @@ struct Run {
     int64_t pos, lo, hi, t0;  // first position; the positions added; row of the call's token at position 0
 };
 
-template <typename T, int W>
-__device__ __forceinline__ void append_run(const AppendArgs &a, const Run &r, int page, int h) {
-    using L = Lay<W>;
-    constexpr int PASSES = 4 / L::RP;
-    __shared__ float tops[8];
+// ... for n heads from h on: their tokens' angles are read once, and a head's rows while the one before it is
+// worked on.
+template <typename T, int W, bool FULL>
+__device__ __forceinline__ void append_run(const AppendArgs &a, const Run &r, int page, int h, int n) {
+    using L = Lay<W, FULL>;
+    constexpr int PASSES = L::RP > 4 ? 1 : 4 / L::RP, CH = L::CH;
+    __shared__ float tops[2][8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = warp >> 2;
     const int ch = lane % L::LPR * 8, row0 = (warp & 3) * 4 + lane / L::LPR;
-    const bool lane_on = ch < L::D;
+    const bool lane_on = ch < L::D && lane / L::LPR < 4;
     const int in_page = (int)(r.pos & ((1 << a.pool.log_page) - 1));
     const int64_t head = a.pool.head(page, kv, h);
     signed char *codes = a.pool.codes + ((head << a.pool.log_page) + in_page) * L::D + ch;
     float *scale = a.pool.scales + (head << (a.pool.log_page - 4)) + (in_page >> 4);
     const int held = (int)max((int64_t)0, r.lo - r.pos);
-    const float old = held ? *scale : 0.f;
-    const T *src = static_cast<const T *>(kv ? a.v : a.k);
     const int64_t sb = kv ? a.v_sb : a.k_sb, ss = kv ? a.v_ss : a.k_ss, sh = kv ? a.v_sh : a.k_sh;
-    float x[PASSES][8];
+    const T *src[PASSES];
     bool on[PASSES];
+    Raw<T> raw[PASSES][CH];
 #pragma unroll
     for (int i = 0; i < PASSES; i++) {
         const int64_t pos = r.pos + row0 + i * L::RP, t = r.t0 + pos;
         on[i] = pos >= r.lo && pos < r.hi && lane_on;
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[i][j] = 0.f;
-        if (on[i]) {
-            const int64_t b = a.S ? t / a.S : 0;
-            load8(src + b * sb + (a.S ? t - b * a.S : t) * ss + h * sh + ch, a.vec & (kv ? 8 : 4), x[i]);
-        }
+        const int64_t b = on[i] && a.S ? t / a.S : 0;
+        src[i] = static_cast<const T *>(kv ? a.v : a.k) + b * sb + (a.S ? t - b * a.S : t) * ss + h * sh + ch;
     }
-    float top = 0.f;
-    if (kv == 0) {
-        float w[8] = {};
-        load_weights<T>(a, a.kw, ch, lane_on, w);
-        const Place p = place_of<W>(a, lane);
+    auto load = [&] {
 #pragma unroll
         for (int i = 0; i < PASSES; i++) {
-            Angles g;
-            const int64_t pos = r.pos + row0 + i * L::RP;
-            if (a.R && on[i]) load_angles(g, a, p, r.t0 + pos, pos);
-            if (a.kw) norm_row<W>(x[i], w, a);
-            if (a.R) {
-                if (!on[i])
+            if (on[i])
 #pragma unroll
-                    for (int j = 0; j < 8; j++) g.c[j] = g.s[j] = 0.f;
-                rotate_row(x[i], g, p, a);
+                for (int c = 0; c < CH; c++) raw[i][c] = load_raw(src[i] + c * L::HALF, a.vec & (kv ? 8 : 4));
+            src[i] += sh;
+        }
+    };
+    load();
+    float old = held ? *scale : 0.f;
+    float w[CH][8] = {};
+    const Place p = place_of<W, FULL>(a, lane);
+    Angles g[PASSES];
+    if (kv == 0) {
+#pragma unroll
+        for (int i = 0; i < PASSES; i++) {
+            const int64_t pos = r.pos + row0 + i * L::RP;
+#pragma unroll
+            for (int j = 0; j < 8; j++) g[i].c[j] = g[i].s[j] = 0.f;
+            if (a.R && on[i]) load_angles(g[i], a, p, r.t0 + pos, pos);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; c++) load_weights<T>(a, a.kw, ch + c * L::HALF, lane_on, w[c]);
+    }
+    for (int y = 0; y < n; y++) {
+        float x[PASSES][CH][8];
+#pragma unroll
+        for (int i = 0; i < PASSES; i++)
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                if (on[i]) {
+                    widen(raw[i][c], x[i][c]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[i][c][j] = 0.f;
+                }
+            }
+        float next = 0.f;
+        if (y + 1 < n) {
+            load();
+            if (held) next = scale[(int64_t)1 << (a.pool.log_page - 4)];
+        }
+        if (kv == 0) {
+#pragma unroll
+            for (int i = 0; i < PASSES; i++) {
+                if (a.kw) norm_row<W, FULL>(x[i], w, a);
+                if (a.R) rotate_row<FULL>(x[i], g[i], p, a);
             }
         }
-    }
+        float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < PASSES; i++)
-        if (on[i])
+        for (int i = 0; i < PASSES; i++)
+            if (on[i])
 #pragma unroll
-            for (int j = 0; j < 8; j++) top = max_nan(top, fabsf(x[i][j]));
+                for (int c = 0; c < CH; c++)
 #pragma unroll
-    for (int m = 1; m < 32; m *= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
-    if (lane == 0) tops[warp] = top;
-    __syncthreads();
-    top = max_nan(max_nan(tops[4 * kv], tops[4 * kv + 1]), max_nan(tops[4 * kv + 2], tops[4 * kv + 3]));
-    // biased exponents: 0 no value but zero, 255 no number
-    const int e_old = (int)(__float_as_uint(old) >> 23) & 255;
-    const int e = max(e_old, top == top ? scale_exponent(top) : 255);
-    const float inv = e == 0 || e == 255 ? 0.f : __uint_as_float((uint32_t)(254 - e) << 23);
+                    for (int j = 0; j < 8; j++) top = max_nan(top, fabsf(x[i][c][j]));
 #pragma unroll
-    for (int i = 0; i < PASSES; i++) {
-        const int row = row0 + i * L::RP;
-        if (on[i]) {
-            uint32_t c[8];
-            // x / scale + 1.5 * 2^23 rounded down: its low byte is the floor
+        for (int m = 1; m < 32; m *= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
+        float *z = tops[y & 1];  // (who writes to it the next time has met the others once more)
+        if (lane == 0) z[warp] = top;
+        if (kv) asm volatile("bar.sync 2, 128;" ::: "memory");  // the 4 warps of the values,
+        else asm volatile("bar.sync 1, 128;" ::: "memory");     // or of the keys
+        top = max_nan(max_nan(z[4 * kv], z[4 * kv + 1]), max_nan(z[4 * kv + 2], z[4 * kv + 3]));
+        // biased exponents: 0 no value but zero, 255 no number
+        const int e_old = (int)(__float_as_uint(old) >> 23) & 255;
+        const int e = max(e_old, top == top ? scale_exponent(top) : 255);
+        const float inv = e == 0 || e == 255 ? 0.f : __uint_as_float((uint32_t)(254 - e) << 23);
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                c[j] = inv > 0.f ? __float_as_uint(__fmaf_rd(x[i][j], inv, 12582912.f)) : 0u;
-            uint2 w;
-            w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-            w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
-            *reinterpret_cast<uint2 *>(codes + (int64_t)row * L::D) = w;
-        } else if (row < held && lane_on && e_old && e > e_old && e < 255) {
-            uint2 *p = reinterpret_cast<uint2 *>(codes + (int64_t)row * L::D);
-            uint2 w = *p;
-            w.x = shift_codes(w.x, e - e_old);
-            w.y = shift_codes(w.y, e - e_old);
-            *p = w;
+        for (int i = 0; i < PASSES; i++) {
+            const int row = row0 + i * L::RP;
+#pragma unroll
+            for (int k = 0; k < CH; k++) {
+                signed char *at = codes + (int64_t)row * L::D + k * L::HALF;
+                if (on[i]) {
+                    uint32_t c[8];
+                    // x / scale + 1.5 * 2^23 rounded down: its low byte is the floor
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        c[j] = inv > 0.f ? __float_as_uint(__fmaf_rd(x[i][k][j], inv, 12582912.f)) : 0u;
+                    uint2 v;
+                    v.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+                    v.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+                    *reinterpret_cast<uint2 *>(at) = v;
+                } else if (row < held && lane_on && e_old && e > e_old && e < 255) {
+                    uint2 v = *reinterpret_cast<uint2 *>(at);
+                    v.x = shift_codes(v.x, e - e_old);
+                    v.y = shift_codes(v.y, e - e_old);
+                    *reinterpret_cast<uint2 *>(at) = v;
+                }
+            }
         }
+        if ((warp & 3) == 0 && lane == 0) *scale = __uint_as_float(e == 255 ? 0x7fc00000u : (uint32_t)e << 23);
+        codes += (int64_t)L::D << a.pool.log_page;
+        scale += (int64_t)1 << (a.pool.log_page - 4);
+        old = next;
     }
-    if ((warp & 3) == 0 && lane == 0) *scale = __uint_as_float(e == 255 ? 0x7fc00000u : (uint32_t)e << 23);
 }
 
-template <typename T, int W>
-__device__ __forceinline__ void keys_and_values(const AppendArgs &a, int slot, int h) {
+// A slot's sequence, and which of its runs of 16 positions: of B sequences of S tokens, `per` runs
+// each, or by cu.  False: none.
+struct Slot {
     int b, k;
-    int64_t c0, n;
-    if (a.S) {
-        b = slot / a.per;
-        k = slot - b * a.per;
-        c0 = (int64_t)b * a.S;
-        n = a.S;
+    int64_t c0, n, i0, i1;  // first row and tokens of the sequence; those of them that have a row
+};
+
+__device__ __forceinline__ bool find_slot(Slot &x, int slot, int B, int64_t S, int64_t T, int per, const int *cu, int *status) {
+    if (S) {
+        x.b = slot / per;
+        x.k = slot - x.b * per;
+        x.c0 = (int64_t)x.b * S;
+        x.n = S;
     } else {
         // a sequence of n tokens has at most n / 16 + 2 runs: slots from cu / 16 + 2 b on are its own
-        const int *cu = a.cu;
-        b = warp_find([=](int i) { return (int64_t)(cu[i] >> 4) + 2 * i; }, a.B, slot);
-        c0 = cu[b];
-        k = slot - (int)((c0 >> 4) + 2 * b);
-        n = cu[b + 1] - c0;
-        if (k < 0) return;
+        x.b = warp_find([=](int i) { return (int64_t)(cu[i] >> 4) + 2 * i; }, B, slot);
+        x.c0 = cu[x.b];
+        x.k = slot - (int)((x.c0 >> 4) + 2 * x.b);
+        x.n = cu[x.b + 1] - x.c0;
+        if (x.k < 0) return false;
     }
-    const int len = a.lengths[b];
-    if (len < 0) return;
     // tokens without a row are skipped
-    int64_t i0 = 0, i1 = n;
-    if (c0 < 0 || c0 + n > a.T) {
-        if (threadIdx.x == 0) atomicOr(a.table.status, kv4::kBadLength);
-        i0 = max((int64_t)0, -c0);
-        i1 = min(n, a.T - c0);
+    x.i0 = 0;
+    x.i1 = x.n;
+    if (x.c0 < 0 || x.c0 + x.n > T) {
+        if (threadIdx.x == 0) atomicOr(status, kv4::kBadLength);
+        x.i0 = max((int64_t)0, -x.c0);
+        x.i1 = min(x.n, T - x.c0);
     }
+    return true;
+}
+
+// The run's positions, for a sequence whose tokens begin at position `start`.
+__device__ __forceinline__ bool run_of(Run &r, const Slot &x, int start) {
+    r.pos = (int64_t)((start >> 4) + x.k) << 4;
+    r.lo = max(r.pos, start + x.i0);
+    r.hi = min(r.pos + kBlock, start + x.i1);
+    r.t0 = x.c0 - start;
+    return r.lo < r.hi;
+}
+
+// The page of a run, or -1, noted in status.
+__device__ __forceinline__ int page_of(const Table &t, int b, int64_t pos) {
+    const int64_t i = pos >> t.log_page;
+    if (i >= t.max_pages) {
+        if (threadIdx.x == 0) atomicOr(t.status, kv4::kBadLength);
+        return -1;
+    }
+    const int page = t.pages[b * t.stride + i];
+    if ((unsigned)page < (unsigned)t.num_pages) return page;
+    if (threadIdx.x == 0) atomicOr(t.status, kv4::kBadPage);
+    return -1;
+}
+
+template <typename T, int W, bool FULL>
+__device__ __forceinline__ void keys_and_values(const AppendArgs &a, int slot, int h) {
+    Slot x;
+    if (!find_slot(x, slot, a.B, a.S, a.T, a.per, a.cu, a.table.status)) return;
+    const int len = a.lengths[x.b];
     Run r;
-    r.pos = (int64_t)((len >> 4) + k) << 4;
-    r.lo = max(r.pos, len + i0);
-    r.hi = min(r.pos + kBlock, len + i1);
-    r.t0 = c0 - len;
-    if (r.lo >= r.hi) return;
-    const int64_t i = r.pos >> a.table.log_page;
-    if (i >= a.table.max_pages) {
-        if (threadIdx.x == 0) atomicOr(a.table.status, kv4::kBadLength);
-        return;
-    }
-    const int page = a.table.pages[b * a.table.stride + i];
-    if ((unsigned)page >= (unsigned)a.table.num_pages) {
-        if (threadIdx.x == 0) atomicOr(a.table.status, kv4::kBadPage);
-        return;
-    }
-    append_run<T, W>(a, r, page, h);
+    if (len < 0 || !run_of(r, x, len)) return;
+    const int page = page_of(a.table, x.b, r.pos);
+    if (page >= 0) append_run<T, W, FULL>(a, r, page, h, min(a.heads, a.Hk - h));
 }
 
 // ------------------------------------------------------------------------- queries
-// kQPasses passes of heads of one token: its angles are read once.
-template <typename T, int W>
+// q_passes passes of heads of one token: its angles are read once.
+template <typename T, int W, bool FULL>
 __device__ __forceinline__ void queries(const AppendArgs &a, int64_t unit) {
-    using L = Lay<W>;
+    using L = Lay<W, FULL>;
+    constexpr int CH = L::CH;
     const int64_t t = unit / a.q_units;
     if (t >= a.T) return;
     const int lane = threadIdx.x & 31, ch = lane % L::LPR * 8;
-    const int h0 = (int)(unit - t * a.q_units) * kQPasses * L::RP + lane / L::LPR;
+    const int h0 = (int)(unit - t * a.q_units) * a.q_passes * L::RP + lane / L::LPR;
     int64_t b = 0, s = t, at = 0;
     bool none = false;  // a row of no sequence
     if (a.S) {
@@ -370,49 +481,65 @@ __device__ __forceinline__ void queries(const AppendArgs &a, int64_t unit) {
         none = a.B == 0 || t < cu[i] || t >= cu[i + 1];
         if (!none && a.R && !a.positions) at = (int64_t)max(0, a.lengths[i]) + t - cu[i];
     }
-    float x[kQPasses][8];
     const T *src = static_cast<const T *>(a.q) + b * a.q_sb + s * a.q_ss + ch;
     T *dst = static_cast<T *>(a.qo) + b * a.qo_sb + s * a.qo_ss + ch;
     const bool lane_on = ch < L::D;
+    Raw<T> raw[kQPasses][CH];
 #pragma unroll
     for (int i = 0; i < kQPasses; i++) {
         const int h = h0 + i * L::RP;
+        if (i < a.q_passes && lane_on && h < a.Hq && !none)
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[i][j] = 0.f;
-        if (lane_on && h < a.Hq && !none) load8(src + h * a.q_sh, a.vec & 1, x[i]);
+            for (int c = 0; c < CH; c++) raw[i][c] = load_raw(src + h * a.q_sh + c * L::HALF, a.vec & 1);
     }
-    const Place p = place_of<W>(a, lane);
+    const Place p = place_of<W, FULL>(a, lane);
     Angles g;
-    float w[8] = {};
+    float w[CH][8] = {};
     if (!none) {
         if (a.R) load_angles(g, a, p, t, at);
-        load_weights<T>(a, a.qw, ch, lane_on, w);
+#pragma unroll
+        for (int c = 0; c < CH; c++) load_weights<T>(a, a.qw, ch + c * L::HALF, lane_on, w[c]);
     }
 #pragma unroll
     for (int i = 0; i < kQPasses; i++) {
+        if (i >= a.q_passes) break;
         const int h = h0 + i * L::RP;
-        if (!none) {
-            if (a.qw) norm_row<W>(x[i], w, a);
-            if (a.R) rotate_row(x[i], g, p, a);
+        const bool on = lane_on && h < a.Hq;
+        float x[CH][8];
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            if (on && !none) {
+                widen(raw[i][c], x[c]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[c][j] = 0.f;
+            }
         }
-        if (lane_on && h < a.Hq) store8(dst + h * a.qo_sh, a.vec & 2, x[i]);
+        if (!none) {
+            if (a.qw) norm_row<W, FULL>(x, w, a);
+            if (a.R) rotate_row<FULL>(x, g, p, a);
+        }
+        if (on)
+#pragma unroll
+            for (int c = 0; c < CH; c++) store8(dst + h * a.qo_sh + c * L::HALF, a.vec & 2, x[c]);
     }
 }
 
-template <typename T, int W>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
-    const int64_t runs = (int64_t)a.slots * a.Hk;
+template <typename T, int W, bool FULL>
+__global__ void __launch_bounds__(kThreads, W <= 4 ? 3 : 2) append_kernel(const __grid_constant__ AppendArgs a) {
+    const int parts = (a.Hk + a.heads - 1) / a.heads;
+    const int64_t runs = (int64_t)a.slots * parts;
     if (blockIdx.x < runs) {
-        const int slot = (int)(blockIdx.x / a.Hk);
-        keys_and_values<T, W>(a, slot, (int)(blockIdx.x - (int64_t)slot * a.Hk));
+        const int slot = (int)(blockIdx.x / parts);
+        keys_and_values<T, W, FULL>(a, slot, (int)(blockIdx.x - (int64_t)slot * parts) * a.heads);
     } else {
-        queries<T, W>(a, ((int64_t)blockIdx.x - runs) * (kThreads / 32) + (threadIdx.x >> 5));
+        queries<T, W, FULL>(a, ((int64_t)blockIdx.x - runs) * (kThreads / 32) + (threadIdx.x >> 5));
     }
 }
 
 // ---------------------------------------------------------------------------- read
 struct ReadArgs {
-    int B, Hk;
+    int B, Hk, per, slots;
     int64_t T, S;
     const int *starts, *cu;
     void *k, *v;
@@ -422,60 +549,70 @@ struct ReadArgs {
     int vec;
 };
 
-// A warp reads the keys or the values of a token, all heads: 8 codes a lane.
+// A warp reads the keys or the values of a head and run of 16 positions: 2 KB in a row at D = 128. 32000
+// tokens of 8 heads, 197 MB, take 39 us, 78 % of the copy rate (a warp a token, whose heads lie a page apart: 45
+// us).
 template <typename T, int W>
-__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadArgs a) {
-    constexpr int CH = 4 * W;  // lanes of a row
-    const int lane = threadIdx.x & 31;
-    const int64_t unit = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), t = unit >> 1;
-    const int kv = (int)unit & 1;
-    if (t >= a.T) return;
-    int64_t b = 0, s = t;
-    int i = 0;
-    int64_t pos = -1;  // no sequence, or a negative start
-    if (a.S) {
-        i = (int)(t / a.S);
-        b = i;
-        s = t - b * a.S;
-        const int start = a.starts ? a.starts[i] : 0;
-        if (start >= 0) pos = start + s;
-    } else if (a.B) {
-        const int *cu = a.cu;
-        if (unit == 0 && lane == 0 && (cu[0] < 0 || cu[a.B] > a.T)) atomicOr(a.table.status, kv4::kBadLength);
-        i = warp_find([=](int j) { return (int64_t)cu[j]; }, a.B, t);
-        if (t >= cu[i] && t < cu[i + 1]) {
-            const int start = a.starts ? a.starts[i] : 0;
-            if (start >= 0) pos = start + t - cu[i];
-        }
-    }
-    int page = -1;
-    if (pos >= 0) {
-        const int64_t at = pos >> a.table.log_page;
-        if (at >= a.table.max_pages) {
-            if (lane == 0) atomicOr(a.table.status, kv4::kBadLength);
-        } else {
-            page = a.table.pages[i * a.table.stride + at];
-            if ((unsigned)page >= (unsigned)a.table.num_pages) {
-                if (lane == 0) atomicOr(a.table.status, kv4::kBadPage);
-                page = -1;
-            }
-        }
-    }
-    const int row = (int)(pos & ((1 << a.table.log_page) - 1));
-    T *dst = static_cast<T *>(kv ? a.v : a.k) + b * a.o_sb + s * a.o_ss;
-    for (int c = lane; c < a.Hk * CH; c += 32) {
-        const int h = c / CH, ch = (c - h * CH) * 8;
-        float x[8] = {};
+__device__ __forceinline__ void read_run(const ReadArgs &a, int slot, int part) {
+    constexpr int UNITS = 2 * W;  // 16 codes each, of a row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Slot x;
+    if (!find_slot(x, slot, a.B, a.S, a.T, a.per, a.cu, a.table.status)) return;
+    const int start = a.starts ? a.starts[x.b] : 0;
+    Run r;
+    if (!run_of(r, x, max(start, 0))) return;
+    const int page = start < 0 ? -1 : page_of(a.table, x.b, r.pos);
+    const int in_page = (int)(r.pos & ((1 << a.pool.log_page) - 1));
+    const int64_t b = a.S ? x.b : 0, s0 = r.t0 + r.pos - b * a.S;  // the run's first row, if it is one
+    const int u = part * (kThreads / 32) + warp;
+    if (u < 2 * a.Hk) {
+        const int kv = u >= a.Hk, h = u - kv * a.Hk;
+        uint4 w[W];
+        float f = 0.f;
         if (page >= 0) {
             const int64_t head = a.pool.head(page, kv, h);
-            const float f = a.pool.scales[(head << (a.pool.log_page - 4)) + (row >> 4)];
-            const uint2 w = *reinterpret_cast<const uint2 *>(a.pool.codes + ((head << a.pool.log_page) + row) * (32 * W) + ch);
-            s8x4_to_f32(w.x, x);
-            s8x4_to_f32(w.y, x + 4);
+            const uint4 *src = reinterpret_cast<const uint4 *>(a.pool.codes + ((head << a.pool.log_page) + in_page) * (32 * W));
+            f = a.pool.scales[(head << (a.pool.log_page - 4)) + (in_page >> 4)];
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = (x[j] + 0.5f) * f;
+            for (int y = 0; y < W; y++) w[y] = src[32 * y + lane];
         }
-        store8(dst + h * a.o_sh + ch, a.vec, x);
+        T *dst = static_cast<T *>(kv ? a.v : a.k) + b * a.o_sb + s0 * a.o_ss + h * a.o_sh;
+#pragma unroll
+        for (int y = 0; y < W; y++) {
+            const int row = (32 * y + lane) / UNITS, ch = (32 * y + lane - row * UNITS) * 16;
+            if (r.pos + row < r.lo || r.pos + row >= r.hi) continue;
+            float z[16] = {};
+            if (page >= 0) {
+                const uint32_t c[4] = {w[y].x, w[y].y, w[y].z, w[y].w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) s8x4_to_f32(c[i], z + 4 * i);
+#pragma unroll
+                for (int i = 0; i < 16; i++) z[i] = (z[i] + 0.5f) * f;
+            }
+            store8(dst + row * a.o_ss + ch, a.vec, z);
+            store8(dst + row * a.o_ss + ch + 8, a.vec, z + 8);
+        }
+    }
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadArgs a) {
+    const int parts = (2 * a.Hk + kThreads / 32 - 1) / (kThreads / 32), runs = a.slots * parts;
+    if ((int)blockIdx.x < runs) {
+        const int slot = blockIdx.x / parts;
+        read_run<T, W>(a, slot, blockIdx.x - slot * parts);
+        return;
+    }
+    // rows of no sequence: zeros
+    const int64_t lo = a.B ? min(max((int64_t)a.cu[0], (int64_t)0), a.T) : a.T, hi = a.B ? min(max((int64_t)a.cu[a.B], lo), a.T) : a.T;
+    const int64_t rows = lo + a.T - hi, warps = (int64_t)(gridDim.x - runs) * (kThreads / 32);
+    for (int64_t i = (int64_t)(blockIdx.x - runs) * (kThreads / 32) + (threadIdx.x >> 5); i < rows; i += warps) {
+        const int64_t at = (i < lo ? i : i - lo + hi) * a.o_ss;
+        for (int c = threadIdx.x & 31; c < 2 * a.Hk * 4 * W; c += 32) {
+            const int u = c / (4 * W), kv = u >= a.Hk;
+            const float z[8] = {};
+            store8(static_cast<T *>(kv ? a.v : a.k) + at + (u - kv * a.Hk) * a.o_sh + (c - u * 4 * W) * 8, a.vec, z);
+        }
     }
 }
 
@@ -565,17 +702,34 @@ extern "C" int fc_kv8_append(const void *q, int64_t q_sb, int64_t q_ss, int64_t 
     return by_dtype(dtype, [&](auto t) {
         return by_head_dim(D, [&](auto w) {
             using E = decltype(t);
-            constexpr int W = decltype(w)::value, heads = kQPasses * Lay<W>::RP;
-            a.q_units = (int)((Hq + heads - 1) / heads);
-            const int64_t blocks = slots * Hk + (T * a.q_units + kThreads / 32 - 1) / (kThreads / 32);
-            if (blocks > 0x7fffffff) {
-                set_error("kv8_append: too many tokens for one call");
-                return FC_ENOTSUP;
+            constexpr int W = decltype(w)::value;
+            auto launch = [&](auto full) {
+                constexpr bool FULL = decltype(full)::value;
+                constexpr int heads = Lay<W, FULL>::RP;  // of a pass
+                // passes of a query warp: one where there are few tokens, more where there are enough for
+                // 32 warps an SM
+                const int64_t loads = (Hq + heads - 1) / heads, want = (32 * (int64_t)num_sms() + T - 1) / T;
+                a.q_passes = (int)((loads + want - 1) / want);
+                if (a.q_passes > kQPasses) a.q_passes = kQPasses;
+                a.q_units = a.q_passes ? (int)((loads + a.q_passes - 1) / a.q_passes) : 0;
+                // heads of a block: as many as leave 3 blocks an SM, up to 8 (8191 tokens, 8 heads: 67 us with
+                // one, 57 with 2, 50 with 8; a single token: 4.1 us with 2, 3.2 with one)
+                a.heads = 1;
+                while (a.heads < 8 && slots * ((Hk + 2 * a.heads - 1) / (2 * a.heads)) >= 3 * (int64_t)num_sms()) a.heads *= 2;
+                const int64_t blocks = slots * ((Hk + a.heads - 1) / a.heads) + (T * a.q_units + kThreads / 32 - 1) / (kThreads / 32);
+                if (blocks > 0x7fffffff) {
+                    set_error("kv8_append: too many tokens for one call");
+                    return FC_ENOTSUP;
+                }
+                if (blocks == 0) return FC_OK;
+                a.slots = (int)slots;
+                append_kernel<E, W, FULL><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+                return check_launch("kv8_append");
+            };
+            if constexpr (W == 4 || W == 8) {
+                if (rotary && rotary_dim == D && !interleaved) return launch(std::true_type());
             }
-            if (blocks == 0) return FC_OK;
-            a.slots = (int)slots;
-            append_kernel<E, W><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-            return check_launch("kv8_append");
+            return launch(std::false_type());
         });
     });
 }
@@ -599,7 +753,11 @@ extern "C" int fc_kv8_read(const signed char *codes, const float *scales, int64_
     a.pool = Pool{const_cast<signed char *>(codes), const_cast<float *>(scales), (int)Hk, ilog2(page_size)};
     a.table = Table{page_table, table_stride, (int)max_pages, (int)num_pages, ilog2(page_size), status};
     a.vec = rows_aligned(k_out, dtype, o_sb, o_ss, o_sh) && rows_aligned(v_out, dtype, o_sb, o_ss, o_sh);
-    const int64_t blocks = (2 * T + kThreads / 32 - 1) / (kThreads / 32);
+    a.per = (int)((S + 30) / 16);
+    a.slots = (int)(a.S ? B * a.per : B ? T / 16 + 2 * B : 0);
+    // (blocks for rows of no sequence)
+    const int64_t rest = cu_seqlens ? (T + 63) / 64 < 32 ? (T + 63) / 64 : 32 : 0, blocks = a.slots * ((2 * Hk + 7) / 8) + rest;
+    if (blocks > 0x7fffffff) { set_error("kv8_read: too many tokens for one call"); return FC_ENOTSUP; }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return by_dtype(dtype, [&](auto t) {
         return by_head_dim(D, [&](auto w) {

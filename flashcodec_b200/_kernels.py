@@ -177,7 +177,8 @@ def reset_workspace(device: torch.device) -> None:
 def _held_workspaces(device: torch.device) -> list:
     """(workspace, whether of a capture) of the current stream."""
     at = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    return [(ws, k[2] != 0) for k, ws in list(_workspaces.items()) if k[:2] == at]
+    return [(ws, k[2] != 0) for held in (_workspaces, _prompt_workspaces)
+            for k, ws in list(held.items()) if k[:2] == at]
 
 
 def _status_word(ws: torch.Tensor, captured: bool) -> torch.Tensor:
@@ -237,6 +238,8 @@ def attn_status_async(device: torch.device, reset: bool = False) -> StatusProbe:
     if reset:
         for ws, _ in held:
             ws[:4].zero_()
+            if any(ws is w for w in _prompt_workspaces.values()):  # a call that gave up may have left its counters
+                ws[:_PROMPT_CLEAR].zero_()
     ev = torch.cuda.Event()
     ev.record(stream)
     return StatusProbe(host, ev)
@@ -734,24 +737,55 @@ def kv8_attn(cache, q_at, dtype, shape, table, lengths, scale, out_at, lse) -> N
 
 
 # ------------------------------------------------------- attention over prompts
+# (device, stream, capture) -> workspace, as for the decode attention; a header with the status word
+# and the arrival counters are zeroed, what lies behind them needs none
+_prompt_workspaces: dict = {}
+_PROMPT_CLEAR = 256 + 4 * (1 << 14)
+
+
+def _prompt_workspace(index, stream, nbytes) -> torch.Tensor:
+    capture = _lib.load().fc_capture_id(stream)
+    key = (index, stream, capture)
+    ws = _prompt_workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _prompt_workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        ws[:_PROMPT_CLEAR].zero_()
+        if capture:
+            captures = [k for k in _prompt_workspaces if k[:2] == key[:2] and k[2]]
+            for k in captures[:-KEPT_CAPTURES]:
+                del _prompt_workspaces[k]
+    return ws
+
+
+def _place(t):
+    """Address, and strides of sequences, tokens and heads."""
+    st = t.stride()
+    return (t.data_ptr(), 0, st[0], st[1]) if len(st) == 3 else (t.data_ptr(), st[0], st[1], st[2])
+
+
 def prompt_attn(q, k, v, cu_q, cu_k, causal, scale, out, lse) -> None:
     """fc_prompt_attn; q, out (T, Hq, D) and k, v (T, Hk, D) packed, or (B, S, H, D) without cu's."""
-    def at(t):
-        return (t.data_ptr(), *((0, *t.stride()[:2]) if t.dim() == 3 else t.stride()[:3]))
-    dev, D = q.device, q.shape[-1]
+    index, shape, keys, lib = q.get_device(), q.shape, k.shape, _lib.load()
+    Hq, Hk, D = shape[-2], keys[-2], shape[-1]
     if cu_q is None:
-        B, Sq, Sk = q.shape[0], q.shape[1], k.shape[1]
-        Tq, Tk = B * Sq, B * Sk
+        B, Sq, Sk = shape[0], shape[1], keys[1]
+        Tq, Tk, cu = B * Sq, B * Sk, (None, None)
     else:
-        B, Sq, Sk, Tq, Tk = cu_q.shape[0] - 1, 0, 0, q.shape[0], k.shape[0]
-    Hq, Hk = q.shape[-2], k.shape[-2]
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        ws = workspace(dev, lib.fc_prompt_attn_workspace_size(B, Tq, Hq, Hk, D))
-        rc = lib.fc_prompt_attn(*at(q), *at(k), *at(v), _code(q.dtype), B, Sq, Sk, Tq, Tk, Hq, Hk, D,
-                                None if cu_q is None else cu_q.data_ptr(),
-                                None if cu_k is None else cu_k.data_ptr(), bool(causal), scale,
-                                *at(out), _p(lse), _p(ws), ws.numel(), _stream(dev))
-    if rc != _lib.FC_OK:
-        reset_workspace(dev)
-    _lib.check(rc, "prompt_attn")
+        B, Sq, Sk, Tq, Tk = cu_q.shape[0] - 1, 0, 0, shape[0], keys[0]
+        cu = cu_q.data_ptr(), cu_k.data_ptr()
+    stream = _raw_stream(index)
+    dtype = _code(q.dtype)
+
+    def call():
+        ws = _prompt_workspace(index, stream, lib.fc_prompt_attn_workspace_size(B, Tq, Hq, Hk, D))
+        rc = lib.fc_prompt_attn(*_place(q), *_place(k), *_place(v), dtype, B, Sq, Sk, Tq, Tk, Hq, Hk, D, *cu,
+                                causal, scale, *_place(out), None if lse is None else lse.data_ptr(),
+                                ws.data_ptr(), ws.numel(), stream)
+        if rc:
+            ws[:_PROMPT_CLEAR].zero_()
+            _lib.check(rc, "prompt_attn")
+    if _current_device() == index:
+        call()
+    else:
+        with torch.cuda.device(index):
+            call()

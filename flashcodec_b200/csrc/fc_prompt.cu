@@ -73,11 +73,16 @@ struct Args {
     int negative;
     int *status;
     int epoch;
+    int split;        // items may be cut along their keys
+    int *counters;    // by (item, head), stream and warp: pieces done, zero between calls
+    int *slots;       // by (item, head) and piece: where its results are
+    float *parts;     // results of pieces, kPart floats each
 };
 
 constexpr int kTile = 128;          // rows of a query tile, keys of a tile
 constexpr int kBox = kTile * 128;   // bytes of 128 rows of 64 channels
 constexpr int kItems = 3;           // items known ahead
+constexpr int kMaxPieces = 256;     // of an item: no more than blocks
 constexpr int kPolyStep = 4;        // every kPolyStep-th pair of weights is a polynomial
 
 template <int DP> struct Cfg {
@@ -267,6 +272,9 @@ struct Item {
     int nt[2];           // key tiles of the streams
     int tiles, first;    // key tiles; the first that holds masked keys
     int valid;           // 0: no more work
+    // an item cut along its keys: the first key, which piece, of how many; its number among the pieces of
+    // all items, and that of the (item, head)
+    int base, piece, pieces, unit, line;
 };
 
 // Keys that token i sees.
@@ -276,64 +284,120 @@ __device__ __forceinline__ int visible(const Args &a, const Sequence &s, int i) 
 
 __device__ __forceinline__ int tiles_of(int keys) { return (int)(((unsigned)keys + kTile - 1) / kTile); }
 
-// Items of a sequence with at least w > 0 key tiles, TP tokens each: those from a token on.
-__device__ __forceinline__ int items_from(const Args &a, const Sequence &s, int w, int TP) {
-    const int n = (s.nq + TP - 1) / TP;
-    if (!a.causal) return tiles_of(s.nk) >= w ? n : 0;
-    if (tiles_of(s.nk) < w) return 0;
-    // item t's last token sees min(nk, nk - nq + (t + 1) TP) keys: more than (w - 1) kTile
-    const int64_t need = (int64_t)(w - 1) * kTile - ((int64_t)s.nk - s.nq);  // (t + 1) TP > need
-    const int64_t t = need < 0 ? 0 : need / TP;
-    return (int)max((int64_t)0, n - t);
-}
+// A piece of an item is no shorter than this many tiles (16/8 heads, D = 128: 1000 tokens, of at most 8 tiles,
+// 31 us with 6, 24 us with 8; 64 tokens over 4096 49 and 45, 48 with 16).
+constexpr int kLeastPiece = 8;
 
-// Item number `rank` of the line of all (sequence, tokens), the ones of most tiles first.  A
-// warp calls it.  Items of no tiles come last.
-__device__ __forceinline__ bool find_item(const Args &a, int64_t rank, int TP, int most, Item &x) {
-    const int lane = threadIdx.x & 31;
-    auto count = [&](int w) {  // items of at least w tiles
-        int64_t n = 0;
-        for (int b = lane; b < a.B; b += 32) {
-            const Sequence s = sequence(a, b);
-            n += w ? items_from(a, s, w, TP) : (s.nq + TP - 1) / TP;
-        }
+// The line of work, as a warp finds its way on it.  Items (sequence, TP tokens) come by their number of
+// tiles, the ones of most first, items of none last.  Where there are fewer than blocks they are cut
+// along their keys, into P = NT * blocks / (all tiles) pieces each, at least 1, and all items' first pieces
+// come first, then the second ones of those that have two, and so on.
+struct Line {
+    const Args &a;
+    int TP, most;
+    Sequence mine;    // of this lane, where there are no more sequences than lanes
+    int64_t tiles;    // of all items and heads, where they are cut
+
+    __device__ __forceinline__ Line(const Args &args, int tp) : a(args), TP(tp), most(0), mine{}, tiles(1) {
+        const int lane = threadIdx.x & 31;
+        if (lane < a.B) mine = sequence(a, lane);
+        for (int b = lane; b < a.B; b += 32) most = max(most, tiles_of(at(b).nk));
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (a.split) {
+            int64_t n = 0;
+            for (int b = lane; b < a.B; b += 32) {
+                const Sequence s = at(b);
+                for (int t = TP; t - TP < s.nq; t += TP) n += tiles_of(visible(a, s, min(t, s.nq) - 1));
+            }
 #pragma unroll
-        for (int o = 16; o; o /= 2) n += __shfl_xor_sync(0xffffffffu, n, o);
-        return n;
-    };
-    if (count(0) <= rank) return false;
-    int lo = 0, hi = most + 1;  // count(lo) > rank >= count(hi)
-    while (hi - lo > 1) {
-        const int mid = lo + (hi - lo) / 2;
-        (count(mid) > rank ? lo : hi) = mid;
-    }
-    int64_t left = rank - count(lo + 1);  // among the items of lo tiles, by sequence
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-        const int b = b0 + lane;
-        int n = 0, t0 = 0;
-        if (b < a.B) {
-            const Sequence s = sequence(a, b);
-            const int all = (s.nq + TP - 1) / TP, ge = lo ? items_from(a, s, lo, TP) : all;
-            n = ge - items_from(a, s, lo + 1, TP);
-            t0 = a.causal ? all - ge : 0;
+            for (int o = 16; o; o /= 2) n += __shfl_xor_sync(0xffffffffu, n, o);
+            tiles = max(n * a.Hk, (int64_t)1);
         }
-        int upto = n;
+    }
+    __device__ __forceinline__ Sequence at(int b) const { return a.B <= 32 ? mine : sequence(a, b); }
+
+    // Items of a sequence with at least w key tiles: those from a token on.
+    __device__ __forceinline__ int items_from(const Sequence &s, int w) const {
+        const int n = (int)(((unsigned)s.nq + TP - 1) / (unsigned)TP);
+        if (w == 0) return n;
+        if (tiles_of(s.nk) < w) return 0;
+        if (!a.causal) return n;
+        // item t's last token sees min(nk, nk - nq + (t + 1) TP) keys: more than (w - 1) kTile
+        const int need = (w - 1) * kTile - s.nk + s.nq;  // (t + 1) TP > need, which is below nq
+        return n - (need < 0 ? 0 : (int)((unsigned)need / (unsigned)TP));
+    }
+    __device__ __forceinline__ int count(int w) const {
+        int n = 0;
+        if (a.B <= 32) n = items_from(mine, w);
+        else for (int b = threadIdx.x & 31; b < a.B; b += 32) n += items_from(at(b), w);
+        return __reduce_add_sync(0xffffffffu, n);
+    }
+    // Tiles from which on an item has a piece p > 0.
+    __device__ __forceinline__ int of_piece(int p) const {
+        const int64_t n = ((p + 1) * tiles + gridDim.x - 1) / gridDim.x;
+        return (int)max(min(n, (int64_t)0x7fffffff), (int64_t)(kLeastPiece * p + 1));
+    }
+
+    // Number `rank` of the line: sequence, head, first token, and piece.
+    __device__ __forceinline__ bool find(int rank, Item &x) const {
+        const int lane = threadIdx.x & 31;
+        int p = 0, n = count(0) * a.Hk;
+        x.unit = rank;
+        while (rank >= n) {
+            if (!a.split || n == 0) return false;
+            rank -= n;
+            n = count(of_piece(++p)) * a.Hk;
+        }
+        x.line = rank;
+        x.piece = p;
+        const int item = rank / a.Hk;
+        x.h = rank - item * a.Hk;
+        int lo = 0, hi = most + 1;  // count(lo) > item >= count(hi)
+        while (hi - lo > 1) {
+            const int mid = lo + (hi - lo) / 2;
+            (count(mid) > item ? lo : hi) = mid;
+        }
+        int left = item - count(lo + 1);  // among the items of lo tiles, by sequence
+        for (int b0 = 0; b0 < a.B; b0 += 32) {
+            int m = 0, t0 = 0;
+            if (b0 + lane < a.B) {
+                const Sequence s = at(b0 + lane);
+                const int all = items_from(s, 0), ge = items_from(s, lo);
+                m = ge - items_from(s, lo + 1);
+                t0 = a.causal ? all - ge : 0;
+            }
+            int upto = m;
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
+            for (int o = 1; o < 32; o *= 2) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned here = __ballot_sync(0xffffffffu, left < upto);
+            if (here) {
+                const int l = __ffs(here) - 1;
+                x.b = b0 + l;
+                x.t = (__shfl_sync(0xffffffffu, t0, l) + left - __shfl_sync(0xffffffffu, upto - m, l)) * TP;
+                return true;
+            }
+            left -= __shfl_sync(0xffffffffu, upto, 31);
         }
-        const unsigned here = __ballot_sync(0xffffffffu, left < upto);
-        if (here) {
-            const int l = __ffs(here) - 1;
-            x.b = b0 + l;
-            x.t = (__shfl_sync(0xffffffffu, t0, l) + (int)left - __shfl_sync(0xffffffffu, upto - n, l)) * TP;
-            return true;
-        }
-        left -= __shfl_sync(0xffffffffu, upto, 31);
+        return false;  // cu_seqlens changed under way
     }
-    return false;  // cu_seqlens changed under way
-}
+
+    // Cuts item x, whose tiles are set, to its piece.
+    __device__ __forceinline__ void cut(Item &x, int streams) const {
+        const int NT = x.tiles;
+        x.pieces = 1;
+        x.base = 0;
+        if (!a.split) return;
+        x.pieces = (int)max(min((int64_t)NT * gridDim.x / tiles, (int64_t)((NT - 1) / kLeastPiece + 1)), (int64_t)1);
+        const int j0 = (int)((int64_t)NT * x.piece / x.pieces), n = (int)((int64_t)NT * (x.piece + 1) / x.pieces) - j0;
+        for (int s = 0; s < streams; s++) x.nt[s] = min(max(x.nt[s] - j0, 0), n);
+        x.tiles = n;
+        x.first = max(x.first - j0, 0);
+        x.base = j0 * kTile;
+    }
+};
 
 // What of shared memory is not tiles.
 template <int DP> struct Small {
@@ -353,6 +417,7 @@ template <int DP, bool F16>
 struct Block {
     using C = Cfg<DP>;
     static constexpr int NQ = C::NQ, LA = C::LA, NU = C::NU, UC = C::UC, NST = C::NST;
+    static constexpr int kPart = kTile * (DP + 2);  // floats of a stream of a piece
 
     const Args &a;
     const uint32_t q_a, ring_a;  // shared memory: queries, ring
@@ -441,7 +506,7 @@ struct Block {
                     mbar_expect_tx(full + at.st, C::STAGE);
 #pragma unroll
                     for (int c = 0; c < UC / 64; c++)
-                        tma_load_4d(ring_a + at.st * C::STAGE + c * kBox, m, u * UC + 64 * c, x.h, x.s.k0 + j * kTile, bb, full + at.st);
+                        tma_load_4d(ring_a + at.st * C::STAGE + c * kBox, m, u * UC + 64 * c, x.h, x.s.k0 + x.base + j * kTile, bb, full + at.st);
                     at.next();
                     round = round || at.st == 0;
                 }
@@ -646,7 +711,7 @@ struct Block {
         for (int it = 0; (item = next<true>(it)); it++) {
             // (rows of no query need no mask: their results go nowhere)
             const int i = item->t + s * a.TQ + tok;
-            const int vis = tok < a.TQ && i < item->s.nq ? visible(a, item->s, i) : 0x7fffffff;
+            const int vis = tok < a.TQ && i < item->s.nq ? visible(a, item->s, i) - item->base : 0x7fffffff;
             Row r{-INFINITY, 0.f};
             const int nt = item->nt[s];
             for (int j = 0; j < nt; j++) {
@@ -668,15 +733,36 @@ struct Block {
         }
     }
 
-    // Outputs of one row.
+    // Outputs of one row, or what they are joined from.
     __device__ __forceinline__ void write(const Item &x, int it, int s, int tok, int head, int nt, const Row &r, uint32_t lanes) const {
         using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
-        const int i = x.t + s * a.TQ + tok, h = x.h * a.G + head;
-        const bool on = tok < a.TQ && i < x.s.nq;
-        const int64_t row = a.cu_q ? x.s.q0 + i : i;
-        T *out = static_cast<T *>(a.out) + (a.cu_q ? 0 : x.b * a.o_sb) + row * a.o_ss + h * a.o_sh;
-        const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
+        const int i = x.t + s * a.TQ + tok, h = x.h * a.G + head, row = threadIdx.x & 127;
+        const bool on = tok < a.TQ && i < x.s.nq, cut = x.pieces > 1;
+        const int64_t at = a.cu_q ? x.s.q0 + i : i;
+        T *out = static_cast<T *>(a.out) + (a.cu_q ? 0 : x.b * a.o_sb) + at * a.o_ss + h * a.o_sh;
+        auto store = [&](float *o, int c, float inv, bool zero) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = zero ? 0u : pack2<F16>(o[k + 2 * e] * inv, o[k + 2 * e + 1] * inv);
+                if (a.o_vec) {
+                    *reinterpret_cast<uint4 *>(out + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        reinterpret_cast<uint16_t *>(out)[c + k + 2 * e] = (uint16_t)w[e];
+                        reinterpret_cast<uint16_t *>(out)[c + k + 2 * e + 1] = (uint16_t)(w[e] >> 16);
+                    }
+                }
+            }
+        };
+        auto log_sum = [&](float ref, float l) {
+            if (on && a.lse)
+                a.lse[(a.cu_q ? at : (int64_t)x.b * a.Sq + i) * a.Hq + h] = l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.693147180559945309f;
+        };
         const bool fix = nt && *reinterpret_cast<volatile int *>(small->bad + (it & 1)) == it + 1;
+        float *part = a.parts + ((int64_t)x.unit * NQ + s) * kPart + row;  // columns of 128 rows, then references and sums
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
             if (c >= a.D) break;
@@ -687,37 +773,70 @@ struct Block {
             }
             if (fix && on) {  // values of the masked tiles that are no numbers
                 const T *v = static_cast<const T *>(a.v) + (a.cu_q ? 0 : x.b * a.v_sb) + x.h * a.v_sh + c;
-                for (int j = x.first * kTile, n = visible(a, x.s, i); j < n; j++)
+                for (int j = x.base + x.first * kTile, n = min(visible(a, x.s, i), x.base + nt * kTile); j < n; j++)
 #pragma unroll
                     for (int k = 0; k < 32; k++) {
                         const float y = Elem<T>::to_f32(v[(int64_t)(x.s.k0 + j) * a.v_ss + k]);
                         if (!(fabsf(y) < INFINITY)) o[k] += y;
                     }
             }
-            if (on) {
+            if (cut) {
+                if (nt)
 #pragma unroll
-                for (int k = 0; k < 32; k += 8) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        w[e] = r.l == 0.f ? 0u : pack2<F16>(o[k + 2 * e] * inv, o[k + 2 * e + 1] * inv);
-                    if (a.o_vec) {
-                        *reinterpret_cast<uint4 *>(out + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            reinterpret_cast<uint16_t *>(out)[c + k + 2 * e] = (uint16_t)w[e];
-                            reinterpret_cast<uint16_t *>(out)[c + k + 2 * e + 1] = (uint16_t)(w[e] >> 16);
-                        }
-                    }
-                }
+                    for (int k = 0; k < 32; k++) part[(c + k) * kTile] = o[k];
+            } else if (on) {
+                store(o, c, r.l == 0.f ? 0.f : 1.f / r.l, r.l == 0.f);
             }
         }
         tc_fence_before();
-        if (on && a.lse) {
-            const int64_t at = ((a.cu_q ? row : (int64_t)x.b * a.Sq + i)) * a.Hq + h;
-            a.lse[at] = r.l == 0.f ? -INFINITY : (r.ref + log2f(r.l)) * 0.693147180559945309f;
+        if (!cut) {
+            log_sum(r.ref, r.l);
+            return;
         }
+        // The warp that is the last one of its rows joins the pieces, in order.
+        part[DP * kTile] = r.ref;
+        part[(DP + 1) * kTile] = nt ? r.l : 0.f;
+        int last = 0;
+        int *slots = a.slots + x.line * kMaxPieces;
+        if ((threadIdx.x & 31) == 0) slots[x.piece] = x.unit;
+        __threadfence();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) {
+            int *counter = a.counters + (x.line * 2 + s) * 4 + (row >> 5);
+            last = atomicAdd(counter, 1) == x.pieces - 1;
+            if (last) *counter = 0;
+            __threadfence();
+        }
+        if (!__shfl_sync(0xffffffffu, last, 0)) return;
+        auto of = [&](int p) { return a.parts + ((int64_t)__ldcg(slots + p) * NQ + s) * kPart + row; };
+        float ref = -INFINITY, l = 0.f;
+        for (int p = 0; p < x.pieces; p++) {
+            const float *z = of(p);
+            if (__ldcg(z + (DP + 1) * kTile) != 0.f) ref = fmaxf(ref, __ldcg(z + DP * kTile));
+        }
+        auto factor = [&](const float *z) {  // references are whole numbers
+            const float e = __ldcg(z + DP * kTile);
+            return e == ref ? 1.f : exp2_fast(e - ref);
+        };
+        for (int p = 0; p < x.pieces; p++) {
+            const float *z = of(p), y = __ldcg(z + (DP + 1) * kTile);
+            if (y != 0.f) l = fmaf(y, factor(z), l);
+        }
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+            if (c >= a.D) break;
+            float o[32] = {};
+#pragma unroll 1
+            for (int p = 0; p < x.pieces; p++) {
+                const float *z = of(p);
+                if (__ldcg(z + (DP + 1) * kTile) == 0.f) continue;
+                const float f = factor(z);
+#pragma unroll
+                for (int k = 0; k < 32; k++) o[k] = fmaf(__ldcg(z + (c + k) * kTile), f, o[k]);
+            }
+            if (on) store(o, c, l == 0.f ? 0.f : 1.f / l, l == 0.f);
+        }
+        log_sum(ref, l);
     }
 
     // ------------------------------------------------------------- helper warps
@@ -725,20 +844,14 @@ struct Block {
     __device__ __forceinline__ void help(int w) {
         const int lane = threadIdx.x & 31;
         int64_t pos = 0;  // where the item's tiles begin
-        const int TP = NQ * a.TQ;
-        int most = 0;
-        if (w == 0) {
-            for (int b = lane; b < a.B; b += 32) most = max(most, tiles_of(sequence(a, b).nk));
-            most = __reduce_max_sync(0xffffffffu, most);
-        }
+        const Line line(a, NQ * a.TQ);
         auto publish = [&](int it) {
             const int slot = it % kItems;
             if (it >= kItems && !wait_warp(small->item_empty + slot, (it / kItems - 1) & 1)) return false;
-            const int64_t n = gridDim.x, c = blockIdx.x, rank = it * n + (it & 1 ? n - 1 - c : c);
+            const int n = gridDim.x, c = blockIdx.x;
             Item x{};
-            x.valid = find_item(a, rank / a.Hk, TP, most, x);
+            x.valid = line.find(it * n + (it & 1 ? n - 1 - c : c), x);
             if (x.valid) {
-                x.h = (int)(rank % a.Hk);
                 x.s = sequence(a, x.b);
                 for (int s = 0; s < NQ; s++) {
                     const int t0 = x.t + s * a.TQ;
@@ -746,6 +859,7 @@ struct Block {
                 }
                 x.tiles = max(x.nt[0], x.nt[1]);
                 x.first = visible(a, x.s, x.t) / kTile;
+                line.cut(x, NQ);
             }
             if (lane == 0) {
                 small->items[slot] = x;
@@ -921,7 +1035,7 @@ bool walkable(const void *p, int64_t sb, int64_t nb, int64_t ss, int64_t ns, int
 }
 
 template <int DP, bool F16>
-int launch(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const Args &a, int64_t items, cudaStream_t st) {
+int launch(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const Args &a, int64_t blocks, cudaStream_t st) {
     using C = Cfg<DP>;
     constexpr int smem = C::NQ * C::QB + C::NST * C::STAGE + (int)sizeof(Small<DP>);
     static_assert(smem <= 232448, "shared memory");
@@ -942,7 +1056,6 @@ int launch(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, 
         }
         ready[dev] = true;
     }
-    const int64_t blocks = items < num_sms() ? items : num_sms();
     prompt_kernel<DP, F16><<<(unsigned)blocks, C::THREADS, smem, st>>>(mq, mk, mv, a);
     return check_launch("prompt_attn");
 }
@@ -954,8 +1067,25 @@ int launch(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, 
 using namespace fc;
 using namespace fc::prompt;
 
+namespace {
+// Tokens of an item, and a bound of the number of (item, head), whatever the lengths.
+int64_t item_tokens(int64_t D, int64_t G) { return (D <= 128 ? 2 : 1) * (kTile / G); }
+int64_t most_items(int64_t B, int64_t Tq, int64_t Hk, int64_t TP) {
+    const int64_t n = (Tq / TP + B) * Hk;
+    return n > 0 ? n : 1;
+}
+// Items are cut along their keys where they are fewer than blocks; there are at most twice as many pieces as blocks then.
+int64_t parts_bytes(int64_t D, int64_t items) {
+    const int64_t DP = D <= 64 ? 64 : D <= 128 ? 128 : D;
+    return items < num_sms() ? 2 * (int64_t)num_sms() * (D <= 128 ? 2 : 1) * kTile * (DP + 2) * 4 : 0;
+}
+constexpr int64_t kSlotsBytes = (int64_t)kMaxPieces * kMaxPieces * 4;
+}  // namespace
+
 extern "C" size_t fc_prompt_attn_workspace_size(int64_t B, int64_t Tq, int64_t Hq, int64_t Hk, int64_t D) {
-    return kWsHeader + kWsUnits * 4;
+    if (Hk <= 0 || Hq < Hk || Hq / Hk > kTile) return kWsHeader + kWsUnits * 4;
+    const int64_t parts = parts_bytes(D, most_items(B, Tq, Hk, item_tokens(D, Hq / Hk)));
+    return (size_t)(kWsHeader + kWsUnits * 4 + (parts ? kSlotsBytes + parts : 0));
 }
 
 extern "C" int fc_prompt_attn(const void *q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const void *k, int64_t k_sb,
@@ -1036,16 +1166,21 @@ extern "C" int fc_prompt_attn(const void *q, int64_t q_sb, int64_t q_ss, int64_t
         ok = ok && encode(&mk, f16, Tk ? k : q, 4, kd, ks, kb) && encode(&mv, f16, Tk ? v : q, 4, kd, vs, kb);
         if (!ok) { set_error("prompt_attn: the tensor maps cannot be made"); return FC_ECUDA; }
     }
-    // no more items than this, whatever the lengths
-    auto items = [&](int nqt) {
-        const int64_t TP = (int64_t)nqt * a.TQ;
-        const int64_t n = (cu_seqlens_q ? Tq / TP + B : B * ((Sq + TP - 1) / TP)) * Hk;
-        return n > 0 ? n : one;
-    };
+    const int64_t items = most_items(B, Tq, Hk, item_tokens(D, a.G));
+    if (items > 0x3fffffff) { set_error("prompt_attn: too many rows"); return FC_ENOTSUP; }
+    // (blocks for pieces: one an SM, where the keys are long enough to be cut at all)
+    const int sms = num_sms() < kMaxPieces ? num_sms() : kMaxPieces;
+    const int64_t keys = cu_seqlens_q ? Tk : Sk;
+    a.split = items < num_sms() && keys > kLeastPiece * kTile;
+    char *ws = static_cast<char *>(workspace) + kWsHeader;
+    a.counters = reinterpret_cast<int *>(ws);
+    a.slots = reinterpret_cast<int *>(ws + kWsUnits * 4);
+    a.parts = reinterpret_cast<float *>(ws + kWsUnits * 4 + kSlotsBytes);
+    const int64_t blocks = a.split ? sms : items < num_sms() ? items : num_sms();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto go = [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
-        return f16 ? launch<DP, true>(mq, mk, mv, a, items(Cfg<DP>::NQ), st) : launch<DP, false>(mq, mk, mv, a, items(Cfg<DP>::NQ), st);
+        return f16 ? launch<DP, true>(mq, mk, mv, a, blocks, st) : launch<DP, false>(mq, mk, mv, a, blocks, st);
     };
     if (D == 64) return go(std::integral_constant<int, 64>());
     if (D <= 128) return go(std::integral_constant<int, 128>());

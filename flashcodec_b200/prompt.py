@@ -22,7 +22,10 @@ def _walkable(name, t):
     if t.stride(-1) != 1:
         raise ValueError(f"{name}: the head dim must have unit stride")
     step = 16 // t.element_size()
-    if t.data_ptr() % 16 or any(n > 1 and (st <= 0 or st % step) for n, st in zip(t.shape[:-1], t.stride()[:-1])):
+    bad = t.data_ptr() % 16
+    for n, st in zip(t.shape[:-1], t.stride()):
+        bad = bad or (n > 1 and (st <= 0 or st % step))
+    if bad:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -49,46 +52,47 @@ def prompt_attention(q, k, v, cu_seqlens=None, cu_seqlens_k=None, *, causal=True
     Scores, softmax and sums are fp32; weights are rounded to q's dtype before they
     meet the values.  It serves and has no gradient.
     """
-    K.require_cuda(q, k, v, cu_seqlens, cu_seqlens_k, out)
+    index, grad = q.get_device(), torch.is_grad_enabled()
     dual = getattr(forward_ad, "_current_level", 0) >= 0  # inside a dual level
-    for t in (q, k, v, out):
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out), ("cu_seqlens", cu_seqlens),
+                    ("cu_seqlens_k", cu_seqlens_k)):
         if t is None:
             continue
-        if torch.is_grad_enabled() and t.requires_grad:
+        if t.get_device() != index or index < 0:
+            K.require_cuda(q, t)
+            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+        if grad and t.requires_grad:
             raise RuntimeError("prompt_attention has no gradient: call it under torch.no_grad()")
         if dual and forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError("prompt_attention has no tangent: pass the primal of a dual tensor")
-    for name, t in (("k", k), ("v", v), ("cu_seqlens", cu_seqlens), ("cu_seqlens_k", cu_seqlens_k), ("out", out)):
-        if t is not None and t.device != q.device:
-            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
     packed = cu_seqlens is not None
-    if q.dim() != (3 if packed else 4):
+    shape, keys, dtype = q.shape, k.shape, q.dtype
+    if len(shape) != (3 if packed else 4):
         raise ValueError("q must be (T, heads, D) with cu_seqlens or (B, S, heads, D) without "
-                         f"(got {tuple(q.shape)})")
-    if k.dim() != q.dim() or k.shape != v.shape or k.shape[-1] != q.shape[-1] or 0 in (q.shape[-2], k.shape[-2]) \
-            or (not packed and k.shape[0] != q.shape[0]):
-        raise ValueError(f"k and v must be alike and go with q (got {tuple(k.shape)}, {tuple(v.shape)} "
-                         f"and {tuple(q.shape)})")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+                         f"(got {tuple(shape)})")
+    if len(keys) != len(shape) or keys != v.shape or keys[-1] != shape[-1] or shape[-2] == 0 or keys[-2] == 0 \
+            or (not packed and keys[0] != shape[0]):
+        raise ValueError(f"k and v must be alike and go with q (got {tuple(keys)}, {tuple(v.shape)} "
+                         f"and {tuple(shape)})")
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError("q, k and v must have one dtype")
-    if cu_seqlens_k is not None and not packed:
+    if packed:
+        for name, t in (("cu_seqlens", cu_seqlens), ("cu_seqlens_k", cu_seqlens_k)):
+            if t is not None and (t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] < 1
+                                  or t.shape != cu_seqlens.shape or not t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous int32 tensor of one entry more than sequences "
+                                 f"(got {t.dtype}, {tuple(t.shape)})")
+        if cu_seqlens_k is None and keys[0] != shape[0]:
+            raise ValueError(f"{keys[0]} keys for {shape[0]} queries need cu_seqlens_k")
+    elif cu_seqlens_k is not None:
         raise ValueError("cu_seqlens_k goes with cu_seqlens")
-    if packed and cu_seqlens_k is None and k.shape[0] != q.shape[0]:
-        raise ValueError(f"{k.shape[0]} keys for {q.shape[0]} queries need cu_seqlens_k")
-    for name, t in (("cu_seqlens", cu_seqlens), ("cu_seqlens_k", cu_seqlens_k)):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < 1
-                              or t.shape != cu_seqlens.shape or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous int32 tensor of one entry more than sequences "
-                             f"(got {t.dtype}, {tuple(t.shape)})")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError("out must have the shape and dtype of q")
-    if out.stride(-1) != 1:
-        raise ValueError("out: the head dim must have unit stride")
+    elif out.shape != shape or out.dtype is not dtype or out.stride(-1) != 1:
+        raise ValueError("out must have the shape and dtype of q, and unit stride along the head dim")
     q, k, v = _walkable("q", q), _walkable("k", k), _walkable("v", v)
-    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
-    K.prompt_attn(q, k, v, cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, causal,
+    lse = torch.empty(shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+    K.prompt_attn(q, k, v, cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, bool(causal),
                   q.shape[-1] ** -0.5 if scale is None else float(scale), out, lse)
     return (out, lse) if return_lse else out
 

@@ -342,3 +342,42 @@ def test_refusals():
     with pytest.raises(NotImplementedError):
         f(big, k[:, :1], v[:, :1], c)
 
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 96, 128, 192, 256])
+def test_cut_along_keys(D, dtype):
+    """Few queries over many keys: blocks share a query tile's keys and the last one joins the results."""
+    lens = [(70, 6000), (3, 2500), (1, 9000), (40, 40), (0, 100)]
+    q, k, v = make(lens, 4, 2, D, dtype)
+    want = check(q, k, v, lens, dtype)
+    args = (q, k, v, cu([n for n, _ in lens]), cu([m for _, m in lens]))
+    for _ in range(3):  # whichever block comes last, the same bits
+        assert torch.equal(fc().prompt_attention(*args), want)
+    check(q, k, v, lens, dtype, causal=False)
+
+
+def test_cut_rows_that_see_little():
+    """Pieces that a row does not see, and rows that see nothing at all."""
+    lens = [(2000, 1500), (300, 4000)]
+    check(*make(lens, 2, 1, 64, "bf16"), lens, "bf16")
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_no_numbers_in_pieces(D):
+    """Of a key tile in the middle, and of one that is not seen by all."""
+    n, m = 40, 5000
+    q, k, v = make([(n, m)], 4, 2, D, "bf16")
+    args = (cu([n]), cu([m]))
+    want = fc().prompt_attention(q, k, v, *args)
+    y = v.clone()
+    y[m - 10, 0] = math.nan  # seen by the last 10 queries
+    out = fc().prompt_attention(q, k, y, *args)
+    assert torch.equal(out[:, 2:], want[:, 2:]) and torch.equal(out[: n - 10, :2], want[: n - 10, :2])
+    assert out[n - 10 + 0:, :2].isnan().all()
+    y = v.clone()
+    y[1000, 1, 7] = math.inf  # seen by all
+    out = fc().prompt_attention(q, k, y, *args)
+    assert torch.equal(out[:, :2], want[:, :2]) and (out[:, 2:, 7] == math.inf).all()
+    same = [d for d in range(D) if d != 7]
+    assert torch.equal(out[:, 2:][..., same], want[:, 2:][..., same])

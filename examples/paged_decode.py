@@ -1,16 +1,17 @@
-"""Continuous batching on the paged 4-bit KV cache.
+"""Continuous batching on the paged KV caches.
 
 Sequences of different lengths share one pool of pages per layer; they join with a
 prompt, grow by a token a step and leave their pages to the next one.  The layers
 are attention blocks with random weights (query and key norms, rotary positions,
-grouped heads): enough to run the four operations as a serving loop does.
+grouped heads): enough to run the operations as a serving loop does.
 
-    append   prompts packed into one call, then one token per sequence and step
-    read     the held keys and values of a prompt, for the prompt's own attention
-    attend   every step's attention, over the pages
-    select   from `sparse_from` tokens on, the pages to attend to
+    append            prompts packed into one call, then one token per sequence and step
+    read              the held keys and values of a prompt, for the prompt's own attention
+    prompt_attention  that attention, all prompts in one call
+    attend            every step's attention, over the pages
+    select            from `sparse_from` tokens on, the pages to attend to (4 bits)
 
-    python examples/paged_decode.py [--layers 4] [--steps 32] [--sparse-from 512]
+    python examples/paged_decode.py [--bits 4] [--layers 4] [--steps 32] [--sparse-from 512]
 """
 
 from __future__ import annotations
@@ -23,7 +24,7 @@ import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
-from flashcodec_b200 import PagedInt4Cache, rotary_table  # noqa: E402
+from flashcodec_b200 import PagedInt4Cache, PagedInt8Cache, prompt_attention, rotary_table  # noqa: E402
 
 
 class Pages:
@@ -47,14 +48,17 @@ class Pages:
 
 
 class Layer:
-    def __init__(self, hq, hk, d, pages, page_size, device, gen):
+    def __init__(self, hq, hk, d, pages, page_size, device, gen, bits):
         w = hq * d
         self.hq, self.hk, self.d = hq, hk, d
         self.qkv = torch.randn((hq + 2 * hk) * d, w, generator=gen, device=device).bfloat16() * w ** -0.5
         self.out = torch.randn(w, w, generator=gen, device=device).bfloat16() * w ** -0.5
         self.q_norm = torch.ones(d, device=device, dtype=torch.bfloat16)
         self.k_norm = torch.ones(d, device=device, dtype=torch.bfloat16)
-        self.cache = PagedInt4Cache(pages, hk, d, page_size=page_size, bounds=True, device=device)
+        if bits == 4:
+            self.cache = PagedInt4Cache(pages, hk, d, page_size=page_size, bounds=True, device=device)
+        else:
+            self.cache = PagedInt8Cache(pages, hk, d, page_size=page_size, device=device)
 
     def heads(self, x):
         y = (x @ self.qkv.t()).unflatten(-1, (-1, self.d))
@@ -68,17 +72,12 @@ class Layer:
     def prompt(self, q, table, cu, starts):
         """Causal attention of packed prompts over what the cache holds of them."""
         k, v = self.cache.read(table, starts, count=q.shape[0], cu_seqlens=cu, dtype=q.dtype)
-        outs = []
-        for a, b in zip(cu.tolist(), cu.tolist()[1:]):
-            o = torch.nn.functional.scaled_dot_product_attention(
-                *(t[a:b].transpose(0, 1)[None] for t in (q, k, v)), is_causal=True, enable_gqa=True)
-            outs.append(o[0].transpose(0, 1))
-        return torch.cat(outs)
+        return prompt_attention(q, k, v, cu)
 
 
 @torch.no_grad()
 def run(layers=4, steps=32, prompts=(37, 5, 700, 129), hq=16, hk=8, d=128, page_size=64,
-        sparse_from=512, count=6, seed=0):
+        sparse_from=512, count=6, seed=0, bits=4):
     """Returns the largest relative difference between a step's attention and the same
     attention computed from the values that the cache holds (dense steps)."""
     dev = torch.device("cuda", torch.cuda.current_device())
@@ -86,7 +85,7 @@ def run(layers=4, steps=32, prompts=(37, 5, 700, 129), hq=16, hk=8, d=128, page_
     rows, most = len(prompts), max(prompts) + steps + 1
     width = -(-most // page_size)
     num_pages = rows * width
-    stack = [Layer(hq, hk, d, num_pages, page_size, dev, gen) for _ in range(layers)]
+    stack = [Layer(hq, hk, d, num_pages, page_size, dev, gen, bits) for _ in range(layers)]
     pages = Pages(num_pages, rows, width, page_size, dev)
     rotary = rotary_table(most, d, base=1e6, device=dev)
 
@@ -108,13 +107,13 @@ def run(layers=4, steps=32, prompts=(37, 5, 700, 129), hq=16, hk=8, d=128, page_
         lens = [n + step + 1 for n in prompts]
         for r, n in enumerate(lens):
             pages.hold(r, n)
-        sparse = max(lens) >= sparse_from and step % 2  # every other step, to show both
+        sparse = bits == 4 and max(lens) >= sparse_from and step % 2  # every other step, to show both
         after = lengths + 1
         x = torch.nn.functional.normalize(x.float(), dim=-1).mul(x.shape[-1] ** 0.5).bfloat16()
         for i, layer in enumerate(stack):
             q = layer.put(x, pages.table, lengths, rotary)
             chosen = layer.cache.select(q, pages.table, after, count) if sparse else None
-            o = layer.cache.attend(q, pages.table, after, selected=chosen)
+            o = layer.cache.attend(q, pages.table, after, **({"selected": chosen} if sparse else {}))
             if step == (steps - 1) // 2 * 2 and i == layers - 1:  # the last dense step
                 worst = max(worst, check(layer, q, o, pages.table, lens))
             x = x + o.flatten(1) @ layer.out.t()
@@ -143,7 +142,8 @@ if __name__ == "__main__":
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--steps", type=int, default=32)
     ap.add_argument("--sparse-from", type=int, default=512)
+    ap.add_argument("--bits", type=int, choices=(4, 8), default=4)
     args = ap.parse_args()
-    err = run(layers=args.layers, steps=args.steps, sparse_from=args.sparse_from)
+    err = run(layers=args.layers, steps=args.steps, sparse_from=args.sparse_from, bits=args.bits)
     print(f"{args.layers} layers, {args.steps} steps: attention over the pages differs from the held values' "
           f"by {err:.2e} (relative)")

@@ -541,3 +541,16 @@ def test_a_prompt_in_chunks():
             err = np.abs(out[b].double().cpu().numpy() - want[0])
             assert (err <= 2.0 ** -8 * np.abs(want[0]) + SLACK["bf16"] * np.abs(v).max()).all()
     cache.check()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_the_serving_example(bits):
+    """Prompts by prompt_attention, steps on either cache: the last dense step differs from the attention
+    computed from the values held by bf16's roundings (norms of a head's outputs: half a step, 2^-8, at most)."""
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parents[1] / "examples" / "paged_decode.py"
+    spec = importlib.util.spec_from_file_location("paged_decode", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.run(layers=2, steps=5, prompts=(37, 5, 300), bits=bits) < 2.0 ** -7

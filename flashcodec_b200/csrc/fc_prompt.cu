@@ -82,6 +82,7 @@ struct Args {
 constexpr int kTile = 128;          // rows of a query tile, keys of a tile
 constexpr int kBox = kTile * 128;   // bytes of 128 rows of 64 channels
 constexpr int kItems = 3;           // items known ahead
+constexpr uint64_t kItemNs = 100 * kWaitNs;  // bound on waits for an item
 constexpr int kMaxPieces = 256;     // of an item: no more than blocks
 constexpr int kPolyStep = 4;        // every kPolyStep-th pair of weights is a polynomial
 
@@ -291,7 +292,9 @@ constexpr int kLeastPiece = 8;
 // The line of work, as a warp finds its way on it.  Items (sequence, TP tokens) come by their number of
 // tiles, the ones of most first, items of none last.  Where there are fewer than blocks they are cut
 // along their keys, into P = NT * blocks / (all tiles) pieces each, at least 1, and all items' first pieces
-// come first, then the second ones of those that have two, and so on.
+// come first, then the second ones of those that have two, and so on.  More sequences than a warp has lanes
+// are not sorted: counting them took longer than the items of 1000 short ones.  Their items are numbered by
+// where the tokens lie, some numbers being left out.
 struct Line {
     const Args &a;
     int TP, most;
@@ -300,21 +303,17 @@ struct Line {
 
     __device__ __forceinline__ Line(const Args &args, int tp) : a(args), TP(tp), most(0), mine{}, tiles(1) {
         const int lane = threadIdx.x & 31;
+        if (a.B > 32) return;
         if (lane < a.B) mine = sequence(a, lane);
-        for (int b = lane; b < a.B; b += 32) most = max(most, tiles_of(at(b).nk));
-        most = __reduce_max_sync(0xffffffffu, most);
+        most = __reduce_max_sync(0xffffffffu, tiles_of(mine.nk));
         if (a.split) {
             int64_t n = 0;
-            for (int b = lane; b < a.B; b += 32) {
-                const Sequence s = at(b);
-                for (int t = TP; t - TP < s.nq; t += TP) n += tiles_of(visible(a, s, min(t, s.nq) - 1));
-            }
+            for (int t = TP; t - TP < mine.nq; t += TP) n += tiles_of(visible(a, mine, min(t, mine.nq) - 1));
 #pragma unroll
             for (int o = 16; o; o /= 2) n += __shfl_xor_sync(0xffffffffu, n, o);
             tiles = max(n * a.Hk, (int64_t)1);
         }
     }
-    __device__ __forceinline__ Sequence at(int b) const { return a.B <= 32 ? mine : sequence(a, b); }
 
     // Items of a sequence with at least w key tiles: those from a token on.
     __device__ __forceinline__ int items_from(const Sequence &s, int w) const {
@@ -327,10 +326,7 @@ struct Line {
         return n - (need < 0 ? 0 : (int)((unsigned)need / (unsigned)TP));
     }
     __device__ __forceinline__ int count(int w) const {
-        int n = 0;
-        if (a.B <= 32) n = items_from(mine, w);
-        else for (int b = threadIdx.x & 31; b < a.B; b += 32) n += items_from(at(b), w);
-        return __reduce_add_sync(0xffffffffu, n);
+        return __reduce_add_sync(0xffffffffu, items_from(mine, w));
     }
     // Tiles from which on an item has a piece p > 0.
     __device__ __forceinline__ int of_piece(int p) const {
@@ -338,11 +334,28 @@ struct Line {
         return (int)max(min(n, (int64_t)0x7fffffff), (int64_t)(kLeastPiece * p + 1));
     }
 
-    // Number `rank` of the line: sequence, head, first token, and piece.
+    // Number `rank` of the line: sequence, head, first token (behind the last one: nothing to do), and piece.
     __device__ __forceinline__ bool find(int rank, Item &x) const {
         const int lane = threadIdx.x & 31;
-        int p = 0, n = count(0) * a.Hk;
         x.unit = rank;
+        if (a.B > 32) {
+            const int item = rank / a.Hk;
+            x.h = rank - item * a.Hk;
+            if (!a.cu_q) {
+                const int each = (a.Sq + TP - 1) / TP;
+                x.b = item / max(each, 1);
+                x.t = (item - x.b * each) * TP;
+                return x.b < a.B;
+            }
+            // a sequence of n tokens has at most n / TP + 1 items: numbers from cu / TP + b on are its own
+            if (item >= a.Tq / TP + a.B) return false;
+            const int *cu = a.cu_q, tp = TP, T = a.Tq;
+            x.b = kv4::warp_find([=](int i) { return (int64_t)(min(max(cu[i], 0), T) / tp) + i; }, a.B, item);
+            const int64_t t = (int64_t)(item - min(max(cu[x.b], 0), T) / tp - x.b) * TP;
+            x.t = (int)min(max(t, (int64_t)0), (int64_t)0x7fffff00);
+            return true;
+        }
+        int p = 0, n = count(0) * a.Hk;
         while (rank >= n) {
             if (!a.split || n == 0) return false;
             rank -= n;
@@ -357,31 +370,20 @@ struct Line {
             const int mid = lo + (hi - lo) / 2;
             (count(mid) > item ? lo : hi) = mid;
         }
-        int left = item - count(lo + 1);  // among the items of lo tiles, by sequence
-        for (int b0 = 0; b0 < a.B; b0 += 32) {
-            int m = 0, t0 = 0;
-            if (b0 + lane < a.B) {
-                const Sequence s = at(b0 + lane);
-                const int all = items_from(s, 0), ge = items_from(s, lo);
-                m = ge - items_from(s, lo + 1);
-                t0 = a.causal ? all - ge : 0;
-            }
-            int upto = m;
+        const int left = item - count(lo + 1);  // among the items of lo tiles, by sequence
+        const int all = items_from(mine, 0), ge = items_from(mine, lo), m = ge - items_from(mine, lo + 1);
+        const int t0 = a.causal ? all - ge : 0;
+        int upto = m;
 #pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const int v = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += v;
-            }
-            const unsigned here = __ballot_sync(0xffffffffu, left < upto);
-            if (here) {
-                const int l = __ffs(here) - 1;
-                x.b = b0 + l;
-                x.t = (__shfl_sync(0xffffffffu, t0, l) + left - __shfl_sync(0xffffffffu, upto - m, l)) * TP;
-                return true;
-            }
-            left -= __shfl_sync(0xffffffffu, upto, 31);
+        for (int o = 1; o < 32; o *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
         }
-        return false;  // cu_seqlens changed under way
+        const unsigned here = __ballot_sync(0xffffffffu, left < upto);
+        if (!here) return false;
+        x.b = __ffs(here) - 1;
+        x.t = (__shfl_sync(0xffffffffu, t0, x.b) + left - __shfl_sync(0xffffffffu, upto - m, x.b)) * TP;
+        return true;
     }
 
     // Cuts item x, whose tiles are set, to its piece.
@@ -430,13 +432,14 @@ struct Block {
           small(reinterpret_cast<Small<DP> *>(smem + NQ * C::QB + NST * C::STAGE)) {}
 
     // Every wait is bounded; one that gives up records the launch and ends the block's work.
-    __device__ __forceinline__ bool wait(uint64_t *bar, unsigned parity) const {
+    // (What waits for the end of an item has more time: kWaitNs are 60,000 tiles.)
+    __device__ __forceinline__ bool wait(uint64_t *bar, unsigned parity, uint64_t limit = kWaitNs) const {
         if (mbar_try_wait(bar, parity)) return true;
         const uint64_t t0 = global_ns();
         for (;;) {
             if (mbar_try_wait_sleep(bar, parity, 20000)) return true;
             if (*static_cast<volatile int *>(&small->abort_s)) return false;
-            if (global_ns() - t0 > kWaitNs) {
+            if (global_ns() - t0 > limit) {
                 atomicMax(a.status, a.epoch);
                 *static_cast<volatile int *>(&small->abort_s) = 1;
                 return false;
@@ -445,15 +448,16 @@ struct Block {
     }
 
     // The same for a whole warp, which goes on or gives up together.
-    __device__ __forceinline__ bool wait_warp(uint64_t *bar, unsigned parity) const {
-        return __all_sync(0xffffffffu, wait(bar, parity));
+    __device__ __forceinline__ bool wait_warp(uint64_t *bar, unsigned parity, uint64_t limit = kWaitNs) const {
+        return __all_sync(0xffffffffu, wait(bar, parity, limit));
     }
 
     // Item `it`, in the ring of items until its readers are done with it; null: no more work, or given up.
     template <bool WARP>
     __device__ __forceinline__ const Item *next(int it) const {
         const int slot = it % kItems;
-        if (!(WARP ? wait_warp(small->item_full + slot, (it / kItems) & 1) : wait(small->item_full + slot, (it / kItems) & 1))) return nullptr;
+        const unsigned parity = (it / kItems) & 1;
+        if (!(WARP ? wait_warp(small->item_full + slot, parity, kItemNs) : wait(small->item_full + slot, parity, kItemNs))) return nullptr;
         return small->items[slot].valid ? small->items + slot : nullptr;
     }
     template <bool WARP>
@@ -847,12 +851,13 @@ struct Block {
         const Line line(a, NQ * a.TQ);
         auto publish = [&](int it) {
             const int slot = it % kItems;
-            if (it >= kItems && !wait_warp(small->item_empty + slot, (it / kItems - 1) & 1)) return false;
+            if (it >= kItems && !wait_warp(small->item_empty + slot, (it / kItems - 1) & 1, kItemNs)) return false;
             const int n = gridDim.x, c = blockIdx.x;
             Item x{};
             x.valid = line.find(it * n + (it & 1 ? n - 1 - c : c), x);
             if (x.valid) {
                 x.s = sequence(a, x.b);
+                x.t = min(x.t, x.s.nq);
                 for (int s = 0; s < NQ; s++) {
                     const int t0 = x.t + s * a.TQ;
                     x.nt[s] = t0 < x.s.nq ? tiles_of(visible(a, x.s, min(t0 + a.TQ, x.s.nq) - 1)) : 0;
@@ -883,7 +888,7 @@ struct Block {
                     // it can be missed, and none passed by a warp that is ahead.)
                     const unsigned parity = seen >> st & 1;
                     seen ^= 1u << st;
-                    if (!wait_warp(small->v_raw + st, parity)) return;
+                    if (!wait_warp(small->v_raw + st, parity, kItemNs)) return;
                     uint4 *v = reinterpret_cast<uint4 *>(ring + st * C::STAGE) + w * 32 + lane;
                     constexpr uint32_t E = F16 ? 0x7c007c00u : 0x7f807f80u, ONE = F16 ? 0x04000400u : 0x00800080u;
 #pragma unroll 4
@@ -1171,7 +1176,7 @@ extern "C" int fc_prompt_attn(const void *q, int64_t q_sb, int64_t q_ss, int64_t
     // (blocks for pieces: one an SM, where the keys are long enough to be cut at all)
     const int sms = num_sms() < kMaxPieces ? num_sms() : kMaxPieces;
     const int64_t keys = cu_seqlens_q ? Tk : Sk;
-    a.split = items < num_sms() && keys > kLeastPiece * kTile;
+    a.split = items < num_sms() && B <= 32 && keys > kLeastPiece * kTile;
     char *ws = static_cast<char *>(workspace) + kWsHeader;
     a.counters = reinterpret_cast<int *>(ws);
     a.slots = reinterpret_cast<int *>(ws + kWsUnits * 4);

@@ -381,3 +381,19 @@ def test_no_numbers_in_pieces(D):
     assert torch.equal(out[:, :2], want[:, :2]) and (out[:, 2:, 7] == math.inf).all()
     same = [d for d in range(D) if d != 7]
     assert torch.equal(out[:, 2:][..., same], want[:, 2:][..., same])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("B", [31, 32, 33, 700])
+def test_numbers_of_sequences(B, causal):
+    """As many as a warp has lanes, one more, and many; empty ones among them; as a batch too."""
+    rng = np.random.default_rng(B)
+    lens = [(int(n), int(n + m)) for n, m in zip(rng.integers(0, 40, B), rng.integers(0, 60, B))]
+    lens[3], lens[7], lens[-1] = (0, 0), (150, 150), (0, 9)
+    check(*make(lens, 2, 1, 64, "bf16"), lens, "bf16", causal=causal)
+    q, k, v = (torch.randn(B, S, H, 64, device="cuda").bfloat16() for S, H in ((5, 4), (9, 2), (9, 2)))
+    out = fc().prompt_attention(q, k, v, causal=causal)
+    flat = fc().prompt_attention(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), cu([5] * B), cu([9] * B), causal=causal)
+    assert torch.equal(out.flatten(0, 1), flat)
+    want, _ = exact(q[-1], k[-1], v[-1], causal)
+    near(out[-1], want, "bf16", v[-1].abs().max().item())

@@ -97,7 +97,11 @@ template <int DP> struct Cfg {
     
     static constexpr int THREADS = 128 * NQ + 128;
     static constexpr int O_COL = 256;                    // TMEM: scores at 0 and 128, outputs from here
-    static_assert(O_COL + NQ * DP <= 512, "TMEM");
+    // Heads of 64 leave room for weights beside the scores: the next scores are made while these are turned
+    // into weights.  Else weights replace scores.
+    static constexpr bool BESIDE = DP == 64;
+    static constexpr int P_COL = BESIDE ? O_COL + NQ * DP : 0, P_STEP = BESIDE ? 64 : kTile;
+    static_assert(O_COL + NQ * DP + (BESIDE ? NQ * 64 : 0) <= 512, "TMEM");
 };
 
 // ------------------------------------------------------------------------ PTX
@@ -408,6 +412,7 @@ template <int DP> struct Small {
     uint64_t kv_full[C::NST], kv_empty[C::NST], v_raw[C::NST], v_half[C::NST];
     uint64_t q_full[2], q_free[2];  // by stream
     uint64_t s_full[2], p_full[4];  // by score buffer: scores; either half of the weights are there
+    uint64_t s_free[2];             // the scores have been read
     uint64_t o_done[2];             // by stream: a product P V is done
     uint64_t item_full[kItems], item_empty[kItems];
     Item items[kItems];
@@ -531,7 +536,7 @@ struct Block {
     __device__ __forceinline__ void multiply() {
         Place at;
         const uint32_t lead = elect();
-        unsigned q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
+        unsigned q_uses[2] = {0, 0}, p_uses[2] = {0, 0}, f_uses[2] = {0, 0};
         constexpr uint32_t id_o = idesc(UC, F16, 1);
         const uint32_t id_s = idesc(kTile, F16, 0) | (uint32_t)a.negative << 13;
         const uint64_t ring_d = sw128_desc(ring_a), q_d = sw128_desc(q_a);
@@ -583,28 +588,46 @@ struct Block {
                 const Place kp = at;
                 const bool more = j + LA < tiles;
                 if (more) at.skip(NU);
+                auto product = [&](int s) {
+                    if (j >= nt[s]) return true;
+                    const int slot = NQ == 2 ? s : j & 1;
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        if (!wait_warp(small->p_full + 2 * slot + half, p_uses[slot] & 1)) return false;
+                        tc_fence_after();
+                        Place p = vp;
+#pragma unroll
+                        for (int u = 0; u < NU; u++, p.next()) {
+                            const uint64_t vd = ring_d + p.st * (C::STAGE >> 4);
+#pragma unroll
+                            for (int k = 4 * half; k < 4 * half + 4; k++)
+                                mma_ts(lead, tmem + C::O_COL + s * DP + u * UC, tmem + C::P_COL + slot * C::P_STEP + k * 8,
+                                       vd + k * (2048 >> 4), id_o, j > 0 || k > 0);
+                        }
+                    }
+                    p_uses[slot]++;
+                    mma_commit(lead, small->o_done + s);
+                    return true;
+                };
+                if constexpr (C::BESIDE) {
+                    if (more) {
+                        if (!full(kp)) return;
+#pragma unroll
+                        for (int s = 0; s < NQ; s++)
+                            if (j + 1 < nt[s] && (!wait_warp(small->s_free + s, (f_uses[s] + j) & 1) || !scores(s, j + 1, kp))) return;
+                        release(kp);
+                    }
+                    if (!full(vp)) return;
+#pragma unroll
+                    for (int s = 0; s < NQ; s++)
+                        if (!product(s)) return;
+                    release(vp);
+                    continue;
+                }
                 if (!full(vp)) return;
 #pragma unroll
                 for (int s = 0; s < NQ; s++) {
-                    if (j < nt[s]) {
-                        const int slot = NQ == 2 ? s : j & 1;
-#pragma unroll
-                        for (int half = 0; half < 2; half++) {
-                            if (!wait_warp(small->p_full + 2 * slot + half, p_uses[slot] & 1)) return;
-                            tc_fence_after();
-                            Place p = vp;
-#pragma unroll
-                            for (int u = 0; u < NU; u++, p.next()) {
-                                const uint64_t vd = ring_d + p.st * (C::STAGE >> 4);
-#pragma unroll
-                                for (int k = 4 * half; k < 4 * half + 4; k++)
-                                    mma_ts(lead, tmem + C::O_COL + s * DP + u * UC, tmem + slot * kTile + k * 8, vd + k * (2048 >> 4),
-                                           id_o, j > 0 || k > 0);
-                            }
-                        }
-                        p_uses[slot]++;
-                        mma_commit(lead, small->o_done + s);
-                    }
+                    if (!product(s)) return;
                     if (s == NQ - 1) release(vp);
                     if (more) {
                         if (s == 0 && !full(kp)) return;
@@ -613,6 +636,7 @@ struct Block {
                     }
                 }
             }
+            for (int s = 0; s < NQ; s++) f_uses[s] += nt[s];
         }
     }
 
@@ -645,11 +669,16 @@ struct Block {
     // 1400).  The product with V begins when the first 64 keys' weights are there.
     template <bool MASK>
     __device__ __forceinline__ bool tile(Row &r, int s, int slot, uint32_t lanes, int lim, bool first, unsigned o_count) const {
-        const uint32_t at = tmem + lanes + slot * kTile;
+        const uint32_t at = tmem + lanes + slot * kTile, to = tmem + lanes + C::P_COL + slot * C::P_STEP;
         float z[kTile];
 #pragma unroll
         for (int c = 0; c < kTile; c += 32) tmem_ld32(at + c, z + c);
         tmem_landed<kTile>(z);
+        if constexpr (C::BESIDE) {
+            tc_fence_before();
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive(small->s_free + slot);
+        }
         if constexpr (MASK) {
 #pragma unroll
             for (int k = 0; k < kTile; k++) z[k] = k < lim ? z[k] : -INFINITY;
@@ -676,10 +705,14 @@ struct Block {
         float2 sum[2] = {};
         uint32_t w[32];
         weigh<!MASK>(z, off2, w, sum);
-        tmem_st32(at, w);
-        if (moved && !first) {  // O waits for the last product
+        // O, and weights beside the scores, wait for the last product.  So does every tile whose scores came
+        // ahead of it: at most one product may be open when the next is waited for, a parity tells no more apart.
+        if (!first && (C::BESIDE || NQ == 1 || moved)) {
             if (!wait_warp(small->o_done + s, (o_count - 1) & 1)) return false;
             tc_fence_after();
+        }
+        tmem_st32(to, w);
+        if (moved && !first) {
 #pragma unroll 1
             for (int c = 0; c < DP; c += 16) {
                 float o[16];
@@ -693,7 +726,7 @@ struct Block {
         }
         ready(slot, 0);
         weigh<!MASK>(z + 64, off2, w, sum);
-        tmem_st32(at + 32, w);
+        tmem_st32(to + 32, w);
         r.l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         ready(slot, 1);
         return true;
@@ -728,8 +761,6 @@ struct Block {
                     return;
                 o_count++;
             }
-            // scores that come two tiles ahead leave two products open: a parity tells one phase from the next only
-            if (NQ == 1 && nt > 1 && !wait_warp(small->o_done + s, o_count & 1)) return;
             if (nt && !wait_warp(small->o_done + s, (o_count - 1) & 1)) return;
             tc_fence_after();
             write(*item, it, s, tok, head, nt, r, lanes);
@@ -943,6 +974,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             mbar_init(m.s_full + i, 1);
             mbar_init(m.p_full + 2 * i, 4);
             mbar_init(m.p_full + 2 * i + 1, 4);
+            mbar_init(m.s_free + i, 4);
             mbar_init(m.o_done + i, 1);
             m.bad[i] = 0;
         }

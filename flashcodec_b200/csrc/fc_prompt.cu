@@ -775,27 +775,54 @@ struct Block {
         const bool on = tok < a.TQ && i < x.s.nq, cut = x.pieces > 1;
         const int64_t at = a.cu_q ? x.s.q0 + i : i;
         T *out = static_cast<T *>(a.out) + (a.cu_q ? 0 : x.b * a.o_sb) + at * a.o_ss + h * a.o_sh;
+        // 32 columns of the warp's rows, in 16-byte pieces that four lanes exchange: a store then has 64 bytes of
+        // 8 rows each, not 16 of 32 (with those an item's outputs took 3 us).
+        const int lane = threadIdx.x & 31, r4 = lane & 3;
+        T *to[4];
+        unsigned rows = __ballot_sync(0xffffffffu, on) >> (lane & ~3);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            to[k] = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), (lane & ~3) + k));
         auto store = [&](float *o, int c, float inv, bool zero) {
+            uint32_t w[4][4];
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-                uint32_t w[4];
+            for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = zero ? 0u : pack2<F16>(o[k + 2 * e] * inv, o[k + 2 * e + 1] * inv);
-                if (a.o_vec) {
-                    *reinterpret_cast<uint4 *>(out + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
-                } else {
+                for (int e = 0; e < 4; e++)
+                    w[k][e] = zero ? 0u : pack2<F16>(o[8 * k + 2 * e] * inv, o[8 * k + 2 * e + 1] * inv);
+            if (!a.o_vec) {
+                if (on)
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            reinterpret_cast<uint16_t *>(out)[c + 8 * k + 2 * e] = (uint16_t)w[k][e];
+                            reinterpret_cast<uint16_t *>(out)[c + 8 * k + 2 * e + 1] = (uint16_t)(w[k][e] >> 16);
+                        }
+                return;
+            }
+#pragma unroll
+            for (int m = 1; m < 4; m *= 2)  // transposed: piece r4 of the four lanes' rows
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (k & m) continue;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        reinterpret_cast<uint16_t *>(out)[c + k + 2 * e] = (uint16_t)w[e];
-                        reinterpret_cast<uint16_t *>(out)[c + k + 2 * e + 1] = (uint16_t)(w[e] >> 16);
+                        const uint32_t give = r4 & m ? w[k][e] : w[k + m][e];
+                        const uint32_t got = __shfl_xor_sync(0xffffffffu, give, m);
+                        if (r4 & m) w[k][e] = got;
+                        else w[k + m][e] = got;
                     }
                 }
-            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (rows >> k & 1) *reinterpret_cast<uint4 *>(to[k] + c + 8 * r4) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
         };
         auto log_sum = [&](float ref, float l) {
             if (on && a.lse)
                 a.lse[(a.cu_q ? at : (int64_t)x.b * a.Sq + i) * a.Hq + h] = l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.693147180559945309f;
         };
+        const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
         const bool fix = nt && *reinterpret_cast<volatile int *>(small->bad + (it & 1)) == it + 1;
         float *part = a.parts + ((int64_t)x.unit * NQ + s) * kPart + row;  // columns of 128 rows, then references and sums
 #pragma unroll 1
@@ -815,12 +842,11 @@ struct Block {
                         if (!(fabsf(y) < INFINITY)) o[k] += y;
                     }
             }
-            if (cut) {
-                if (nt)
+            if (!cut) {
+                store(o, c, inv, r.l == 0.f);
+            } else if (nt) {
 #pragma unroll
-                    for (int k = 0; k < 32; k++) part[(c + k) * kTile] = o[k];
-            } else if (on) {
-                store(o, c, r.l == 0.f ? 0.f : 1.f / r.l, r.l == 0.f);
+                for (int k = 0; k < 32; k++) part[(c + k) * kTile] = o[k];
             }
         }
         tc_fence_before();
@@ -869,7 +895,7 @@ struct Block {
 #pragma unroll
                 for (int k = 0; k < 32; k++) o[k] = fmaf(__ldcg(z + (c + k) * kTile), f, o[k]);
             }
-            if (on) store(o, c, l == 0.f ? 0.f : 1.f / l, l == 0.f);
+            store(o, c, l == 0.f ? 0.f : 1.f / l, l == 0.f);
         }
         log_sum(ref, l);
     }

@@ -18,8 +18,9 @@
 // 2^-39 of the row's largest); fp16 and fp32 ones are two fp16 parts (22 bits).
 //
 // Weights.  Base-2 softmax with a running maximum per row, and a running maximum r of the
-// values' scales: weight * scale / r, at most 1, is the fp16 operand (powers of two: the
-// product is rounded once, to 11 bits; for fp16 and fp32 queries to two parts).  The products
+// values' scales: weight * scale / r * 2^14, at most 2^14, is the fp16 operand (powers of two: the
+// product is rounded once, to 11 bits; for fp16 and fp32 queries to two parts).  Those bits are
+// kept of values down to 2^-28 of the largest, whose weight may be nothing.  The products
 // of a chunk are summed by themselves and added in rounded fp32, which takes the factor of a
 // new maximum along for nothing.
 //
@@ -53,6 +54,7 @@ struct AttnArgs {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr float kNone = -3e38f;  // the maximum of a row that has seen no token
+constexpr float kUp = 0x1p14f;   // what an fp16 weight is multiplied by
 
 __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -286,7 +288,7 @@ struct Attn {
         inv_ref = __uint_as_float((254u << 23) - __float_as_uint(top));
         float ratio[BLOCKS];
 #pragma unroll
-        for (int y = 0; y < BLOCKS; y++) ratio[y] = vs[y] * inv_ref;
+        for (int y = 0; y < BLOCKS; y++) ratio[y] = vs[y] * inv_ref * kUp;
         float g[NT][2];
         uint32_t wb[BLOCKS][NT][PARTS][2];
 #pragma unroll
@@ -412,7 +414,7 @@ struct Attn {
     }
     // v / s in units of u
     __device__ __forceinline__ static float result(float v, float s, float u) {
-        return s == 0.f ? 0.f : v / s * u;
+        return s == 0.f ? 0.f : v / s * (u / kUp);
     }
 
     // Joins the warps; whole: the outputs are final, else they go to `part`: [row][D], then

@@ -554,3 +554,24 @@ def test_the_serving_example(bits):
     example = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(example)
     assert example.run(layers=2, steps=5, prompts=(37, 5, 300), bits=bits) < 2.0 ** -7
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_a_large_value_of_no_weight(dtype):
+    """A token whose values are 2^16 times larger and whose weight is nothing costs the others no bits: bounds
+    with M the largest |value| that has a weight."""
+    n, D = 300, 64
+    g = torch.Generator().manual_seed(5)
+    k, v = torch.randn(n, 1, D, generator=g), torch.randn(n, 1, D, generator=g)
+    q = torch.ones(1, 2, D)
+    k[40:56] = -40.0  # a run that no query attends to: scores of -320, weights of e^-300
+    v[40:56] *= 2.0 ** 16
+    table, pages = table_of([n], 16)
+    cache = new_cache(pages, 1, D, 16)
+    cache.append(None, k[None].cuda(), v[None].cuda(), table, i32([0]))
+    held = tuple(kv8.values(*kv8.quantise(x.numpy())) for x in (k, v))
+    out = cache.attend(q.to(DT[dtype]).cuda(), table, i32([n]))
+    want, _ = kv8.attention(q.numpy(), *held, D ** -0.5)
+    rest = np.concatenate([held[1][:40], held[1][56:]])
+    err = np.abs(out.double().cpu().numpy() - want)
+    assert (err <= HALF_STEP[dtype] * np.abs(want) + SLACK[dtype] * np.abs(rest).max()).all()

@@ -312,13 +312,16 @@ constexpr int kLeastPiece = 8;
 struct Line {
     const Args &a;
     int TP, most;
+    unsigned inv;     // 2^32 / TP, rounded up (not of 1)
     Sequence mine;    // of this lane, where there are no more sequences than lanes
+    int all;          // its items
     int64_t tiles;    // of all items and heads, where they are cut
 
-    __device__ __forceinline__ Line(const Args &args, int tp) : a(args), TP(tp), most(0), mine{}, tiles(1) {
+    __device__ __forceinline__ Line(const Args &args, int tp) : a(args), TP(tp), most(0), inv(0xffffffffu / (unsigned)tp + 1), mine{}, all(0), tiles(1) {
         const int lane = threadIdx.x & 31;
         if (a.B > 32) return;
         if (lane < a.B) mine = sequence(a, lane);
+        all = over((unsigned)mine.nq + TP - 1);
         most = __reduce_max_sync(0xffffffffu, tiles_of(mine.nk));
         if (a.split) {
             int64_t n = 0;
@@ -329,19 +332,21 @@ struct Line {
         }
     }
 
-    // Items of a sequence with at least w key tiles: those from a token on.
-    __device__ __forceinline__ int items_from(const Sequence &s, int w) const {
-        const int n = (int)(((unsigned)s.nq + TP - 1) / (unsigned)TP);
-        if (w == 0) return n;
-        if (tiles_of(s.nk) < w) return 0;
-        if (!a.causal) return n;
+    // n / TP: the product is right up to 2^24 at least, since TP * inv passes 2^32 by less than 2^8.
+    __device__ __forceinline__ int over(unsigned n) const {
+        return (int)(TP == 1 ? n : n < 1u << 24 ? __umulhi(n, inv) : n / (unsigned)TP);
+    }
+
+    // Items of this lane's sequence with at least w key tiles: those from a token on.
+    __device__ __forceinline__ int items_from(int w) const {
+        if (w == 0) return all;
+        if (tiles_of(mine.nk) < w) return 0;
+        if (!a.causal) return all;
         // item t's last token sees min(nk, nk - nq + (t + 1) TP) keys: more than (w - 1) kTile
-        const int need = (w - 1) * kTile - s.nk + s.nq;  // (t + 1) TP > need, which is below nq
-        return n - (need < 0 ? 0 : (int)((unsigned)need / (unsigned)TP));
+        const int need = (w - 1) * kTile - mine.nk + mine.nq;  // (t + 1) TP > need, which is below nq
+        return all - (need < 0 ? 0 : over((unsigned)need));
     }
-    __device__ __forceinline__ int count(int w) const {
-        return __reduce_add_sync(0xffffffffu, items_from(mine, w));
-    }
+    __device__ __forceinline__ int count(int w) const { return __reduce_add_sync(0xffffffffu, items_from(w)); }
     // Tiles from which on an item has a piece p > 0.
     __device__ __forceinline__ int of_piece(int p) const {
         const int64_t n = ((p + 1) * tiles + gridDim.x - 1) / gridDim.x;
@@ -385,7 +390,7 @@ struct Line {
             (count(mid) > item ? lo : hi) = mid;
         }
         const int left = item - count(lo + 1);  // among the items of lo tiles, by sequence
-        const int all = items_from(mine, 0), ge = items_from(mine, lo), m = ge - items_from(mine, lo + 1);
+        const int ge = items_from(lo), m = ge - items_from(lo + 1);
         const int t0 = a.causal ? all - ge : 0;
         int upto = m;
 #pragma unroll
@@ -689,9 +694,14 @@ struct Block {
             __syncwarp();
             if ((threadIdx.x & 31) == 0) mbar_arrive(small->s_free + slot);
         }
-        if constexpr (MASK) {
+        if constexpr (MASK) {  // 32 keys at a time, where one of the warp's rows does not see them all
+            const int least = __reduce_min_sync(0xffffffffu, lim);
 #pragma unroll
-            for (int k = 0; k < kTile; k++) z[k] = k < lim ? z[k] : -INFINITY;
+            for (int c = 0; c < kTile; c += 32)
+                if (least < c + 32) {
+#pragma unroll
+                    for (int k = c; k < c + 32; k++) z[k] = k < lim ? z[k] : -INFINITY;
+                }
         }
         float m[8] = {z[0], z[1], z[2], z[3], z[4], z[5], z[6], z[7]};
 #pragma unroll

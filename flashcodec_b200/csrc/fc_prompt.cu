@@ -39,8 +39,8 @@
 // load, where the power cap holds the clock near 1.5 GHz.  A pair of tiles takes 2970 cycles where the products
 // alone would take 2050: a stream's softmax (1790: 200 to read the scores, 230 for the maximum, 600 for each
 // half's weights, 150 to store them) and its next two products follow one another, and two streams are all
-// that TMEM holds.  517 tokens 16 us, 8191 packed in 7 prompts 172 us, 512 tokens over up to 30000 keys
-// (14/2 heads, D = 64, fp16) 98 us.  Heads of 64: 0.67 PFLOP/s, half a tile's products for the same softmax.
+// that TMEM holds.  517 tokens 16 us, 8191 packed in 7 prompts 167 us, 512 tokens over up to 30000 keys
+// (14/2 heads, D = 64, fp16) 95 us.  Heads of 64: 0.67 PFLOP/s, half a tile's products for the same softmax.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

@@ -83,7 +83,8 @@ struct Args {
     int negative;
     int *status;
     int epoch;
-    int split;        // items may be cut along their keys
+    int split;        // items may be cut along their keys,
+    int items;        // if there are no more (item, head) than this: what the workspace is made for
     int *counters;    // by (item, head), stream and warp: pieces done, zero between calls
     int *slots;       // by (item, head) and piece: where its results are
     float *parts;     // results of pieces, kPart floats each
@@ -315,15 +316,19 @@ struct Line {
     unsigned inv;     // 2^32 / TP, rounded up (not of 1)
     Sequence mine;    // of this lane, where there are no more sequences than lanes
     int all;          // its items
+    // Items are cut along their keys.  (cu_seqlens that fall again are sequences that overlap, and more items
+    // than the rows that there are could be: the workspace has no room for their pieces.)
+    bool split;
     int64_t tiles;    // of all items and heads, where they are cut
 
-    __device__ __forceinline__ Line(const Args &args, int tp) : a(args), TP(tp), most(0), inv(0xffffffffu / (unsigned)tp + 1), mine{}, all(0), tiles(1) {
+    __device__ __forceinline__ Line(const Args &args, int tp) : a(args), TP(tp), most(0), inv(0xffffffffu / (unsigned)tp + 1), mine{}, all(0), split(false), tiles(1) {
         const int lane = threadIdx.x & 31;
         if (a.B > 32) return;
         if (lane < a.B) mine = sequence(a, lane);
         all = over((unsigned)mine.nq + TP - 1);
         most = __reduce_max_sync(0xffffffffu, tiles_of(mine.nk));
-        if (a.split) {
+        split = a.split && (int64_t)__reduce_add_sync(0xffffffffu, all) * a.Hk <= a.items;
+        if (split) {
             int64_t n = 0;
             for (int t = TP; t - TP < mine.nq; t += TP) n += tiles_of(visible(a, mine, min(t, mine.nq) - 1));
 #pragma unroll
@@ -376,7 +381,7 @@ struct Line {
         }
         int p = 0, n = count(0) * a.Hk;
         while (rank >= n) {
-            if (!a.split || n == 0) return false;
+            if (!split || n == 0) return false;
             rank -= n;
             n = count(of_piece(++p)) * a.Hk;
         }
@@ -410,7 +415,7 @@ struct Line {
         const int NT = x.tiles;
         x.pieces = 1;
         x.base = 0;
-        if (!a.split) return;
+        if (!split) return;
         x.pieces = (int)max(min((int64_t)NT * gridDim.x / tiles, (int64_t)((NT - 1) / kLeastPiece + 1)), (int64_t)1);
         const int j0 = (int)((int64_t)NT * x.piece / x.pieces), n = (int)((int64_t)NT * (x.piece + 1) / x.pieces) - j0;
         for (int s = 0; s < streams; s++) x.nt[s] = min(max(x.nt[s] - j0, 0), n);
@@ -1255,6 +1260,7 @@ extern "C" int fc_prompt_attn(const void *q, int64_t q_sb, int64_t q_ss, int64_t
     const int sms = num_sms() < kMaxPieces ? num_sms() : kMaxPieces;
     const int64_t keys = cu_seqlens_q ? Tk : Sk;
     a.split = items < num_sms() && B <= 32 && keys > kLeastPiece * kTile;
+    a.items = (int)items;
     char *ws = static_cast<char *>(workspace) + kWsHeader;
     a.counters = reinterpret_cast<int *>(ws);
     a.slots = reinterpret_cast<int *>(ws + kWsUnits * 4);

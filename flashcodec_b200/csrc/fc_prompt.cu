@@ -376,7 +376,8 @@ struct Line {
             const int *cu = a.cu_q, tp = TP, T = a.Tq;
             x.b = kv4::warp_find([=](int i) { return (int64_t)(min(max(cu[i], 0), T) / tp) + i; }, a.B, item);
             const int64_t t = (int64_t)(item - min(max(cu[x.b], 0), T) / tp - x.b) * TP;
-            x.t = (int)min(max(t, (int64_t)0), (int64_t)0x7fffff00);
+            // (a number of none: before the first sequence's, or left out)
+            x.t = (int)(t < 0 ? (int64_t)0x7fffff00 : min(t, (int64_t)0x7fffff00));
             return true;
         }
         int p = 0, n = count(0) * a.Hk;

@@ -51,3 +51,24 @@ def test_sequences_that_overlap_stay_in_the_workspace():
     for i in rows[:4]:  # nothing seen in the short ones
         want = exact(q[i:i + 1], k[:m - n + i + 1], v[:m - n + i + 1])[0][0]
         assert np.minimum(np.abs(out[i] - want), np.abs(out[i])).max() <= lim
+
+
+@pytest.mark.parametrize("lead", [0, 7, 1500])
+@pytest.mark.parametrize("B,n", [(33, 50), (700, 13)])
+def test_many_sequences_behind_rows_of_no_sequence(B, n, lead):
+    """More sequences than a warp has lanes, not from row 0 on: in place and beside are the same bits, each
+    item being computed once; rows of no sequence get zeros.  (Keys of one tile: no row takes another reference.)"""
+    T = lead + B * n + 20
+    q, k, v = make([(T, T)], 4, 2, 64, "bf16", B + lead)
+    c = i32([lead + n * b for b in range(B + 1)])
+    want, lse = fc().prompt_attention(q, k, v, c, return_lse=True)
+    assert not want[:lead].any() and not want[-20:].any()
+    assert torch.isneginf(lse[:lead]).all() and torch.isneginf(lse[-20:]).all()
+    for b in (0, 1, B // 2, B - 1):
+        at = slice(lead + b * n, lead + b * n + n)
+        near(want[at], exact(q[at], k[at], v[at])[0], "bf16", v[at].abs().max().item())
+    assert torch.equal(want[lead:-20], fc().prompt_attention(q[lead:-20], k[lead:-20], v[lead:-20], c - lead))
+    for _ in range(3):
+        mine = q.clone()
+        assert fc().prompt_attention(mine, k, v, c, out=mine) is mine and torch.equal(mine, want)
+    assert fc().attention_status().value() == 0

@@ -291,6 +291,9 @@ struct Item {
     // an item cut along its keys: the first key, which piece, of how many; its number among the pieces of
     // all items, and that of the (item, head)
     int base, piece, pieces, unit, line;
+    // a masked value was no number: set by the helpers, which may be as far ahead of the softmax as items are
+    // known, so it has its place with the item
+    int bad;
 };
 
 // Keys that token i sees.
@@ -437,7 +440,7 @@ template <int DP> struct Small {
     uint64_t o_done[2];             // by stream: a product P V is done
     uint64_t item_full[kItems], item_empty[kItems];
     Item items[kItems];
-    int abort_s, bad[2];            // bad: by item, its number + 1 if a value was no number
+    int abort_s;
     uint32_t tmem;
 };
 
@@ -789,13 +792,13 @@ struct Block {
             }
             if (nt && !wait_warp(small->o_done + s, (o_count - 1) & 1)) return;
             tc_fence_after();
-            write(*item, it, s, tok, head, nt, r, lanes);
+            write(*item, s, tok, head, nt, r, lanes);
             done<true>(it);
         }
     }
 
     // Outputs of one row, or what they are joined from.
-    __device__ __forceinline__ void write(const Item &x, int it, int s, int tok, int head, int nt, const Row &r, uint32_t lanes) const {
+    __device__ __forceinline__ void write(const Item &x, int s, int tok, int head, int nt, const Row &r, uint32_t lanes) const {
         using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
         const int i = x.t + s * a.TQ + tok, h = x.h * a.G + head, row = threadIdx.x & 127;
         const bool on = tok < a.TQ && i < x.s.nq, cut = x.pieces > 1;
@@ -849,7 +852,7 @@ struct Block {
                 a.lse[(a.cu_q ? at : (int64_t)x.b * a.Sq + i) * a.Hq + h] = l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.693147180559945309f;
         };
         const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
-        const bool fix = nt && *reinterpret_cast<volatile int *>(small->bad + (it & 1)) == it + 1;
+        const bool fix = nt && *const_cast<const volatile int *>(&x.bad);
         float *part = a.parts + ((int64_t)x.unit * NQ + s) * kPart + row;  // columns of 128 rows, then references and sums
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
@@ -988,7 +991,7 @@ struct Block {
                             v[i * 64] = make_uint4(zero(y.x), zero(y.y), zero(y.z), zero(y.w));
                         }
                     }
-                    if (any) *reinterpret_cast<volatile int *>(small->bad + (it & 1)) = it + 1;
+                    if (any) *const_cast<volatile int *>(&item->bad) = 1;
                     fence_async_smem();
                     __syncwarp();
                     if (w == 0 && !wait_warp(small->v_half + st, parity)) return;
@@ -1028,7 +1031,6 @@ prompt_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             mbar_init(m.p_full + 2 * i + 1, 4);
             mbar_init(m.s_free + i, 4);
             mbar_init(m.o_done + i, 1);
-            m.bad[i] = 0;
         }
         for (int i = 0; i < kItems; i++) {
             mbar_init(m.item_full + i, 1);

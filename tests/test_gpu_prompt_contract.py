@@ -72,3 +72,28 @@ def test_many_sequences_behind_rows_of_no_sequence(B, n, lead):
         mine = q.clone()
         assert fc().prompt_attention(mine, k, v, c, out=mine) is mine and torch.equal(mine, want)
     assert fc().attention_status().value() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 192])
+@pytest.mark.parametrize("Hq,Hk", [(2, 1), (8, 8)])
+def test_no_numbers_in_many_sequences(D, Hq, Hk):
+    """Every sequence holds an infinity and a NaN among its values, in tiles that are looked through; empty ones
+    lie between them.  Outputs are finite where fp64's are, for every item and whatever is under way beside it."""
+    rng = np.random.default_rng(D + Hk)
+    B = 700 // Hk
+    lens = [int(n) if rng.random() < 0.6 else 0 for n in rng.integers(2, 40, B)]
+    c = cu(lens)
+    q, k, v = make([(sum(lens), sum(lens))], Hq, Hk, D, "bf16", B)
+    a, finite = 0, torch.ones(sum(lens), Hq, D, dtype=torch.bool)
+    for n in lens:
+        if n:
+            i, j = sorted(rng.integers(0, n, 2).tolist())
+            d, h, G = int(rng.integers(0, D - 1)), int(rng.integers(0, Hk)), Hq // Hk
+            v[a + i, h, d], v[a + j, h, d + 1] = math.inf, math.nan
+            finite[a + i:a + n, h * G:h * G + G, d] = False
+            finite[a + j:a + n, h * G:h * G + G, d + 1] = False
+        a += n
+    for _ in range(5):
+        out = fc().prompt_attention(q, k, v, c)
+        assert torch.equal(out.isfinite().cpu(), finite)
+    assert fc().attention_status().value() == 0

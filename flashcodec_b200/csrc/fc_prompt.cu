@@ -95,6 +95,7 @@ constexpr int kBox = kTile * 128;   // bytes of 128 rows of 64 channels
 constexpr int kItems = 3;           // items known ahead
 constexpr uint64_t kItemNs = 100 * kWaitNs;  // bound on waits for an item
 constexpr int kMaxPieces = 256;     // of an item: no more than blocks
+constexpr int kNoRow = 0x7fffffff;   // keys that a row of no query sees
 constexpr int kPolyStep = 4;        // every kPolyStep-th pair of weights is a polynomial
 
 template <int DP> struct Cfg {
@@ -692,7 +693,7 @@ struct Block {
     // cycles while products are running (four of 32 keys, each waited for: 1800 cycles a tile instead of
     // 1400).  The product with V begins when the first 64 keys' weights are there.
     template <bool MASK>
-    __device__ __forceinline__ bool tile(Row &r, int s, int slot, uint32_t lanes, int lim, bool first, unsigned o_count) const {
+    __device__ __forceinline__ bool tile(Row &r, int s, int slot, uint32_t lanes, int lim, bool on, bool first, unsigned o_count) const {
         const uint32_t at = tmem + lanes + slot * kTile, to = tmem + lanes + C::P_COL + slot * C::P_STEP;
         float z[kTile];
 #pragma unroll
@@ -720,9 +721,11 @@ struct Block {
 #pragma unroll
         for (int e = 0; e < 8; e++) m[e] = fmaxf(m[e], z[120 + e]);
         const float top = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
-        // the reference follows only a maximum that is 2^8 above it: weights stay below 2^8
+        // The reference follows only a maximum that is 2^8 above it: weights stay below 2^8.  A warp's rows move
+        // theirs together; rows of no query, which hold the next sequence's queries or nothing that was written,
+        // do not ask for it: another reference is another rounding of the weights.
         float f = 1.f;
-        const bool moved = __any_sync(0xffffffffu, fmaf(top, a.scale, -r.ref) > 8.f);
+        const bool moved = __any_sync(0xffffffffu, on && fmaf(top, a.scale, -r.ref) > 8.f);
         if (moved) {
             const float n = fmaxf(r.ref, ceilf(top * a.scale)), d = r.ref - n;  // d <= 0, no number where both are infinite
             f = d == 0.f ? 1.f : d > -126.f ? __int_as_float(((int)d + 127) << 23) : 0.f;
@@ -777,7 +780,7 @@ struct Block {
         for (int it = 0; (item = next<true>(it)); it++) {
             // (rows of no query need no mask: their results go nowhere)
             const int i = item->t + s * a.TQ + tok;
-            const int vis = tok < a.TQ && i < item->s.nq ? visible(a, item->s, i) - item->base : 0x7fffffff;
+            const int vis = tok < a.TQ && i < item->s.nq ? visible(a, item->s, i) - item->base : kNoRow;
             Row r{-INFINITY, 0.f};
             const int nt = item->nt[s];
             for (int j = 0; j < nt; j++) {
@@ -785,8 +788,9 @@ struct Block {
                 if (!wait_warp(small->s_full + slot, s_uses[NQ == 2 ? 0 : slot]++ & 1)) return;
                 tc_fence_after();
                 const int lim = vis - j * kTile;
-                if (__any_sync(0xffffffffu, lim < kTile) ? !tile<true>(r, s, slot, lanes, lim, j == 0, o_count)
-                                                         : !tile<false>(r, s, slot, lanes, lim, j == 0, o_count))
+                const bool on = vis != kNoRow;
+                if (__any_sync(0xffffffffu, lim < kTile) ? !tile<true>(r, s, slot, lanes, lim, on, j == 0, o_count)
+                                                         : !tile<false>(r, s, slot, lanes, lim, on, j == 0, o_count))
                     return;
                 o_count++;
             }

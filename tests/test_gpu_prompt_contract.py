@@ -97,3 +97,39 @@ def test_no_numbers_in_many_sequences(D, Hq, Hk):
         out = fc().prompt_attention(q, k, v, c)
         assert torch.equal(out.isfinite().cpu(), finite)
     assert fc().attention_status().value() == 0
+
+
+@pytest.mark.parametrize("Hq,Hk", [(3, 1), (14, 2), (20, 4)])
+@pytest.mark.parametrize("D", [64, 128, 192])
+@pytest.mark.parametrize("many", [False, True])
+def test_rows_of_no_query_change_no_bits(D, Hq, Hk, many):
+    """Groups that do not divide 128 leave rows of a query tile without a query, and a sequence's last tile holds
+    the next one's: with scores that grow, in place and beside, after whatever other calls left behind, the same bits."""
+    lens = [(300, 300), (5, 260), (129, 400), (41, 41), (700, 700), (77, 390)] * (6 if many else 1)
+    q, k, v = make(lens, Hq, Hk, D, "bf16", Hq)
+    k = (k.float() * torch.linspace(0, 8, k.shape[0], device="cuda").sin()[:, None, None] * 4).bfloat16()
+    args = cu([n for n, _ in lens]), cu([m for _, m in lens])
+    want = fc().prompt_attention(q, k, v, *args)
+    for a, b, (n, m) in ((0, 0, lens[0]), (300, 300, lens[1])):
+        # (sums of |q k| up to 700 here: scores off by 2^-11, 2^-12 more than near() has, which is 2^-4 of its 2^-8)
+        near(want[a:a + n], exact(q[a:a + n], k[b:b + m], v[b:b + m])[0], "bf16", (1 + 2.0 ** -4) * v[b:b + m].abs().max().item())
+    for size in (1.0, 300.0, -300.0):
+        x = torch.full((4000, 16, D), size, dtype=q.dtype, device="cuda")
+        fc().prompt_attention(x, x, x, i32([0, 4000]))  # (other rows of shared memory)
+        assert torch.equal(fc().prompt_attention(q, k, v, *args), want)
+        mine = q.clone()
+        fc().prompt_attention(mine, k, v, *args, out=mine)
+        assert torch.equal(mine, want)
+    # neighbours of other sizes
+    other = q.clone()
+    a = 0
+    for i, (n, _) in enumerate(lens):
+        if i % 2:
+            other[a:a + n] *= 64
+        a += n
+    out = fc().prompt_attention(other, k, v, *args)
+    a = 0
+    for i, (n, _) in enumerate(lens):
+        if i % 2 == 0:
+            assert torch.equal(out[a:a + n], want[a:a + n])
+        a += n

@@ -227,13 +227,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // 2^x without the special function units, whose 16 lanes would otherwise take as long as both
 // products of a tile: 2^round(x) put into the exponent, 2^f on [-1/2, 1/2] as a polynomial
 // (least largest relative error, by reweighted least squares: 2^-13.7 of degree 3 for bf16
-// weights, 2^-18.5 of degree 4 for fp16 ones).  From -125 down the result is no weight any more;
-// a NaN stays one.  x is at most 8 or no number.
+// weights, 2^-18.5 of degree 4 for fp16 ones).  From -127 down the result is 0.  The power of two is a factor, not
+// an addition to the exponent's bits, which would turn a NaN into a number.  x is at most 8 or no number.
 template <bool F16>
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
     auto low = [](float v) {
         float y;
-        asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(v), "f"(-125.f));
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(v), "f"(-127.f));
         return y;
     };
     x = make_float2(low(x.x), low(x.y));
@@ -252,9 +252,9 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
         p = __ffma2_rn(f, p, c2(0.6932609677314758f));
         p = __ffma2_rn(f, p, c2(0.9999280571937561f));
     }
-    p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
-    p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
-    return p;
+    // (t = 1.5 * 2^23 + n: its low bits are n, in two's complement; at n = -127 the factor is 0)
+    auto power = [](float v) { return __int_as_float((__float_as_int(v) << 23) + 0x3f800000); };
+    return __fmul2_rn(p, make_float2(power(t.x), power(t.y)));
 }
 
 template <bool F16>

@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_prompt import check, cu, exact, fc, i32, make, near
+from test_gpu_prompt import cu, exact, fc, i32, make, near, near_lse
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +133,39 @@ def test_rows_of_no_query_change_no_bits(D, Hq, Hk, many):
         if i % 2 == 0:
             assert torch.equal(out[a:a + n], want[a:a + n])
         a += n
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 96, 128, 192, 256])
+def test_a_key_that_is_no_number(D, dtype):
+    """Wherever it lies in a tile that all rows see, the rows that see it are NaN, log-sums too, and no other."""
+    n = 400
+    q, k, v = (t.to(dtype) for t in make([(n, n)], 4, 2, D, "bf16"))
+    want = fc().prompt_attention(q, k, v, cu([n]), return_lse=True)
+    for j in [*range(8), 121, 126, 127, 260, 263]:
+        y = k.clone()
+        y[j, 0, 3] = math.nan
+        got = fc().prompt_attention(q, y, v, cu([n]), return_lse=True)
+        for g, w in zip(got, want):
+            assert torch.equal(g[:, 2:], w[:, 2:]) and torch.equal(g[:j, :2], w[:j, :2])
+            assert g[j:, :2].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 192])
+def test_keys_that_weigh_nothing(D, dtype):
+    """Keys whose scores are infinite below: no weight, wherever they lie in a tile; others as without them."""
+    n = 400
+    q, k, v = (t.to(dtype) for t in make([(n, n)], 2, 1, D, "bf16"))
+    q[..., 0] = 1.0
+    for j in range(8):
+        none = torch.zeros(n, dtype=torch.bool)
+        none[40 + j:200:8] = True
+        y = k.clone()
+        y[none, 0, 0] = -math.inf
+        out, lse = fc().prompt_attention(q, y, v, cu([n]), return_lse=True)
+        rest = ~none
+        for i in (300, 399):
+            want, wl = exact(q[i:i + 1], k[:i + 1][rest[:i + 1]], v[:i + 1][rest[:i + 1]])
+            near(out[i:i + 1], want, "bf16" if dtype is torch.bfloat16 else "fp16", v.abs().max().item())
+            near_lse(lse[i:i + 1], wl)

@@ -96,6 +96,10 @@ constexpr int kItems = 3;           // items known ahead
 constexpr uint64_t kItemNs = 100 * kWaitNs;  // bound on waits for an item
 constexpr int kMaxPieces = 256;     // of an item: no more than blocks
 constexpr int kNoRow = 0x7fffffff;   // keys that a row of no query sees
+// fp16 weights are held 2^7 times larger (at most 2^15, the largest being above 2^6): each is off by 2^-11 of
+// itself or by 2^-25, 2^-31 of the row's sum, so that a tail of 2^20 keys costs no more than another 2^-11.
+// (Unscaled, 32768 keys of 2^-25 the largest's weight were nothing, in a sum that counted them as 2^-10.)
+template <bool F16> constexpr float kUp = F16 ? 7.f : 0.f;
 constexpr int kPolyStep = 4;        // every kPolyStep-th pair of weights is a polynomial
 
 template <int DP> struct Cfg {
@@ -228,7 +232,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // products of a tile: 2^round(x) put into the exponent, 2^f on [-1/2, 1/2] as a polynomial
 // (least largest relative error, by reweighted least squares: 2^-13.7 of degree 3 for bf16
 // weights, 2^-18.5 of degree 4 for fp16 ones).  From -127 down the result is 0.  The power of two is a factor, not
-// an addition to the exponent's bits, which would turn a NaN into a number.  x is at most 8 or no number.
+// an addition to the exponent's bits, which would turn a NaN into a number.  x is at most 15 or no number.
 template <bool F16>
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
     auto low = [](float v) {
@@ -732,7 +736,7 @@ struct Block {
             r.ref = n;
             r.l *= f;
         }
-        const float off = r.ref == -INFINITY ? 0.f : -r.ref;
+        const float off = r.ref == -INFINITY ? 0.f : kUp<F16> - r.ref;
         const float2 off2 = make_float2(off, off);
         float2 sum[2] = {};
         uint32_t w[32];
@@ -853,7 +857,7 @@ struct Block {
         };
         auto log_sum = [&](float ref, float l) {
             if (on && a.lse)
-                a.lse[(a.cu_q ? at : (int64_t)x.b * a.Sq + i) * a.Hq + h] = l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.693147180559945309f;
+                a.lse[(a.cu_q ? at : (int64_t)x.b * a.Sq + i) * a.Hq + h] = l == 0.f ? -INFINITY : (ref - kUp<F16> + log2f(l)) * 0.693147180559945309f;
         };
         const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
         const bool fix = nt && *const_cast<const volatile int *>(&x.bad);

@@ -169,3 +169,23 @@ def test_keys_that_weigh_nothing(D, dtype):
             want, wl = exact(q[i:i + 1], k[:i + 1][rest[:i + 1]], v[:i + 1][rest[:i + 1]])
             near(out[i:i + 1], want, "bf16" if dtype is torch.bfloat16 else "fp16", v.abs().max().item())
             near_lse(lse[i:i + 1], wl)
+
+
+@pytest.mark.parametrize("n,m,Hq,Hk", [(3, 32769, 2, 1), (9216, 32769, 4, 4)])
+@pytest.mark.parametrize("at", [0, 20000])
+def test_a_tail_of_small_weights(n, m, Hq, Hk, at):
+    """32768 keys of 2^-25 the weight of one whose value is zero: fp16 weights keep them, cut along the keys and
+    not.  Held 2^7 times larger, each is off by 2^-25 of a sum above 2^6: 2^-31 M a key; scores and exponentials
+    (polynomials: 2^-18.5, which is 2^-18 with fp32's own) and the output's rounding, 2^-11, are of the result."""
+    D = 64
+    q = torch.zeros(n, Hq, D, dtype=torch.float16, device="cuda")
+    k = torch.zeros(m, Hk, D, dtype=torch.float16, device="cuda")
+    v = torch.ones(m, Hk, D, dtype=torch.float16, device="cuda")
+    q[..., 0], k[at, :, 0], v[at] = 8.0, 17.33, 0.0
+    tail = (m - 1) * math.exp(-k[at, 0, 0].item())
+    out, lse = fc().prompt_attention(q, k, v, cu([n]), cu([m]), causal=False, return_lse=True)
+    want = tail / (1 + tail)
+    err = (out.double() - want).abs().max().item()
+    assert err <= (2.0 ** -11 + 2.0 ** -18) * want + m * 2.0 ** -31, f"{out.flatten()[0].item()} for {want}"
+    assert (lse.double() - (k[at, 0, 0].item() + math.log1p(tail))).abs().max() <= 2.0 ** -12
+    assert fc().attention_status().value() == 0

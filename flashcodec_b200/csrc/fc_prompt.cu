@@ -789,7 +789,8 @@ struct Block {
             const int nt = item->nt[s];
             for (int j = 0; j < nt; j++) {
                 const int slot = NQ == 2 ? s : j & 1;
-                if (!wait_warp(small->s_full + slot, s_uses[NQ == 2 ? 0 : slot]++ & 1)) return;
+                // (the first scores come when the other stream is done with its tiles of the item before)
+                if (!wait_warp(small->s_full + slot, s_uses[NQ == 2 ? 0 : slot]++ & 1, j ? kWaitNs : kItemNs)) return;
                 tc_fence_after();
                 const int lim = vis - j * kTile;
                 const bool on = vis != kNoRow;

@@ -189,3 +189,22 @@ def test_a_tail_of_small_weights(n, m, Hq, Hk, at):
     assert err <= (2.0 ** -11 + 2.0 ** -18) * want + m * 2.0 ** -31, f"{out.flatten()[0].item()} for {want}"
     assert (lse.double() - (k[at, 0, 0].item() + math.log1p(tail))).abs().max() <= 2.0 ** -12
     assert fc().attention_status().value() == 0
+
+
+def test_a_stream_that_waits_for_a_long_one():
+    """100 queries over 2^25 keys (a third of a second, one query tile), and items of two tiles behind it on the
+    same block: the second tile's warps wait for longer than any product takes, and do not give up."""
+    m, n, B, D = 1 << 25, 200, 300, 64
+    lens = [(100, m)] + [(n, n)] * (B - 1)
+    k = torch.zeros(m + n * (B - 1), 1, D, dtype=torch.bfloat16, device="cuda")
+    q, k[m:], _ = make([(100 + n * (B - 1), n * (B - 1))], 1, 1, D, "bf16")
+    out, lse = fc().prompt_attention(q, k, k, cu([a for a, _ in lens]), cu([b for _, b in lens]), return_lse=True)
+    assert fc().attention_status(reset=True).value() == 0
+    assert not out[:100].any()
+    # equal scores of zero: weights of one, whose sum is exact
+    seen = torch.arange(m - 99, m + 1, device="cuda").double().log()
+    assert (lse[:100, 0].double() - seen).abs().max() <= 2.0 ** -19
+    for b in range(1, B, 23):
+        a, c = 100 + n * (b - 1), m + n * (b - 1)
+        x = k[c:c + n]
+        near(out[a:a + n], exact(q[a:a + n], x, x)[0], "bf16", x.abs().max().item())

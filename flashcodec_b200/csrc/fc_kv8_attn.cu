@@ -318,10 +318,12 @@ struct Attn {
                     float w[2];
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const float p = exp2_fast(s[y][nt][2 * j + x] - M[nt][x]);
+                        const float z = s[y][nt][2 * j + x], p = exp2_fast(z - M[nt][x]);
                         l[nt][x] += p;
-                        // a weight of zero is zero whatever the scale: the tokens may be behind the last one
-                        w[x] = p == 0.f ? 0.f : p * ratio[y];
+                        // A token that is not seen has no weight, whatever the scale: it may be behind the last
+                        // one.  (Not every weight of zero: values that are no numbers stay so where a weight is
+                        // below fp32, as it may be beside one block's largest score and not beside another's.)
+                        w[x] = z == -INFINITY ? 0.f : p * ratio[y];
                         ws[nt][x] += w[x];
                     }
                     const __half2 hi = __floats2half2_rn(w[0], w[1]);

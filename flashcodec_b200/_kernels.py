@@ -236,9 +236,11 @@ def attn_status_async(device: torch.device, reset: bool = False) -> StatusProbe:
     words = [_status_word(*w) for w in held]
     host.copy_(words[0] if len(words) == 1 else torch.stack(words).amax(0), non_blocking=True)
     if reset:
-        for ws, _ in held:
+        for ws, captured in held:
             ws[:4].zero_()
-            if any(ws is w for w in _prompt_workspaces.values()):  # a call that gave up may have left its counters
+            # An eager call that gave up may have left its counters.  A graph zeroes its own when it is replayed,
+            # and may be under way on another stream now.
+            if not captured and any(ws is w for w in _prompt_workspaces.values()):
                 ws[:_PROMPT_CLEAR].zero_()
     ev = torch.cuda.Event()
     ev.record(stream)

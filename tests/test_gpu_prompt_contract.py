@@ -208,3 +208,27 @@ def test_a_stream_that_waits_for_a_long_one():
         a, c = 100 + n * (b - 1), m + n * (b - 1)
         x = k[c:c + n]
         near(out[a:a + n], exact(q[a:a + n], x, x)[0], "bf16", x.abs().max().item())
+
+
+def test_clearing_the_status_leaves_the_counters_of_graphs():
+    """A graph may be under way on another stream when its capture's stream clears the status words."""
+    from flashcodec_b200 import _kernels as K
+    lens = [(40, 3000)]
+    q, k, v = make(lens, 4, 2, 64, "bf16")
+    args = (q, k, v, cu([40]), cu([3000]))
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fc().prompt_attention(*args)
+    with torch.cuda.graph(graph, stream=side):
+        fc().prompt_attention(*args)
+    graph.replay()
+    torch.cuda.synchronize()
+    held = {key[2] != 0: ws for key, ws in K._prompt_workspaces.items() if key[1] == side.cuda_stream}
+    for ws in held.values():
+        ws[256:260] = 7  # as if a row's pieces were on their way
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        assert fc().attention_status(reset=True).value() == 0
+    side.synchronize()
+    assert held[True][256:260].tolist() == [7] * 4 and held[False][256:260].tolist() == [0] * 4

@@ -158,7 +158,8 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     key = (device.index, stream, _lib.load().fc_capture_id(stream))
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(max(nbytes, 4096), dtype=torch.uint8, device=device)
+        with torch.inference_mode(False):  # it is written to in whatever mode a later call comes
+            ws = torch.zeros(max(nbytes, 4096), dtype=torch.uint8, device=device)
         _workspaces[key] = ws
         captures = [k for k in _workspaces if k[:2] == key[:2] and k[2]]
         for k in captures[:-KEPT_CAPTURES]:
@@ -635,7 +636,8 @@ def _kv4_workspace(what, sizes, units, index, stream, cache="kv4"):
     if units > ws.units:
         nbytes = getattr(_lib.load(), f"fc_{cache}_{what}_workspace_size")(*sizes)
         if nbytes > ws.bytes:
-            ws.buffer = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+            with torch.inference_mode(False):  # as for the decode attention
+                ws.buffer = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
             ws.address, ws.bytes = ws.buffer.data_ptr(), nbytes
             ws.clear()
         ws.units = units
@@ -750,7 +752,8 @@ def _prompt_workspace(index, stream, nbytes) -> torch.Tensor:
     key = (index, stream, capture)
     ws = _prompt_workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _prompt_workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        with torch.inference_mode(False):  # as for the decode attention
+            ws = _prompt_workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
         ws[:_PROMPT_CLEAR].zero_()
         if capture:
             captures = [k for k in _prompt_workspaces if k[:2] == key[:2] and k[2]]

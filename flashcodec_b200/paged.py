@@ -142,7 +142,8 @@ class _PagedCache:
         self.num_pages, self.num_kv_heads = int(num_pages), int(num_kv_heads)
         self.head_dim, self.page_size = int(head_dim), int(page_size)
         self.page_bytes = K.kv4_page_bytes(self.num_kv_heads, self.head_dim, self.page_size)
-        self._status = torch.zeros(1, dtype=torch.int32, device=dev)
+        with torch.inference_mode(False):  # what a cache holds can be written to in any mode
+            self._status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._index, self._scale, self._lib = dev.index, self.head_dim ** -0.5, _lib.load()
         self._status_ptr = self._status.data_ptr()
 
@@ -320,13 +321,14 @@ class PagedInt4Cache(_PagedCache):
     def __init__(self, num_pages, num_kv_heads, head_dim, page_size=64, bounds=False,
                  device="cuda"):
         super().__init__(num_pages, num_kv_heads, head_dim, page_size, device)
-        self._pool = torch.empty(self.num_pages, self.page_bytes, dtype=torch.uint8, device=self.device)
         self._bounds = self._exponents = None
-        if bounds:
-            self._bounds = torch.zeros(self.num_pages, self.num_kv_heads, 2, self.head_dim,
-                                       dtype=torch.int8, device=self.device)
-            self._exponents = torch.zeros(self.num_pages, self.num_kv_heads, dtype=torch.int32,
-                                          device=self.device)
+        with torch.inference_mode(False):
+            self._pool = torch.empty(self.num_pages, self.page_bytes, dtype=torch.uint8, device=self.device)
+            if bounds:
+                self._bounds = torch.zeros(self.num_pages, self.num_kv_heads, 2, self.head_dim,
+                                           dtype=torch.int8, device=self.device)
+                self._exponents = torch.zeros(self.num_pages, self.num_kv_heads, dtype=torch.int32,
+                                              device=self.device)
         self._pool_args = (self._pool.data_ptr(), self.num_pages, self.num_kv_heads, self.head_dim,
                            self.page_size)
         self._bounds_args = (self._bounds.data_ptr(), self._exponents.data_ptr()) if bounds \
@@ -463,8 +465,9 @@ class PagedInt8Cache(_PagedCache):
         super().__init__(num_pages, num_kv_heads, head_dim, page_size, device)
         self.page_bytes = 2 * self.num_kv_heads * self.page_size * (4 * self.head_dim + 1) // 4
         at = (self.num_pages, 2, self.num_kv_heads)
-        self._codes = torch.empty(*at, self.page_size, self.head_dim, dtype=torch.int8, device=self.device)
-        self._scales = torch.zeros(*at, self.page_size // 16, dtype=torch.float32, device=self.device)
+        with torch.inference_mode(False):
+            self._codes = torch.empty(*at, self.page_size, self.head_dim, dtype=torch.int8, device=self.device)
+            self._scales = torch.zeros(*at, self.page_size // 16, dtype=torch.float32, device=self.device)
         self._pool_args = (self._codes.data_ptr(), self._scales.data_ptr(), self.num_pages,
                            self.num_kv_heads, self.head_dim, self.page_size)
 

@@ -35,3 +35,26 @@ def test_values_that_are_no_numbers_and_weigh_nothing(D, dtype):
                 assert torch.equal(nan[:, :, 2:], fine[:, :, 2:]) and torch.equal(inf[:, :, 2:], fine[:, :, 2:])
             else:  # not seen
                 assert torch.equal(nan, fine) and torch.equal(inf, fine) and fine.isfinite().all()
+
+
+@pytest.mark.parametrize("made_in_inference_mode", [True, False])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_caches_and_calls_in_inference_mode(bits, made_in_inference_mode):
+    """A cache made in inference mode is checked, cleared and restored outside of it, and the other way round."""
+    make = fc().PagedInt8Cache if bits == 8 else (lambda *a, **kw: fc().PagedInt4Cache(*a, bounds=True, **kw))
+    x = torch.randn(1, 20, 2, 64, device="cuda")
+    with torch.inference_mode(made_in_inference_mode):
+        cache = make(4, 2, 64, page_size=16)
+        cache.append(None, x, x, i32([[0, 1]]), i32([0]))
+        cache.append(None, x, x, i32([[0, 9]]), i32([0]))  # a page outside the pool
+        want = cache.attend(x[:, 0], i32([[0, 1]]), i32([20]))
+        fc().prompt_attention(x[0].half(), x[0].half(), x[0].half(), i32([0, 20]))
+    with torch.inference_mode(not made_in_inference_mode):
+        with pytest.raises(fc()._lib.FlashCodecError, match="page outside"):
+            cache.check()
+        cache.check()
+        assert fc().attention_status(reset=True).value() == 0
+        held = [cache.pool] if bits == 4 else [cache.codes, cache.scales]
+        for t in held:
+            t.copy_(t.clone())
+        assert torch.equal(cache.attend(x[:, 0], i32([[0, 1]]), i32([20])), want)

@@ -199,8 +199,8 @@ def attn_status(device: torch.device) -> int:
 class StatusProbe:
     """A copy of an attention status word in flight to pinned host memory.
 
-    0 means every decode-attention call on that stream's workspace since the
-    last reset produced valid output; a positive value is the launch number of
+    0 means every decode or prompt attention call on that stream's workspaces since
+    the last reset produced valid output; a positive value is the launch number of
     a call whose bounded wait gave up (its output is invalid)."""
 
     def __init__(self, host: torch.Tensor, event: torch.cuda.Event | None):
@@ -221,7 +221,7 @@ class StatusProbe:
         v = self.value()
         if v:
             raise _lib.FlashCodecError(
-                _lib.FC_ECUDA, f"decode attention launch {v} gave up waiting for a staged "
+                _lib.FC_ECUDA, f"attention launch {v} gave up waiting for a staged "
                 "tile (bounded wait); its output is invalid")
 
 

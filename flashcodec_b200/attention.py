@@ -112,9 +112,9 @@ def codec_decode_attention(query, key_stream, value_stream, scale=None, impl="au
 
 
 def attention_status(device=None, reset=False):
-    """Failure status of the decode-attention calls issued on the current
-    stream of ``device``, without synchronising (an extension: the reference
-    kernels have no failure status).
+    """Failure status of the codec decode-attention and ``prompt_attention`` calls
+    issued on the current stream of ``device``, without synchronising (an
+    extension: the reference kernels have no failure status).
 
     Every wait inside the attention kernels is bounded; a call whose wait
     gave up leaves invalid output and records its launch number in the

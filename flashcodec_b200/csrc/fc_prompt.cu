@@ -26,7 +26,8 @@
 // What is masked.  Scores are replaced, not added to, so a NaN there is gone.  A value that no
 // weight but zero meets could still turn a sum into a NaN, so the tiles that hold masked keys
 // (one or two of an item) are looked through in shared memory: what is no number becomes zero
-// there, and is added in plain arithmetic to the rows that do see it.
+// there, and is added in plain arithmetic to the rows that do see it (an infinity whose weight is nothing then
+// makes an infinity, where one in a tile without a mask makes a NaN).
 //
 // Work.  Items (sequence, KV head, TQ or 2 TQ tokens) are dealt out to one block an SM, the
 // longest first, back and forth; every block finds its own from the lengths, which are on the
@@ -34,13 +35,13 @@
 // their keys, and the last warp to finish a row's pieces joins them, in order.  No block waits for
 // another.
 //
-// 16384 tokens, 32/8 heads, D = 128, bf16, causal (2.2 TFLOP): 1.74 ms in short runs, 1.27 PFLOP/s, 76 % of
-// the burst rate of a library product; 1.98 ms (1.11 PFLOP/s, 81 % of its sustained rate) under sustained
+// 16384 tokens, 32/8 heads, D = 128, bf16, causal (2.2 TFLOP): 1.77 ms in short runs, 1.25 PFLOP/s, 75 % of
+// the burst rate of a library product; 2.0 ms (1.1 PFLOP/s, 80 % of its sustained rate) under sustained
 // load, where the power cap holds the clock near 1.5 GHz.  A pair of tiles takes 2970 cycles where the products
 // alone would take 2050: a stream's softmax (1790: 200 to read the scores, 230 for the maximum, 600 for each
 // half's weights, 150 to store them) and its next two products follow one another, and two streams are all
-// that TMEM holds.  517 tokens 16 us, 8191 packed in 7 prompts 167 us, 512 tokens over up to 30000 keys
-// (14/2 heads, D = 64, fp16) 95 us.  Heads of 64: 0.67 PFLOP/s, half a tile's products for the same softmax.
+// that TMEM holds.  517 tokens 16 us, 8191 packed in 7 prompts 168 us, 512 tokens over up to 30000 keys
+// (14/2 heads, D = 64, fp16) 98 us.  Heads of 64: 0.67 PFLOP/s, half a tile's products for the same softmax.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -100,7 +101,9 @@ constexpr int kNoRow = 0x7fffffff;   // keys that a row of no query sees
 // itself or by 2^-25, 2^-31 of the row's sum, so that a tail of 2^20 keys costs no more than another 2^-11.
 // (Unscaled, 32768 keys of 2^-25 the largest's weight were nothing, in a sum that counted them as 2^-10.)
 template <bool F16> constexpr float kUp = F16 ? 7.f : 0.f;
-constexpr int kPolyStep = 4;        // every kPolyStep-th pair of weights is a polynomial
+// Every kPolyStep-th pair of weights of a tile without a mask is a polynomial.  8192 tokens, 32/8 heads, D = 128,
+// bf16: 440 us, 452 with none; fp16 462 and 467; 16/8 heads, D = 64, fp16 202 and 205, bf16 no difference.
+constexpr int kPolyStep = 4;
 
 template <int DP> struct Cfg {
     static constexpr int NQ = DP <= 128 ? 2 : 1;         // streams

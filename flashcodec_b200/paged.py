@@ -456,7 +456,9 @@ class PagedInt8Cache(_PagedCache):
     the codes held are then shifted, and equal those of the run quantised at once: what
     is stored does not depend on how tokens are split into calls.  A run with an infinity
     or a NaN reads as NaN.  A run whose tokens were dropped keeps its scale until its
-    first position is appended anew.
+    first position is appended anew: the tokens before them have then lost the bits that
+    their scale took (all of them, if one was no number).  Drafts that may be rejected are
+    better verified before they are appended.
     """
 
     _bits = 8

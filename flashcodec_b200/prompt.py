@@ -49,8 +49,11 @@ def prompt_attention(q, k, v, cu_seqlens=None, cu_seqlens_k=None, *, causal=True
     Returns the outputs in q's shape and dtype, and with ``return_lse`` the natural
     log of the softmax sums, q.shape[:-1] fp32.
 
-    Scores, softmax and sums are fp32; weights are rounded to q's dtype before they
-    meet the values.  It serves and has no gradient.
+    Scores, softmax and sums are fp32 (a quarter of the exponentials to 2^-13 with
+    bf16, 2^-18 with fp16); weights are rounded to q's dtype before they meet the
+    values (fp16: or by 2^-31 of their row's sum).  The products' sums cut, at
+    2^-24 of the sum of weight * |value| for every 16 keys: 2^-11 of it at 131072 keys.
+    Values beyond 2^128 / (256 * keys) may overflow.  It serves and has no gradient.
     """
     index, grad = q.get_device(), torch.is_grad_enabled()
     dual = getattr(forward_ad, "_current_level", 0) >= 0  # inside a dual level

@@ -741,7 +741,9 @@ FC_API int fc_kv8_attn(const void *q, int dtype, int64_t B, int64_t Sq, int64_t 
  * (B, Sk, Hk, D), Tq = B Sq, Tk = B Sk, cu_seqlens NULL.
  * Query i of n_q sees the keys 0 .. n_k - n_q + i with `causal` (the last query sees all),
  * else all n_k; one that sees none gets zeros.  A key or value that a query does not see
- * does not touch its output, whatever it holds.
+ * does not touch its output, whatever it holds; a score that is no number makes the output and
+ * the log-sum NaN, an infinite value whose weight rounds to nothing an infinity or a NaN.
+ * cu_seqlens that fall again make sequences that overlap, whose rows each of them writes.
  * lse (as q without D) fp32 or NULL: the natural logarithm of the softmax sums, -inf
  * where a query sees nothing.  out must not overlap k or v; it may be q itself, but
  * must not overlap it otherwise.

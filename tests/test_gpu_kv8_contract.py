@@ -58,3 +58,49 @@ def test_caches_and_calls_in_inference_mode(bits, made_in_inference_mode):
         for t in held:
             t.copy_(t.clone())
         assert torch.equal(cache.attend(x[:, 0], i32([[0, 1]]), i32([20])), want)
+
+
+def test_a_pool_beyond_32_bits():
+    """Pages whose codes lie beyond 2^32 bytes are appended to, read and attended to as those at the front."""
+    Hk, D, page, n = 8, 128, 64, 150
+    num = (9 << 29) // (2 * Hk * page * D) + 8
+    cache = fc().PagedInt8Cache(num, Hk, D, page_size=page)
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.randn(1, n, Hk, D, generator=g).cuda() for _ in range(2))
+    q = torch.randn(1, 16, D, generator=g).cuda()
+    got = []
+    for first in (0, num - 3):
+        table = i32([[first, first + 2, first + 1]])
+        cache.append(None, k, v, table, i32([0]))
+        got.append((*cache.read(table, count=n, dtype=torch.float32), cache.attend(q, table, i32([n]))))
+    cache.check()
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    assert (got[0][0] - k).abs().max() <= 2.0 ** -7 * k.abs().max()
+
+
+def test_calls_on_two_streams_at_once():
+    """Steps of two caches and prompts that are cut, issued to two streams in turn, without waiting: each gives what it
+    gives alone."""
+    work = []
+    for i, lens in enumerate(([40, 900, 3], [4000])):
+        g = torch.Generator().manual_seed(i)
+        B, m = len(lens), max(lens)
+        cache = new_cache(B * 64, 2, 128, 64)
+        table = torch.arange(B * 64, dtype=torch.int32, device="cuda").view(B, 64)
+        k = torch.randn(B, m, 2, 128, generator=g).bfloat16().cuda()
+        cache.append(None, k, k, table, i32([0] * B))
+        q = torch.randn(B, 8, 128, generator=g).bfloat16().cuda()
+        x = torch.randn(20, 8, 128, generator=g).bfloat16().cuda()
+        work.append((cache, table, i32(lens), q, (x, k[0], k[0], i32([0, 20]), i32([0, m]))))
+    run = lambda w: (w[0].attend(w[3], w[1], w[2]), fc().prompt_attention(*w[4]))  # noqa: E731
+    want = [run(w) for w in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for _ in range(100):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs.append((i, run(work[i])))
+    torch.cuda.synchronize()
+    for i, out in outs:
+        assert all(torch.equal(x, y) for x, y in zip(out, want[i]))

@@ -232,3 +232,24 @@ def test_clearing_the_status_leaves_the_counters_of_graphs():
         assert fc().attention_status(reset=True).value() == 0
     side.synchronize()
     assert held[True][256:260].tolist() == [7] * 4 and held[False][256:260].tolist() == [0] * 4
+
+
+def test_a_graph_of_many_sequences():
+    """More sequences than a warp has lanes, captured: replays follow cu_seqlens, rows in front included."""
+    B, T = 40, 900
+    q, k, v = make([(T, T)], 4, 2, 128, "bf16")
+    c = i32([20 * b for b in range(B + 1)])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fc().prompt_attention(q, k, v, c)
+    rng = np.random.default_rng(0)
+    for lead in (0, 300, 0, 5):
+        lens = rng.multinomial(T - lead - 30, rng.dirichlet([0.4] * B))
+        c.copy_(i32((lead + np.concatenate([[0], np.cumsum(lens)])).tolist()))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, fc().prompt_attention(q, k, v, c))
+        assert not out[:lead].any() and not out[-30:].any()
+        b = int(lens.argmax())
+        at = slice(int(c[b]), int(c[b + 1]))
+        near(out[at], exact(q[at], k[at], v[at])[0], "bf16", v[at].abs().max().item())
